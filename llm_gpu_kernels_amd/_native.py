@@ -5,7 +5,7 @@ There is no fallback: if the library is missing, every entry point raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_int32, c_size_t, c_uint32, c_void_p, POINTER
+from ctypes import c_int32, c_int64, c_size_t, c_uint32, c_void_p, POINTER
 from pathlib import Path
 
 import os
@@ -56,6 +56,37 @@ class GqaDesc(ctypes.Structure):
                 ("scale", ctypes.c_float), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
+GQA_BF16, GQA_FP16 = 0, 1
+GQA_STATUS_BAD_BOUNDS, GQA_STATUS_BAD_PAGE = 1, 2
+
+
+class GqaPackedDesc(ctypes.Structure):
+    _fields_ = [(n, c_int32) for n in ("N", "S", "Hq", "Hkv", "D", "dtype")] + \
+               [(n, c_void_p) for n in ("q", "k", "v", "out", "starts")] + \
+               [(n, c_int64) for n in ("q_stride", "k_stride", "v_stride")] + \
+               [("scale", ctypes.c_float), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class GqaPagedDesc(ctypes.Structure):
+    _fields_ = [(n, c_int32) for n in ("B", "Hq", "Hkv", "D", "P", "page", "M", "dtype")] + \
+               [(n, c_void_p) for n in ("q", "k", "v", "out", "tables", "lengths")] + \
+               [("q_stride", c_int64), ("table_stride", c_int64), ("k_strides", c_int64 * 3),
+                ("v_strides", c_int64 * 3), ("scale", ctypes.c_float), ("workspace", c_void_p),
+                ("workspace_bytes", c_size_t)]
+
+
+KV_STATUS_BAD_ROW, KV_STATUS_NOT_EMPTY, KV_STATUS_OUT_OF_PAGES = 1, 2, 4
+KV_STATUS_TOO_LONG, KV_STATUS_BAD_COUNT, KV_STATUS_BAD_STATE = 8, 16, 32
+KV_MAX_SEQUENCES, KV_MAX_PAGES, KV_MAX_TOKENS = 1024, 1 << 20, 1 << 20
+
+
+class KvCacheDesc(ctypes.Structure):
+    _fields_ = [(n, c_int32) for n in ("pages", "page_size", "kv_heads", "head_dim", "layers", "sequences",
+                                       "max_pages", "max_tokens")] + \
+               [(n, c_void_p) for n in ("k", "v", "tables", "lengths", "refs", "starts", "slots", "status",
+                                        "workspace")] + [("workspace_bytes", c_size_t)]
+
+
 # name -> (restype, argtypes); the complete exported ABI of include/*.h.
 SIGNATURES = {
     "moe_abi_version": (c_int32, []),
@@ -81,6 +112,25 @@ SIGNATURES = {
     "gqa_seg_plan_create": (c_int32, [POINTER(c_void_p), POINTER(GqaDesc)]),
     "gqa_seg_plan_run": (c_int32, [c_void_p, c_void_p]),
     "gqa_seg_plan_destroy": (None, [c_void_p]),
+    "gqa_packed_workspace_bytes": (c_int32, [POINTER(GqaPackedDesc), POINTER(c_size_t)]),
+    "gqa_packed_plan_create": (c_int32, [POINTER(c_void_p), POINTER(GqaPackedDesc)]),
+    "gqa_packed_plan_run": (c_int32, [c_void_p, c_void_p]),
+    "gqa_packed_plan_read_status": (c_int32, [c_void_p, c_void_p, POINTER(c_uint32)]),
+    "gqa_packed_plan_destroy": (None, [c_void_p]),
+    "gqa_paged_workspace_bytes": (c_int32, [POINTER(GqaPagedDesc), POINTER(c_size_t)]),
+    "gqa_paged_plan_create": (c_int32, [POINTER(c_void_p), POINTER(GqaPagedDesc)]),
+    "gqa_paged_plan_run": (c_int32, [c_void_p, c_void_p]),
+    "gqa_paged_plan_read_status": (c_int32, [c_void_p, c_void_p, POINTER(c_uint32)]),
+    "gqa_paged_plan_destroy": (None, [c_void_p]),
+    "kv_cache_workspace_bytes": (c_int32, [POINTER(KvCacheDesc), POINTER(c_size_t)]),
+    "kv_cache_create": (c_int32, [POINTER(c_void_p), POINTER(KvCacheDesc)]),
+    "kv_cache_reserve": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p]),
+    "kv_cache_append": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_void_p]),
+    "kv_cache_fork": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
+    "kv_cache_free": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p]),
+    "kv_cache_compact": (c_int32, [c_void_p, c_void_p]),
+    "kv_cache_read_status": (c_int32, [c_void_p, c_void_p, POINTER(c_uint32)]),
+    "kv_cache_destroy": (None, [c_void_p]),
 }
 
 _LIB = None

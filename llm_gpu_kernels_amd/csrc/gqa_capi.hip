@@ -17,6 +17,16 @@ namespace moe {
 int capi_fail(int code, const char *fmt, ...);  // moe_capi.hip (thread-local message)
 }
 
+struct gqa_packed_plan {
+  moe::GqaPackedArgs a;
+  int device;
+};
+
+struct gqa_paged_plan {
+  moe::GqaPagedArgs a;
+  int device;
+};
+
 struct gqa_seg_plan {
   moe::GqaArgs a;
   moe::GqaShape shape;
@@ -74,9 +84,185 @@ int device_cus(int *device, int *cus) {
   return MOE_OK;
 }
 
+constexpr int kMaxGroup = 64;
+
+int validate_heads(int Hq, int Hkv, int D, int dtype) {
+  using moe::capi_fail;
+  if (D != 64 && D != 128) return capi_fail(MOE_EINVAL, "head_dim must be 64 or 128 (got %d)", D);
+  if (Hkv < 1 || Hq < 1 || Hq % Hkv || Hq / Hkv > kMaxGroup || Hq > (1 << 16))
+    return capi_fail(MOE_EINVAL, "Hq must be a positive multiple of Hkv, at most %d times it (got %d, %d)", kMaxGroup, Hq,
+                     Hkv);
+  if (dtype != GQA_BF16 && dtype != GQA_FP16) return capi_fail(MOE_EINVAL, "unknown dtype %d", dtype);
+  return MOE_OK;
+}
+
+int check_stride(const char *what, int64_t stride, int64_t least) {
+  if (stride < least || stride > kMaxTokenStride || stride % 8)
+    return moe::capi_fail(MOE_EINVAL, "%s must be in [%lld, %lld] and a multiple of 8 (got %lld)", what, (long long)least,
+                          (long long)kMaxTokenStride, (long long)stride);
+  return MOE_OK;
+}
+
+float scale_or_default(float scale, int D) {
+  return scale > 0.f && scale < INFINITY ? scale : 1.0f / sqrtf((float)D);
+}
+
+int validate_packed_sizes(const gqa_packed_desc *d) {
+  using moe::capi_fail;
+  if (!d) return capi_fail(MOE_EINVAL, "null descriptor");
+  if (const int rc = validate_heads(d->Hq, d->Hkv, d->D, d->dtype)) return rc;
+  if (d->N < 0 || (int64_t)d->N * (d->Hq / d->Hkv) >= 1LL << 30)
+    return capi_fail(MOE_EINVAL, "N must be >= 0 and N * Hq / Hkv < 2^30 (got %d)", d->N);
+  if (d->S < 0 || d->S > (1 << 20)) return capi_fail(MOE_EINVAL, "S must be in [0, 2^20] (got %d)", d->S);
+  return MOE_OK;
+}
+
+int validate_packed(const gqa_packed_desc *d) {
+  using moe::capi_fail;
+  if (const int rc = validate_packed_sizes(d)) return rc;
+  if (d->N == 0 || d->S == 0) return MOE_OK;
+  if (!d->q || !d->k || !d->v || !d->out || !aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out))
+    return capi_fail(MOE_EINVAL, "q/k/v/out must be non-null and 16-byte aligned");
+  if (!d->starts || ((uintptr_t)d->starts & 3u)) return capi_fail(MOE_EINVAL, "starts must be given");
+  int rc = check_stride("q token stride", d->q_stride, (int64_t)d->Hq * d->D);
+  if (!rc) rc = check_stride("k token stride", d->k_stride, (int64_t)d->Hkv * d->D);
+  if (!rc) rc = check_stride("v token stride", d->v_stride, (int64_t)d->Hkv * d->D);
+  return rc;
+}
+
+size_t packed_workspace(const gqa_packed_desc *) { return 256; }
+
+int validate_paged_sizes(const gqa_paged_desc *d) {
+  using moe::capi_fail;
+  if (!d) return capi_fail(MOE_EINVAL, "null descriptor");
+  if (const int rc = validate_heads(d->Hq, d->Hkv, d->D, d->dtype)) return rc;
+  if (d->B < 0 || d->B > (1 << 16)) return capi_fail(MOE_EINVAL, "B must be in [0, 2^16] (got %d)", d->B);
+  if (d->page < 16 || d->page > 1024 || d->page % 16)
+    return capi_fail(MOE_EINVAL, "page must be a multiple of 16 up to 1024 (got %d)", d->page);
+  if (d->P < 1 || d->M < 1 || (int64_t)d->M * d->page >= 1LL << 31)
+    return capi_fail(MOE_EINVAL, "P and M must be positive and M * page < 2^31 (got %d, %d)", d->P, d->M);
+  return MOE_OK;
+}
+
+int validate_paged(const gqa_paged_desc *d) {
+  using moe::capi_fail;
+  if (const int rc = validate_paged_sizes(d)) return rc;
+  if (d->B == 0) return MOE_OK;
+  if (!d->q || !d->k || !d->v || !d->out || !aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out))
+    return capi_fail(MOE_EINVAL, "q/k/v/out must be non-null and 16-byte aligned");
+  if (!d->tables || !d->lengths || ((uintptr_t)d->tables & 3u) || ((uintptr_t)d->lengths & 3u))
+    return capi_fail(MOE_EINVAL, "tables and lengths must be given");
+  if (d->table_stride < d->M) return capi_fail(MOE_EINVAL, "table_stride must be at least M = %d", d->M);
+  int rc = check_stride("q row stride", d->q_stride, (int64_t)d->Hq * d->D);
+  for (int kv = 0; !rc && kv < 2; ++kv) {
+    const int64_t *st = kv ? d->v_strides : d->k_strides;
+    if (st[0] < 8 || st[0] % 8 || st[1] < 8 || st[1] % 8)
+      return capi_fail(MOE_EINVAL, "page and head strides must be positive multiples of 8");
+    rc = check_stride("page row stride", st[2], d->D);
+  }
+  return rc;
+}
+
+size_t paged_workspace(const gqa_paged_desc *) { return 256; }
+
+int need_workspace(const void *workspace, size_t have, size_t need) {
+  if (!workspace || !aligned16(workspace) || have < need)
+    return moe::capi_fail(MOE_ESPACE, "workspace has %zu bytes, needs %zu, 16-byte aligned", have, need);
+  return MOE_OK;
+}
+
+// Runs `launch` with a plan's device current.
+template <typename F>
+int on_device(int device, const char *what, F launch) {
+  int prev = -1;
+  hipError_t e = hipGetDevice(&prev);
+  if (e == hipSuccess && prev != device) e = hipSetDevice(device);
+  if (e == hipSuccess) e = launch();
+  if (prev >= 0 && prev != device) (void)hipSetDevice(prev);
+  if (e != hipSuccess) return moe::capi_fail(MOE_EDEVICE, "%s: %s", what, hipGetErrorString(e));
+  return MOE_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+int gqa_packed_workspace_bytes(const gqa_packed_desc *d, size_t *bytes) {
+  if (const int rc = validate_packed_sizes(d)) return rc;
+  if (!bytes) return moe::capi_fail(MOE_EINVAL, "null bytes");
+  *bytes = packed_workspace(d);
+  return MOE_OK;
+}
+
+int gqa_packed_plan_create(gqa_packed_plan **out, const gqa_packed_desc *d) {
+  if (!out) return moe::capi_fail(MOE_EINVAL, "null plan pointer");
+  *out = nullptr;
+  int rc = validate_packed(d), dev = 0, cus = 0;
+  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, packed_workspace(d));
+  if (!rc) rc = device_cus(&dev, &cus);
+  if (rc) return rc;
+  gqa_packed_plan *p = new (std::nothrow) gqa_packed_plan;
+  if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");
+  p->a = moe::GqaPackedArgs{(const uint16_t *)d->q, (const uint16_t *)d->k, (const uint16_t *)d->v, (uint16_t *)d->out,
+                            d->starts, d->q_stride, d->k_stride, d->v_stride, d->N, d->S, d->Hq, d->Hkv, d->D, d->dtype,
+                            scale_or_default(d->scale, d->D), (uint32_t *)d->workspace};
+  p->device = dev;
+  *out = p;
+  return MOE_OK;
+}
+
+int gqa_packed_plan_run(gqa_packed_plan *p, void *stream) {
+  if (!p) return moe::capi_fail(MOE_EINVAL, "null plan");
+  if (p->a.N == 0 || p->a.S == 0) return MOE_OK;
+  return on_device(p->device, "packed gqa launch", [&] { return moe::launch_gqa_packed(p->a, (hipStream_t)stream); });
+}
+
+int gqa_packed_plan_read_status(gqa_packed_plan *p, void *stream, uint32_t *flags) {
+  if (!p || !flags) return moe::capi_fail(MOE_EINVAL, "null plan or flags");
+  return on_device(p->device, "status",
+                   [&] { return moe::read_and_clear_status(p->a.status, flags, (hipStream_t)stream); });
+}
+
+void gqa_packed_plan_destroy(gqa_packed_plan *p) { delete p; }
+
+int gqa_paged_workspace_bytes(const gqa_paged_desc *d, size_t *bytes) {
+  if (const int rc = validate_paged_sizes(d)) return rc;
+  if (!bytes) return moe::capi_fail(MOE_EINVAL, "null bytes");
+  *bytes = paged_workspace(d);
+  return MOE_OK;
+}
+
+int gqa_paged_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d) {
+  if (!out) return moe::capi_fail(MOE_EINVAL, "null plan pointer");
+  *out = nullptr;
+  int rc = validate_paged(d), dev = 0, cus = 0;
+  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, paged_workspace(d));
+  if (!rc) rc = device_cus(&dev, &cus);
+  if (rc) return rc;
+  gqa_paged_plan *p = new (std::nothrow) gqa_paged_plan;
+  if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");
+  p->a = moe::GqaPagedArgs{(const uint16_t *)d->q, (const uint16_t *)d->k, (const uint16_t *)d->v, (uint16_t *)d->out,
+                           d->tables, d->lengths, d->q_stride, d->table_stride, d->k_strides[0], d->k_strides[1],
+                           d->k_strides[2], d->v_strides[0], d->v_strides[1], d->v_strides[2], d->B, d->Hq, d->Hkv, d->D,
+                           d->P, d->page, d->M, d->dtype, scale_or_default(d->scale, d->D), (uint32_t *)d->workspace};
+  p->device = dev;
+  *out = p;
+  return MOE_OK;
+}
+
+int gqa_paged_plan_run(gqa_paged_plan *p, void *stream) {
+  if (!p) return moe::capi_fail(MOE_EINVAL, "null plan");
+  if (p->a.B == 0) return MOE_OK;
+  return on_device(p->device, "paged gqa launch", [&] { return moe::launch_gqa_paged(p->a, (hipStream_t)stream); });
+}
+
+int gqa_paged_plan_read_status(gqa_paged_plan *p, void *stream, uint32_t *flags) {
+  if (!p || !flags) return moe::capi_fail(MOE_EINVAL, "null plan or flags");
+  return on_device(p->device, "status",
+                   [&] { return moe::read_and_clear_status(p->a.status, flags, (hipStream_t)stream); });
+}
+
+void gqa_paged_plan_destroy(gqa_paged_plan *p) { delete p; }
 
 int gqa_seg_workspace_bytes(const gqa_seg_desc *d, size_t *bytes) {
   int dev = 0, cus = 0;

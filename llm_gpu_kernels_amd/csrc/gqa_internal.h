@@ -41,4 +41,32 @@ hipError_t launch_gqa_prefill(const GqaArgs &a, int nsplit, hipStream_t s);
 size_t gqa_partial_bytes(int T, int Hq, int nsplit);
 hipError_t launch_gqa(const GqaArgs &a, GqaShape shape, hipStream_t s);
 
+// Packed prompts (gqa_packed.hip).  dtype: GQA_BF16 or GQA_FP16.
+struct GqaPackedArgs {
+  const uint16_t *q, *k, *v;             // [N, H, D], token strides in elements
+  uint16_t *out;                         // [N, Hq, D] contiguous
+  const int32_t *starts;                 // [S + 1]
+  int64_t q_stride, k_stride, v_stride;
+  int N, S, Hq, Hkv, D, dtype;
+  float scale;
+  uint32_t *status;
+};
+hipError_t launch_gqa_packed(const GqaPackedArgs &a, hipStream_t s);
+
+// One new token per sequence over a paged cache (gqa_paged.hip).
+struct GqaPagedArgs {
+  const uint16_t *q, *k, *v;             // q [B, Hq, D]; k, v: pages
+  uint16_t *out;                         // [B, Hq, D] contiguous
+  const int32_t *tables, *lengths;
+  int64_t q_stride, table_stride;
+  int64_t k_page, k_head, k_row, v_page, v_head, v_row;  // strides in elements
+  int B, Hq, Hkv, D, P, page, M, dtype;
+  float scale;
+  uint32_t *status;
+};
+hipError_t launch_gqa_paged(const GqaPagedArgs &a, hipStream_t s);
+
+// Synchronises `s`, reads a status word and enqueues its clearing.
+hipError_t read_and_clear_status(uint32_t *status, uint32_t *flags, hipStream_t s);
+
 }  // namespace moe

@@ -1,0 +1,444 @@
+// Paged key-value cache on gfx950: pages handed out, shared, given back and
+// moved, and the keys and values of new tokens written to their slots.
+//
+// All decisions are integer work over a few thousand words and are taken by one
+// workgroup (no grid-wide synchronisation, and the pages come out in the same
+// order every time); what moves bytes (copies of pages, slots, table rows) is a
+// second launch over the whole chip that reads the decisions.
+#include "common.h"
+#include "../../include/kv_mi355x.h"
+#include "kv_internal.h"
+
+namespace moe {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;  // one row of the cache each
+constexpr int kWaves = kPlanThreads / kWave;
+constexpr int kScanPages = 8;       // pages of a thread per scanned chunk
+static_assert(KV_MAX_SEQUENCES <= kPlanThreads, "a thread per row");
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Exclusive sum over the workgroup's threads and the total.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *lds, uint64_t *total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t x = v;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const uint64_t y = __shfl_up(x, o, kWave);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // the last scan's sums have been read
+  if (lane == kWave - 1) lds[wave] = x;
+  __syncthreads();
+  uint64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const uint64_t s = lds[w];
+    if (w < wave) before += s;
+    all += s;
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// One bit per page of a thread's eight: in use.
+__device__ __forceinline__ uint32_t used_bits(const KvState &s, int first) {
+  uint32_t bits = 0;
+  if (first + kScanPages <= s.pages) {
+    const int4 a = *(const int4 *)(s.refs + first), b = *(const int4 *)(s.refs + first + 4);
+    bits = (a.x > 0) | (a.y > 0) << 1 | (a.z > 0) << 2 | (a.w > 0) << 3 | (b.x > 0) << 4 | (b.y > 0) << 5 |
+           (b.z > 0) << 6 | (b.w > 0) << 7;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kScanPages; ++i)
+      if (first + i < s.pages && s.refs[first + i] > 0) bits |= 1u << i;
+  }
+  return bits;
+}
+__device__ __forceinline__ uint32_t valid_bits(const KvState &s, int first) {
+  const int n = s.pages - first;
+  return n >= kScanPages ? 0xffu : n > 0 ? (1u << n) - 1u : 0u;
+}
+
+// Pages, lengths and slots of a reserve.  Thread s is row s.
+__global__ __launch_bounds__(kPlanThreads) void kv_reserve_plan(KvState s, const int32_t *counts, int stride) {
+  __shared__ uint64_t sums[kWaves];
+  __shared__ int last_page[kPlanThreads], need_at[kPlanThreads + 1], row_len[kPlanThreads];
+  __shared__ int copy_at[kPlanThreads];  // the row's copy's number, -1: none
+  const int row = threadIdx.x;
+  const bool live = row < s.sequences;
+  const int cap = s.max_pages * s.page_size;  // < 2^31
+  int len = live ? s.lengths[row] : 0, count = live ? counts[row] : 0;
+  uint32_t bad = 0;
+  if (len < 0 || len > cap) {
+    bad |= KV_STATUS_BAD_STATE;
+    len = 0;
+  }
+  if (count < 0 || count > s.max_tokens || (stride > 0 && count > stride)) {
+    bad |= KV_STATUS_BAD_COUNT;
+    count = 0;
+  }
+  if (count > cap - len) {
+    bad |= KV_STATUS_TOO_LONG;
+    count = 0;
+  }
+  // A shared, partly filled last page.
+  int last = -1, holders = 0;
+  if (count > 0 && len % s.page_size) {
+    const int p = s.tables[(int64_t)row * s.max_pages + len / s.page_size];
+    if (p < 0 || p >= s.pages) {
+      bad |= KV_STATUS_BAD_STATE;
+    } else if ((holders = s.refs[p]) > 1) {
+      last = p;
+    }
+  }
+  last_page[row] = last;
+  row_len[row] = len;
+  __syncthreads();
+  bool copy = last >= 0;
+  if (copy) {
+    int growing = 0;
+    bool later = false;
+    for (int j = 0; j < s.sequences; ++j) {
+      const bool same = last_page[j] == last;
+      growing += same;
+      later |= same && j > row;
+    }
+    copy = growing < holders || later;
+  }
+  const int used = ceil_div(len, s.page_size);
+  const int need = ceil_div(len + count, s.page_size) - used + copy;
+  uint64_t all, copies;
+  const uint64_t mine = block_scan((uint64_t)need << 32 | (uint32_t)count, sums, &all);
+  const int my_copy = (int)block_scan(copy, sums, &copies);
+  const int total = (int)(all >> 32), tokens = (int)(all & 0xffffffffu);
+  if (tokens > s.max_tokens) bad |= KV_STATUS_BAD_COUNT;
+  need_at[row] = (int)(mine >> 32);
+  if (row == 0) need_at[kPlanThreads] = total;
+  copy_at[row] = copy ? my_copy : -1;
+
+  bool refuse = __syncthreads_or(bad != 0);
+  if (!refuse && total > 0) {
+    int found = 0;
+    for (int base = 0; base < s.pages && found < total; base += kPlanThreads * kScanPages) {
+      const int first = base + row * kScanPages;
+      uint32_t free_bits = first < s.pages ? ~used_bits(s, first) & valid_bits(s, first) : 0u;
+      uint64_t n;
+      int at = found + (int)block_scan(__popc(free_bits), sums, &n);
+      for (; free_bits && at < total; free_bits &= free_bits - 1, ++at) s.list[at] = first + __ffs(free_bits) - 1;
+      found += (int)n;
+    }
+    if (found < total) {
+      bad |= KV_STATUS_OUT_OF_PAGES;
+      refuse = true;
+    }
+  }
+  if (bad) atomicOr(s.status, bad);
+  if (refuse) {
+    for (int i = row; i <= s.sequences; i += kPlanThreads) s.starts[i] = 0;
+    if (row == 0) *s.num_moves = 0;
+    return;
+  }
+  __syncthreads();  // list is complete
+  for (int i = row; i < total; i += kPlanThreads) {
+    // The row whose pages i lies among: the last one that starts at or before i.
+    int lo = 0, hi = s.sequences - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (need_at[mid] <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    const int page = s.list[i], nth = i - need_at[lo], c = copy_at[lo], l = row_len[lo];
+    int column = ceil_div(l, s.page_size) + nth;
+    if (c >= 0) {
+      --column;  // the copy takes the last page's place
+      if (nth == 0) {
+        s.move_src[c] = last_page[lo];
+        s.move_dst[c] = page;
+        atomicSub(s.refs + last_page[lo], 1);
+      }
+    }
+    s.tables[(int64_t)lo * s.max_pages + column] = page;
+    s.refs[page] = 1;
+  }
+  if (live) {
+    s.lengths[row] = len + count;
+    s.starts[row] = (int)(mine & 0xffffffffu);
+  }
+  if (row == 0) {
+    s.starts[s.sequences] = tokens;
+    *s.num_moves = (int)copies;
+  }
+}
+
+// Copies the moves' pages in every layer, keys and values, in pieces of kPiece
+// bytes that the workgroups take in turn.
+constexpr int kPiece = 16384;
+__device__ __forceinline__ void copy_moves(const KvState &s, int block, int blocks) {
+  const int n = *s.num_moves;
+  if (n == 0) return;
+  const int64_t page_bytes = (int64_t)s.kv_heads * s.page_size * s.head_dim * 2;
+  const int pieces = (int)((page_bytes + kPiece - 1) / kPiece);
+  const int64_t total = (int64_t)n * 2 * s.layers * pieces;
+  for (int64_t u = block; u < total; u += blocks) {
+    const int piece = (int)(u % pieces);
+    const int64_t rest = u / pieces;
+    const int plane = (int)(rest % (2 * s.layers)), m = (int)(rest / (2 * s.layers));
+    uint8_t *const base = (uint8_t *)(plane < s.layers ? s.k : s.v) +
+                          (int64_t)(plane < s.layers ? plane : plane - s.layers) * s.pages * page_bytes +
+                          (int64_t)piece * kPiece;
+    const uint8_t *const from = base + s.move_src[m] * page_bytes;
+    uint8_t *const to = base + s.move_dst[m] * page_bytes;
+    const int bytes = (int)min((int64_t)kPiece, page_bytes - (int64_t)piece * kPiece);
+    for (int o = threadIdx.x * 16; o < bytes; o += blockDim.x * 16) *(u32x4 *)(to + o) = *(const u32x4 *)(from + o);
+  }
+}
+
+constexpr int kWideThreads = 256;
+constexpr int kCopyBlocks = 1024;
+
+// Slots of the reserved tokens and the copies of shared pages.
+__global__ __launch_bounds__(kWideThreads) void kv_reserve_finish(KvState s, int stride, int slot_blocks) {
+  if ((int)blockIdx.x >= slot_blocks) {
+    copy_moves(s, blockIdx.x - slot_blocks, gridDim.x - slot_blocks);
+    return;
+  }
+  for (int i = blockIdx.x * kWideThreads + threadIdx.x; i < s.max_tokens; i += slot_blocks * kWideThreads) {
+    int row = s.sequences, nth = 0;
+    if (stride > 0) {
+      row = i / stride;
+      nth = i % stride;
+    } else if (i < s.starts[s.sequences]) {
+      int lo = 0, hi = s.sequences - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s.starts[mid] <= i) lo = mid;
+        else hi = mid - 1;
+      }
+      row = lo;
+      nth = i - s.starts[lo];
+    }
+    int64_t slot = -1;
+    if (row < s.sequences) {
+      const int count = s.starts[row + 1] - s.starts[row];
+      if (nth < count) {
+        const int at = s.lengths[row] - count + nth;
+        slot = (int64_t)s.tables[(int64_t)row * s.max_pages + at / s.page_size] * s.page_size + at % s.page_size;
+      }
+    }
+    s.slots[i] = slot;
+  }
+}
+
+// 16 bytes of a token's keys and of its values per thread.
+__global__ __launch_bounds__(kWideThreads) void kv_append(KvState s, int layer, const uint16_t *k, const uint16_t *v,
+                                                         int64_t k_stride, int64_t v_stride, int n) {
+  const int chunks = s.kv_heads * s.head_dim / 8;  // of a token
+  const int64_t total = (int64_t)n * chunks;
+  const int64_t cells = (int64_t)s.pages * s.page_size, plane = (int64_t)layer * cells * s.kv_heads * s.head_dim;
+  for (int64_t u = (int64_t)blockIdx.x * kWideThreads + threadIdx.x; u < total; u += (int64_t)gridDim.x * kWideThreads) {
+    const int token = (int)(u / chunks), c = (int)(u % chunks) * 8;
+    const int64_t slot = s.slots[token];
+    if (slot < 0 || slot >= cells) continue;
+    const int head = c / s.head_dim, d = c % s.head_dim;
+    const int64_t page = slot / s.page_size;
+    const int row = (int)(slot % s.page_size);
+    const int64_t to = plane + ((page * s.kv_heads + head) * s.page_size + row) * s.head_dim + d;
+    *(u32x4 *)(s.k + to) = *(const u32x4 *)(k + token * k_stride + c);
+    *(u32x4 *)(s.v + to) = *(const u32x4 *)(v + token * v_stride + c);
+  }
+}
+
+// Pages of a row that hold tokens; -1 (and a status) for a length out of range.
+__device__ __forceinline__ int row_pages(const KvState &s, int row) {
+  const int len = s.lengths[row];
+  if (len < 0 || len > s.max_pages * s.page_size) {
+    if (threadIdx.x == 0) atomicOr(s.status, KV_STATUS_BAD_STATE);
+    return -1;
+  }
+  return ceil_div(len, s.page_size);
+}
+
+// Fork: pair i may go ahead.  Rows are as before the call, since lengths are
+// written by a later launch.
+__device__ __forceinline__ bool fork_ok(const KvState &s, const int32_t *src, const int32_t *dst, int i, bool report) {
+  const int a = src[i], b = dst[i];
+  if (a < 0 || b < 0) return false;
+  uint32_t bad = 0;
+  if (a >= s.sequences || b >= s.sequences) {
+    bad = KV_STATUS_BAD_ROW;
+  } else {
+    bool taken = s.lengths[b] != 0;
+    for (int j = 0; j < i && !taken; ++j) taken = dst[j] == b && src[j] >= 0 && src[j] < s.sequences;
+    if (taken) bad = KV_STATUS_NOT_EMPTY;
+  }
+  if (bad && report) atomicOr(s.status, bad);
+  return bad == 0;
+}
+
+// One workgroup per pair: the table row, and one more holder of its pages.
+__global__ __launch_bounds__(kWideThreads) void kv_fork_rows(KvState s, const int32_t *src, const int32_t *dst) {
+  const int i = blockIdx.x;
+  if (!fork_ok(s, src, dst, i, threadIdx.x == 0)) return;
+  const int n = row_pages(s, src[i]);
+  const int32_t *const from = s.tables + (int64_t)src[i] * s.max_pages;
+  int32_t *const to = s.tables + (int64_t)dst[i] * s.max_pages;
+  for (int c = threadIdx.x; c < n; c += kWideThreads) {
+    const int p = from[c];
+    to[c] = p;
+    if (p >= 0 && p < s.pages) atomicAdd(s.refs + p, 1);
+    else atomicOr(s.status, KV_STATUS_BAD_STATE);
+  }
+}
+__global__ __launch_bounds__(kPlanThreads) void kv_fork_lengths(KvState s, const int32_t *src, const int32_t *dst, int n) {
+  const int i = threadIdx.x;
+  int len = -1;
+  if (i < n && fork_ok(s, src, dst, i, false)) {
+    len = s.lengths[src[i]];
+    if (len > s.max_pages * s.page_size) len = -1;
+  }
+  __syncthreads();  // every length has been read
+  if (len >= 0) s.lengths[dst[i]] = len;
+}
+
+__global__ __launch_bounds__(kWideThreads) void kv_free(KvState s, const int32_t *rows) {
+  const int row = rows[blockIdx.x];
+  if (row < 0) return;
+  if (row >= s.sequences) {
+    if (threadIdx.x == 0) atomicOr(s.status, KV_STATUS_BAD_ROW);
+    return;
+  }
+  for (int j = 0; j < (int)blockIdx.x; ++j)
+    if (rows[j] == row) return;  // named before
+  const int n = row_pages(s, row);
+  int32_t *const table = s.tables + (int64_t)row * s.max_pages;
+  for (int c = threadIdx.x; c < n; c += kWideThreads) {
+    const int p = table[c];
+    table[c] = -1;
+    if (p >= 0 && p < s.pages) atomicSub(s.refs + p, 1);
+    else atomicOr(s.status, KV_STATUS_BAD_STATE);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) s.lengths[row] = 0;
+}
+
+// Moves of a compaction: with U pages in use, the free pages below U in order
+// take the used pages from U on in order.
+__global__ __launch_bounds__(kPlanThreads) void kv_compact_plan(KvState s) {
+  __shared__ uint64_t sums[kWaves];
+  uint64_t n = 0;
+  int used = 0;
+  for (int base = 0; base < s.pages; base += kPlanThreads * kScanPages) {
+    const int first = base + threadIdx.x * kScanPages;
+    if (first < s.pages) used += __popc(used_bits(s, first));
+  }
+  (void)block_scan(used, sums, &n);
+  const int U = (int)n;
+  // Free pages below U and used ones from U on, numbered.
+  int holes = 0, movers = 0;
+  for (int base = 0; base < s.pages; base += kPlanThreads * kScanPages) {
+    const int first = base + threadIdx.x * kScanPages;
+    uint32_t hole = 0, mover = 0;
+    if (first < s.pages) {
+      const uint32_t u = used_bits(s, first);
+      const int k = U - first;
+      const uint32_t below = k >= kScanPages ? 0xffu : k > 0 ? (1u << k) - 1u : 0u;
+      hole = ~u & below & valid_bits(s, first);
+      mover = u & ~below;
+    }
+    const uint64_t at = block_scan((uint64_t)__popc(hole) << 32 | __popc(mover), sums, &n);
+    int h = holes + (int)(at >> 32), m = movers + (int)(at & 0xffffffffu);
+    for (; hole; hole &= hole - 1) s.move_dst[h++] = first + __ffs(hole) - 1;
+    for (; mover; mover &= mover - 1) s.move_src[m++] = first + __ffs(mover) - 1;
+    holes += (int)(n >> 32);
+    movers += (int)(n & 0xffffffffu);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < movers; i += kPlanThreads) {
+    const int a = s.move_src[i], b = s.move_dst[i];
+    s.moved_to[a] = b;
+    s.refs[b] = s.refs[a];
+    s.refs[a] = 0;
+  }
+  if (threadIdx.x == 0) {
+    *s.num_moves = movers;
+    s.status[1] = (uint32_t)U;
+  }
+}
+
+// Tables of the rows (a workgroup each in turn) and the pages' bytes.
+__global__ __launch_bounds__(kWideThreads) void kv_compact_finish(KvState s, int row_blocks) {
+  if ((int)blockIdx.x >= row_blocks) {
+    copy_moves(s, blockIdx.x - row_blocks, gridDim.x - row_blocks);
+    return;
+  }
+  const int U = (int)s.status[1];
+  for (int row = blockIdx.x; row < s.sequences; row += row_blocks) {
+    const int n = row_pages(s, row);
+    int32_t *const table = s.tables + (int64_t)row * s.max_pages;
+    for (int c = threadIdx.x; c < n; c += kWideThreads) {
+      const int p = table[c];
+      if (p >= 0 && p < U) continue;
+      const int to = p >= U && p < s.pages ? s.moved_to[p] : -1;
+      if (to >= 0 && to < U) table[c] = to;
+      else atomicOr(s.status, KV_STATUS_BAD_STATE);
+    }
+  }
+}
+
+}  // namespace
+
+namespace {
+size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+}  // namespace
+
+size_t kv_workspace_bytes(int pages) { return 256 + 4 * align256((size_t)pages * 4); }
+
+void kv_bind_workspace(KvState *s, void *workspace) {
+  uint8_t *const w = (uint8_t *)workspace;
+  const size_t each = align256((size_t)s->pages * 4);
+  s->num_moves = (int32_t *)w;
+  s->move_src = (int32_t *)(w + 256);
+  s->move_dst = (int32_t *)(w + 256 + each);
+  s->list = (int32_t *)(w + 256 + 2 * each);
+  s->moved_to = (int32_t *)(w + 256 + 3 * each);
+}
+
+hipError_t launch_kv_reserve(const KvState &s, const int32_t *counts, int stride, hipStream_t st) {
+  hipLaunchKernelGGL(kv_reserve_plan, dim3(1), dim3(kPlanThreads), 0, st, s, counts, stride);
+  const int slot_blocks = min((s.max_tokens + kWideThreads - 1) / kWideThreads, 256);
+  hipLaunchKernelGGL(kv_reserve_finish, dim3(slot_blocks + kCopyBlocks), dim3(kWideThreads), 0, st, s, stride,
+                     slot_blocks);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_append(const KvState &s, int layer, const uint16_t *k, const uint16_t *v, int64_t k_stride,
+                            int64_t v_stride, int n, hipStream_t st) {
+  const int64_t total = (int64_t)n * (s.kv_heads * s.head_dim / 8);
+  const int64_t want = (total + kWideThreads - 1) / kWideThreads;
+  hipLaunchKernelGGL(kv_append, dim3((uint32_t)(want < 65536 ? want : 65536)), dim3(kWideThreads), 0, st, s, layer, k, v,
+                     k_stride, v_stride, n);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_fork(const KvState &s, const int32_t *src, const int32_t *dst, int n, hipStream_t st) {
+  hipLaunchKernelGGL(kv_fork_rows, dim3(n), dim3(kWideThreads), 0, st, s, src, dst);
+  hipLaunchKernelGGL(kv_fork_lengths, dim3(1), dim3(kPlanThreads), 0, st, s, src, dst, n);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_free(const KvState &s, const int32_t *rows, int n, hipStream_t st) {
+  hipLaunchKernelGGL(kv_free, dim3(n), dim3(kWideThreads), 0, st, s, rows);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_compact(const KvState &s, hipStream_t st) {
+  hipLaunchKernelGGL(kv_compact_plan, dim3(1), dim3(kPlanThreads), 0, st, s);
+  const int row_blocks = min(s.sequences, 256);
+  hipLaunchKernelGGL(kv_compact_finish, dim3(row_blocks + kCopyBlocks), dim3(kWideThreads), 0, st, s, row_blocks);
+  return hipGetLastError();
+}
+
+}  // namespace moe
