@@ -24,7 +24,7 @@ struct gqa_packed_plan {
 
 struct gqa_paged_plan {
   moe::GqaPagedArgs a;
-  int device;
+  int device, cus;
 };
 
 struct gqa_seg_plan {
@@ -141,6 +141,11 @@ int validate_paged_sizes(const gqa_paged_desc *d) {
     return capi_fail(MOE_EINVAL, "page must be a multiple of 16 up to 1024 (got %d)", d->page);
   if (d->P < 1 || d->M < 1 || (int64_t)d->M * d->page >= 1LL << 31)
     return capi_fail(MOE_EINVAL, "P and M must be positive and M * page < 2^31 (got %d, %d)", d->P, d->M);
+  // 32-key steps over all sequences and blocks of 16 query heads are counted in 32 bits.
+  const int64_t steps = (int64_t)d->B * d->Hkv * ((d->Hq / d->Hkv + 15) / 16);
+  if (steps > (1LL << 30) / (((int64_t)d->M * d->page + 31) / 32))
+    return capi_fail(MOE_EINVAL, "B * Hkv * M * page / 32 must be at most 2^30 (B %d, Hkv %d, M %d, page %d)", d->B,
+                     d->Hkv, d->M, d->page);
   return MOE_OK;
 }
 
@@ -163,7 +168,7 @@ int validate_paged(const gqa_paged_desc *d) {
   return rc;
 }
 
-size_t paged_workspace(const gqa_paged_desc *) { return 256; }
+size_t paged_workspace(const gqa_paged_desc *d, int cus) { return moe::gqa_paged_workspace(d->B, d->Hq, d->Hkv, d->D, cus); }
 
 int need_workspace(const void *workspace, size_t have, size_t need) {
   if (!workspace || !aligned16(workspace) || have < need)
@@ -226,26 +231,30 @@ int gqa_packed_plan_read_status(gqa_packed_plan *p, void *stream, uint32_t *flag
 void gqa_packed_plan_destroy(gqa_packed_plan *p) { delete p; }
 
 int gqa_paged_workspace_bytes(const gqa_paged_desc *d, size_t *bytes) {
-  if (const int rc = validate_paged_sizes(d)) return rc;
-  if (!bytes) return moe::capi_fail(MOE_EINVAL, "null bytes");
-  *bytes = paged_workspace(d);
-  return MOE_OK;
+  int rc = validate_paged_sizes(d), dev = 0, cus = 0;
+  if (!rc && !bytes) rc = moe::capi_fail(MOE_EINVAL, "null bytes");
+  if (!rc) rc = device_cus(&dev, &cus);
+  if (!rc) *bytes = paged_workspace(d, cus);
+  return rc;
 }
 
 int gqa_paged_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d) {
   if (!out) return moe::capi_fail(MOE_EINVAL, "null plan pointer");
   *out = nullptr;
   int rc = validate_paged(d), dev = 0, cus = 0;
-  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, paged_workspace(d));
+  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, 256);
   if (!rc) rc = device_cus(&dev, &cus);
+  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, paged_workspace(d, cus));
   if (rc) return rc;
   gqa_paged_plan *p = new (std::nothrow) gqa_paged_plan;
   if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");
   p->a = moe::GqaPagedArgs{(const uint16_t *)d->q, (const uint16_t *)d->k, (const uint16_t *)d->v, (uint16_t *)d->out,
                            d->tables, d->lengths, d->q_stride, d->table_stride, d->k_strides[0], d->k_strides[1],
                            d->k_strides[2], d->v_strides[0], d->v_strides[1], d->v_strides[2], d->B, d->Hq, d->Hkv, d->D,
-                           d->P, d->page, d->M, d->dtype, scale_or_default(d->scale, d->D), (uint32_t *)d->workspace};
+                           d->P, d->page, d->M, d->dtype, scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr};
+  moe::gqa_paged_bind(&p->a, d->workspace);
   p->device = dev;
+  p->cus = cus;
   *out = p;
   return MOE_OK;
 }
@@ -253,7 +262,7 @@ int gqa_paged_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d) {
 int gqa_paged_plan_run(gqa_paged_plan *p, void *stream) {
   if (!p) return moe::capi_fail(MOE_EINVAL, "null plan");
   if (p->a.B == 0) return MOE_OK;
-  return on_device(p->device, "paged gqa launch", [&] { return moe::launch_gqa_paged(p->a, (hipStream_t)stream); });
+  return on_device(p->device, "paged gqa launch", [&] { return moe::launch_gqa_paged(p->a, p->cus, (hipStream_t)stream); });
 }
 
 int gqa_paged_plan_read_status(gqa_paged_plan *p, void *stream, uint32_t *flags) {

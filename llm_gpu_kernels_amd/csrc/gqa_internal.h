@@ -63,8 +63,13 @@ struct GqaPagedArgs {
   int B, Hq, Hkv, D, P, page, M, dtype;
   float scale;
   uint32_t *status;
+  int32_t *pieces;                       // {first slot, pieces (0: none, written at once)} per
+                                         // (sequence, block of query heads)
+  float *partial;                        // [2 per wave][rows]{m, l, O[D]}
 };
-hipError_t launch_gqa_paged(const GqaPagedArgs &a, hipStream_t s);
+size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int cus);
+void gqa_paged_bind(GqaPagedArgs *a, void *workspace);
+hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s);
 
 // Synchronises `s`, reads a status word and enqueues its clearing.
 hipError_t read_and_clear_status(uint32_t *status, uint32_t *flags, hipStream_t s);

@@ -1,82 +1,532 @@
 // Attention of one new token per sequence over a paged cache on gfx950.
+//
+//   out[b][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[b][h] . k_j - max),
+//   over the lengths[b] keys of row b; head h reads KV head h / (Hq / Hkv).
+//
+// Every K and V byte is used by one KV head's queries only (at most 16 rows of
+// an MFMA), so the cache's bytes bound it, and what counts is that every wave
+// has loads in flight all the time and that all of them end together:
+//   * the work is one flat list of 32-key steps, (sequence, KV head, step), cut
+//     into equal ranges, one per wave of a grid that fills the chip once.  Waves
+//     work for themselves (no barrier): a wave's next step is loaded while the
+//     present one computes, across the ends of sequences too;
+//   * a wave's range may end inside a (sequence, head).  Such pieces leave their
+//     (max, sum, O) in the workspace and a second launch joins them in the order
+//     of the keys; whole ones are written at once;
+//   * K and V rows go from HBM to LDS in whole rows (buffer loads with an LDS
+//     destination, a descriptor per 16-key block: a block lies in one page),
+//     permuted within a row so that the operand reads have no bank conflicts.
+// Scores are computed transposed, S^T = K Q^T, so they land in the A layout of
+// the P.V product; V comes back transposed with ds_read_b64_tr_b16.
 #include "common.h"
 #include "../../include/gqa_mi355x.h"
+#include "gqa_dev.h"
 #include "gqa_internal.h"
 
 namespace moe {
 
+using namespace gqa;
+
 namespace {
 
-__device__ __forceinline__ float to_f32(uint16_t x, int dtype) {
-  return dtype == GQA_FP16 ? (float)__builtin_bit_cast(_Float16, x) : bf16_bits_to_f32(x);
+constexpr int kStep = 32;       // keys of a step
+constexpr int kBlock = 16;      // keys that lie in one page
+constexpr int kRows = 16;       // query rows of an MFMA
+constexpr int kWaves = 4;       // per workgroup; only the LDS is shared out by it
+
+// LDS of a wave: 32 rows of K, 32 of V, 16 of Q.  Row i's 16-byte chunk c lies
+// at place c ^ swizzle(i) of its row: the sixteen lanes that read one chunk of
+// sixteen K rows, and the sixteen that read two chunks of four V rows, meet
+// sixteen (eight) different bank groups.
+template <int D> constexpr int kStage = kStep * D * 2;
+template <int D> constexpr int kWaveLds = 5 * kStage<D> / 2;
+template <int D> constexpr int kWorkgroups = 160 * 1024 / (kWaves * kWaveLds<D>);  // per CU
+template <int D>
+__device__ __forceinline__ int swizzle_k(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+template <int D>
+__device__ __forceinline__ int swizzle_v(int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
+
+// K fragments (key block kt, 32-dim slice ks) -> k[2 ks + kt], and Q's.
+template <int D>
+__device__ __forceinline__ void read_kq(uint32_t base, const uint32_t (&at)[D / 32], u32x4 (&k)[D / 16], u32x4 (&q)[D / 32]) {
+  if constexpr (D == 128) {
+    asm volatile(
+        "ds_read_b128 %0, %12\n\t"
+        "ds_read_b128 %8, %12 offset:16384\n\t"
+        "ds_read_b128 %1, %12 offset:4096\n\t"
+        "ds_read_b128 %2, %13\n\t"
+        "ds_read_b128 %9, %13 offset:16384\n\t"
+        "ds_read_b128 %3, %13 offset:4096\n\t"
+        "ds_read_b128 %4, %14\n\t"
+        "ds_read_b128 %10, %14 offset:16384\n\t"
+        "ds_read_b128 %5, %14 offset:4096\n\t"
+        "ds_read_b128 %6, %15\n\t"
+        "ds_read_b128 %11, %15 offset:16384\n\t"
+        "ds_read_b128 %7, %15 offset:4096\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3]), "=&v"(k[4]), "=&v"(k[5]), "=&v"(k[6]), "=&v"(k[7]),
+          "=&v"(q[0]), "=&v"(q[1]), "=&v"(q[2]), "=&v"(q[3])
+        : "v"(base + at[0]), "v"(base + at[1]), "v"(base + at[2]), "v"(base + at[3])
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b128 %0, %6\n\t"
+        "ds_read_b128 %4, %6 offset:8192\n\t"
+        "ds_read_b128 %1, %6 offset:2048\n\t"
+        "ds_read_b128 %2, %7\n\t"
+        "ds_read_b128 %5, %7 offset:8192\n\t"
+        "ds_read_b128 %3, %7 offset:2048\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3]), "=&v"(q[0]), "=&v"(q[1])
+        : "v"(base + at[0]), "v"(base + at[1])
+        : "memory");
+  }
 }
-__device__ __forceinline__ uint16_t from_f32(float x, int dtype) {
-  return dtype == GQA_FP16 ? __builtin_bit_cast(uint16_t, (_Float16)x) : (uint16_t)f32_to_bf16_bits(x);
+// V of 16 dims dt and the lane group's keys 4 g + 0..3 -> v[2 dt], keys 16
+// further -> v[2 dt + 1].  ds_read_b64_tr_b16: within 16 lanes, lane 4 a + b
+// receives element b of the 8-byte rows addressed by lanes a, a + 4, a + 8, a + 12.
+template <int D>
+__device__ __forceinline__ void read_v(uint32_t base, u32x2 (&v)[D / 8]) {
+  const uint32_t a0 = base, a1 = base ^ 32, a2 = base ^ 64, a3 = base ^ 96;
+  if constexpr (D == 128) {
+    const uint32_t a4 = base ^ 128, a5 = base ^ 160, a6 = base ^ 192, a7 = base ^ 224;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %16\n\t"
+        "ds_read_b64_tr_b16 %1, %16 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %2, %17\n\t"
+        "ds_read_b64_tr_b16 %3, %17 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %4, %18\n\t"
+        "ds_read_b64_tr_b16 %5, %18 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %6, %19\n\t"
+        "ds_read_b64_tr_b16 %7, %19 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %8, %20\n\t"
+        "ds_read_b64_tr_b16 %9, %20 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %10, %21\n\t"
+        "ds_read_b64_tr_b16 %11, %21 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %12, %22\n\t"
+        "ds_read_b64_tr_b16 %13, %22 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %14, %23\n\t"
+        "ds_read_b64_tr_b16 %15, %23 offset:4096\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]),
+          "=&v"(v[8]), "=&v"(v[9]), "=&v"(v[10]), "=&v"(v[11]), "=&v"(v[12]), "=&v"(v[13]), "=&v"(v[14]), "=&v"(v[15])
+        : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "v"(a4), "v"(a5), "v"(a6), "v"(a7)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %2, %9\n\t"
+        "ds_read_b64_tr_b16 %3, %9 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %4, %10\n\t"
+        "ds_read_b64_tr_b16 %5, %10 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %6, %11\n\t"
+        "ds_read_b64_tr_b16 %7, %11 offset:2048\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+        : "v"(a0), "v"(a1), "v"(a2), "v"(a3)
+        : "memory");
+  }
 }
 
-// One wave per sequence and query head, a key per lane and step.
-__global__ __launch_bounds__(64) void gqa_paged_simple(GqaPagedArgs a) {
-  __shared__ float qs[128], ps[64];
-  __shared__ int64_t rows[64];
-  const int b = blockIdx.x, head = blockIdx.y, kvh = head / (a.Hq / a.Hkv), lane = threadIdx.x;
-  int len = a.lengths[b];
-  if (len < 0 || len > a.M * a.page) {
-    if (lane == 0) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
-    len = max(0, min(len, a.M * a.page));
+// Read by scalar loads: the tables do not change while the kernel runs.
+__device__ __forceinline__ int uniform_load(const int32_t *p) {
+  return *(const __attribute__((address_space(4))) int32_t *)(const __attribute__((address_space(4))) void *)p;
+}
+
+// A step: up to 32 keys of one (sequence, head block).  All fields are the same
+// in every lane.
+struct Step {
+  int b, head;       // sequence, block of up to 16 query heads
+  int s, steps;      // number among the steps of its (sequence, head block)
+  int page[2], row[2], n[2];  // its 16-key blocks: page, first row, keys (0: none)
+};
+
+template <int D, bool F16>
+__global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(GqaPagedArgs a) {
+  constexpr int kSlices = D / 32;               // 32-dim slices of a row
+  constexpr int kTiles = D / 16;                // 16-dim tiles of O
+  constexpr int kLoads = kBlock * D * 2 / 1024; // loads of a block
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = sgpr(threadIdx.x >> 6);
+  const int worker = sgpr(blockIdx.x * kWaves + wave), workers = gridDim.x * kWaves;
+  const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows, heads = a.Hkv * blocks;
+  const int cap = a.M * a.page;
+  uint8_t *const kst = smem + wave * kWaveLds<D>, *const vst = kst + kStage<D>, *const qst = vst + kStage<D>;
+
+  // ---- the wave's range of the flat list ----
+  // Lengths of 64 sequences from `base` on, one per lane.
+  auto lengths_at = [&](int base) __attribute__((always_inline)) {
+    const int i = base + lane, raw = i < a.B ? a.lengths[i] : 0, len = max(0, min(raw, cap));
+    if (raw != len) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
+    return len;
+  };
+  auto steps_of = [](int len) __attribute__((always_inline)) { return (len + kStep - 1) / kStep; };
+  int window = 0, lens = lengths_at(0);
+  int sum = steps_of(lens);
+  for (int base = kWave; base < a.B; base += kWave) sum += steps_of(lengths_at(base));
+  const int all = sgpr(wave_sum_i(sum)) * heads;          // < 2^31, checked on the host
+  const int per = (all + workers - 1) / workers;          // steps of a wave
+  if ((int64_t)worker * per >= all) return;
+  const int first = worker * per;
+  int left = min(per, all - first);
+  int before = 0;  // steps in the sequences before the window
+  int incl;        // running sum within the window
+  for (;;) {
+    incl = steps_of(lens) * heads;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int y = __shfl_up(incl, o, kWave);
+      if (lane >= o) incl += y;
+    }
+    const int in_window = __builtin_amdgcn_readlane(incl, 63);
+    if (first < before + in_window) break;
+    before += in_window;
+    window += kWave;
+    if (window >= a.B) return;  // only if lengths change meanwhile
+    lens = lengths_at(window);
   }
-  for (int d = lane; d < a.D; d += 64) qs[d] = to_f32(a.q[b * a.q_stride + head * a.D + d], a.dtype);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int base = 0; base < len; base += 64) {
-    const int j = base + lane, n = min(64, len - base);
-    float s = -INFINITY;
-    int64_t vrow = -1;
-    if (lane < n) {
-      const int p = a.tables[b * a.table_stride + j / a.page], r = j % a.page;
-      if (p < 0 || p >= a.P) {
-        atomicOr(a.status, GQA_STATUS_BAD_PAGE);
-      } else {
-        const uint16_t *kp = a.k + p * a.k_page + kvh * a.k_head + r * a.k_row;
-        vrow = p * a.v_page + kvh * a.v_head + r * a.v_row;
-        s = 0.f;
-        for (int d = 0; d < a.D; ++d) s += qs[d] * to_f32(kp[d], a.dtype);
-        s *= a.scale;
+  const int at = sgpr(__builtin_ctzll(__builtin_amdgcn_ballot_w64(before + incl > first)));
+  int b = window + at, len = __builtin_amdgcn_readlane(lens, at), steps = steps_of(len);
+  const int rest = first - (before + (at ? __builtin_amdgcn_readlane(incl, at - 1 < 0 ? 0 : at - 1) : 0));
+  int head = rest / steps, s = rest % steps;
+  const int per_page = a.page / kBlock;
+  int page_at = 2 * s / per_page, block_at = 2 * s % per_page;  // of the next step's first block
+
+  // The next step of the range; none left: no keys.
+  auto next_step = [&]() __attribute__((always_inline)) {
+    Step t;
+    t.b = b;
+    t.head = head;
+    t.s = s;
+    t.steps = steps;
+    const int n = left > 0 ? min(kStep, len - kStep * s) : 0;
+    t.n[0] = min(kBlock, n);
+    t.n[1] = max(0, n - kBlock);
+    t.row[0] = block_at * kBlock;
+    const int32_t *const table = a.tables + (int64_t)b * a.table_stride;
+    t.page[0] = n > 0 ? uniform_load(table + page_at) : 0;
+    if (++block_at == per_page) {
+      block_at = 0;
+      ++page_at;
+    }
+    t.row[1] = block_at * kBlock;
+    t.page[1] = n > kBlock ? uniform_load(table + page_at) : 0;
+    if (++block_at == per_page) {
+      block_at = 0;
+      ++page_at;
+    }
+    if (--left > 0 && ++s == steps) {
+      s = page_at = block_at = 0;
+      if (++head == heads) {
+        head = 0;
+        int i = b - window + 1;
+        for (;;) {
+          const uint64_t some = __builtin_amdgcn_ballot_w64(lens > 0);
+          const uint64_t later = i < kWave ? some >> i << i : 0ull;
+          if (later) {
+            i = sgpr(__builtin_ctzll(later));
+            break;
+          }
+          window += kWave;
+          if (window >= a.B) {  // only if lengths change meanwhile
+            left = i = 0;
+            break;
+          }
+          lens = lengths_at(window);
+          i = 0;
+        }
+        if (left > 0) {
+          b = window + i;
+          len = __builtin_amdgcn_readlane(lens, i);
+          steps = steps_of(len);
+        }
       }
     }
-    float mx = s;
-    for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn, alpha = expf(m - ref);
-    const float p = vrow >= 0 ? expf(s - ref) : 0.f;
-    float sum = p;
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    return t;
+  };
+
+  // ---- loads ----
+  // Load j of a block, lane l: 16 bytes of row (64 j + l) / (D / 8), which land
+  // at place (64 j + l) % (D / 8) of that row.
+  uint32_t k_off[kLoads], v_off[kLoads], q_off[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const int row = (64 * j + lane) / (D / 8), place = lane % (D / 8);
+    k_off[j] = (uint32_t)row * (uint32_t)(2 * a.k_row) + 16 * (place ^ swizzle_k<D>(row));
+    v_off[j] = (uint32_t)row * (uint32_t)(2 * a.v_row) + 16 * (place ^ swizzle_v<D>(row));
+    q_off[j] = (uint32_t)row * (2 * D) + 16 * (place ^ swizzle_k<D>(row));
+  }
+  // Keys of a block that are there: none of a page outside the cache.
+  auto usable = [&](const Step &t, int i) __attribute__((always_inline)) {
+    return (uint32_t)t.page[i] < (uint32_t)a.P ? t.n[i] : 0;
+  };
+  auto issue = [&](const Step &t, const uint16_t *pages, int64_t page_st, int64_t head_st, int64_t row_st,
+                   const uint32_t (&off)[kLoads], uint8_t *stage) __attribute__((always_inline)) {
+    const int64_t head_at = (t.head / blocks) * head_st;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int n = usable(t, i);
+      const uint16_t *const base = pages + (n ? t.page[i] * page_st + head_at + t.row[i] * row_st : 0);
+      const auto rs = buffer(base, n ? (uint32_t)(n - 1) * (uint32_t)(2 * row_st) + 2 * D : 0u);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) load_lds16(rs, stage + (i * kLoads + j) * 1024, off[j]);
+    }
+  };
+  auto issue_k = [&](const Step &t) __attribute__((always_inline)) {
+    issue(t, a.k, a.k_page, a.k_head, a.k_row, k_off, kst);
+    asm volatile("" ::: "memory");  // the counted waits rely on the order
+  };
+  auto issue_v = [&](const Step &t) __attribute__((always_inline)) {
+    issue(t, a.v, a.v_page, a.v_head, a.v_row, v_off, vst);
+    asm volatile("" ::: "memory");
+  };
+  auto issue_q = [&](const Step &t) __attribute__((always_inline)) {
+    const int kvh = t.head / blocks, part = t.head % blocks, rows = min(kRows, group - kRows * part);
+    const uint16_t *const base = a.q + t.b * a.q_stride + (int64_t)(kvh * group + kRows * part) * D;
+    const auto rs = buffer(base, (uint32_t)rows * 2 * D);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) load_lds16(rs, qst + j * 1024, q_off[j]);
+    asm volatile("" ::: "memory");
+  };
+
+  // ---- operand addresses ----
+  uint32_t k_at[kSlices];  // chunk 4 ks + g of row r
+#pragma unroll
+  for (int ks = 0; ks < kSlices; ++ks) k_at[ks] = (uint32_t)(r * 2 * D + 16 * ((4 * ks + g) ^ swizzle_k<D>(r)));
+  const uint32_t k_base = lds_addr(kst);
+  const int v_row = 4 * g + (r >> 2);  // the lane addresses dims 4 (r % 4) .. of this key
+  const uint32_t v_base = lds_addr(vst) + (uint32_t)(v_row * 2 * D + 16 * (((r & 3) >> 1) ^ swizzle_v<D>(v_row)) + 8 * (r & 1));
+
+  // Softmax state of query row r (this lane's keys only in l), base-2 domain; O:
+  // rows 4 g + i, dims 16 dt + r.
+  float m_run = -INFINITY, l_run = 0.f;
+  f32x4 o[kTiles];
+#pragma unroll
+  for (int dt = 0; dt < kTiles; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float sl2 = a.scale * kLog2e;
+  int piece_from = s, piece_unit = first;  // where the present piece began
+  int unit = first;
+  bool bad_page = false;
+
+  Step cur = next_step(), nx = next_step();
+  issue_q(cur);
+  issue_k(cur);
+  issue_v(cur);
+  while (cur.n[0] > 0) {
+    // K (and Q) have landed once at most V's loads remain.
+    wait_vmcnt<2 * kLoads>();
+    u32x4 kf[2 * kSlices], qf[kSlices];
+    read_kq<D>(k_base, k_at, kf, qf);
+    f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int ks = 0; ks < kSlices; ++ks)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) sc[kt] = mfma16x16<F16>(kf[2 * ks + kt], qf[ks], sc[kt]);
+    if (nx.b != cur.b || nx.head != cur.head) issue_q(nx);
+    issue_k(nx);
+    // Lane: keys 16 kt + 4 g + i of query row r.
+    const int n0 = usable(cur, 0), n1 = usable(cur, 1);
+    if (n0 + n1 < kStep) {
+      bad_page |= n0 != cur.n[0] || n1 != cur.n[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[0][i] = 4 * g + i < n0 ? sc[0][i] : -INFINITY;
+        sc[1][i] = 4 * g + i < n1 ? sc[1][i] : -INFINITY;
+      }
+    }
+    const float lmax = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                             fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3]))) * sl2;
+    if (__builtin_amdgcn_ballot_w64(lmax > m_run + kRescaleSlack)) {
+      const float m_new = fmaxf(m_run, quad_max(lmax));
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+      l_run *= alpha;
+      m_run = m_new;
+      float al[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, 4 * g + i, kWave);
+#pragma unroll
+      for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[dt][i] *= al[i];
+    }
+    const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+    float p[2][4];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], sl2, neg_m));
+    l_run += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+    // Probabilities in the type of V: half a step each, against fp32 sums of both.
+    const u32x4 pa = {pack2<F16>(p[0][0], p[0][1]), pack2<F16>(p[0][2], p[0][3]), pack2<F16>(p[1][0], p[1][1]),
+                      pack2<F16>(p[1][2], p[1][3])};
+    // V has landed once at most the next K's loads remain.
+    wait_vmcnt<2 * kLoads>();
+    u32x2 vr[2 * kTiles];
+    read_v<D>(v_base, vr);
+    issue_v(nx);
+#pragma unroll
+    for (int dt = 0; dt < kTiles; ++dt)
+      o[dt] = mfma16x16<F16>(pa, u32x4{vr[2 * dt][0], vr[2 * dt][1], vr[2 * dt + 1][0], vr[2 * dt + 1][1]}, o[dt]);
+
+    // ---- the end of a piece ----
+    const bool pair_ends = cur.s + 1 == cur.steps;
+    if (pair_ends || nx.n[0] == 0) {
+      const int kvh = cur.head / blocks, part = cur.head % blocks, rows = min(kRows, group - kRows * part);
+      const int64_t head0 = (int64_t)cur.b * a.Hq + kvh * group + kRows * part;
+      const float l = quad_sum(l_run);
+      const bool whole = pair_ends && piece_from == 0;
+      const int slot = 2 * worker + (piece_unit == first ? 0 : 1);
+      if (piece_from == 0 && lane == 0) {
+        // Pieces of the (sequence, head block): this one, then the first pieces
+        // of the following waves.
+        const int last = (piece_unit + cur.steps - 1) / per;
+        a.pieces[2 * (cur.b * heads + cur.head)] = slot;
+        a.pieces[2 * (cur.b * heads + cur.head) + 1] = whole ? 0 : last - worker + 1;
+      }
+      float L[4], M[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        L[i] = __shfl(l, 4 * g + i, kWave);
+        M[i] = __shfl(m_run, 4 * g + i, kWave);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 4 * g + i;
+        if (row >= rows) continue;
+        if (whole) {
+          const float inv = L[i] == 0.f ? 0.f : 1.0f / L[i];
+          uint16_t *const op = a.out + (head0 + row) * D + r;
+#pragma unroll
+          for (int dt = 0; dt < kTiles; ++dt) op[16 * dt] = (uint16_t)pack2<F16>(o[dt][i] * inv, 0.f);
+        } else {
+          float *const pp = a.partial + ((int64_t)slot * min(group, kRows) + row) * (D + 2);
+          if (r == 0) {
+            pp[0] = M[i];
+            pp[1] = L[i];
+          }
+#pragma unroll
+          for (int dt = 0; dt < kTiles; ++dt) pp[2 + 16 * dt + r] = o[dt][i];
+        }
+      }
+      m_run = -INFINITY;
+      l_run = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < kTiles; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      piece_from = 0;
+      piece_unit = unit + 1;
+    }
+    ++unit;
+    cur = nx;
+    nx = next_step();
+  }
+  wait_vmcnt<0>();  // the last (empty) step's loads write LDS
+  if (bad_page && lane == 0) atomicOr(a.status, GQA_STATUS_BAD_PAGE);
+}
+
+// Joins the pieces of a (sequence, head block), in the order of the keys: eight
+// groups of threads take every eighth piece of 32 dims of a row, and the eight
+// states are joined in order.  A piece without a usable key (m = -inf) has
+// weight 0, a row without any is 0; NaN passes through.  Sequences of length 0
+// get their zeros here.
+constexpr int kMergeThreads = 256;
+template <bool F16>
+__global__ __launch_bounds__(kMergeThreads) void gqa_paged_merge(GqaPagedArgs a, int D) {
+  constexpr int kGroups = kMergeThreads / 32;
+  __shared__ float sm[kGroups], sl[kGroups], so[kGroups][32];
+  const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows, heads = a.Hkv * blocks;
+  const int b = blockIdx.x / heads, head = blockIdx.x % heads;
+  const int kvh = head / blocks, part = head % blocks, rows = min(kRows, group - kRows * part);
+  const int d = threadIdx.x & 31, pg = threadIdx.x >> 5;
+  const bool empty = a.lengths[b] <= 0;
+  const int slot = a.pieces[2 * blockIdx.x], n = empty ? 0 : a.pieces[2 * blockIdx.x + 1];
+  if (!empty && n == 0) return;  // written by the wave that had all of it
+  const int slices = D / 32, per_slot = min(group, kRows);
+  for (int item = blockIdx.y; item < rows * slices; item += gridDim.y) {
+    const int row = item / slices, at = 32 * (item % slices) + d;
+    uint16_t *const op = a.out + (((int64_t)b * a.Hq + kvh * group + kRows * part + row) * D + at);
+    if (empty) {
+      if (pg == 0) *op = 0;
+      continue;
+    }
+    float M = -INFINITY, den = 0.f, num = 0.f;
+    for (int i = pg; i < n; i += kGroups) {
+      // The first piece's slot, then the first slot of each following wave.
+      const float *const pp = a.partial + ((int64_t)(i == 0 ? slot : (slot / 2 + i) * 2) * per_slot + row) * (D + 2);
+      const float m = pp[0], l = pp[1], x = pp[2 + at];
+      const float m_new = fmaxf(M, m), ref = m_new == -INFINITY ? 0.f : m_new;
+      const float wa = exp2f(M - ref), wb = exp2f(m - ref);
+      den = den * wa + l * wb;
+      num = num * wa + x * wb;
+      M = m_new;
+    }
+    __syncthreads();  // the last item's states have been read
+    if (d == 0) {
+      sm[pg] = M;
+      sl[pg] = den;
+    }
+    so[pg][d] = num;
     __syncthreads();
-    ps[lane] = p;
-    rows[lane] = vrow;
-    __syncthreads();
-    l = l * alpha + sum;
-    m = mn;
-    o0 *= alpha;
-    o1 *= alpha;
-    for (int i = 0; i < n; ++i) {
-      if (rows[i] < 0) continue;
-      const uint16_t *vp = a.v + rows[i];
-      o0 += ps[i] * to_f32(vp[lane], a.dtype);
-      if (a.D > 64) o1 += ps[i] * to_f32(vp[64 + lane], a.dtype);
+    if (pg == 0) {
+      M = sm[0];
+      for (int i = 1; i < kGroups; ++i) M = fmaxf(M, sm[i]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      den = num = 0.f;
+      for (int i = 0; i < kGroups; ++i) {
+        const float w = exp2f(sm[i] - ref);
+        den += w * sl[i];
+        num += w * so[i][d];
+      }
+      const float v = den == 0.f ? 0.f : num / den;
+      *op = (uint16_t)pack2<F16>(v, 0.f);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  uint16_t *op = a.out + ((int64_t)b * a.Hq + head) * a.D;
-  op[lane] = from_f32(o0 * inv, a.dtype);
-  if (a.D > 64) op[64 + lane] = from_f32(o1 * inv, a.dtype);
 }
 
 __global__ void clear_word(uint32_t *w) { *w = 0; }
 
+template <int D, bool F16>
+hipError_t launch(const GqaPagedArgs &a, int cus, hipStream_t s) {
+  auto k = gqa_paged_kernel<D, F16>;
+  constexpr int lds = kWaves * kWaveLds<D>;
+  static const bool attr = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds) ==
+                           hipSuccess;
+  if (!attr) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(k, dim3(cus * kWorkgroups<D>), dim3(64 * kWaves), lds, s, a);
+  const int group = a.Hq / a.Hkv, heads = a.Hkv * ((group + kRows - 1) / kRows);
+  // Few (sequence, head block)s: their rows and dims on workgroups of their own.
+  const int items = min(group, kRows) * (D / 32), pairs = a.B * heads;
+  const int spread = pairs >= 1024 ? 1 : min(items, (1024 + pairs - 1) / pairs);
+  hipLaunchKernelGGL(gqa_paged_merge<F16>, dim3(pairs, spread), dim3(kMergeThreads), 0, s, a, D);
+  return hipGetLastError();
+}
+
+int waves_of(int D, int cus) { return cus * kWaves * (D == 128 ? kWorkgroups<128> : kWorkgroups<64>); }
+
+size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
 }  // namespace
 
-hipError_t launch_gqa_paged(const GqaPagedArgs &a, hipStream_t s) {
-  hipLaunchKernelGGL(gqa_paged_simple, dim3(a.B, a.Hq), dim3(64), 0, s, a);
-  return hipGetLastError();
+// {status words; two words per (sequence, head block); the pieces' states}
+size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int cus) {
+  const int group = Hq / Hkv, rows = group < kRows ? group : kRows;
+  const size_t pairs = (size_t)B * Hkv * ((group + kRows - 1) / kRows);
+  return 256 + align256(8 * pairs) + (size_t)2 * waves_of(D, cus) * rows * (D + 2) * sizeof(float);
+}
+
+void gqa_paged_bind(GqaPagedArgs *a, void *workspace) {
+  uint8_t *const w = (uint8_t *)workspace;
+  const int group = a->Hq / a->Hkv;
+  const size_t pairs = (size_t)a->B * a->Hkv * ((group + kRows - 1) / kRows);
+  a->status = (uint32_t *)w;
+  a->pieces = (int32_t *)(w + 256);
+  a->partial = (float *)(w + 256 + align256(8 * pairs));
+}
+
+hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s) {
+  if (a.D == 128) return a.dtype == GQA_FP16 ? launch<128, true>(a, cus, s) : launch<128, false>(a, cus, s);
+  return a.dtype == GQA_FP16 ? launch<64, true>(a, cus, s) : launch<64, false>(a, cus, s);
 }
 
 hipError_t read_and_clear_status(uint32_t *status, uint32_t *flags, hipStream_t s) {
