@@ -3,18 +3,19 @@
 //   out[t][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[t][h] . k_j - max),
 //   over the keys j of t's sequence up to t; head h reads KV head h / G.
 //
-// Long prompts are bound by the matrix cores, and next to them by the LDS: an
-// MFMA operand read is used for as many query rows as the wave holds.  So a
-// workgroup owns 256 query rows of one KV head (a sequence's tokens with their G
-// heads side by side, row = token * G + head, whatever G is) and each of its
-// four waves, one per SIMD, owns 64: two blocks of 32 that share every K and V
-// operand.  With one wave per SIMD nothing else fills its pauses, so the wave
+// Long prompts are bound by the matrix cores and, next to them, by the issue of
+// the softmax's vector instructions.  A workgroup owns 256 query rows of one KV
+// head (a sequence's tokens with their G heads side by side, row = token * G +
+// head, whatever G is), each of its eight waves, two per SIMD, 32 of them.  A wave
 // overlaps its own work: per 32 keys
-//   A: S^T = K Q^T of the next 32 keys (MFMA) beside the exponentials of these,
-//   B: O^T += V^T P^T of these (MFMA) beside the sums and the next maxima,
+//   A: S^T = K Q^T of the next 32 keys (MFMA) beside the exponentials and sums of
+//      these,
+//   B: O^T += V^T P^T of these (MFMA) beside the next maxima,
 // with the operands of each read from LDS one phase ahead.  A lane holds sixteen
-// scores of one query per block (the partner lane l ^ 32 the other sixteen), so
-// the online softmax is lane-local and P is the B operand of O^T as it lies.
+// scores of one query (the partner lane l ^ 32 the other sixteen), so the online
+// softmax is lane-local and P is the B operand of O^T as it lies.  (Four waves of
+// 64 rows, one per SIMD, read half as much from LDS but cannot issue more than one
+// instruction in four cycles: 1.03 PFLOP/s at 16384 tokens.)
 //
 // K and V come in stages of 64 keys, global -> LDS in whole rows (buffer loads
 // with an LDS destination; keys behind the sequence's end read as zeros), three
@@ -31,29 +32,41 @@ using namespace gqa;
 namespace {
 
 constexpr int kTileRows = 256;  // query rows of a workgroup
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
+constexpr int kWaveRows = 32;
 constexpr int kStageKeys = 64;
 constexpr int kSlots = 4;
 constexpr int kWindow = 4;      // sequences per lane that a search looks at together
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 // Row i of a stage's K (V) tile holds its 16-byte chunk c at place c ^ swizzle(i):
-// sixteen lanes that read one chunk of sixteen K rows, or two chunks of four V
-// rows, then meet different bank groups.
+// sixteen lanes that read one chunk of sixteen K rows, or 32 lanes that read four
+// chunks of four V rows, then meet sixteen different bank groups.
 template <int D>
 __device__ __forceinline__ int swizzle_k(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
 template <int D>
-__device__ __forceinline__ int swizzle_v(int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
+__device__ __forceinline__ int swizzle_v(int row) { return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
 
-// 16 bytes per lane from a buffer straight into LDS at `dst` + 16 l.  As inline
+// 16 bytes per lane from a buffer straight into LDS at `dst` + 16 l (load j 1024 j
+// further).  As inline
 // assembly (it has no output register): the compiler would make every later LDS
 // read wait for all such loads in flight; the kernel waits with exact counts.
 // (Nothing else in this kernel uses m0.)
-__device__ __forceinline__ void load_lds(u32x4 rsrc, uint32_t dst, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(dst), "v"(off), "s"(rsrc)
-               : "memory");
+template <int N>
+__device__ __forceinline__ void load_lds(u32x4 rsrc, uint32_t dst, const uint32_t (&off)[N]) {
+  static_assert(N == 1 || N == 2, "loads of a wave");
+  if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
+        :
+        : "s"(dst), "v"(off[0]), "v"(off[1]), "s"(rsrc)
+        : "memory", "scc");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(dst), "v"(off[0]), "s"(rsrc)
+                 : "memory");
 }
 __device__ __forceinline__ u32x4 buffer_words(const void *base, uint32_t bytes) {
   const uint64_t b = sgpr64((uint64_t)base);
@@ -80,22 +93,15 @@ __device__ __forceinline__ f32x2_t halves(float x) {
   const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return f32x2_t{__uint_as_float(h[0]), __uint_as_float(h[1])};
 }
-// MFMA results stay in AGPRs and are read and written by these.  As plain
-// arithmetic, the rare rescale of O would make the compiler move all of O to VGPRs
-// and back at every step; and across a branch it can miss that an MFMA's result is
-// not there yet (it takes up to 19 wait states for 16 passes).  Before the first
-// read: acc_settle(), or two later MFMAs (each waits for the one before).
-__device__ __forceinline__ float acc_read(float x) {
-  float t;
-  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(t) : "a"(x));
-  return t;
-}
-__device__ __forceinline__ float acc_write(float t) {
-  float x;
-  asm volatile("v_accvgpr_write_b32 %0, %1" : "=a"(x) : "v"(t));
+// An MFMA's results take up to 19 wait states, and across a branch the compiler can
+// miss that they are not there yet.  Where they are read in another block than
+// the MFMA's, mfma_settle() stands before, or two later MFMAs (each waits for the
+// one before), and pin() keeps the reads behind that.
+__device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 3" ::: "memory"); }
+__device__ __forceinline__ float pin(float x) {
+  asm volatile("" : "+v"(x));
   return x;
 }
-__device__ __forceinline__ void acc_settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 template <bool F16>
 __device__ __forceinline__ bool not_finite2(uint32_t w) {
   constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;
@@ -186,40 +192,44 @@ __device__ __forceinline__ Rows find_rows(const GqaPackedArgs &a, int G, int ite
   return Rows{0, 0, 0};
 }
 
-// The 64 rows of a wave from row0 on, a row per lane and a key per step, in plain
-// fp32: for waves that meet a V that only some of their rows see and that is not
-// finite.  A key that a row does not see touches nothing of it.
+// The rows of a wave from row0 on, a row per pair of lanes l, l + 32 (each with half
+// of the dims) and a key per step, in plain fp32: for waves that meet a V that only
+// some of their rows see and that is not finite.  A key that a row does not see
+// touches nothing of it.
 template <int D, bool F16>
 __device__ __forceinline__ void take_rows(const GqaPackedArgs &a, const Rows &w, int kvh, int row0, int tok_hi) {
-  const int G = a.Hq / a.Hkv, rows = w.len * G;
-  const int row = min(row0 + (int)(threadIdx.x & 63), rows - 1), tok = row / G, head = kvh * G + row % G;
-  const uint16_t *const qp = a.q + (int64_t)(w.start + tok) * a.q_stride + (int64_t)head * D;
-  u32x4 q[D / 8];
+  constexpr int kPart = D / 16;  // 16-byte chunks of a lane
+  const int G = a.Hq / a.Hkv, rows = w.len * G, lane = threadIdx.x & 63;
+  const int row = min(row0 + lane % kWaveRows, rows - 1), tok = row / G, head = kvh * G + row % G;
+  const int first = lane / kWaveRows * (D / 2);  // of the lane's dims
+  const uint16_t *const qp = a.q + (int64_t)(w.start + tok) * a.q_stride + (int64_t)head * D + first;
+  u32x4 q[kPart];
 #pragma unroll
-  for (int c = 0; c < D / 8; ++c) q[c] = *(const u32x4 *)(qp + 8 * c);
-  float o[D], m = -INFINITY, l = 0.f;
+  for (int c = 0; c < kPart; ++c) q[c] = *(const u32x4 *)(qp + 8 * c);
+  float o[8 * kPart], m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int d = 0; d < D; ++d) o[d] = 0.f;
+  for (int d = 0; d < 8 * kPart; ++d) o[d] = 0.f;
   const float sl2 = a.scale * kLog2e;
 #pragma clang loop unroll(disable)
   for (int key = 0; key <= tok_hi; ++key) {
-    const uint16_t *const kp = a.k + (int64_t)(w.start + key) * a.k_stride + (int64_t)kvh * D;
-    const uint16_t *const vp = a.v + (int64_t)(w.start + key) * a.v_stride + (int64_t)kvh * D;
+    const uint16_t *const kp = a.k + (int64_t)(w.start + key) * a.k_stride + (int64_t)kvh * D + first;
+    const uint16_t *const vp = a.v + (int64_t)(w.start + key) * a.v_stride + (int64_t)kvh * D + first;
     float dot = 0.f;
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
+    for (int c = 0; c < kPart; ++c) {
       const u32x4 x = *(const u32x4 *)(kp + 8 * c);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        dot = __builtin_fmaf(element<F16>(q[c], i), element<F16>(x, i), dot);
+      for (int i = 0; i < 8; ++i) dot = __builtin_fmaf(element<F16>(q[c], i), element<F16>(x, i), dot);
     }
+    const f32x2_t both = halves(dot);
     const bool seen = key <= tok;
-    const float sc = seen ? dot * sl2 : -INFINITY, m_new = fmaxf(m, sc), ref = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = exp2f(m - ref), p = seen ? exp2f(sc - ref) : 0.f;
-    m = m_new;
-    l = l * alpha + p;
+    const float sc = seen ? (both[0] + both[1]) * sl2 : -INFINITY;
+    const float m_new = fmaxf(m, sc), ref = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = exp2f(m - ref), p = exp2f(sc - ref);
+    m = seen ? m_new : m;
+    l = seen ? l * alpha + p : l;
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
+    for (int c = 0; c < kPart; ++c) {
       const u32x4 x = *(const u32x4 *)(vp + 8 * c);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -228,16 +238,16 @@ __device__ __forceinline__ void take_rows(const GqaPackedArgs &a, const Rows &w,
       }
     }
   }
-  if (row0 + (int)(threadIdx.x & 63) >= rows) return;
+  if (row0 + lane % kWaveRows >= rows) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  uint32_t *const op = (uint32_t *)(a.out + ((int64_t)(w.start + tok) * a.Hq + head) * D);
+  uint32_t *const op = (uint32_t *)(a.out + ((int64_t)(w.start + tok) * a.Hq + head) * D + first);
 #pragma unroll
-  for (int d = 0; d < D; d += 2) op[d / 2] = pack2<F16>(o[d] * inv, o[d + 1] * inv);
+  for (int d = 0; d < 8 * kPart; d += 2) op[d / 2] = pack2<F16>(o[d] * inv, o[d + 1] * inv);
 }
 
 template <int D, bool F16>
-__global__ __launch_bounds__(64 * kWaves, 1) void gqa_packed_kernel(GqaPackedArgs a) {
-  constexpr int kSteps = D / 16;                    // QK MFMAs per block and half stage
+__global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArgs a) {
+  constexpr int kSteps = D / 16;                    // QK MFMAs per half stage
   constexpr int kDims = D / 32;                     // 32-dim tiles of O
   constexpr int kTile = kStageKeys * D * 2;         // bytes of a stage's K (or V)
   constexpr int kLoads = kTile / 1024 / kWaves;     // of K (or V) per wave and stage
@@ -257,12 +267,12 @@ __global__ __launch_bounds__(64 * kWaves, 1) void gqa_packed_kernel(GqaPackedArg
   if (w.len == 0) return;
 
   const int rows = w.len * G;                                           // of the sequence
-  const int row0 = w.tile * kTileRows + 64 * wave;                      // of the wave
+  const int row0 = w.tile * kTileRows + kWaveRows * wave;                      // of the wave
   const int keys = min(w.len, (w.tile * kTileRows + kTileRows - 1) / G + 1);  // that the workgroup sees
   const int stages = (keys + kStageKeys - 1) / kStageKeys;
   // The wave's half stages of 32 keys: all up to its last token's, the first
   // `full` of them seen by all of its tokens.
-  const int tok_lo = row0 / G, tok_hi = min(w.len - 1, (row0 + 63) / G);
+  const int tok_lo = row0 / G, tok_hi = min(w.len - 1, (row0 + kWaveRows - 1) / G);
   const int nhalf = row0 < rows ? tok_hi / 32 + 1 : 0, full = (tok_lo + 1) / 32;
 
   // ---- loads ----
@@ -282,10 +292,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void gqa_packed_kernel(GqaPackedArg
     const u32x4 krs = buffer_words(k0 + (int64_t)first * a.k_stride, (uint32_t)(n - 1) * ksb + 2 * D);
     const u32x4 vrs = buffer_words(v0 + (int64_t)first * a.v_stride, (uint32_t)(n - 1) * vsb + 2 * D);
     const uint32_t dst = sgpr((int)(lds0 + (st % kSlots) * (2 * kTile) + wave * kLoads * 1024));
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) load_lds(krs, dst + j * 1024, k_off[j]);
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) load_lds(vrs, dst + kTile + j * 1024, v_off[j]);
+    load_lds(krs, dst, k_off);
+    load_lds(vrs, dst + kTile, v_off);
   };
   // Stage st is there for every wave, and every wave is done with stage st - 2,
   // whose slot takes stage st + 2.
@@ -300,16 +308,11 @@ __global__ __launch_bounds__(64 * kWaves, 1) void gqa_packed_kernel(GqaPackedArg
   if (stages > 1) issue(1);
 
   // ---- operands ----
-  u32x4 qf[2][kSteps];
-  int lim[2];  // the lane's token per block: the last key that it sees
+  const int row = min(row0 + r, rows - 1), tok = row / G;  // the lane's; tok: the last key that it sees
+  const int64_t at_q = (int64_t)(w.start + tok), head = kvh * G + row % G;
+  u32x4 qf[kSteps];
 #pragma unroll
-  for (int blk = 0; blk < 2; ++blk) {
-    const int row = min(row0 + 32 * blk + r, rows - 1), tok = row / G;
-    lim[blk] = tok;
-    const uint16_t *const qp = a.q + (int64_t)(w.start + tok) * a.q_stride + (int64_t)(kvh * G + row % G) * D + 8 * h;
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) qf[blk][ks] = *(const u32x4 *)(qp + 16 * ks);
-  }
+  for (int ks = 0; ks < kSteps; ++ks) qf[ks] = *(const u32x4 *)(a.q + at_q * a.q_stride + head * D + 8 * h + 16 * ks);
   // K fragment ks: row r, chunk 2 ks + h.  V: the lane addresses dims 16 (gi % 2)
   // + 4 x .. of 32, key 4 h + c.
   const uint32_t k_at = (uint32_t)(r * 2 * D + 16 * (h ^ swizzle_k<D>(r)));
@@ -318,182 +321,175 @@ __global__ __launch_bounds__(64 * kWaves, 1) void gqa_packed_kernel(GqaPackedArg
 
   u32x4 kf[kSteps], vf[2][kDims];
   auto half_base = [&](int hf) { return lds0 + (uint32_t)((hf / 2) % kSlots * (2 * kTile) + (hf & 1) * (kTile / 2)); };
-  auto read_k = [&](int hf) __attribute__((always_inline)) {
-    const uint32_t at = half_base(hf) + k_at;
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) kf[ks] = lds_b128(at ^ (32 * ks));
+  // Operand reads, spread over the MFMAs before their use: all at once they would
+  // not fit the registers, and the waves' bursts would wait for each other.
+  auto read_k = [&](int hf, int ks) __attribute__((always_inline)) {
+    kf[ks] = lds_b128((half_base(hf) + k_at) ^ (32 * ks));
   };
-  auto read_v = [&](int hf) __attribute__((always_inline)) {
-    const uint32_t at = half_base(hf) + v_at;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int db = 0; db < kDims; ++db) {
-        const u32x2 lo = lds_tr16((at ^ (64 * db)) + j * 32 * D), hi = lds_tr16((at ^ (64 * db)) + j * 32 * D + 16 * D);
-        vf[j][db] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-      }
+  auto read_v = [&](int hf, int j, int db) __attribute__((always_inline)) {
+    const uint32_t at = ((half_base(hf) + v_at) ^ (64 * db)) + j * 32 * D;
+    const u32x2 lo = lds_tr16(at), hi = lds_tr16(at + 16 * D);
+    vf[j][db] = u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
 
   const float sl2 = a.scale * kLog2e;
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};  // base-2 domain; l of this lane's keys
-  f32x16 o[2][kDims];
+  float m_run = -INFINITY, l_run = 0.f;  // base-2 domain; l of this lane's keys
+  f32x16 o[kDims], s0, s1;
 #pragma unroll
-  for (int blk = 0; blk < 2; ++blk)
+  for (int db = 0; db < kDims; ++db)
 #pragma unroll
-    for (int db = 0; db < kDims; ++db)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[blk][db][i] = 0.f;
+    for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+  float mx = -INFINITY;  // of the raw scores of the half at hand
 
-  float s[2][16], mx[2];  // raw scores of the half at hand, and their maxima
-  f32x16 sn[2];           // the next half's
-  // Pairs of scores (b, i), (b, i + 1): b = x / 8, i = 2 (x % 8), x = 0..15.
-  auto take_next = [&](int x) __attribute__((always_inline)) {
-    const int b = x / 8, i = 2 * (x % 8);
-    s[b][i] = acc_read(sn[b][i]);
-    s[b][i + 1] = acc_read(sn[b][i + 1]);
-    mx[b] = fmaxf(fmaxf(s[b][i], s[b][i + 1]), i ? mx[b] : -INFINITY);
-  };
-  bool redo = false;
-  sync(0);
-  if (nhalf > 0) {
-    read_k(0);
+  // One half: its scores in s; the next half's come into sn.
+  // The second four waves, each beside one of the first on its SIMD, meet them at
+  // the barrier a phase earlier in their own work, so that one's exponentials fall
+  // beside the other's MFMAs.
+  auto half = [&](int hf, f32x16 &s, f32x16 &sn) __attribute__((always_inline)) {
+    if (wave >= kWaves / 2 && !(hf & 1) && hf / 2 + 1 < stages) sync(hf / 2 + 1);
+    if (hf >= full) {
+      const int last = tok - 32 * hf - 4 * h;
+      mx = -INFINITY;
 #pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sn[blk][i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) sn[blk] = mfma32x32<F16>(kf[ks], qf[blk][ks], sn[blk]);
-    }
-    if (nhalf > 1) read_k(1);
-    acc_settle();
-#pragma unroll
-    for (int x = 0; x < 16; ++x) take_next(x);
-  }
-  for (int hf = 0; hf < nhalf; ++hf) {
-    const bool masked = hf >= full;
-    if (masked) {
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
-        const int last = lim[blk] - 32 * hf - 4 * h;
-        mx[blk] = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[blk][i] = 8 * (i >> 2) + (i & 3) <= last ? s[blk][i] : -INFINITY;
-          mx[blk] = fmaxf(mx[blk], s[blk][i]);
-        }
+      for (int i = 0; i < 16; ++i) {
+        s[i] = 8 * (i >> 2) + (i & 3) <= last ? s[i] : -INFINITY;
+        mx = fmaxf(mx, s[i]);
       }
     }
-    const bool grow = mx[0] * sl2 > m_run[0] + kRescaleSlack || mx[1] * sl2 > m_run[1] + kRescaleSlack;
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-      acc_settle();
+    if (__builtin_amdgcn_ballot_w64(mx * sl2 > m_run + kRescaleSlack)) {
+      mfma_settle();
+      const f32x2_t both = halves(mx * sl2);
+      const float m_new = fmaxf(m_run, fmaxf(both[0], both[1]));
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+      l_run *= alpha;
+      m_run = m_new;
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
-        const f32x2_t both = halves(mx[blk] * sl2);
-        const float m_new = fmaxf(m_run[blk], fmaxf(both[0], both[1]));
-        const float alpha = __builtin_amdgcn_exp2f(m_run[blk] - (m_new == -INFINITY ? 0.f : m_new));
-        l_run[blk] *= alpha;
-        m_run[blk] = m_new;
+      for (int db = 0; db < kDims; ++db)
 #pragma unroll
-        for (int db = 0; db < kDims; ++db)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[blk][db][i] = acc_write(acc_read(o[blk][db][i]) * alpha);
-      }
+        for (int i = 0; i < 16; ++i) o[db][i] = pin(o[db][i]) * alpha;
     }
-    const float neg_m[2] = {m_run[0] == -INFINITY ? 0.f : -m_run[0], m_run[1] == -INFINITY ? 0.f : -m_run[1]};
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) asm volatile("" : "+a"(qf[blk][ks]));  // Q stays in AGPRs
+    const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
 
     // A: the next half's scores beside this one's exponentials.  (Behind the
-    // wave's last half kf holds keys that nothing asks for.)
-    read_v(hf);
+    // wave's last half these are of rows in the ring that nothing asks for.)
+#pragma unroll
+    for (int ks = kSteps / 2; ks < kSteps; ++ks) read_k(hf + 1, ks);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int blk = 0; blk < 2; ++blk)
+    for (int i = 0; i < 16; ++i) sn[i] = 0.f;
+    u32x4 pb[2];
+    float sum0 = 0.f, sum1 = 0.f, p0 = 0.f, p1 = 0.f;
+    // Pair x of probabilities (in the type of V: half a step each, against fp32
+    // sums of both) and of the sums; a pair later than its exponentials.
+    auto take = [&](int x) __attribute__((always_inline)) {
+      uint32_t w = pack2<F16>(p0, p1);
+      sum0 += p0;
+      sum1 += p1;
+      asm volatile("" : "+v"(w), "+v"(sum0), "+v"(sum1));  // here, not where they are used
+      pb[x / 4][x % 4] = w;
+    };
+    constexpr int kEach = 8 / kSteps;  // pairs of scores per MFMA
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sn[blk][i] = 0.f;
-    u32x4 pb[2][2];
+    for (int m = 0; m < kSteps; ++m) {
+      sn = mfma32x32<F16>(kf[m], qf[m], sn);
 #pragma unroll
-    for (int m = 0; m < 2 * kSteps; ++m) {
-      sn[m & 1] = mfma32x32<F16>(kf[m >> 1], qf[m & 1][m >> 1], sn[m & 1]);
-#pragma unroll
-      for (int x = 8 / kSteps * m; x < 8 / kSteps * (m + 1); ++x) {
-        const int b = x / 8, i = 2 * (x % 8);
-        float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], sl2, neg_m[b]));
-        float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i + 1], sl2, neg_m[b]));
-        // Probabilities in the type of V: half a step each, against fp32 sums of both.
-        uint32_t w = pack2<F16>(p0, p1);
-        asm volatile("" : "+v"(p0), "+v"(p1), "+v"(w));  // here, not where they are used
-        s[b][i] = p0;
-        s[b][i + 1] = p1;
-        pb[b][i / 8][(i / 2) % 4] = w;
+      for (int x = kEach * m; x < kEach * (m + 1); ++x) {
+        const float e0 = pin(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * x], sl2, neg_m)));
+        const float e1 = pin(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * x + 1], sl2, neg_m)));
+        if (x > 0) take(x - 1);
+        p0 = e0;
+        p1 = e1;
       }
+      if (m == kSteps - 1) take(7);
+      // V's first keys beside the first half of the MFMAs, the others (in the place
+      // of K fragments that are done with) beside the second.
+      if (m < kSteps / 2) read_v(hf, 0, m % kDims);
+      else read_v(hf, 1, m % kDims);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (!(hf & 1) && hf / 2 + 1 < stages) sync(hf / 2 + 1);
+    l_run += sum0 + sum1;
+    if (wave < kWaves / 2 && !(hf & 1) && hf / 2 + 1 < stages) sync(hf / 2 + 1);
 
-    // B: O of this half beside its sums and the next half's maxima (from the
-    // third MFMA on: the scores are there then).
-    if (hf + 2 < nhalf) read_k(hf + 2);
-    if (masked) {
-      // A probability of 0 times a V that is not finite is NaN: rows before such a
-      // V would not be what they are without it.
-      bool bad = false;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int db = 0; db < kDims; ++db)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) bad |= not_finite2<F16>(vf[j][db][c]);
-      redo |= __builtin_amdgcn_ballot_w64(bad) != 0;
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-    constexpr int kPv = 4 * kDims;
+    // B: O of this half beside the next half's maxima (from the third MFMA on: the
+    // scores are there then).
+    constexpr int kPv = 2 * kDims;
+    mx = -INFINITY;
 #pragma unroll
     for (int m = 0; m < kPv; ++m) {
-      const int blk = m & 1, db = (m >> 1) % kDims, j = m / (2 * kDims);
-      o[blk][db] = mfma32x32<F16>(vf[j][db], pb[blk][j], o[blk][db]);
+      o[m % kDims] = mfma32x32<F16>(vf[m / kDims][m % kDims], pb[m / kDims], o[m % kDims]);
 #pragma unroll
-      for (int x = m < 2 ? 0 : 16 * (m - 2) / (kPv - 2); x < (m < 2 ? 0 : 16 * (m - 1) / (kPv - 2)); ++x) {
-        const int b = x / 8, i = 2 * (x % 8);
-        sum[b][0] += s[b][i];
-        sum[b][1] += s[b][i + 1];
-        take_next(x);
-        asm volatile("" : "+v"(sum[b][0]), "+v"(sum[b][1]), "+v"(mx[b]));
+      for (int x = m < 2 ? 0 : 8 * (m - 2) / (kPv - 2); x < (m < 2 ? 0 : 8 * (m - 1) / (kPv - 2)); ++x) {
+        sn[2 * x] = pin(sn[2 * x]);
+        sn[2 * x + 1] = pin(sn[2 * x + 1]);
+        mx = pin(fmaxf(fmaxf(sn[2 * x], sn[2 * x + 1]), mx));
       }
+      if (m >= kDims) read_k(hf + 2, m - kDims);
       __builtin_amdgcn_sched_barrier(0);
     }
+  };
+
+  sync(0);
+  if (nhalf > 0) {
 #pragma unroll
-    for (int blk = 0; blk < 2; ++blk) l_run[blk] += sum[blk][0] + sum[blk][1];
+    for (int ks = 0; ks < kSteps; ++ks) read_k(0, ks);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s0[i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) s0 = mfma32x32<F16>(kf[ks], qf[ks], s0);
+#pragma unroll
+    for (int ks = 0; ks < kSteps / 2; ++ks) read_k(1, ks);
+    mfma_settle();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s0[i] = pin(s0[i]);
+      mx = fmaxf(mx, s0[i]);
+    }
+    for (int hf = 0; hf < nhalf; hf += 2) {
+      half(hf, s0, s1);
+      if (hf + 1 == nhalf) break;
+      half(hf + 1, s1, s0);
+    }
   }
   // The stages that other waves still read.
   for (int st = (nhalf + 1) / 2 + 1; st < stages; ++st) sync(st);
-  if (__builtin_expect(redo, 0)) {
-    take_rows<D, F16>(a, w, kvh, row0, tok_hi);
-    return;
-  }
-  acc_settle();
+  mfma_settle();
 
+  // In the masked halves a probability of 0 stood before values that the row does
+  // not see, and 0 times one that is not finite is NaN.  Looked for only where O is
+  // not finite; then the wave takes its rows again, slowly.
+  float zero = 0.f;
 #pragma unroll
-  for (int blk = 0; blk < 2; ++blk) {
-    const f32x2_t both = halves(l_run[blk]);
-    const float L = both[0] + both[1], inv = L == 0.f ? 0.f : 1.0f / L;
-    const int row = row0 + 32 * blk + r;
-    if (row >= rows) continue;
-    // Lane (r, h): dims 32 db + 8 q + 4 h + i of its row.
-    uint16_t *const op = a.out + ((int64_t)(w.start + lim[blk]) * a.Hq + kvh * G + row % G) * D + 4 * h;
+  for (int db = 0; db < kDims; ++db)
 #pragma unroll
-    for (int db = 0; db < kDims; ++db)
+    for (int i = 0; i < 16; ++i) {
+      o[db][i] = pin(o[db][i]);
+      zero = __builtin_fmaf(o[db][i], 0.f, zero);
+    }
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(zero != 0.f) != 0, 0)) {
+    bool bad = false;
+    for (int key = 32 * full + lane / kChunks; key < min(32 * nhalf, w.len); key += 64 / kChunks) {
+      const u32x4 v = *(const u32x4 *)(v0 + (int64_t)key * a.v_stride + 8 * (lane % kChunks));
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        u32x2 v;
-        v[0] = pack2<F16>(acc_read(o[blk][db][4 * q]) * inv, acc_read(o[blk][db][4 * q + 1]) * inv);
-        v[1] = pack2<F16>(acc_read(o[blk][db][4 * q + 2]) * inv, acc_read(o[blk][db][4 * q + 3]) * inv);
-        *(u32x2 *)(op + 32 * db + 8 * q) = v;
-      }
+      for (int c = 0; c < 4; ++c) bad |= not_finite2<F16>(v[c]);
+    }
+    if (nhalf > 0 && __builtin_amdgcn_ballot_w64(bad)) {
+      take_rows<D, F16>(a, w, kvh, row0, tok_hi);
+      return;
+    }
   }
+  const f32x2_t both = halves(l_run);
+  const float L = both[0] + both[1], inv = L == 0.f ? 0.f : 1.0f / L;
+  // Lane (r, h): dims 32 db + 8 q + 4 h + i of its row.
+  uint16_t *const op = a.out + (at_q * a.Hq + head) * D + 4 * h;
+#pragma unroll
+  for (int db = 0; db < kDims; ++db)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      u32x2 v;
+      v[0] = pack2<F16>(o[db][4 * q] * inv, o[db][4 * q + 1] * inv);
+      v[1] = pack2<F16>(o[db][4 * q + 2] * inv, o[db][4 * q + 3] * inv);
+      if (row0 + r < rows) *(u32x2 *)(op + 32 * db + 8 * q) = v;
+    }
 }
 
 template <int D, bool F16>
