@@ -147,7 +147,7 @@ __device__ __forceinline__ Rows find_rows(const GqaPackedArgs &a, int G, int ite
       int c = 0;
 #pragma unroll
       for (int i = 0; i < kWindow; ++i) c += longer(i, s);
-      return sgpr(wave_sum_i(c));
+      return wave_total(c);
     };
     const bool sorted = a.S <= kWave * kWindow;
     const int total = count(0);
@@ -172,12 +172,7 @@ __device__ __forceinline__ Rows find_rows(const GqaPackedArgs &a, int G, int ite
 #pragma unroll
     for (int i = 0; i < kWindow; ++i) {
       const int rest = stages ? longer(i, stages) : 0, c = (stages ? longer(i, stages - 1) : tiles(i)) - rest;
-      int incl = c;
-#pragma unroll
-      for (int o = 1; o < kWave; o <<= 1) {
-        const int y = __shfl_up(incl, o, kWave);
-        if (lane >= o) incl += y;
-      }
+      const int incl = wave_scan(c);
       const int here = __builtin_amdgcn_readlane(incl, 63);
       if (left < here) {
         const int at = sgpr(__builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > left)));

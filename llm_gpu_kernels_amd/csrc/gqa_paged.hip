@@ -33,6 +33,7 @@ constexpr int kStep = 32;       // keys of a step
 constexpr int kBlock = 16;      // keys that lie in one page
 constexpr int kRows = 16;       // query rows of an MFMA
 constexpr int kWaves = 4;       // per workgroup; only the LDS is shared out by it
+constexpr int kWindow = 4;      // sequences per lane whose lengths a wave holds
 
 // LDS of a wave: 32 rows of K, 32 of V, 16 of Q.  Row i's 16-byte chunk c lies
 // at place c ^ swizzle(i) of its row: the sixteen lanes that read one chunk of
@@ -156,40 +157,86 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
   uint8_t *const kst = smem + wave * kWaveLds<D>, *const vst = kst + kStage<D>, *const qst = vst + kStage<D>;
 
   // ---- the wave's range of the flat list ----
-  // Lengths of 64 sequences from `base` on, one per lane.
-  auto lengths_at = [&](int base) __attribute__((always_inline)) {
-    const int i = base + lane, raw = i < a.B ? a.lengths[i] : 0, len = max(0, min(raw, cap));
-    if (raw != len) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
-    return len;
+  // Lengths of 64 kWindow sequences from `window` on: i-th of a lane at 64 i + lane.
+  int window = 0, lens[kWindow];
+  auto load_lengths = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kWindow; ++i) {
+      const int at = window + kWave * i + lane;
+      lens[i] = at < a.B ? a.lengths[at] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kWindow; ++i) {
+      const int ok = max(0, min(lens[i], cap));
+      if (lens[i] != ok) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
+      lens[i] = ok;
+    }
   };
   auto steps_of = [](int len) __attribute__((always_inline)) { return (len + kStep - 1) / kStep; };
-  int window = 0, lens = lengths_at(0);
-  int sum = steps_of(lens);
-  for (int base = kWave; base < a.B; base += kWave) sum += steps_of(lengths_at(base));
-  const int all = sgpr(wave_sum_i(sum)) * heads;          // < 2^31, checked on the host
+  int sum = 0;
+  for (;; window += kWave * kWindow) {
+    load_lengths();
+#pragma unroll
+    for (int i = 0; i < kWindow; ++i) sum += steps_of(lens[i]);
+    if (window + kWave * kWindow >= a.B) break;
+  }
+  const int all = wave_total(sum) * heads;                // < 2^31, checked on the host
   const int per = (all + workers - 1) / workers;          // steps of a wave
   if ((int64_t)worker * per >= all) return;
   const int first = worker * per;
   int left = min(per, all - first);
-  int before = 0;  // steps in the sequences before the window
-  int incl;        // running sum within the window
-  for (;;) {
-    incl = steps_of(lens) * heads;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int y = __shfl_up(incl, o, kWave);
-      if (lane >= o) incl += y;
-    }
-    const int in_window = __builtin_amdgcn_readlane(incl, 63);
-    if (first < before + in_window) break;
-    before += in_window;
-    window += kWave;
-    if (window >= a.B) return;  // only if lengths change meanwhile
-    lens = lengths_at(window);
+  if (window > 0) {
+    window = 0;
+    load_lengths();
   }
-  const int at = sgpr(__builtin_ctzll(__builtin_amdgcn_ballot_w64(before + incl > first)));
-  int b = window + at, len = __builtin_amdgcn_readlane(lens, at), steps = steps_of(len);
-  const int rest = first - (before + (at ? __builtin_amdgcn_readlane(incl, at - 1 < 0 ? 0 : at - 1) : 0));
+  // The sequence where the range begins, and the steps before it.
+  int b = -1, len = 0, before = 0;
+  while (b < 0) {
+#pragma unroll
+    for (int i = 0; i < kWindow; ++i) {
+      const int incl = before + wave_scan(steps_of(lens[i]) * heads);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(incl > first);
+      if (b < 0) {
+        if (past) {
+          const int at = sgpr(__builtin_ctzll(past));
+          b = window + kWave * i + at;
+          len = __builtin_amdgcn_readlane(lens[i], at);
+          before = __builtin_amdgcn_readlane(incl, at) - steps_of(len) * heads;
+        } else {
+          before = __builtin_amdgcn_readlane(incl, 63);
+        }
+      }
+    }
+    if (b < 0) {
+      window += kWave * kWindow;
+      if (window >= a.B) return;  // only if lengths change meanwhile
+      load_lengths();
+    }
+  }
+  int steps = steps_of(len);
+  // The next sequence that has keys, from `from` on; -1 only if lengths change
+  // meanwhile.
+  auto next_sequence = [&](int from) __attribute__((always_inline)) {
+    for (;;) {
+      int found = -1;
+#pragma unroll
+      for (int i = 0; i < kWindow; ++i) {
+        const int lo = max(0, from - window - kWave * i);
+        const uint64_t some = __builtin_amdgcn_ballot_w64(lens[i] > 0);
+        const uint64_t later = lo < kWave ? some >> lo << lo : 0ull;
+        if (found < 0 && later) {
+          const int at = sgpr(__builtin_ctzll(later));
+          found = window + kWave * i + at;
+          len = __builtin_amdgcn_readlane(lens[i], at);
+        }
+      }
+      if (found >= 0) return found;
+      window += kWave * kWindow;
+      if (window >= a.B) return -1;
+      load_lengths();
+    }
+  };
+  const int rest = first - before;
   int head = rest / steps, s = rest % steps;
   const int per_page = a.page / kBlock;
   int page_at = 2 * s / per_page, block_at = 2 * s % per_page;  // of the next step's first block
@@ -221,25 +268,11 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
       s = page_at = block_at = 0;
       if (++head == heads) {
         head = 0;
-        int i = b - window + 1;
-        for (;;) {
-          const uint64_t some = __builtin_amdgcn_ballot_w64(lens > 0);
-          const uint64_t later = i < kWave ? some >> i << i : 0ull;
-          if (later) {
-            i = sgpr(__builtin_ctzll(later));
-            break;
-          }
-          window += kWave;
-          if (window >= a.B) {  // only if lengths change meanwhile
-            left = i = 0;
-            break;
-          }
-          lens = lengths_at(window);
-          i = 0;
-        }
-        if (left > 0) {
-          b = window + i;
-          len = __builtin_amdgcn_readlane(lens, i);
+        const int next = next_sequence(b + 1);
+        if (next < 0) {
+          left = 0;
+        } else {
+          b = next;
           steps = steps_of(len);
         }
       }
@@ -425,63 +458,68 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
   if (bad_page && lane == 0) atomicOr(a.status, GQA_STATUS_BAD_PAGE);
 }
 
-// Joins the pieces of a (sequence, head block), in the order of the keys: eight
-// groups of threads take every eighth piece of 32 dims of a row, and the eight
-// states are joined in order.  A piece without a usable key (m = -inf) has
-// weight 0, a row without any is 0; NaN passes through.  Sequences of length 0
-// get their zeros here.
-constexpr int kMergeThreads = 256;
+// Joins the pieces of a (sequence, head block), in the order of the keys: a thread
+// per element of O where there are enough of them, else groups of threads take
+// every groups-th piece and their states are joined in order; kBatch pieces' loads
+// are in flight together.  A piece without a usable key (m = -inf) has weight 0, a
+// row without any is 0; NaN passes through.  Sequences of length 0 get their zeros
+// here.
+constexpr int kMergeThreads = 512;
+constexpr int kBatch = 8;
+struct State {
+  float m, l, o;
+  __device__ __forceinline__ void join(float m2, float l2, float o2) {
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
+    const float wa = __builtin_amdgcn_exp2f(m - ref), wb = __builtin_amdgcn_exp2f(m2 - ref);
+    l = l * wa + l2 * wb;
+    o = o * wa + o2 * wb;
+    m = top;
+  }
+};
 template <bool F16>
-__global__ __launch_bounds__(kMergeThreads) void gqa_paged_merge(GqaPagedArgs a, int D) {
-  constexpr int kGroups = kMergeThreads / 32;
-  __shared__ float sm[kGroups], sl[kGroups], so[kGroups][32];
+__global__ __launch_bounds__(kMergeThreads) void gqa_paged_merge(GqaPagedArgs a, int chunk) {
+  __shared__ State states[kMergeThreads];
   const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows, heads = a.Hkv * blocks;
   const int b = blockIdx.x / heads, head = blockIdx.x % heads;
   const int kvh = head / blocks, part = head % blocks, rows = min(kRows, group - kRows * part);
-  const int d = threadIdx.x & 31, pg = threadIdx.x >> 5;
+  const int per_slot = min(group, kRows), groups = kMergeThreads / chunk;
+  const int e = blockIdx.y * chunk + threadIdx.x % chunk, mine = threadIdx.x / chunk;  // element, group
   const bool empty = a.lengths[b] <= 0;
   const int slot = a.pieces[2 * blockIdx.x], n = empty ? 0 : a.pieces[2 * blockIdx.x + 1];
   if (!empty && n == 0) return;  // written by the wave that had all of it
-  const int slices = D / 32, per_slot = min(group, kRows);
-  for (int item = blockIdx.y; item < rows * slices; item += gridDim.y) {
-    const int row = item / slices, at = 32 * (item % slices) + d;
-    uint16_t *const op = a.out + (((int64_t)b * a.Hq + kvh * group + kRows * part + row) * D + at);
-    if (empty) {
-      if (pg == 0) *op = 0;
-      continue;
-    }
-    float M = -INFINITY, den = 0.f, num = 0.f;
-    for (int i = pg; i < n; i += kGroups) {
+  const bool live = e < rows * a.D;
+  const int row = live ? e / a.D : 0, d = live ? e % a.D : 0;
+  uint16_t *const op = a.out + (((int64_t)b * a.Hq + kvh * group + kRows * part + row) * a.D + d);
+  if (empty) {
+    if (live && mine == 0) *op = 0;
+    return;
+  }
+  State st = {-INFINITY, 0.f, 0.f};
+  for (int i = mine; i < n; i += groups * kBatch) {
+    float m[kBatch], l[kBatch], x[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
       // The first piece's slot, then the first slot of each following wave.
-      const float *const pp = a.partial + ((int64_t)(i == 0 ? slot : (slot / 2 + i) * 2) * per_slot + row) * (D + 2);
-      const float m = pp[0], l = pp[1], x = pp[2 + at];
-      const float m_new = fmaxf(M, m), ref = m_new == -INFINITY ? 0.f : m_new;
-      const float wa = exp2f(M - ref), wb = exp2f(m - ref);
-      den = den * wa + l * wb;
-      num = num * wa + x * wb;
-      M = m_new;
+      const int at = min(i + j * groups, n - 1);
+      const float *const pp = a.partial + ((int64_t)(at == 0 ? slot : (slot / 2 + at) * 2) * per_slot + row) * (a.D + 2);
+      m[j] = pp[0];
+      l[j] = pp[1];
+      x[j] = pp[2 + d];
     }
-    __syncthreads();  // the last item's states have been read
-    if (d == 0) {
-      sm[pg] = M;
-      sl[pg] = den;
-    }
-    so[pg][d] = num;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (i + j * groups < n) st.join(m[j], l[j], x[j]);
+  }
+  if (groups > 1) {
+    states[threadIdx.x] = st;
     __syncthreads();
-    if (pg == 0) {
-      M = sm[0];
-      for (int i = 1; i < kGroups; ++i) M = fmaxf(M, sm[i]);
-      const float ref = M == -INFINITY ? 0.f : M;
-      den = num = 0.f;
-      for (int i = 0; i < kGroups; ++i) {
-        const float w = exp2f(sm[i] - ref);
-        den += w * sl[i];
-        num += w * so[i][d];
-      }
-      const float v = den == 0.f ? 0.f : num / den;
-      *op = (uint16_t)pack2<F16>(v, 0.f);
+    if (mine > 0) return;
+    for (int g = 1; g < groups; ++g) {
+      const State o = states[g * chunk + threadIdx.x];
+      st.join(o.m, o.l, o.o);
     }
   }
+  if (live) *op = (uint16_t)pack2<F16>(st.l == 0.f ? 0.f : st.o / st.l, 0.f);
 }
 
 __global__ void clear_word(uint32_t *w) { *w = 0; }
@@ -495,10 +533,13 @@ hipError_t launch(const GqaPagedArgs &a, int cus, hipStream_t s) {
   if (!attr) return hipErrorInvalidValue;
   hipLaunchKernelGGL(k, dim3(cus * kWorkgroups<D>), dim3(64 * kWaves), lds, s, a);
   const int group = a.Hq / a.Hkv, heads = a.Hkv * ((group + kRows - 1) / kRows);
-  // Few (sequence, head block)s: their rows and dims on workgroups of their own.
-  const int items = min(group, kRows) * (D / 32), pairs = a.B * heads;
-  const int spread = pairs >= 1024 ? 1 : min(items, (1024 + pairs - 1) / pairs);
-  hipLaunchKernelGGL(gqa_paged_merge<F16>, dim3(pairs, spread), dim3(kMergeThreads), 0, s, a, D);
+  // Elements per merge workgroup: all of a (sequence, head block) up to a thread
+  // each; fewer where that leaves CUs without a workgroup.
+  const int elements = min(group, kRows) * D, pairs = a.B * heads;
+  int chunk = kMergeThreads;
+  while (chunk > 32 && (chunk >= 2 * elements || (int64_t)pairs * ((elements + chunk - 1) / chunk) < cus)) chunk /= 2;
+  hipLaunchKernelGGL(gqa_paged_merge<F16>, dim3(pairs, (elements + chunk - 1) / chunk), dim3(kMergeThreads), 0, s, a,
+                     chunk);
   return hipGetLastError();
 }
 
