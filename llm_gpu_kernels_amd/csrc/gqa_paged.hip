@@ -151,7 +151,7 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = sgpr(threadIdx.x >> 6);
-  const int worker = sgpr(blockIdx.x * kWaves + wave), workers = gridDim.x * kWaves;
+  const int worker = sgpr(wave * gridDim.x + blockIdx.x), workers = gridDim.x * kWaves;  // few steps: on many CUs
   const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows, heads = a.Hkv * blocks;
   const int cap = a.M * a.page;
   uint8_t *const kst = smem + wave * kWaveLds<D>, *const vst = kst + kStage<D>, *const qst = vst + kStage<D>;
@@ -458,68 +458,85 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
   if (bad_page && lane == 0) atomicOr(a.status, GQA_STATUS_BAD_PAGE);
 }
 
-// Joins the pieces of a (sequence, head block), in the order of the keys: a thread
-// per element of O where there are enough of them, else groups of threads take
-// every groups-th piece and their states are joined in order; kBatch pieces' loads
-// are in flight together.  A piece without a usable key (m = -inf) has weight 0, a
-// row without any is 0; NaN passes through.  Sequences of length 0 get their zeros
-// here.
-constexpr int kMergeThreads = 512;
+// Joins the pieces of a (sequence, head block), in the order of the keys.  A thread
+// takes two elements of O of all pieces, or, where there are too few elements to
+// fill the chip, of every groups-th piece, and the groups are joined in order;
+// kBatch pieces' loads are in flight together.  A piece without a usable key (m =
+// -inf) has weight 0, a row without any is 0; NaN passes through.  Sequences of
+// length 0 get their zeros here.
+constexpr int kMergeThreads = 256;
 constexpr int kBatch = 8;
 struct State {
-  float m, l, o;
-  __device__ __forceinline__ void join(float m2, float l2, float o2) {
-    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
-    const float wa = __builtin_amdgcn_exp2f(m - ref), wb = __builtin_amdgcn_exp2f(m2 - ref);
-    l = l * wa + l2 * wb;
-    o = o * wa + o2 * wb;
-    m = top;
-  }
+  float m, l;
+  f32x2_t o;
 };
 template <bool F16>
 __global__ __launch_bounds__(kMergeThreads) void gqa_paged_merge(GqaPagedArgs a, int chunk) {
   __shared__ State states[kMergeThreads];
   const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows, heads = a.Hkv * blocks;
   const int b = blockIdx.x / heads, head = blockIdx.x % heads;
-  const int kvh = head / blocks, part = head % blocks, rows = min(kRows, group - kRows * part);
-  const int per_slot = min(group, kRows), groups = kMergeThreads / chunk;
-  const int e = blockIdx.y * chunk + threadIdx.x % chunk, mine = threadIdx.x / chunk;  // element, group
   const bool empty = a.lengths[b] <= 0;
   const int slot = a.pieces[2 * blockIdx.x], n = empty ? 0 : a.pieces[2 * blockIdx.x + 1];
   if (!empty && n == 0) return;  // written by the wave that had all of it
+  const int kvh = head / blocks, part = head % blocks, rows = min(kRows, group - kRows * part);
+  const int per_slot = min(group, kRows), groups = kMergeThreads / chunk;
+  const int e = 2 * (blockIdx.y * chunk + threadIdx.x % chunk), mine = threadIdx.x / chunk;  // element, group
+  const int half = a.D == 128 ? 7 : 6;                                                       // log2 D
   const bool live = e < rows * a.D;
-  const int row = live ? e / a.D : 0, d = live ? e % a.D : 0;
-  uint16_t *const op = a.out + (((int64_t)b * a.Hq + kvh * group + kRows * part + row) * a.D + d);
+  const int row = live ? e >> half : 0, d = e & (a.D - 1);
+  uint32_t *const op = (uint32_t *)(a.out + (((int64_t)b * a.Hq + kvh * group + kRows * part + row) * a.D + d));
   if (empty) {
     if (live && mine == 0) *op = 0;
     return;
   }
-  State st = {-INFINITY, 0.f, 0.f};
+  // Piece 0 lies in `slot`, the i-th in the first slot of the i-th following wave
+  // (32-bit offsets: the states take 35 MB at most).
+  const uint32_t row_bytes = (uint32_t)(a.D + 2) * 4, slot_bytes = (uint32_t)per_slot * row_bytes;
+  const uint8_t *const base = (const uint8_t *)a.partial;
+  const uint32_t own = (uint32_t)row * row_bytes, first = (uint32_t)(slot / 2 * 2) * slot_bytes + own;
+  State st = {-INFINITY, 0.f, f32x2_t{0.f, 0.f}};
   for (int i = mine; i < n; i += groups * kBatch) {
-    float m[kBatch], l[kBatch], x[kBatch];
+    f32x2_t ml[kBatch], x[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      // The first piece's slot, then the first slot of each following wave.
       const int at = min(i + j * groups, n - 1);
-      const float *const pp = a.partial + ((int64_t)(at == 0 ? slot : (slot / 2 + at) * 2) * per_slot + row) * (a.D + 2);
-      m[j] = pp[0];
-      l[j] = pp[1];
-      x[j] = pp[2 + d];
+      const uint32_t off = at ? first + (uint32_t)at * 2 * slot_bytes : (uint32_t)slot * slot_bytes + own;
+      ml[j] = *(const f32x2_t *)(base + off);
+      x[j] = *(const f32x2_t *)(base + off + 8 + 4 * d);
     }
+    float top = st.m;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (i + j * groups < n) st.join(m[j], l[j], x[j]);
+    for (int j = 0; j < kBatch; ++j) top = i + j * groups < n ? fmaxf(top, ml[j][0]) : top;
+    const float ref = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(st.m - ref);
+    st.m = top;
+    st.l *= old;
+    st.o[0] *= old;
+    st.o[1] *= old;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (i + j * groups >= n) break;
+      const float w = __builtin_amdgcn_exp2f(ml[j][0] - ref);
+      st.l = __builtin_fmaf(w, ml[j][1], st.l);
+      st.o[0] = __builtin_fmaf(w, x[j][0], st.o[0]);
+      st.o[1] = __builtin_fmaf(w, x[j][1], st.o[1]);
+    }
   }
   if (groups > 1) {
     states[threadIdx.x] = st;
     __syncthreads();
     if (mine > 0) return;
     for (int g = 1; g < groups; ++g) {
-      const State o = states[g * chunk + threadIdx.x];
-      st.join(o.m, o.l, o.o);
+      const State y = states[g * chunk + threadIdx.x];
+      const float top = fmaxf(st.m, y.m), ref = top == -INFINITY ? 0.f : top;
+      const float wa = __builtin_amdgcn_exp2f(st.m - ref), wb = __builtin_amdgcn_exp2f(y.m - ref);
+      st.m = top;
+      st.l = st.l * wa + y.l * wb;
+      st.o[0] = st.o[0] * wa + y.o[0] * wb;
+      st.o[1] = st.o[1] * wa + y.o[1] * wb;
     }
   }
-  if (live) *op = (uint16_t)pack2<F16>(st.l == 0.f ? 0.f : st.o / st.l, 0.f);
+  const float inv = st.l == 0.f ? 0.f : 1.0f / st.l;
+  if (live) *op = pack2<F16>(st.o[0] * inv, st.o[1] * inv);
 }
 
 __global__ void clear_word(uint32_t *w) { *w = 0; }
@@ -533,13 +550,13 @@ hipError_t launch(const GqaPagedArgs &a, int cus, hipStream_t s) {
   if (!attr) return hipErrorInvalidValue;
   hipLaunchKernelGGL(k, dim3(cus * kWorkgroups<D>), dim3(64 * kWaves), lds, s, a);
   const int group = a.Hq / a.Hkv, heads = a.Hkv * ((group + kRows - 1) / kRows);
-  // Elements per merge workgroup: all of a (sequence, head block) up to a thread
-  // each; fewer where that leaves CUs without a workgroup.
-  const int elements = min(group, kRows) * D, pairs = a.B * heads;
+  // Threads per piece in a merge workgroup: all of a (sequence, head block), two
+  // elements each; fewer, and pieces shared out over groups, while that leaves CUs
+  // without a workgroup.
+  const int need = min(group, kRows) * D / 2, pairs = a.B * heads;
   int chunk = kMergeThreads;
-  while (chunk > 32 && (chunk >= 2 * elements || (int64_t)pairs * ((elements + chunk - 1) / chunk) < cus)) chunk /= 2;
-  hipLaunchKernelGGL(gqa_paged_merge<F16>, dim3(pairs, (elements + chunk - 1) / chunk), dim3(kMergeThreads), 0, s, a,
-                     chunk);
+  while (chunk > 16 && (chunk >= 2 * need || (int64_t)pairs * ((need + chunk - 1) / chunk) < cus)) chunk /= 2;
+  hipLaunchKernelGGL(gqa_paged_merge<F16>, dim3(pairs, (need + chunk - 1) / chunk), dim3(kMergeThreads), 0, s, a, chunk);
   return hipGetLastError();
 }
 
