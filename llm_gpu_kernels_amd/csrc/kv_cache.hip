@@ -20,27 +20,37 @@ static_assert(KV_MAX_SEQUENCES <= kPlanThreads, "a thread per row");
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Exclusive sum over the workgroup's threads and the total.
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *lds, uint64_t *total) {
+// Exclusive sums over the workgroup's threads of two numbers and of a flag, and the
+// totals.
+struct Scan {
+  int a, b, flag, all_a, all_b, all_flag;
+};
+struct ScanLds {
+  int a[kWaves], b[kWaves], flag[kWaves];
+};
+__device__ __forceinline__ Scan block_scan(int a, int b, bool flag, ScanLds *lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t x = v;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const uint64_t y = __shfl_up(x, o, kWave);
-    if (lane >= o) x += y;
-  }
+  const int ia = wave_scan(a), ib = wave_scan(b);
+  const uint64_t set = __builtin_amdgcn_ballot_w64(flag);
   __syncthreads();  // the last scan's sums have been read
-  if (lane == kWave - 1) lds[wave] = x;
+  if (lane == kWave - 1) {
+    lds->a[wave] = ia;
+    lds->b[wave] = ib;
+    lds->flag[wave] = (int)__popcll(set);
+  }
   __syncthreads();
-  uint64_t before = 0, all = 0;
+  Scan r = {ia - a, ib - b, (int)__popcll(set & lanemask_lt()), 0, 0, 0};
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    const uint64_t s = lds[w];
-    if (w < wave) before += s;
-    all += s;
+    const int wa = lds->a[w], wb = lds->b[w], wf = lds->flag[w];
+    r.a += w < wave ? wa : 0;
+    r.b += w < wave ? wb : 0;
+    r.flag += w < wave ? wf : 0;
+    r.all_a += wa;
+    r.all_b += wb;
+    r.all_flag += wf;
   }
-  *total = all;
-  return before + x - v;
+  return r;
 }
 
 // One bit per page of a thread's eight: in use.
@@ -62,15 +72,21 @@ __device__ __forceinline__ uint32_t valid_bits(const KvState &s, int first) {
   return n >= kScanPages ? 0xffu : n > 0 ? (1u << n) - 1u : 0u;
 }
 
-// Pages, lengths and slots of a reserve.  Thread s is row s.
+// Pages, lengths and slots of a reserve.  Thread s is row s.  One workgroup, so
+// what bounds it is the chain of dependent loads: the first pages' holders are
+// loaded beside the rows, and short lists of pages stay in LDS.
+constexpr int kListLds = 4096;
 __global__ __launch_bounds__(kPlanThreads) void kv_reserve_plan(KvState s, const int32_t *counts, int stride) {
-  __shared__ uint64_t sums[kWaves];
-  __shared__ int last_page[kPlanThreads], need_at[kPlanThreads + 1], row_len[kPlanThreads];
+  __shared__ ScanLds sums;
+  __shared__ __attribute__((aligned(16))) int last_page[kPlanThreads];
+  __shared__ int need_at[kPlanThreads], row_len[kPlanThreads];
   __shared__ int copy_at[kPlanThreads];  // the row's copy's number, -1: none
+  __shared__ int list_lds[kListLds];
   const int row = threadIdx.x;
   const bool live = row < s.sequences;
   const int cap = s.max_pages * s.page_size;  // < 2^31
   int len = live ? s.lengths[row] : 0, count = live ? counts[row] : 0;
+  uint32_t used0 = row * kScanPages < s.pages ? used_bits(s, row * kScanPages) : 0u;
   uint32_t bad = 0;
   if (len < 0 || len > cap) {
     bad |= KV_STATUS_BAD_STATE;
@@ -96,39 +112,41 @@ __global__ __launch_bounds__(kPlanThreads) void kv_reserve_plan(KvState s, const
   }
   last_page[row] = last;
   row_len[row] = len;
-  __syncthreads();
   bool copy = last >= 0;
-  if (copy) {
-    int growing = 0;
-    bool later = false;
-    for (int j = 0; j < s.sequences; ++j) {
-      const bool same = last_page[j] == last;
-      growing += same;
-      later |= same && j > row;
+  __syncthreads();
+  if (__builtin_amdgcn_ballot_w64(copy)) {
+    int growing = 0, later = -1;  // rows that grow on this page, the last of them
+#pragma unroll 4
+    for (int j = 0; j < s.sequences; j += 4) {
+      const int4 p = *(const int4 *)(last_page + j);
+      growing += (p.x == last) + (p.y == last) + (p.z == last) + (p.w == last);
+      later = p.x == last ? j : later;
+      later = p.y == last ? j + 1 : later;
+      later = p.z == last ? j + 2 : later;
+      later = p.w == last ? j + 3 : later;
     }
-    copy = growing < holders || later;
+    copy = copy && (growing < holders || later > row);
   }
   const int used = ceil_div(len, s.page_size);
-  const int need = ceil_div(len + count, s.page_size) - used + copy;
-  uint64_t all, copies;
-  const uint64_t mine = block_scan((uint64_t)need << 32 | (uint32_t)count, sums, &all);
-  const int my_copy = (int)block_scan(copy, sums, &copies);
-  const int total = (int)(all >> 32), tokens = (int)(all & 0xffffffffu);
+  const int need = ceil_div(len + count, s.page_size) - used + copy;  // <= 2^16 + 1
+  const Scan sc = block_scan(need, count, copy, &sums);  // sums below 2^27 and 2^31
+  const int total = sc.all_a, tokens = sc.all_b;
   if (tokens > s.max_tokens) bad |= KV_STATUS_BAD_COUNT;
-  need_at[row] = (int)(mine >> 32);
-  if (row == 0) need_at[kPlanThreads] = total;
-  copy_at[row] = copy ? my_copy : -1;
+  need_at[row] = sc.a;
+  copy_at[row] = copy ? sc.flag : -1;
 
   bool refuse = __syncthreads_or(bad != 0);
+  int32_t *const list = total <= kListLds ? list_lds : s.list;
   if (!refuse && total > 0) {
     int found = 0;
     for (int base = 0; base < s.pages && found < total; base += kPlanThreads * kScanPages) {
       const int first = base + row * kScanPages;
-      uint32_t free_bits = first < s.pages ? ~used_bits(s, first) & valid_bits(s, first) : 0u;
-      uint64_t n;
-      int at = found + (int)block_scan(__popc(free_bits), sums, &n);
-      for (; free_bits && at < total; free_bits &= free_bits - 1, ++at) s.list[at] = first + __ffs(free_bits) - 1;
-      found += (int)n;
+      if (base > 0) used0 = first < s.pages ? used_bits(s, first) : 0u;
+      uint32_t free_bits = ~used0 & valid_bits(s, first);
+      const Scan f = block_scan(__popc(free_bits), 0, false, &sums);
+      int at = found + f.a;
+      for (; free_bits && at < total; free_bits &= free_bits - 1, ++at) list[at] = first + __ffs(free_bits) - 1;
+      found += f.all_a;
     }
     if (found < total) {
       bad |= KV_STATUS_OUT_OF_PAGES;
@@ -150,7 +168,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_reserve_plan(KvState s, const
       if (need_at[mid] <= i) lo = mid;
       else hi = mid - 1;
     }
-    const int page = s.list[i], nth = i - need_at[lo], c = copy_at[lo], l = row_len[lo];
+    const int page = list[i], nth = i - need_at[lo], c = copy_at[lo], l = row_len[lo];
     int column = ceil_div(l, s.page_size) + nth;
     if (c >= 0) {
       --column;  // the copy takes the last page's place
@@ -165,11 +183,11 @@ __global__ __launch_bounds__(kPlanThreads) void kv_reserve_plan(KvState s, const
   }
   if (live) {
     s.lengths[row] = len + count;
-    s.starts[row] = (int)(mine & 0xffffffffu);
+    s.starts[row] = sc.b;
   }
   if (row == 0) {
     s.starts[s.sequences] = tokens;
-    *s.num_moves = (int)copies;
+    *s.num_moves = sc.all_flag;
   }
 }
 
@@ -261,30 +279,31 @@ __device__ __forceinline__ int row_pages(const KvState &s, int row) {
   return ceil_div(len, s.page_size);
 }
 
-// Fork: pair i may go ahead.  Rows are as before the call, since lengths are
-// written by a later launch.
-__device__ __forceinline__ bool fork_ok(const KvState &s, const int32_t *src, const int32_t *dst, int i, bool report) {
-  const int a = src[i], b = dst[i];
-  if (a < 0 || b < 0) return false;
-  uint32_t bad = 0;
-  if (a >= s.sequences || b >= s.sequences) {
-    bad = KV_STATUS_BAD_ROW;
-  } else {
-    bool taken = s.lengths[b] != 0;
-    for (int j = 0; j < i && !taken; ++j) taken = dst[j] == b && src[j] >= 0 && src[j] < s.sequences;
-    if (taken) bad = KV_STATUS_NOT_EMPTY;
-  }
-  if (bad && report) atomicOr(s.status, bad);
-  return bad == 0;
+// A pair of a fork: 0 if it may go ahead, else why not (KV_STATUS_*; ~0: left out
+// by the caller).  Rows are as before the call: lengths are written by a later
+// launch.  `named` says that an earlier pair that goes by valid rows names dst.
+__device__ __forceinline__ bool fork_rows_valid(const KvState &s, int a, int b) {
+  return a >= 0 && b >= 0 && a < s.sequences && b < s.sequences;
+}
+__device__ __forceinline__ uint32_t fork_status(const KvState &s, int a, int b, bool named) {
+  if (a < 0 || b < 0) return ~0u;
+  if (!fork_rows_valid(s, a, b)) return KV_STATUS_BAD_ROW;
+  return named || s.lengths[b] != 0 ? KV_STATUS_NOT_EMPTY : 0u;
 }
 
 // One workgroup per pair: the table row, and one more holder of its pages.
 __global__ __launch_bounds__(kWideThreads) void kv_fork_rows(KvState s, const int32_t *src, const int32_t *dst) {
-  const int i = blockIdx.x;
-  if (!fork_ok(s, src, dst, i, threadIdx.x == 0)) return;
-  const int n = row_pages(s, src[i]);
-  const int32_t *const from = s.tables + (int64_t)src[i] * s.max_pages;
-  int32_t *const to = s.tables + (int64_t)dst[i] * s.max_pages;
+  const int i = blockIdx.x, a = src[i], b = dst[i];
+  bool named = false;
+  for (int j = threadIdx.x; j < i; j += kWideThreads) named |= dst[j] == b && fork_rows_valid(s, src[j], b);
+  const uint32_t why = fork_status(s, a, b, __syncthreads_or(named));
+  if (why) {
+    if (threadIdx.x == 0 && why != ~0u) atomicOr(s.status, why);
+    return;
+  }
+  const int n = row_pages(s, a);
+  const int32_t *const from = s.tables + (int64_t)a * s.max_pages;
+  int32_t *const to = s.tables + (int64_t)b * s.max_pages;
   for (int c = threadIdx.x; c < n; c += kWideThreads) {
     const int p = from[c];
     to[c] = p;
@@ -292,26 +311,28 @@ __global__ __launch_bounds__(kWideThreads) void kv_fork_rows(KvState s, const in
     else atomicOr(s.status, KV_STATUS_BAD_STATE);
   }
 }
+// A thread per pair; the first pair that names a row by valid rows owns it.
 __global__ __launch_bounds__(kPlanThreads) void kv_fork_lengths(KvState s, const int32_t *src, const int32_t *dst, int n) {
-  const int i = threadIdx.x;
-  int len = -1;
-  if (i < n && fork_ok(s, src, dst, i, false)) {
-    len = s.lengths[src[i]];
-    if (len > s.max_pages * s.page_size) len = -1;
-  }
+  __shared__ int owner[kPlanThreads];
+  const int i = threadIdx.x, a = i < n ? src[i] : -1, b = i < n ? dst[i] : -1;
+  const bool valid = fork_rows_valid(s, a, b);
+  const int len = valid ? s.lengths[a] : -1, old = valid ? s.lengths[b] : -1;
+  owner[i] = kPlanThreads;
   __syncthreads();  // every length has been read
-  if (len >= 0) s.lengths[dst[i]] = len;
+  if (valid) atomicMin(owner + b, i);
+  __syncthreads();
+  if (valid && owner[b] == i && old == 0 && len >= 0 && len <= s.max_pages * s.page_size) s.lengths[b] = len;
 }
 
 __global__ __launch_bounds__(kWideThreads) void kv_free(KvState s, const int32_t *rows) {
   const int row = rows[blockIdx.x];
-  if (row < 0) return;
+  bool named = false;  // before
+  for (int j = threadIdx.x; j < (int)blockIdx.x; j += kWideThreads) named |= rows[j] == row;
+  if (__syncthreads_or(named) || row < 0) return;
   if (row >= s.sequences) {
     if (threadIdx.x == 0) atomicOr(s.status, KV_STATUS_BAD_ROW);
     return;
   }
-  for (int j = 0; j < (int)blockIdx.x; ++j)
-    if (rows[j] == row) return;  // named before
   const int n = row_pages(s, row);
   int32_t *const table = s.tables + (int64_t)row * s.max_pages;
   for (int c = threadIdx.x; c < n; c += kWideThreads) {
@@ -327,33 +348,29 @@ __global__ __launch_bounds__(kWideThreads) void kv_free(KvState s, const int32_t
 // Moves of a compaction: with U pages in use, the free pages below U in order
 // take the used pages from U on in order.
 __global__ __launch_bounds__(kPlanThreads) void kv_compact_plan(KvState s) {
-  __shared__ uint64_t sums[kWaves];
-  uint64_t n = 0;
+  __shared__ ScanLds sums;
+  const int chunk = kPlanThreads * kScanPages, mine = threadIdx.x * kScanPages;
   int used = 0;
-  for (int base = 0; base < s.pages; base += kPlanThreads * kScanPages) {
-    const int first = base + threadIdx.x * kScanPages;
-    if (first < s.pages) used += __popc(used_bits(s, first));
+  uint32_t bits = 0;
+  for (int base = 0; base < s.pages; base += chunk) {
+    bits = base + mine < s.pages ? used_bits(s, base + mine) : 0u;
+    used += __popc(bits);
   }
-  (void)block_scan(used, sums, &n);
-  const int U = (int)n;
+  const int U = block_scan(used, 0, false, &sums).all_a;
   // Free pages below U and used ones from U on, numbered.
   int holes = 0, movers = 0;
-  for (int base = 0; base < s.pages; base += kPlanThreads * kScanPages) {
-    const int first = base + threadIdx.x * kScanPages;
-    uint32_t hole = 0, mover = 0;
-    if (first < s.pages) {
-      const uint32_t u = used_bits(s, first);
-      const int k = U - first;
-      const uint32_t below = k >= kScanPages ? 0xffu : k > 0 ? (1u << k) - 1u : 0u;
-      hole = ~u & below & valid_bits(s, first);
-      mover = u & ~below;
-    }
-    const uint64_t at = block_scan((uint64_t)__popc(hole) << 32 | __popc(mover), sums, &n);
-    int h = holes + (int)(at >> 32), m = movers + (int)(at & 0xffffffffu);
+  for (int base = 0; base < s.pages; base += chunk) {
+    const int first = base + mine;
+    if (s.pages > chunk) bits = first < s.pages ? used_bits(s, first) : 0u;
+    const int k = U - first;
+    const uint32_t below = k >= kScanPages ? 0xffu : k > 0 ? (1u << k) - 1u : 0u;
+    uint32_t hole = ~bits & below & valid_bits(s, first), mover = bits & ~below;
+    const Scan sc = block_scan(__popc(hole), __popc(mover), false, &sums);
+    int h = holes + sc.a, m = movers + sc.b;
     for (; hole; hole &= hole - 1) s.move_dst[h++] = first + __ffs(hole) - 1;
     for (; mover; mover &= mover - 1) s.move_src[m++] = first + __ffs(mover) - 1;
-    holes += (int)(n >> 32);
-    movers += (int)(n & 0xffffffffu);
+    holes += sc.all_a;
+    movers += sc.all_b;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < movers; i += kPlanThreads) {

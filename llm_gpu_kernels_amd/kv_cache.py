@@ -16,7 +16,7 @@ import ctypes
 import torch
 
 from . import _native as N
-from .attention import _check_int32, _check_rows, _token_stride
+from .attention import _check_int32
 
 __all__ = ["PagedKVCache"]
 
@@ -83,6 +83,21 @@ class PagedKVCache:
     def _stream(self):
         return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
 
+    def _token_stride(self, t, name):
+        """Token stride of new keys or values (alignment is checked by the library)."""
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        heads, dim = self.kv_heads, self.head_dim
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != dim or t.dtype != self.dtype or t.device != self.device:
+            raise ValueError(f"{name} must be {self.dtype} [n, {heads}, {dim}] on {self.device}")
+        s0, s1, s2 = t.stride()
+        if shape[0] == 0:
+            return heads * dim
+        if s2 != 1 or (heads > 1 and s1 != dim):
+            raise ValueError(f"{name} must have inner strides ({dim}, 1)")
+        return s0 if shape[0] > 1 else heads * dim
+
     def _rows(self, t, name):
         if not isinstance(t, torch.Tensor) or t.ndim != 1:
             raise ValueError(f"{name} must be an int32 tensor [n]")
@@ -110,16 +125,11 @@ class PagedKVCache:
         """Write token i's keys and values ([n, kv_heads, head_dim], the heads of
         a token side by side) to ``slots[i]`` of a layer, for every i < n whose
         slot is not -1."""
-        for t, name in ((k, "k"), (v, "v")):
-            _check_rows(t, name)
-            if t.dtype != self.dtype or tuple(t.shape[1:]) != (self.kv_heads, self.head_dim):
-                raise ValueError(f"{name} must be {self.dtype} [n, {self.kv_heads}, {self.head_dim}]")
-            if t.device != self.device:
-                raise ValueError(f"{name} must be on {self.device}")
+        ks, vs = self._token_stride(k, "k"), self._token_stride(v, "v")
         if k.shape[0] != v.shape[0]:
             raise ValueError("k and v must have the same number of tokens")
-        N.check(N.lib().kv_cache_append(self._cache, int(layer), k.data_ptr(), v.data_ptr(), _token_stride(k, "k"),
-                                        _token_stride(v, "v"), k.shape[0], self._stream()), "append")
+        N.check(N.lib().kv_cache_append(self._cache, int(layer), k.data_ptr(), v.data_ptr(), ks, vs, k.shape[0],
+                                        self._stream()), "append")
 
     def fork(self, src, dst):
         """Row ``dst[i]``, which must be empty, starts as a copy of row ``src[i]``
