@@ -111,9 +111,13 @@ int validate_packed_sizes(const gqa_packed_desc *d) {
   using moe::capi_fail;
   if (!d) return capi_fail(MOE_EINVAL, "null descriptor");
   if (const int rc = validate_heads(d->Hq, d->Hkv, d->D, d->dtype)) return rc;
-  if (d->N < 0 || (int64_t)d->N * (d->Hq / d->Hkv) >= 1LL << 30)
-    return capi_fail(MOE_EINVAL, "N must be >= 0 and N * Hq / Hkv < 2^30 (got %d)", d->N);
   if (d->S < 0 || d->S > (1 << 20)) return capi_fail(MOE_EINVAL, "S must be in [0, 2^20] (got %d)", d->S);
+  // The kernel divides numbers of query rows below 2^26, and its workgroups (one
+  // per 256 query rows and one per sequence) are counted in 31 bits.
+  if (d->N < 0 || (int64_t)d->N * (d->Hq / d->Hkv) + 256 >= 1LL << 26 ||
+      ((int64_t)d->N * (d->Hq / d->Hkv) / 256 + d->S + 8) * d->Hkv >= 1LL << 30)
+    return capi_fail(MOE_EINVAL, "N must be >= 0, N * Hq / Hkv below 2^26 - 256 and N * Hq / 256 + S * Hkv below 2^30 (got %d)",
+                     d->N);
   return MOE_OK;
 }
 
@@ -130,7 +134,7 @@ int validate_packed(const gqa_packed_desc *d) {
   return rc;
 }
 
-size_t packed_workspace(const gqa_packed_desc *) { return 256; }
+size_t packed_workspace(const gqa_packed_desc *d) { return moe::gqa_packed_workspace(d->N, d->Hq, d->Hkv, d->S); }
 
 int validate_paged_sizes(const gqa_paged_desc *d) {
   using moe::capi_fail;
@@ -210,7 +214,9 @@ int gqa_packed_plan_create(gqa_packed_plan **out, const gqa_packed_desc *d) {
   if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");
   p->a = moe::GqaPackedArgs{(const uint16_t *)d->q, (const uint16_t *)d->k, (const uint16_t *)d->v, (uint16_t *)d->out,
                             d->starts, d->q_stride, d->k_stride, d->v_stride, d->N, d->S, d->Hq, d->Hkv, d->D, d->dtype,
-                            scale_or_default(d->scale, d->D), (uint32_t *)d->workspace};
+                            scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0};
+  moe::gqa_packed_bind(&p->a, d->workspace);
+  moe::gqa_packed_constants(&p->a);
   p->device = dev;
   *out = p;
   return MOE_OK;

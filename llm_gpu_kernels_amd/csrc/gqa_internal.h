@@ -50,7 +50,15 @@ struct GqaPackedArgs {
   int N, S, Hq, Hkv, D, dtype;
   float scale;
   uint32_t *status;
+  int32_t *num_tiles, *tiles, *tile_sums;  // workspace
+  // Set by gqa_packed_constants: the group Hq / Hkv; log2 of the XCDs that share a
+  // class of KV heads, and a class's heads; ceil(2^32 / G).
+  int G, class_xcds, per_class;
+  uint32_t G_magic;
 };
+size_t gqa_packed_workspace(int N, int Hq, int Hkv, int S);
+void gqa_packed_bind(GqaPackedArgs *a, void *workspace);
+void gqa_packed_constants(GqaPackedArgs *a);
 hipError_t launch_gqa_packed(const GqaPackedArgs &a, hipStream_t s);
 
 // One new token per sequence over a paged cache (gqa_paged.hip).

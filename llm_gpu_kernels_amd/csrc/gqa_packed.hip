@@ -20,6 +20,7 @@
 // K and V come in stages of 64 keys, global -> LDS in whole rows (buffer loads
 // with an LDS destination; keys behind the sequence's end read as zeros), three
 // stages ahead in a ring of four, with one barrier per stage.
+#include <stdlib.h>
 #include "common.h"
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"
@@ -31,12 +32,10 @@ using namespace gqa;
 
 namespace {
 
-constexpr int kTileRows = 256;  // query rows of a workgroup
-constexpr int kWaves = 8;
-constexpr int kWaveRows = 32;
-constexpr int kStageKeys = 64;
-constexpr int kSlots = 4;
-constexpr int kWindow = 4;      // sequences per lane that a search looks at together
+constexpr int kWaveRows = 32;   // query rows of a wave
+constexpr int kStageKeys = 32;
+template <int WAVES> constexpr int kTileRows = kWaveRows * WAVES;  // of a workgroup
+template <int WAVES> constexpr int kSlots = WAVES == 4 ? 5 : 8;    // of the ring of stages
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 // Row i of a stage's K (V) tile holds its 16-byte chunk c at place c ^ swizzle(i):
@@ -79,6 +78,11 @@ __device__ __forceinline__ u32x4 lds_b128(uint32_t at) {
   return u32x4{at, 0u, 0u, 0u};
 #endif
 }
+__device__ __forceinline__ void lds_write_b64(uint32_t at, u32x2 v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  *(GQA_AS_LDS u32x2 *)at = v;
+#endif
+}
 // Within each group of 16 lanes, lane 4a + b receives element b of the 8-byte
 // rows addressed by lanes a, a + 4, a + 8, a + 12.
 __device__ __forceinline__ u32x2 lds_tr16(uint32_t at) {
@@ -113,78 +117,111 @@ __device__ __forceinline__ float element(u32x4 x, int i) {
   return to_f32<F16>(i & 1 ? x[i / 2] >> 16 : x[i / 2] & 0xffffu);
 }
 
-// A workgroup's rows: tile `tile` (kTileRows query rows) of the sequence that
-// starts at token `start` and has `len`.
+// A workgroup's rows: tile `tile` of the sequence that starts at token `start` and
+// has `len`.
 struct Rows {
-  int start, len, tile;
+  int start, len, tile, none;
 };
 
-// The item-th tile of all sequences.  Up to 64 kWindow sequences: in descending
-// number of 64-key stages (the longest start first), found by bisection over
-// that number, with every wave counting for itself: a sequence of n tokens has
-// T = ceil(n G / 256) tiles, tile t sees min(n, (256 t + 255) / G + 1) keys, so
-// T - min(T, G s / 4) of them have more than s stages.  More sequences: in
-// order, since no one tile weighs much there.  len 0: no such tile.
-__device__ __forceinline__ Rows find_rows(const GqaPackedArgs &a, int G, int item) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < a.S; base += kWave * kWindow) {
-    int b[kWindow], n[kWindow];
+// n / d for n < 2^26, d <= 64 and magic = ceil(2^32 / d).
+__device__ __forceinline__ int quotient(int n, int d, uint32_t magic) {
+  return d == 1 ? n : (int)__umulhi((uint32_t)n, magic);
+}
+
+// Sequence s, its bounds forced into [0, N].
+__device__ __forceinline__ Rows sequence(const GqaPackedArgs &a, int s) {
+  const int lo = a.starts[s], hi = a.starts[s + 1], b = max(0, min(lo, a.N));
+  if (lo < 0 || hi < lo || hi > a.N) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
+  return Rows{b, max(0, min(hi, a.N) - b), 0, 0};
+}
+
+// The list of all sequences' tiles of R rows, those that see the most keys first
+// (the last workgroups to run are short then).  One workgroup sorts them by counting
+// in kClasses classes of equally many stages; the order within a class does not
+// matter to any result.  A search of every workgroup for its own tile took 3 to 5 us
+// of its 10 to 50.
+constexpr int kPlanThreads = 1024;
+constexpr int kClasses = kPlanThreads;
+constexpr int kPlanLds = 2048;  // sequences whose tile sums lie in LDS
+__device__ __forceinline__ int plan_scan(int x, int *lds, int *total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, incl = wave_scan(x);
+  __syncthreads();  // the last scan's sums have been read
+  if (lane == kWave - 1) lds[wave] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < kWindow; ++i) {
-      const int s = base + kWave * i + lane;
-      const int lo = s < a.S ? a.starts[s] : 0, hi = s < a.S ? a.starts[s + 1] : 0;
-      b[i] = max(0, min(lo, a.N));
-      n[i] = max(0, min(hi, a.N) - b[i]);
-      if (lo < 0 || hi < lo || hi > a.N) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
-    }
-    auto tiles = [&](int i) { return (n[i] * G + kTileRows - 1) / kTileRows; };
-    auto longer = [&](int i, int s) {
-      const int T = tiles(i);
-      return n[i] > kStageKeys * s ? T - min(T, G * s / 4) : 0;
-    };
-    static_assert(kTileRows == 4 * kStageKeys, "G s / 4 above");
-    auto count = [&](int s) {
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < kWindow; ++i) c += longer(i, s);
-      return wave_total(c);
-    };
-    const bool sorted = a.S <= kWave * kWindow;
-    const int total = count(0);
-    if (item >= total) {
-      if (sorted) break;
-      item -= total;
-      continue;
-    }
-    int above = 0, stages = 0;  // tiles with more stages; stages of this one (0: in order)
-    if (sorted && a.S > 1) {
-      int lo = 1, hi = (a.N + kStageKeys - 1) / kStageKeys;  // count(hi) is 0
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (count(mid) <= item) hi = mid;
-        else lo = mid + 1;
-      }
-      stages = lo;
-      above = count(lo);
-    }
-    // The (item - above)-th of the tiles of that class, in order.
-    int left = item - above;
-#pragma unroll
-    for (int i = 0; i < kWindow; ++i) {
-      const int rest = stages ? longer(i, stages) : 0, c = (stages ? longer(i, stages - 1) : tiles(i)) - rest;
-      const int incl = wave_scan(c);
-      const int here = __builtin_amdgcn_readlane(incl, 63);
-      if (left < here) {
-        const int at = sgpr(__builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > left)));
-        const int nth = left - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(c, at));
-        const int T = __builtin_amdgcn_readlane(tiles(i), at) - __builtin_amdgcn_readlane(rest, at);
-        return Rows{__builtin_amdgcn_readlane(b[i], at), __builtin_amdgcn_readlane(n[i], at), T - 1 - nth};
-      }
-      left -= here;
-    }
-    break;
+  for (int w = 0; w < kPlanThreads / kWave; ++w) {
+    const int v = lds[w];
+    before += w < wave ? v : 0;
+    all += v;
   }
-  return Rows{0, 0, 0};
+  *total = all;
+  return before + incl - x;
+}
+template <bool LDS>  // S <= kPlanLds
+__global__ __launch_bounds__(kPlanThreads) void gqa_packed_plan(GqaPackedArgs a, int R) {
+  __shared__ int waves[kPlanThreads / kWave], count[kClasses], longest;
+  // Tiles before a sequence, and the sequences: [S + 1], [S].
+  __shared__ int sums[LDS ? kPlanLds + 1 : 1], first[LDS ? kPlanLds : 1], length[LDS ? kPlanLds : 1];
+  auto tiles_before = [&](int s) { return LDS ? sums[s] : a.tile_sums[s]; };
+  const int tid = threadIdx.x;
+  if (tid == 0) longest = 0;
+  count[tid] = 0;
+  int total = 0, most_here = 0;
+  for (int base = 0; base < a.S; base += kPlanThreads) {
+    const int s = base + tid;
+    Rows q = {0, 0, 0, 0};
+    if (s < a.S) q = sequence(a, s);
+    int all;
+    const int at = total + plan_scan((q.len * a.G + R - 1) / R, waves, &all);
+    if (s < a.S) {
+      if (LDS) {
+        sums[s] = at;
+        first[s] = q.start;
+        length[s] = q.len;
+      } else {
+        a.tile_sums[s] = at;
+      }
+    }
+    total += all;
+    most_here = max(most_here, q.len);
+  }
+  if (most_here > 0) atomicMax(&longest, most_here);
+  if (tid == 0) *a.num_tiles = total;
+  __syncthreads();
+  const int most = max(1, (longest + kStageKeys - 1) / kStageKeys);
+  struct Tile {
+    Rows w;
+    int cls;
+  };
+  auto tile_at = [&](int i) __attribute__((always_inline)) {
+    int lo = 0, hi = a.S - 1;  // the last sequence with at most i tiles before it
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (tiles_before(mid) <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    Rows w = LDS ? Rows{first[lo], length[lo], 0, 0} : sequence(a, lo);
+    w.tile = i - tiles_before(lo);
+    const int keys = min(w.len, quotient(w.tile * R + R - 1, a.G, a.G_magic) + 1);
+    const int shorter = most - (keys + kStageKeys - 1) / kStageKeys;  // 0 .. most - 1
+    return Tile{w, most <= kClasses ? shorter : (int)((int64_t)shorter * (kClasses - 1) / most)};
+  };
+  Tile mine = {};
+  for (int i = tid; i < total; i += kPlanThreads) {
+    const Tile t = tile_at(i);
+    if (i == tid) mine = t;
+    atomicAdd(count + t.cls, 1);
+  }
+  __syncthreads();
+  int all;
+  const int at = plan_scan(count[tid], waves, &all);
+  count[tid] = at;
+  __syncthreads();
+  for (int i = tid; i < total; i += kPlanThreads) {
+    const Tile t = i == tid ? mine : tile_at(i);
+    ((Rows *)a.tiles)[atomicAdd(count + t.cls, 1)] = t.w;
+  }
 }
 
 // The rows of a wave from row0 on, a row per pair of lanes l, l + 32 (each with half
@@ -194,8 +231,9 @@ __device__ __forceinline__ Rows find_rows(const GqaPackedArgs &a, int G, int ite
 template <int D, bool F16>
 __device__ __forceinline__ void take_rows(const GqaPackedArgs &a, const Rows &w, int kvh, int row0, int tok_hi) {
   constexpr int kPart = D / 16;  // 16-byte chunks of a lane
-  const int G = a.Hq / a.Hkv, rows = w.len * G, lane = threadIdx.x & 63;
-  const int row = min(row0 + lane % kWaveRows, rows - 1), tok = row / G, head = kvh * G + row % G;
+  const int G = a.G, rows = w.len * G, lane = threadIdx.x & 63;
+  const int row = min(row0 + lane % kWaveRows, rows - 1), tok = quotient(row, G, a.G_magic);
+  const int head = kvh * G + row - tok * G;
   const int first = lane / kWaveRows * (D / 2);  // of the lane's dims
   const uint16_t *const qp = a.q + (int64_t)(w.start + tok) * a.q_stride + (int64_t)head * D + first;
   u32x4 q[kPart];
@@ -240,35 +278,51 @@ __device__ __forceinline__ void take_rows(const GqaPackedArgs &a, const Rows &w,
   for (int d = 0; d < 8 * kPart; d += 2) op[d / 2] = pack2<F16>(o[d] * inv, o[d + 1] * inv);
 }
 
-template <int D, bool F16>
-__global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArgs a) {
+template <int D, bool F16, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void gqa_packed_kernel(GqaPackedArgs a) {
+  constexpr int kR = kTileRows<WAVES>, kRing = kSlots<WAVES>;
   constexpr int kSteps = D / 16;                    // QK MFMAs per half stage
   constexpr int kDims = D / 32;                     // 32-dim tiles of O
   constexpr int kTile = kStageKeys * D * 2;         // bytes of a stage's K (or V)
-  constexpr int kLoads = kTile / 1024 / kWaves;     // of K (or V) per wave and stage
+  constexpr int kLoads = kTile / 1024 / WAVES;      // of K (or V) per wave and stage
   constexpr int kChunks = D / 8;                    // 16-byte chunks of a row
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const int wave = sgpr(threadIdx.x >> 6);
-  const int G = a.Hq / a.Hkv;
+  const int G = a.G;
+  // Beside the waves of another workgroup on the CU, the dependent steps outside of
+  // the loop go first.
+  __builtin_amdgcn_s_setprio(3);
 
   // Workgroups go round the eight XCDs; the tiles of one KV head stay on the
   // XCDs of its class, which share K and V through their L2.
   const int xcd = blockIdx.x % kXcds, slot8 = blockIdx.x / kXcds;
-  const int classes = a.Hkv % 8 == 0 ? 8 : a.Hkv % 4 == 0 ? 4 : a.Hkv % 2 == 0 ? 2 : 1;
-  const int in_class = slot8 * (kXcds / classes) + xcd / classes, per_class = a.Hkv / classes;
-  const int kvh = sgpr(xcd % classes + classes * (in_class % per_class));
-  const Rows w = find_rows(a, G, sgpr(in_class / per_class));
-  if (w.len == 0) return;
+  const int in_class = (slot8 << a.class_xcds) + (xcd >> (3 - a.class_xcds)), nth = in_class / a.per_class;
+  const int kvh = (xcd & (7 >> a.class_xcds)) + ((in_class - nth * a.per_class) << (3 - a.class_xcds));
+  Rows w;
+  if (a.S == 1) {
+    w = sequence(a, 0);
+    const int T = (w.len * G + kR - 1) / kR;
+    if (nth >= T) return;
+    w.tile = T - 1 - nth;  // the longest first
+  } else {
+    // Scalar loads: the list does not change while the kernel runs.
+    typedef const __attribute__((address_space(4))) int *Uniform;
+    const Uniform list = (Uniform)(const __attribute__((address_space(4))) void *)a.tiles + 4 * (int64_t)nth;
+    const int num = *(Uniform)(const __attribute__((address_space(4))) void *)a.num_tiles;
+    w = Rows{list[0], list[1], list[2], 0};  // the list has room for the whole grid
+    if (nth >= num) return;
+  }
 
   const int rows = w.len * G;                                           // of the sequence
-  const int row0 = w.tile * kTileRows + kWaveRows * wave;                      // of the wave
-  const int keys = min(w.len, (w.tile * kTileRows + kTileRows - 1) / G + 1);  // that the workgroup sees
+  const int row0 = w.tile * kR + kWaveRows * wave;                      // of the wave
+  const int keys = min(w.len, quotient(w.tile * kR + kR - 1, G, a.G_magic) + 1);  // that the workgroup sees
   const int stages = (keys + kStageKeys - 1) / kStageKeys;
-  // The wave's half stages of 32 keys: all up to its last token's, the first
-  // `full` of them seen by all of its tokens.
-  const int tok_lo = row0 / G, tok_hi = min(w.len - 1, (row0 + kWaveRows - 1) / G);
-  const int nhalf = row0 < rows ? tok_hi / 32 + 1 : 0, full = (tok_lo + 1) / 32;
+  // The wave's stages: all up to its last token's key, the first `full` of them seen
+  // by all of its tokens.
+  const int tok_lo = quotient(row0, G, a.G_magic);
+  const int tok_hi = min(w.len - 1, quotient(row0 + kWaveRows - 1, G, a.G_magic));
+  const int own = row0 < rows ? tok_hi / kStageKeys + 1 : 0, full = (tok_lo + 1) / kStageKeys;
 
   // ---- loads ----
   const uint32_t lds0 = lds_addr(smem);
@@ -286,25 +340,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArg
     const int first = st * kStageKeys, n = min(kStageKeys, w.len - first);
     const u32x4 krs = buffer_words(k0 + (int64_t)first * a.k_stride, (uint32_t)(n - 1) * ksb + 2 * D);
     const u32x4 vrs = buffer_words(v0 + (int64_t)first * a.v_stride, (uint32_t)(n - 1) * vsb + 2 * D);
-    const uint32_t dst = sgpr((int)(lds0 + (st % kSlots) * (2 * kTile) + wave * kLoads * 1024));
+    const uint32_t dst = sgpr((int)(lds0 + st % kRing * (2 * kTile) + wave * kLoads * 1024));
     load_lds(krs, dst, k_off);
     load_lds(vrs, dst + kTile, v_off);
   };
-  // Stage st is there for every wave, and every wave is done with stage st - 2,
-  // whose slot takes stage st + 2.
+  // In step st of the loop: stage st + 2 is there for every wave, and every wave is
+  // done with stage st - 1, whose slot takes the next one.
   auto sync = [&](int st) __attribute__((always_inline)) {
-    if (st + 1 < stages) wait_vmcnt<2 * kLoads>();
+    if (st + kRing - 2 < stages) wait_vmcnt<2 * kLoads * (kRing - 4)>();
     else wait_vmcnt<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (st + 2 < stages) issue(st + 2);
+    if (st + kRing - 1 < stages) issue(st + kRing - 1);
   };
-  issue(0);
-  if (stages > 1) issue(1);
+  // Three stages ahead of Q, since loads return in order; the others behind it.
+  for (int st = 0; st < min(3, stages); ++st) issue(st);
 
   // ---- operands ----
-  const int row = min(row0 + r, rows - 1), tok = row / G;  // the lane's; tok: the last key that it sees
-  const int64_t at_q = (int64_t)(w.start + tok), head = kvh * G + row % G;
+  const int row = min(row0 + r, rows - 1), tok = quotient(row, G, a.G_magic);  // the lane's; tok: the last key that it sees
+  const int64_t at_q = (int64_t)(w.start + tok), head = kvh * G + row - tok * G;
   u32x4 qf[kSteps];
 #pragma unroll
   for (int ks = 0; ks < kSteps; ++ks) qf[ks] = *(const u32x4 *)(a.q + at_q * a.q_stride + head * D + 8 * h + 16 * ks);
@@ -315,14 +369,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArg
   const uint32_t v_at = (uint32_t)(kTile + v_key * 2 * D + 16 * (v_chunk ^ swizzle_v<D>(v_key)) + 8 * (lane & 1));
 
   u32x4 kf[kSteps], vf[2][kDims];
-  auto half_base = [&](int hf) { return lds0 + (uint32_t)((hf / 2) % kSlots * (2 * kTile) + (hf & 1) * (kTile / 2)); };
   // Operand reads, spread over the MFMAs before their use: all at once they would
   // not fit the registers, and the waves' bursts would wait for each other.
-  auto read_k = [&](int hf, int ks) __attribute__((always_inline)) {
-    kf[ks] = lds_b128((half_base(hf) + k_at) ^ (32 * ks));
+  auto slot_base = [&](int st) { return lds0 + (uint32_t)(st % kRing * (2 * kTile)); };
+  auto read_k = [&](int st, int ks) __attribute__((always_inline)) {
+    kf[ks] = lds_b128((slot_base(st) + k_at) ^ (32 * ks));
   };
-  auto read_v = [&](int hf, int j, int db) __attribute__((always_inline)) {
-    const uint32_t at = ((half_base(hf) + v_at) ^ (64 * db)) + j * 32 * D;
+  auto read_v = [&](int st, int j, int db) __attribute__((always_inline)) {
+    const uint32_t at = ((slot_base(st) + v_at) ^ (64 * db)) + j * 32 * D;
     const u32x2 lo = lds_tr16(at), hi = lds_tr16(at + 16 * D);
     vf[j][db] = u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
@@ -334,16 +388,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArg
   for (int db = 0; db < kDims; ++db)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
-  float mx = -INFINITY;  // of the raw scores of the half at hand
+  float mx = -INFINITY;  // of the raw scores of the stage at hand
 
-  // One half: its scores in s; the next half's come into sn.
-  // The second four waves, each beside one of the first on its SIMD, meet them at
+  // One stage: its scores in s; the next one's come into sn.
+  // Of eight waves the second four, each beside one of the first on its SIMD, meet them at
   // the barrier a phase earlier in their own work, so that one's exponentials fall
   // beside the other's MFMAs.
-  auto half = [&](int hf, f32x16 &s, f32x16 &sn) __attribute__((always_inline)) {
-    if (wave >= kWaves / 2 && !(hf & 1) && hf / 2 + 1 < stages) sync(hf / 2 + 1);
-    if (hf >= full) {
-      const int last = tok - 32 * hf - 4 * h;
+  auto step = [&](int st, f32x16 &s, f32x16 &sn) __attribute__((always_inline)) {
+    if (WAVES == 8 && wave >= WAVES / 2 && st + 2 < stages) sync(st);
+    if (st >= full) {
+      const int last = tok - kStageKeys * st - 4 * h;
       mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -365,10 +419,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArg
     }
     const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
 
-    // A: the next half's scores beside this one's exponentials.  (Behind the
-    // wave's last half these are of rows in the ring that nothing asks for.)
+    // A: the next stage's scores beside this one's exponentials.  (Behind the
+    // wave's last stage these are of rows in the ring that nothing asks for.)
 #pragma unroll
-    for (int ks = kSteps / 2; ks < kSteps; ++ks) read_k(hf + 1, ks);
+    for (int ks = kSteps / 2; ks < kSteps; ++ks) read_k(st + 1, ks);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 16; ++i) sn[i] = 0.f;
@@ -398,14 +452,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArg
       if (m == kSteps - 1) take(7);
       // V's first keys beside the first half of the MFMAs, the others (in the place
       // of K fragments that are done with) beside the second.
-      if (m < kSteps / 2) read_v(hf, 0, m % kDims);
-      else read_v(hf, 1, m % kDims);
+      if (m < kSteps / 2) read_v(st, 0, m % kDims);
+      else read_v(st, 1, m % kDims);
       __builtin_amdgcn_sched_barrier(0);
     }
     l_run += sum0 + sum1;
-    if (wave < kWaves / 2 && !(hf & 1) && hf / 2 + 1 < stages) sync(hf / 2 + 1);
+    if ((WAVES == 4 || wave < WAVES / 2) && st + 2 < stages) sync(st);
 
-    // B: O of this half beside the next half's maxima (from the third MFMA on: the
+    // B: O of this stage beside the next one's maxima (from the third MFMA on: the
     // scores are there then).
     constexpr int kPv = 2 * kDims;
     mx = -INFINITY;
@@ -418,13 +472,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArg
         sn[2 * x + 1] = pin(sn[2 * x + 1]);
         mx = pin(fmaxf(fmaxf(sn[2 * x], sn[2 * x + 1]), mx));
       }
-      if (m >= kDims) read_k(hf + 2, m - kDims);
+      if (m >= kDims) read_k(st + 2, m - kDims);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  sync(0);
-  if (nhalf > 0) {
+  wait_vmcnt<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  for (int st = 3; st < min(kRing - 1, stages); ++st) issue(st);
+  __builtin_amdgcn_s_setprio(0);
+  if (own > 0) {
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) read_k(0, ks);
 #pragma unroll
@@ -439,17 +497,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArg
       s0[i] = pin(s0[i]);
       mx = fmaxf(mx, s0[i]);
     }
-    for (int hf = 0; hf < nhalf; hf += 2) {
-      half(hf, s0, s1);
-      if (hf + 1 == nhalf) break;
-      half(hf + 1, s1, s0);
+    for (int st = 0; st < own; st += 2) {
+      step(st, s0, s1);
+      if (st + 1 == own) break;
+      step(st + 1, s1, s0);
     }
   }
+  __builtin_amdgcn_s_setprio(3);
   // The stages that other waves still read.
-  for (int st = (nhalf + 1) / 2 + 1; st < stages; ++st) sync(st);
+  for (int st = own; st + 2 < stages; ++st) sync(st);
   mfma_settle();
 
-  // In the masked halves a probability of 0 stood before values that the row does
+  // In the masked stages a probability of 0 stood before values that the row does
   // not see, and 0 times one that is not finite is NaN.  Looked for only where O is
   // not finite; then the wave takes its rows again, slowly.
   float zero = 0.f;
@@ -462,20 +521,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArg
     }
   if (__builtin_expect(__builtin_amdgcn_ballot_w64(zero != 0.f) != 0, 0)) {
     bool bad = false;
-    for (int key = 32 * full + lane / kChunks; key < min(32 * nhalf, w.len); key += 64 / kChunks) {
+    for (int key = kStageKeys * full + lane / kChunks; key < min(kStageKeys * own, w.len); key += 64 / kChunks) {
       const u32x4 v = *(const u32x4 *)(v0 + (int64_t)key * a.v_stride + 8 * (lane % kChunks));
 #pragma unroll
       for (int c = 0; c < 4; ++c) bad |= not_finite2<F16>(v[c]);
     }
-    if (nhalf > 0 && __builtin_amdgcn_ballot_w64(bad)) {
+    if (own > 0 && __builtin_amdgcn_ballot_w64(bad)) {
       take_rows<D, F16>(a, w, kvh, row0, tok_hi);
       return;
     }
   }
   const f32x2_t both = halves(l_run);
   const float L = both[0] + both[1], inv = L == 0.f ? 0.f : 1.0f / L;
-  // Lane (r, h): dims 32 db + 8 q + 4 h + i of its row.
-  uint16_t *const op = a.out + (at_q * a.Hq + head) * D + 4 * h;
+  // Lane (r, h) holds dims 32 db + 8 q + 4 h + i of its row.  Through LDS, in slots that
+  // no stage is read from any more (at most the last three are), to whole rows:
+  // stores of 8 bytes in each of 32 rows took longer than all of the rest here.
+  const uint32_t tile = lds0 + (uint32_t)((stages + wave / 2) % kRing * (2 * kTile) + (wave & 1) * kTile);
 #pragma unroll
   for (int db = 0; db < kDims; ++db)
 #pragma unroll
@@ -483,30 +544,69 @@ __global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArg
       u32x2 v;
       v[0] = pack2<F16>(o[db][4 * q] * inv, o[db][4 * q + 1] * inv);
       v[1] = pack2<F16>(o[db][4 * q + 2] * inv, o[db][4 * q + 3] * inv);
-      if (row0 + r < rows) *(u32x2 *)(op + 32 * db + 8 * q) = v;
+      lds_write_b64(tile + (uint32_t)(r * 2 * D + 16 * ((4 * db + q) ^ swizzle_k<D>(r)) + 8 * h), v);
     }
+#pragma unroll
+  for (int i = 0; i < kWaveRows * kChunks / 64; ++i) {
+    const int x = (64 * i + lane) / kChunks, c = lane % kChunks, at = row0 + x, t = quotient(at, G, a.G_magic);
+    const u32x4 v = lds_b128(tile + (uint32_t)(x * 2 * D + 16 * (c ^ swizzle_k<D>(x))));
+    if (at < rows) *(u32x4 *)(a.out + ((int64_t)(w.start + t) * a.Hq + kvh * G + at - t * G) * D + 8 * c) = v;
+  }
 }
 
-template <int D, bool F16>
+// Every sequence ends in at most one tile that is not full.
+int64_t max_tiles(int N, int G, int S, int R) { return (int64_t)N * G / R + (S < N ? S : N); }
+
+template <int D, bool F16, int WAVES>
 hipError_t launch(const GqaPackedArgs &a, hipStream_t s) {
-  auto k = gqa_packed_kernel<D, F16>;
-  constexpr int lds = kSlots * 2 * kStageKeys * D * 2;
+  auto k = gqa_packed_kernel<D, F16, WAVES>;
+  constexpr int lds = kSlots<WAVES> * 2 * kStageKeys * D * 2;
   static const bool attr = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds) ==
                            hipSuccess;
   if (!attr) return hipErrorInvalidValue;
-  // Every sequence ends in at most one tile that is not full.
-  const int64_t tiles = (int64_t)a.N * (a.Hq / a.Hkv) / kTileRows + (a.S < a.N ? a.S : a.N);
-  const int classes = a.Hkv % 8 == 0 ? 8 : a.Hkv % 4 == 0 ? 4 : a.Hkv % 2 == 0 ? 2 : 1;
-  const int64_t in_class = tiles * (a.Hkv / classes), per_xcd = (in_class + kXcds / classes - 1) / (kXcds / classes);
-  hipLaunchKernelGGL(k, dim3((uint32_t)(per_xcd * kXcds)), dim3(64 * kWaves), lds, s, a);
+  const int64_t tiles = max_tiles(a.N, a.G, a.S, kTileRows<WAVES>);
+  const int64_t per_xcd = (tiles * a.per_class + (1 << a.class_xcds) - 1) >> a.class_xcds;
+  if (a.S > 1)
+    hipLaunchKernelGGL(a.S <= kPlanLds ? gqa_packed_plan<true> : gqa_packed_plan<false>, dim3(1), dim3(kPlanThreads), 0, s,
+                       a, kTileRows<WAVES>);
+  hipLaunchKernelGGL(k, dim3((uint32_t)(per_xcd * kXcds)), dim3(64 * WAVES), lds, s, a);
   return hipGetLastError();
 }
 
 }  // namespace
 
+void gqa_packed_constants(GqaPackedArgs *a) {
+  a->G = a->Hq / a->Hkv;
+  a->G_magic = (uint32_t)(((1ull << 32) + a->G - 1) / a->G);
+  // KV heads go round 8, 4, 2 or 1 classes of XCDs.
+  a->class_xcds = a->Hkv % 8 == 0 ? 0 : a->Hkv % 4 == 0 ? 1 : a->Hkv % 2 == 0 ? 2 : 3;
+  a->per_class = a->Hkv >> (3 - a->class_xcds);
+}
+
+namespace {
+size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+// Tiles of the smaller size, and what the grid's rounding up to whole XCDs adds.
+size_t list_entries(int N, int G, int S) { return (size_t)max_tiles(N, G, S, kTileRows<4>) + kXcds; }
+}  // namespace
+
+// {status and number of tiles; the tiles; the sums of the tiles before a sequence}
+size_t gqa_packed_workspace(int N, int Hq, int Hkv, int S) {
+  return 256 + align256(list_entries(N, Hq / Hkv, S) * sizeof(Rows)) + ((size_t)S + 1) * 4;
+}
+
+void gqa_packed_bind(GqaPackedArgs *a, void *workspace) {
+  uint8_t *const w = (uint8_t *)workspace;
+  a->status = (uint32_t *)w;
+  a->num_tiles = (int32_t *)(w + 128);
+  a->tiles = (int32_t *)(w + 256);
+  a->tile_sums = (int32_t *)(w + 256 + align256(list_entries(a->N, a->Hq / a->Hkv, a->S) * sizeof(Rows)));
+}
+
 hipError_t launch_gqa_packed(const GqaPackedArgs &a, hipStream_t s) {
-  if (a.D == 128) return a.dtype == GQA_FP16 ? launch<128, true>(a, s) : launch<128, false>(a, s);
-  return a.dtype == GQA_FP16 ? launch<64, true>(a, s) : launch<64, false>(a, s);
+  const bool f16 = a.dtype == GQA_FP16;
+  if (getenv("PK8") && a.D == 128) return f16 ? launch<128, true, 8>(a, s) : launch<128, false, 8>(a, s);
+  if (a.D == 128) return f16 ? launch<128, true, 4>(a, s) : launch<128, false, 4>(a, s);
+  return f16 ? launch<64, true, 4>(a, s) : launch<64, false, 4>(a, s);
 }
 
 }  // namespace moe
