@@ -19,7 +19,7 @@ int capi_fail(int code, const char *fmt, ...);  // moe_capi.hip (thread-local me
 
 struct gqa_packed_plan {
   moe::GqaPackedArgs a;
-  int device;
+  int device, cus;
 };
 
 struct gqa_paged_plan {
@@ -214,10 +214,11 @@ int gqa_packed_plan_create(gqa_packed_plan **out, const gqa_packed_desc *d) {
   if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");
   p->a = moe::GqaPackedArgs{(const uint16_t *)d->q, (const uint16_t *)d->k, (const uint16_t *)d->v, (uint16_t *)d->out,
                             d->starts, d->q_stride, d->k_stride, d->v_stride, d->N, d->S, d->Hq, d->Hkv, d->D, d->dtype,
-                            scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0};
+                            scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0, 0};
   moe::gqa_packed_bind(&p->a, d->workspace);
   moe::gqa_packed_constants(&p->a);
   p->device = dev;
+  p->cus = cus;
   *out = p;
   return MOE_OK;
 }
@@ -225,7 +226,7 @@ int gqa_packed_plan_create(gqa_packed_plan **out, const gqa_packed_desc *d) {
 int gqa_packed_plan_run(gqa_packed_plan *p, void *stream) {
   if (!p) return moe::capi_fail(MOE_EINVAL, "null plan");
   if (p->a.N == 0 || p->a.S == 0) return MOE_OK;
-  return on_device(p->device, "packed gqa launch", [&] { return moe::launch_gqa_packed(p->a, (hipStream_t)stream); });
+  return on_device(p->device, "packed gqa launch", [&] { return moe::launch_gqa_packed(p->a, p->cus, (hipStream_t)stream); });
 }
 
 int gqa_packed_plan_read_status(gqa_packed_plan *p, void *stream, uint32_t *flags) {

@@ -53,13 +53,13 @@ struct GqaPackedArgs {
   int32_t *num_tiles, *tiles, *tile_sums;  // workspace
   // Set by gqa_packed_constants: the group Hq / Hkv; log2 of the XCDs that share a
   // class of KV heads, and a class's heads; ceil(2^32 / G).
-  int G, class_xcds, per_class;
+  int G, class_xcds, per_class, listed;
   uint32_t G_magic;
 };
 size_t gqa_packed_workspace(int N, int Hq, int Hkv, int S);
 void gqa_packed_bind(GqaPackedArgs *a, void *workspace);
 void gqa_packed_constants(GqaPackedArgs *a);
-hipError_t launch_gqa_packed(const GqaPackedArgs &a, hipStream_t s);
+hipError_t launch_gqa_packed(const GqaPackedArgs &a, int cus, hipStream_t s);
 
 // One new token per sequence over a paged cache (gqa_paged.hip).
 struct GqaPagedArgs {
