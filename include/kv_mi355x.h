@@ -52,7 +52,7 @@ typedef struct kv_cache_desc {
   int32_t *tables, *lengths, *refs, *starts;
   int64_t *slots;
   uint32_t *status;
-  void *workspace; /* >= kv_cache_workspace_bytes(); scratch of a call */
+  void *workspace; /* >= kv_cache_workspace_bytes(), zeroed once; scratch of a call */
   size_t workspace_bytes;
 } kv_cache_desc;
 

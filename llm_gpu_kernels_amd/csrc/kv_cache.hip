@@ -280,8 +280,7 @@ __device__ __forceinline__ int row_pages(const KvState &s, int row) {
 }
 
 // A pair of a fork: 0 if it may go ahead, else why not (KV_STATUS_*; ~0: left out
-// by the caller).  Rows are as before the call: lengths are written by a later
-// launch.  `named` says that an earlier pair that goes by valid rows names dst.
+// by the caller).  Rows are as before the call: lengths are written at its end.  `named` says that an earlier pair that goes by valid rows names dst.
 __device__ __forceinline__ bool fork_rows_valid(const KvState &s, int a, int b) {
   return a >= 0 && b >= 0 && a < s.sequences && b < s.sequences;
 }
@@ -291,37 +290,59 @@ __device__ __forceinline__ uint32_t fork_status(const KvState &s, int a, int b, 
   return named || s.lengths[b] != 0 ? KV_STATUS_NOT_EMPTY : 0u;
 }
 
-// One workgroup per pair: the table row, and one more holder of its pages.
-__global__ __launch_bounds__(kWideThreads) void kv_fork_rows(KvState s, const int32_t *src, const int32_t *dst) {
+// One workgroup per pair: the table row, and one more holder of its pages.  The
+// last one to finish sets the lengths: no other reads them any more then.
+__device__ __forceinline__ void fork_lengths(const KvState &s, const int32_t *src, const int32_t *dst, int n);
+__global__ __launch_bounds__(kWideThreads) void kv_fork(KvState s, const int32_t *src, const int32_t *dst) {
   const int i = blockIdx.x, a = src[i], b = dst[i];
   bool named = false;
   for (int j = threadIdx.x; j < i; j += kWideThreads) named |= dst[j] == b && fork_rows_valid(s, src[j], b);
   const uint32_t why = fork_status(s, a, b, __syncthreads_or(named));
   if (why) {
     if (threadIdx.x == 0 && why != ~0u) atomicOr(s.status, why);
-    return;
+  } else {
+    const int n = row_pages(s, a);
+    const int32_t *const from = s.tables + (int64_t)a * s.max_pages;
+    int32_t *const to = s.tables + (int64_t)b * s.max_pages;
+    for (int c = threadIdx.x; c < n; c += kWideThreads) {
+      const int p = from[c];
+      to[c] = p;
+      if (p >= 0 && p < s.pages) atomicAdd(s.refs + p, 1);
+      else atomicOr(s.status, KV_STATUS_BAD_STATE);
+    }
   }
-  const int n = row_pages(s, a);
-  const int32_t *const from = s.tables + (int64_t)a * s.max_pages;
-  int32_t *const to = s.tables + (int64_t)b * s.max_pages;
-  for (int c = threadIdx.x; c < n; c += kWideThreads) {
-    const int p = from[c];
-    to[c] = p;
-    if (p >= 0 && p < s.pages) atomicAdd(s.refs + p, 1);
-    else atomicOr(s.status, KV_STATUS_BAD_STATE);
-  }
-}
-// A thread per pair; the first pair that names a row by valid rows owns it.
-__global__ __launch_bounds__(kPlanThreads) void kv_fork_lengths(KvState s, const int32_t *src, const int32_t *dst, int n) {
-  __shared__ int owner[kPlanThreads];
-  const int i = threadIdx.x, a = i < n ? src[i] : -1, b = i < n ? dst[i] : -1;
-  const bool valid = fork_rows_valid(s, a, b);
-  const int len = valid ? s.lengths[a] : -1, old = valid ? s.lengths[b] : -1;
-  owner[i] = kPlanThreads;
-  __syncthreads();  // every length has been read
-  if (valid) atomicMin(owner + b, i);
+  __shared__ bool last;
+  __syncthreads();  // every thread has read what it reads of lengths
+  if (threadIdx.x == 0) last = atomicAdd(s.arrived, 1) == (int)gridDim.x - 1;
   __syncthreads();
-  if (valid && owner[b] == i && old == 0 && len >= 0 && len <= s.max_pages * s.page_size) s.lengths[b] = len;
+  if (!last) return;
+  if (threadIdx.x == 0) atomicExch(s.arrived, 0);
+  fork_lengths(s, src, dst, gridDim.x);
+}
+// The first pair that names a row by valid rows owns it.
+__device__ __forceinline__ void fork_lengths(const KvState &s, const int32_t *src, const int32_t *dst, int n) {
+  constexpr int kEach = KV_MAX_SEQUENCES / kWideThreads;  // pairs of a thread
+  __shared__ int owner[KV_MAX_SEQUENCES];
+  int to[kEach], len[kEach], old[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = k * kWideThreads + threadIdx.x, a = i < n ? src[i] : -1, b = i < n ? dst[i] : -1;
+    const bool valid = fork_rows_valid(s, a, b);
+    to[k] = valid ? b : -1;
+    len[k] = valid ? s.lengths[a] : -1;
+    old[k] = valid ? s.lengths[b] : -1;
+    owner[i] = KV_MAX_SEQUENCES;
+  }
+  __syncthreads();  // every length has been read
+#pragma unroll
+  for (int k = 0; k < kEach; ++k)
+    if (to[k] >= 0) atomicMin(owner + to[k], k * kWideThreads + (int)threadIdx.x);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kEach; ++k)
+    if (to[k] >= 0 && owner[to[k]] == k * kWideThreads + (int)threadIdx.x && old[k] == 0 && len[k] >= 0 &&
+        len[k] <= s.max_pages * s.page_size)
+      s.lengths[to[k]] = len[k];
 }
 
 __global__ __launch_bounds__(kWideThreads) void kv_free(KvState s, const int32_t *rows) {
@@ -417,6 +438,7 @@ void kv_bind_workspace(KvState *s, void *workspace) {
   uint8_t *const w = (uint8_t *)workspace;
   const size_t each = align256((size_t)s->pages * 4);
   s->num_moves = (int32_t *)w;
+  s->arrived = (int32_t *)(w + 128);
   s->move_src = (int32_t *)(w + 256);
   s->move_dst = (int32_t *)(w + 256 + each);
   s->list = (int32_t *)(w + 256 + 2 * each);
@@ -441,8 +463,7 @@ hipError_t launch_kv_append(const KvState &s, int layer, const uint16_t *k, cons
 }
 
 hipError_t launch_kv_fork(const KvState &s, const int32_t *src, const int32_t *dst, int n, hipStream_t st) {
-  hipLaunchKernelGGL(kv_fork_rows, dim3(n), dim3(kWideThreads), 0, st, s, src, dst);
-  hipLaunchKernelGGL(kv_fork_lengths, dim3(1), dim3(kPlanThreads), 0, st, s, src, dst, n);
+  hipLaunchKernelGGL(kv_fork, dim3(n), dim3(kWideThreads), 0, st, s, src, dst);
   return hipGetLastError();
 }
 

@@ -13,9 +13,10 @@ struct KvState {
   int32_t *tables, *lengths, *refs, *starts;
   int64_t *slots;
   uint32_t *status;
-  // Scratch: {count of moves, ...}, the moves' source and target pages, the
+  // Scratch: the count of moves, the workgroups of a fork that have finished (0
+  // between calls), the moves' source and target pages, the
   // pages of a reserve (or of a compaction) in order, and where a moved page went.
-  int32_t *num_moves, *move_src, *move_dst, *list, *moved_to;
+  int32_t *num_moves, *arrived, *move_src, *move_dst, *list, *moved_to;
 };
 
 size_t kv_workspace_bytes(int pages);
