@@ -583,7 +583,7 @@ hipError_t launch(GqaPackedArgs a, int cus, hipStream_t s) {
   // The order matters once some workgroups start after others; up to 64 sequences a
   // wave finds its tile by itself (four prompts of up to 48 tokens: 6.5 us, 9.7 with
   // the list).
-  a.listed = a.S > kWave || (a.S > 1 && per_xcd * kXcds > 2 * cus);
+  a.listed = a.S > kWave || (a.S > 1 && per_xcd * kXcds > 4 * cus);
   if (a.listed)
     hipLaunchKernelGGL(a.S <= kPlanLds ? gqa_packed_plan<true> : gqa_packed_plan<false>, dim3(1), dim3(kPlanThreads), 0, s,
                        a);
