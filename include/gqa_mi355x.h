@@ -77,9 +77,9 @@ void gqa_seg_plan_destroy(gqa_seg_plan *p);
 #define GQA_FP16 1
 
 /* Device status bits, latched until read (gqa_*_plan_read_status clears them). */
-#define GQA_STATUS_BAD_BOUNDS 1u /* starts not ascending within [0, N] (rows of out that two
-                                    sequences then claim are undefined), or a cache length
-                                    outside [0, M * page]: taken as the nearest within     */
+#define GQA_STATUS_BAD_BOUNDS 1u /* starts not ascending within [0, N]: each taken as the largest
+                                    up to it, at most N; or a cache length outside [0, M *
+                                    page]: taken as the nearest within                       */
 #define GQA_STATUS_BAD_PAGE 2u   /* a page number outside [0, P): its keys were left out   */
 
 /*

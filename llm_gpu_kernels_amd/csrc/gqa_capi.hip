@@ -112,12 +112,14 @@ int validate_packed_sizes(const gqa_packed_desc *d) {
   if (!d) return capi_fail(MOE_EINVAL, "null descriptor");
   if (const int rc = validate_heads(d->Hq, d->Hkv, d->D, d->dtype)) return rc;
   if (d->S < 0 || d->S > (1 << 20)) return capi_fail(MOE_EINVAL, "S must be in [0, 2^20] (got %d)", d->S);
-  // The kernel divides numbers of query rows below 2^26, and its workgroups (one
-  // per 256 query rows and one per sequence) are counted in 31 bits.
-  if (d->N < 0 || (int64_t)d->N * (d->Hq / d->Hkv) + 256 >= 1LL << 26 ||
-      ((int64_t)d->N * (d->Hq / d->Hkv) / 256 + d->S + 8) * d->Hkv >= 1LL << 30)
-    return capi_fail(MOE_EINVAL, "N must be >= 0, N * Hq / Hkv below 2^26 - 256 and N * Hq / 256 + S * Hkv below 2^30 (got %d)",
-                     d->N);
+  // The kernel divides numbers of query rows below 2^26; a grid has fewer than 2^32
+  // threads, 256 per 128 query rows and per sequence, for every KV head.
+  const int64_t rows = (int64_t)d->N * (d->Hq / d->Hkv);
+  if (d->N < 0 || rows >= (1LL << 26) - 256 ||
+      (rows / 128 + (d->S < d->N ? d->S : d->N) + 8) * d->Hkv >= (1LL << 24) - 8)
+    return capi_fail(MOE_EINVAL,
+                     "N must be >= 0, N * Hq / Hkv below 2^26 - 256 and N * Hq / 128 + S * Hkv below 2^24 (got N %d, S %d)",
+                     d->N, d->S);
   return MOE_OK;
 }
 
@@ -147,6 +149,8 @@ int validate_paged_sizes(const gqa_paged_desc *d) {
     return capi_fail(MOE_EINVAL, "P and M must be positive and M * page < 2^31 (got %d, %d)", d->P, d->M);
   // 32-key steps over all sequences and blocks of 16 query heads are counted in 32 bits.
   const int64_t steps = (int64_t)d->B * d->Hkv * ((d->Hq / d->Hkv + 15) / 16);
+  if (steps >= 1LL << 24)  // (a grid has fewer than 2^32 threads)
+    return capi_fail(MOE_EINVAL, "B * Hkv * ceil(Hq / Hkv / 16) must be below 2^24 (got B %d, Hkv %d)", d->B, d->Hkv);
   if (steps > (1LL << 30) / (((int64_t)d->M * d->page + 31) / 32))
     return capi_fail(MOE_EINVAL, "B * Hkv * M * page / 32 must be at most 2^30 (B %d, Hkv %d, M %d, page %d)", d->B,
                      d->Hkv, d->M, d->page);

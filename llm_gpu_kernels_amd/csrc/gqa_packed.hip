@@ -131,14 +131,26 @@ __device__ __forceinline__ int quotient(int n, int d, uint32_t magic) {
   return d == 1 ? n : (int)__umulhi((uint32_t)n, magic);
 }
 
-// Sequence s, its bounds forced into [0, N].
-__device__ __forceinline__ Rows sequence(const GqaPackedArgs &a, int s) {
-  const int lo = a.starts[s], hi = a.starts[s + 1], b = max(0, min(lo, a.N));
-  if (lo < 0 || hi < lo || hi > a.N) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
-  return Rows{b, max(0, min(hi, a.N) - b), 0, 0};
+// Bound s of the sequences as given, forced into [0, N].
+__device__ __forceinline__ int bound(const GqaPackedArgs &a, int s) { return max(0, min(a.starts[s], a.N)); }
+// Reports bounds that are not what they are taken as.
+__device__ __forceinline__ void check_bounds(const GqaPackedArgs &a, int s, const Rows &q) {
+  if (a.starts[s] != q.start || a.starts[s + 1] != q.start + q.len) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
+}
+// Running maximum over the wave's lanes of numbers that are not negative (steps as
+// in wave_scan).  Bounds are taken as the largest so far, so that sequences never
+// overlap and there are no more tiles than the list has room for.
+__device__ __forceinline__ int wave_max_scan(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return x;
 }
 
-// The list of all sequences' tiles of R rows, those that see the most keys first
+// The list of all sequences' tiles, those that see the most keys first
 // (the last workgroups to run are short then).  One workgroup sorts them by counting
 // in kClasses classes of equally many stages; the order within a class does not
 // matter to any result.  A search of every workgroup for its own tile took 3 to 5 us
@@ -161,30 +173,49 @@ __device__ __forceinline__ int plan_scan(int x, int *lds, int *total) {
   *total = all;
   return before + incl - x;
 }
+// The largest of the earlier threads' numbers (not negative) and of all.
+__device__ __forceinline__ int plan_max_scan(int x, int *lds, int *top) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, incl = wave_max_scan(x);
+  __syncthreads();
+  if (lane == kWave - 1) lds[wave] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / kWave; ++w) {
+    const int v = lds[w];
+    before = max(before, w < wave ? v : 0);
+    all = max(all, v);
+  }
+  *top = all;
+  return max(before, incl);
+}
 template <bool LDS>  // S <= kPlanLds
 __global__ __launch_bounds__(kPlanThreads) void gqa_packed_plan(GqaPackedArgs a) {
   __shared__ int waves[kPlanThreads / kWave], count[kClasses], longest;
-  // Tiles before a sequence, and the sequences: [S + 1], [S].
-  __shared__ int sums[LDS ? kPlanLds + 1 : 1], first[LDS ? kPlanLds : 1], length[LDS ? kPlanLds : 1];
-  auto tiles_before = [&](int s) { return LDS ? sums[s] : a.tile_sums[s]; };
+  // Tiles before a sequence, and the sequences' starts and lengths, [S] each.
+  __shared__ int lds[3][LDS ? kPlanLds : 1];
+  int *const sums = LDS ? lds[0] : a.tile_sums;
+  int *const first = LDS ? lds[1] : a.tile_sums + a.S;
+  int *const length = LDS ? lds[2] : a.tile_sums + 2 * a.S;
   const int tid = threadIdx.x;
   if (tid == 0) longest = 0;
   count[tid] = 0;
-  int total = 0, most_here = 0;
+  int total = 0, top = 0, most_here = 0;
   for (int base = 0; base < a.S; base += kPlanThreads) {
     const int s = base + tid;
+    int here, all;
     Rows q = {0, 0, 0, 0};
-    if (s < a.S) q = sequence(a, s);
-    int all;
+    q.start = max(top, plan_max_scan(s < a.S ? bound(a, s) : 0, waves, &here));
+    if (s < a.S) {
+      q.len = max(0, bound(a, s + 1) - q.start);
+      check_bounds(a, s, q);
+    }
+    top = max(top, here);
     const int at = total + plan_scan((q.len * a.G + kTileRows - 1) / kTileRows, waves, &all);
     if (s < a.S) {
-      if (LDS) {
-        sums[s] = at;
-        first[s] = q.start;
-        length[s] = q.len;
-      } else {
-        a.tile_sums[s] = at;
-      }
+      sums[s] = at;
+      first[s] = q.start;
+      length[s] = q.len;
     }
     total += all;
     most_here = max(most_here, q.len);
@@ -201,11 +232,10 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_packed_plan(GqaPackedArgs a)
     int lo = 0, hi = a.S - 1;  // the last sequence with at most i tiles before it
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (tiles_before(mid) <= i) lo = mid;
+      if (sums[mid] <= i) lo = mid;
       else hi = mid - 1;
     }
-    Rows w = LDS ? Rows{first[lo], length[lo], 0, 0} : sequence(a, lo);
-    w.tile = i - tiles_before(lo);
+    const Rows w = {first[lo], length[lo], i - sums[lo], 0};
     const int keys = min(w.len, quotient(w.tile * kTileRows + kTileRows - 1, a.G, a.G_magic) + 1);
     const int shorter = most - (keys + kStageKeys - 1) / kStageKeys;  // 0 .. most - 1
     return Tile{w, most <= kClasses ? shorter : (int)((int64_t)shorter * (kClasses - 1) / most)};
@@ -303,8 +333,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void gqa_packed_kernel(GqaPackedArg
   const int kvh = (xcd & (7 >> a.class_xcds)) + ((in_class - nth * a.per_class) << (3 - a.class_xcds));
   Rows w;
   if (!a.listed) {  // S <= 64: in the order of the sequences, each one's longest first
-    Rows q = {0, 0, 0, 0};
-    if (lane < a.S) q = sequence(a, lane);
+    Rows q = {wave_max_scan(lane < a.S ? bound(a, lane) : 0), 0, 0, 0};
+    if (lane < a.S) {
+      q.len = max(0, bound(a, lane + 1) - q.start);
+      check_bounds(a, lane, q);
+    }
     const int T = (q.len * G + kTileRows - 1) / kTileRows, incl = wave_scan(T);
     const uint64_t behind = __builtin_amdgcn_ballot_w64(incl > nth);
     if (!behind) return;
@@ -607,9 +640,9 @@ size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 size_t list_entries(int N, int G, int S) { return (size_t)max_tiles(N, G, S) + kXcds; }
 }  // namespace
 
-// {status and number of tiles; the tiles; the sums of the tiles before a sequence}
+// {status and number of tiles; the tiles; three numbers per sequence}
 size_t gqa_packed_workspace(int N, int Hq, int Hkv, int S) {
-  return 256 + align256(list_entries(N, Hq / Hkv, S) * sizeof(Rows)) + ((size_t)S + 1) * 4;
+  return 256 + align256(list_entries(N, Hq / Hkv, S) * sizeof(Rows)) + (S <= kPlanLds ? 0 : (size_t)S * 12);
 }
 
 void gqa_packed_bind(GqaPackedArgs *a, void *workspace) {

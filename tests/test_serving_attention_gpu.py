@@ -180,6 +180,36 @@ def test_packed_bad_starts(gpu_device):
     assert torch.equal(plan.run(), clean)
 
 
+@pytest.mark.parametrize("count", [5, 64, 100, 3000])
+def test_packed_starts_without_order(count, gpu_device):
+    """Starts in any order are taken as the largest so far within [0, N], found by
+    a wave, by the sorted list and by the list of many sequences."""
+    n = 400
+    q, k, v, _, _ = _packed([n], 4, 2, 64, torch.bfloat16, gpu_device)
+    g = torch.Generator().manual_seed(count)
+    raw = torch.randint(-200, 700, (count + 1,), generator=g)
+    if count > 64:  # most of them within a narrow range, rising slowly
+        raw = (torch.arange(count + 1) * n // count + torch.randint(-30, 30, (count + 1,), generator=g))
+    raw[0] = 7
+    starts = torch.cummax(raw.clamp(0, n), 0).values.tolist()
+    out = torch.full((n, 4, 64), 3.0, dtype=torch.bfloat16, device=gpu_device)
+    plan = prepare_packed_gqa(q, k, v, raw.to(torch.int32).to(gpu_device), out)
+    _check_packed(plan, starts)
+    assert (out[:7] == 3).all() and (out[starts[-1]:] == 3).all()
+    with pytest.raises(ValueError, match="starts"):
+        plan.check_inputs()
+
+
+@pytest.mark.parametrize("count", [2100, 5000])
+def test_packed_many_sequences_listed(count, gpu_device):
+    """More sequences than the sorting workgroup holds in LDS."""
+    lengths = [(5 * i) % 7 for i in range(count)]
+    q, k, v, starts, on_gpu = _packed(lengths, 2, 1, 64, torch.bfloat16, gpu_device)
+    plan = prepare_packed_gqa(q, k, v, on_gpu)
+    _check_packed(plan, starts)
+    plan.check_inputs()
+
+
 # ---- paged decode -----------------------------------------------------------------
 
 

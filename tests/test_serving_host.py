@@ -34,7 +34,7 @@ def _packed(**kw):
 
 @pytest.mark.parametrize("bad", [
     dict(D=96), dict(D=256), dict(Hq=31), dict(Hkv=0), dict(Hq=0), dict(Hq=65, Hkv=1), dict(dtype=2), dict(N=-1),
-    dict(N=1 << 29), dict(S=-1), dict(S=(1 << 20) + 1), dict(q=None), dict(k=BASE + 8), dict(out=None), dict(starts=None),
+    dict(N=1 << 29), dict(N=1 << 24), dict(S=1 << 20, N=1 << 22, Hq=32, Hkv=32), dict(S=-1), dict(S=(1 << 20) + 1), dict(q=None), dict(k=BASE + 8), dict(out=None), dict(starts=None),
     dict(starts=BASE + 2), dict(q_stride=4088), dict(k_stride=1028), dict(v_stride=0), dict(k_stride=(1 << 25) + 8),
     dict(workspace=None), dict(workspace_bytes=0),
 ])
@@ -61,7 +61,7 @@ def _paged(**kw):
 
 @pytest.mark.parametrize("bad", [
     dict(D=80), dict(Hq=12), dict(Hq=520, Hkv=8), dict(dtype=-1), dict(B=-1), dict(B=(1 << 16) + 1), dict(page=0),
-    dict(page=8), dict(page=24), dict(page=2048), dict(P=0), dict(M=0), dict(M=1 << 27), dict(q=None), dict(k=BASE + 4),
+    dict(page=8), dict(page=24), dict(page=2048), dict(P=0), dict(M=0), dict(M=1 << 27), dict(M=1 << 22), dict(B=1 << 16, Hq=1024, Hkv=1024, M=1), dict(q=None), dict(k=BASE + 4),
     dict(v=None), dict(tables=None), dict(lengths=BASE + 1), dict(table_stride=19), dict(q_stride=4092),
     dict(k_strides=(16384, 2048, 120)), dict(k_strides=(0, 2048, 128)), dict(v_strides=(16384, 2044, 128)),
     dict(v_strides=(16384, 2048, (1 << 25) + 8)), dict(workspace=None), dict(workspace_bytes=0),
