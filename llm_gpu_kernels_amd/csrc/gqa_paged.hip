@@ -465,7 +465,7 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
 // -inf) has weight 0, a row without any is 0; NaN passes through.  Sequences of
 // length 0 get their zeros here.
 constexpr int kMergeThreads = 256;
-constexpr int kBatch = 8;
+constexpr int kBatch = 16;
 struct State {
   float m, l;
   f32x2_t o;

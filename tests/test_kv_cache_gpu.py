@@ -264,3 +264,29 @@ def test_large_pages_and_offsets(gpu_device):
     assert c.tables[:2, 0].tolist() == [0, 1] and c.read_status() == 0 and c.used_pages.item() == 2
     for p in (0, 1):
         assert torch.equal(c.k[0, p, :, :5], row.transpose(0, 1)) and torch.equal(c.v[0, p, :, :5], -row.transpose(0, 1))
+
+
+def test_as_many_pages_and_tokens_as_allowed(gpu_device):
+    """2^20 pages, all but some at the end in use, and a reserve of 2^20 tokens."""
+    pages, tokens = N.KV_MAX_PAGES, N.KV_MAX_TOKENS
+    c = PagedKVCache(pages, 16, 1, 64, sequences=3, max_pages=pages, max_tokens=tokens, device=gpu_device)
+    c.refs[:pages - 70000] = 1
+    c.reserve(_i32([tokens - 1000, 0, 1000], gpu_device))
+    need = [-(-(tokens - 1000) // 16), 0, 63]
+    first = pages - 70000
+    assert c.read_status() == 0 and c.lengths.tolist() == [tokens - 1000, 0, 1000]
+    ids = torch.arange(first, first + sum(need), dtype=torch.int32, device=gpu_device)
+    assert torch.equal(c.tables[0, :need[0]], ids[:need[0]]) and torch.equal(c.tables[2, :63], ids[need[0]:])
+    at = torch.arange(tokens, device=gpu_device)
+    row_start = torch.where(at < tokens - 1000, 0, tokens - 1000)
+    page = torch.where(at < tokens - 1000, first, first + need[0]) + (at - row_start) // 16
+    assert torch.equal(c.slots, page * 16 + (at - row_start) % 16)
+    c.refs[:first] = 0
+    c.refs[5] = 1
+    c.k[0, first + 3].fill_(3.0)
+    c.compact()
+    assert c.read_status() == 0 and c.used_pages.item() == sum(need) + 1
+    # Pages below the count that are free, in order, took the used ones from it on.
+    free = torch.tensor([p for p in range(sum(need) + 1) if p != 5], device=gpu_device)
+    assert torch.equal(c.tables[0, :need[0]].long(), free[:need[0]]) and (c.k[0, free[3]] == 3).all()
+    assert c.refs[:sum(need) + 1].min() == 1 and c.refs[sum(need) + 1:].max() == 0

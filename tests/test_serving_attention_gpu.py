@@ -490,3 +490,62 @@ def test_serving_a_batch(gpu_device):
     assert c.read_status() == 0
     for p in plans:
         p.check_inputs()
+
+
+def test_packed_offsets_past_32_bits(gpu_device):
+    """Token strides that put the last keys, values and queries more than 2^32
+    bytes from the base."""
+    n, wide = 70000, 1 << 16
+    base = torch.empty(n, wide, dtype=torch.bfloat16, device=gpu_device)
+    assert base.numel() * 2 > 1 << 33
+    g = torch.Generator(device=gpu_device).manual_seed(5)
+    q, k, v = (base[:, i * 4096:i * 4096 + h * 64].unflatten(1, (h, 64)) for i, h in enumerate((8, 1, 1)))
+    for t in (q, k, v):
+        t.copy_(torch.randn(t.shape, generator=g, device=gpu_device))
+    starts = [0, 69300, 69301, 70000]
+    plan = prepare_packed_gqa(q, k, v, torch.tensor(starts, dtype=torch.int32, device=gpu_device))
+    qc, kc, vc = q.cpu(), k.cpu(), v.cpu()
+    for t in (0, 31, 4097, 32768, 69299, 69300, 69301, 69999):
+        first = max(s for s in starts[:-1] if s <= t)
+        ref, bound = S.attention_rows(qc[t], kc[first:t + 1], vc[first:t + 1])
+        _assert_close(plan.output[t], ref, bound, t + 1 - first, 6.0)
+    plan.check_inputs()
+
+
+def test_paged_as_many_rows_as_allowed(gpu_device):
+    """2^16 sequences of 0 to 3 pages that share 50 pages."""
+    b, pages = 1 << 16, 50
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn(pages, 1, 16, 64, generator=g).to(torch.float16).to(gpu_device) for _ in range(2))
+    tables = torch.randint(0, pages, (b, 3), generator=g, dtype=torch.int32)
+    lengths = torch.randint(0, 49, (b,), generator=g, dtype=torch.int32)
+    q = torch.randn(b, 2, 64, generator=g).to(torch.float16)
+    plan = prepare_paged_gqa(q.to(gpu_device), k, v, tables.to(gpu_device), lengths.to(gpu_device))
+    rows = list(range(0, b, 997)) + [b - 1]
+    ref, bound = S.paged_attention(q[rows], k.cpu(), v.cpu(), tables[rows].tolist(), lengths[rows].tolist())
+    _assert_close(plan.output[rows], ref, bound, 48, 5.0)
+    assert (plan.output[(lengths == 0).to(gpu_device)] == 0).all()
+    plan.check_inputs()
+
+
+def test_two_plans_on_two_streams(gpu_device):
+    """Plans of their own run side by side, with the same inputs and pages."""
+    q, k, v, starts, on_gpu = _packed([900, 3, 400], 16, 4, 128, torch.bfloat16, gpu_device)
+    pq, pk, pv, tables, gt, gl = _paged([2000, 5, 700], 16, 4, 128, 16, torch.bfloat16, gpu_device)
+    packed = [prepare_packed_gqa(q, k, v, on_gpu) for _ in range(2)]
+    paged = [prepare_paged_gqa(pq, pk, pv, gt, gl) for _ in range(2)]
+    want = packed[0].output.clone(), paged[0].output.clone()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device=gpu_device) for _ in range(2)]
+    for _ in range(3):
+        for p in packed + paged:
+            p.output.zero_()
+        torch.cuda.synchronize()
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                for _ in range(4):
+                    (packed if i else paged)[i].run()
+                    (paged if i else packed)[i].run()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(packed[i].output, want[0]) and torch.equal(paged[i].output, want[1])
