@@ -93,5 +93,15 @@ __device__ __forceinline__ float quad_sum(float x) {
   return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
+// An MFMA's results take up to 19 wait states, and across a branch the compiler can
+// miss that they are not there yet.  Where they are read in another block than
+// the MFMA's, mfma_settle() stands before, or two later MFMAs (each waits for the
+// one before), and pin() keeps the reads behind that.
+__device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 3" ::: "memory"); }
+__device__ __forceinline__ float pin(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 }  // namespace gqa
 }  // namespace moe

@@ -100,15 +100,6 @@ __device__ __forceinline__ f32x2_t halves(float x) {
   const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return f32x2_t{__uint_as_float(h[0]), __uint_as_float(h[1])};
 }
-// An MFMA's results take up to 19 wait states, and across a branch the compiler can
-// miss that they are not there yet.  Where they are read in another block than
-// the MFMA's, mfma_settle() stands before, or two later MFMAs (each waits for the
-// one before), and pin() keeps the reads behind that.
-__device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 3" ::: "memory"); }
-__device__ __forceinline__ float pin(float x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
 template <bool F16>
 __device__ __forceinline__ bool not_finite2(uint32_t w) {
   constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;

@@ -13,11 +13,19 @@
 //   * a wave's range may end inside a (sequence, head).  Such pieces leave their
 //     (max, sum, O) in the workspace and a second launch joins them in the order
 //     of the keys; whole ones are written at once;
+//   * where even a full table is a few steps per wave, a workgroup takes a
+//     (sequence, head) instead, its waves' states are joined in LDS, and the second
+//     launch falls away (team_of() has the rule);
 //   * K and V rows go from HBM to LDS in whole rows (buffer loads with an LDS
 //     destination, a descriptor per 16-key block: a block lies in one page),
 //     permuted within a row so that the operand reads have no bank conflicts.
 // Scores are computed transposed, S^T = K Q^T, so they land in the A layout of
 // the P.V product; V comes back transposed with ds_read_b64_tr_b16.
+//
+// Measured, a copy of 2 GiB running at 5.0 TB/s: one sequence of 131072 tokens, 8 KV heads
+// of 128 (537 MB), 97 us and 6.5 us for the join, 5.2 TB/s; 64 sequences of 1 to 8192 (289
+// MB), 60 and 7 us, 4.3 TB/s; by teams, 200 sequences of 16 to 2000, 2 KV heads of 64 (52
+// MB), 14 us.
 #include "common.h"
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"
@@ -143,8 +151,12 @@ struct Step {
   int page[2], row[2], n[2];  // its 16-key blocks: page, first row, keys (0: none)
 };
 
-template <int D, bool F16>
-__global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(GqaPagedArgs a) {
+// TEAM 0: a range of the flat list per wave.  TEAM > 0: a workgroup of TEAM waves per
+// (sequence, head block), each taking every TEAM-th step, whose states are joined in
+// LDS at the end.
+template <int D, bool F16, int TEAM>
+__global__ __launch_bounds__(64 * (TEAM ? TEAM : kWaves), TEAM == 8 ? 1 : kWorkgroups<D>)
+void gqa_paged_kernel(GqaPagedArgs a) {
   constexpr int kSlices = D / 32;               // 32-dim slices of a row
   constexpr int kTiles = D / 16;                // 16-dim tiles of O
   constexpr int kLoads = kBlock * D * 2 / 1024; // loads of a block
@@ -152,11 +164,13 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = sgpr(threadIdx.x >> 6);
   const int worker = sgpr(wave * gridDim.x + blockIdx.x), workers = gridDim.x * kWaves;  // few steps: on many CUs
+  constexpr bool kList = TEAM == 0;
   const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows, heads = a.Hkv * blocks;
   const int cap = a.M * a.page;
   uint8_t *const kst = smem + wave * kWaveLds<D>, *const vst = kst + kStage<D>, *const qst = vst + kStage<D>;
 
-  // ---- the wave's range of the flat list ----
+  // ---- the wave's range of the flat list, or its first step ----
+  auto steps_of = [](int keys) __attribute__((always_inline)) { return (keys + kStep - 1) / kStep; };
   // Lengths of 64 kWindow sequences from `window` on: i-th of a lane at 64 i + lane.
   int window = 0, lens[kWindow];
   auto load_lengths = [&]() __attribute__((always_inline)) {
@@ -172,48 +186,64 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
       lens[i] = ok;
     }
   };
-  auto steps_of = [](int len) __attribute__((always_inline)) { return (len + kStep - 1) / kStep; };
-  int sum = 0;
-  for (;; window += kWave * kWindow) {
-    load_lengths();
+  int b = -1, len = 0, head, s;           // of the next step, with its sequence's length
+  int steps, left;                        // of its (sequence, head block), of the wave
+  int per = 1, first = 0;                 // steps of a wave, the wave's first in the list
+  if constexpr (kList) {
+    int sum = 0;
+    for (;; window += kWave * kWindow) {
+      load_lengths();
 #pragma unroll
-    for (int i = 0; i < kWindow; ++i) sum += steps_of(lens[i]);
-    if (window + kWave * kWindow >= a.B) break;
-  }
-  const int all = wave_total(sum) * heads;                // < 2^31, checked on the host
-  const int per = (all + workers - 1) / workers;          // steps of a wave
-  if ((int64_t)worker * per >= all) return;
-  const int first = worker * per;
-  int left = min(per, all - first);
-  if (window > 0) {
-    window = 0;
-    load_lengths();
-  }
-  // The sequence where the range begins, and the steps before it.
-  int b = -1, len = 0, before = 0;
-  while (b < 0) {
-#pragma unroll
-    for (int i = 0; i < kWindow; ++i) {
-      const int incl = before + wave_scan(steps_of(lens[i]) * heads);
-      const uint64_t past = __builtin_amdgcn_ballot_w64(incl > first);
-      if (b < 0) {
-        if (past) {
-          const int at = sgpr(__builtin_ctzll(past));
-          b = window + kWave * i + at;
-          len = __builtin_amdgcn_readlane(lens[i], at);
-          before = __builtin_amdgcn_readlane(incl, at) - steps_of(len) * heads;
-        } else {
-          before = __builtin_amdgcn_readlane(incl, 63);
-        }
-      }
+      for (int i = 0; i < kWindow; ++i) sum += steps_of(lens[i]);
+      if (window + kWave * kWindow >= a.B) break;
     }
-    if (b < 0) {
-      window += kWave * kWindow;
-      if (window >= a.B) return;  // only if lengths change meanwhile
+    const int all = wave_total(sum) * heads;                // < 2^31, checked on the host
+    per = (all + workers - 1) / workers;
+    if ((int64_t)worker * per >= all) return;
+    first = worker * per;
+    left = min(per, all - first);
+    if (window > 0) {
+      window = 0;
       load_lengths();
     }
+    // The sequence where the range begins, and the steps before it.
+    int before = 0;
+    while (b < 0) {
+#pragma unroll
+      for (int i = 0; i < kWindow; ++i) {
+        const int incl = before + wave_scan(steps_of(lens[i]) * heads);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(incl > first);
+        if (b < 0) {
+          if (past) {
+            const int at = sgpr(__builtin_ctzll(past));
+            b = window + kWave * i + at;
+            len = __builtin_amdgcn_readlane(lens[i], at);
+            before = __builtin_amdgcn_readlane(incl, at) - steps_of(len) * heads;
+          } else {
+            before = __builtin_amdgcn_readlane(incl, 63);
+          }
+        }
+      }
+      if (b < 0) {
+        window += kWave * kWindow;
+        if (window >= a.B) return;  // only if lengths change meanwhile
+        load_lengths();
+      }
+    }
+    steps = steps_of(len);
+    const int rest = first - before;
+    head = rest / steps;
+    s = rest % steps;
+  } else {
+    b = blockIdx.x / heads;
+    head = blockIdx.x % heads;
+    const int raw = a.lengths[b];
+    len = sgpr(max(0, min(raw, cap)));
+    if (raw != len && threadIdx.x == 0) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
+    steps = steps_of(len);
+    s = wave;
+    left = s < steps ? (steps - s + TEAM - 1) / TEAM : 0;
   }
-  int steps = steps_of(len);
   // The next sequence that has keys, from `from` on; -1 only if lengths change
   // meanwhile.
   auto next_sequence = [&](int from) __attribute__((always_inline)) {
@@ -236,8 +266,6 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
       load_lengths();
     }
   };
-  const int rest = first - before;
-  int head = rest / steps, s = rest % steps;
   const int per_page = a.page / kBlock;
   int page_at = 2 * s / per_page, block_at = 2 * s % per_page;  // of the next step's first block
 
@@ -264,7 +292,13 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
       block_at = 0;
       ++page_at;
     }
-    if (--left > 0 && ++s == steps) {
+    if constexpr (!kList) {
+      --left;
+      s += TEAM;
+      block_at += 2 * (TEAM - 1);
+      page_at += block_at / per_page;
+      block_at %= per_page;
+    } else if (--left > 0 && ++s == steps) {
       s = page_at = block_at = 0;
       if (++head == heads) {
         head = 0;
@@ -405,7 +439,7 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
 
     // ---- the end of a piece ----
     const bool pair_ends = cur.s + 1 == cur.steps;
-    if (pair_ends || nx.n[0] == 0) {
+    if (kList && (pair_ends || nx.n[0] == 0)) {
       const int kvh = cur.head / blocks, part = cur.head % blocks, rows = min(kRows, group - kRows * part);
       const int64_t head0 = (int64_t)cur.b * a.Hq + kvh * group + kRows * part;
       const float l = quad_sum(l_run);
@@ -456,6 +490,47 @@ __global__ __launch_bounds__(64 * kWaves, kWorkgroups<D>) void gqa_paged_kernel(
   }
   wait_vmcnt<0>();  // the last (empty) step's loads write LDS
   if (bad_page && lane == 0) atomicOr(a.status, GQA_STATUS_BAD_PAGE);
+
+  if constexpr (!kList) {
+    // The waves' states, each in its own part of the LDS: O, then m and l per row.
+    const int kvh = head / blocks, part = head % blocks, rows = min(kRows, group - kRows * part);
+    const float l = quad_sum(l_run);
+    float *const mine = (float *)kst;
+    mfma_settle();
+    if (g == 0) {
+      mine[kRows * D + r] = m_run;
+      mine[kRows * D + kRows + r] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * g + i < rows) {
+#pragma unroll
+        for (int dt = 0; dt < kTiles; ++dt) mine[(4 * g + i) * D + 16 * dt + r] = pin(o[dt][i]);
+      }
+    __syncthreads();
+    uint32_t *const out = (uint32_t *)(a.out + ((int64_t)b * a.Hq + kvh * group + kRows * part) * D);
+    for (int e = 2 * threadIdx.x; e < rows * D; e += 2 * 64 * TEAM) {
+      const int row = e / D;
+      float m[TEAM], top = -INFINITY, den = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+      for (int w = 0; w < TEAM; ++w) {
+        m[w] = ((const float *)(smem + w * kWaveLds<D>))[kRows * D + row];
+        top = fmaxf(top, m[w]);
+      }
+      const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < TEAM; ++w) {
+        const float *const x = (const float *)(smem + w * kWaveLds<D>);
+        const float f = __builtin_amdgcn_exp2f(m[w] - ref);
+        const f32x2_t v = *(const f32x2_t *)(x + e);
+        den = __builtin_fmaf(f, x[kRows * D + kRows + row], den);
+        o0 = __builtin_fmaf(f, v[0], o0);
+        o1 = __builtin_fmaf(f, v[1], o1);
+      }
+      const float inv = den == 0.f ? 0.f : 1.0f / den;
+      out[e / 2] = pack2<F16>(o0 * inv, o1 * inv);
+    }
+  }
 }
 
 // Joins the pieces of a (sequence, head block), in the order of the keys.  A thread
@@ -541,26 +616,52 @@ __global__ __launch_bounds__(kMergeThreads) void gqa_paged_merge(GqaPagedArgs a,
 
 __global__ void clear_word(uint32_t *w) { *w = 0; }
 
-template <int D, bool F16>
-hipError_t launch(const GqaPagedArgs &a, int cus, hipStream_t s) {
-  auto k = gqa_paged_kernel<D, F16>;
-  constexpr int lds = kWaves * kWaveLds<D>;
+int waves_of(int D, int cus) { return cus * kWaves * (D == 128 ? kWorkgroups<128> : kWorkgroups<64>); }
+
+// Waves of a workgroup per (sequence, head block), or 0 for the list and its merge,
+// by the steps of a full table.  A team needs no second launch (4 to 7 us), but has all
+// of its sequence, however long it is.  So: eight waves if all teams then run at
+// once, else four (short prologues overlap; 2048 teams, lengths 1..512: 42 us, by
+// eight 53); and a team only if one with a full table has at most 16 steps a wave, and
+// not many more than half of what the list would give a wave.  Heads of 128, all of
+// one length, list and team: 8 x 128 keys 9.2, 4.7 us; 128 x 512 keys 14.0, 7.8; 128 x
+// 2048 keys 28, 22; 2048 of 1..1024 keys 98, 80; one sequence of 2048 keys among
+// 15 of 40: 13.0, 13.7.  Left to the list: 8 x 2048 keys 10.1, 13.6; 8 x 4096 keys
+// 11.8, 22.5.
+int team_of(int64_t pairs, int64_t steps, int64_t waves) {
+  const int team = 8 * pairs <= waves ? 8 : 4;
+  const int64_t listed = (pairs * steps + waves - 1) / waves, teamed = (steps + team - 1) / team;
+  return teamed <= 16 && teamed <= listed / 2 + 6 ? team : 0;
+}
+
+template <int D, bool F16, int TEAM>
+hipError_t launch_kernel(const GqaPagedArgs &a, int grid, hipStream_t s) {
+  auto k = gqa_paged_kernel<D, F16, TEAM>;
+  constexpr int waves = TEAM ? TEAM : kWaves, lds = waves * kWaveLds<D>;
   static const bool attr = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds) ==
                            hipSuccess;
   if (!attr) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(k, dim3(cus * kWorkgroups<D>), dim3(64 * kWaves), lds, s, a);
-  const int group = a.Hq / a.Hkv, heads = a.Hkv * ((group + kRows - 1) / kRows);
+  hipLaunchKernelGGL(k, dim3(grid), dim3(64 * waves), lds, s, a);
+  return hipGetLastError();
+}
+
+template <int D, bool F16>
+hipError_t launch(const GqaPagedArgs &a, int cus, hipStream_t s) {
+  const int group = a.Hq / a.Hkv, heads = a.Hkv * ((group + kRows - 1) / kRows), pairs = a.B * heads;
+  const int team = team_of(pairs, ((int64_t)a.M * a.page + kStep - 1) / kStep, waves_of(D, cus));
+  if (team == 8) return launch_kernel<D, F16, 8>(a, pairs, s);
+  if (team == 4) return launch_kernel<D, F16, 4>(a, pairs, s);
+  const hipError_t e = launch_kernel<D, F16, 0>(a, cus * kWorkgroups<D>, s);
+  if (e != hipSuccess) return e;
   // Threads per piece in a merge workgroup: all of a (sequence, head block), two
   // elements each; fewer, and pieces shared out over groups, while that leaves CUs
   // without a workgroup.
-  const int need = min(group, kRows) * D / 2, pairs = a.B * heads;
+  const int need = min(group, kRows) * D / 2;
   int chunk = kMergeThreads;
   while (chunk > 16 && (chunk >= 2 * need || (int64_t)pairs * ((need + chunk - 1) / chunk) < cus)) chunk /= 2;
   hipLaunchKernelGGL(gqa_paged_merge<F16>, dim3(pairs, (need + chunk - 1) / chunk), dim3(kMergeThreads), 0, s, a, chunk);
   return hipGetLastError();
 }
-
-int waves_of(int D, int cus) { return cus * kWaves * (D == 128 ? kWorkgroups<128> : kWorkgroups<64>); }
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 

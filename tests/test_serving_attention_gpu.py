@@ -10,6 +10,7 @@ pytestmark = pytest.mark.gpu
 
 HEADS = [(32, 8, 128), (8, 8, 128), (12, 4, 64), (14, 2, 64), (6, 6, 64), (16, 1, 128), (40, 2, 128), (64, 1, 64)]
 TYPES = [torch.bfloat16, torch.float16]
+WIDE = [False, True]  # tables of decode attention
 
 
 def _assert_close(out, ref, bound, keys, vmax):
@@ -213,12 +214,13 @@ def test_packed_many_sequences_listed(count, gpu_device):
 # ---- paged decode -----------------------------------------------------------------
 
 
-def _paged(lengths, hq, hkv, d, page, dtype, device, order="heads", spare=3, seed=0):
+def _paged(lengths, hq, hkv, d, page, dtype, device, order="heads", spare=3, seed=0, wide=False):
     """Pages in a shuffled order; the places behind each sequence's end and the
-    spare pages hold NaN, table entries behind the last page an impossible one."""
+    spare pages hold NaN, table entries behind the last page an impossible one.
+    Wide tables have room for many more pages (another way to share the work out)."""
     g = torch.Generator().manual_seed(seed + sum(lengths) + page)
     used = [-(-n // page) for n in lengths]
-    count, width = sum(used) + spare, max(used) + 2
+    count, width = sum(used) + spare, 1000 if wide else max(used) + 2
     perm = torch.randperm(count, generator=g).tolist()
     shape = (count, hkv, page, d) if order == "heads" else (count, page, hkv, d)
     kv = [torch.randn(shape, generator=g).to(dtype) for _ in range(2)]
@@ -254,11 +256,12 @@ def _check_paged(plan, tables, lengths, scale=None):
             assert (plan.output[b] == 0).all()
 
 
+@pytest.mark.parametrize("wide", WIDE)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hq,hkv,d", HEADS)
-def test_paged_heads(hq, hkv, d, dtype, gpu_device):
+def test_paged_heads(hq, hkv, d, dtype, wide, gpu_device):
     lengths = [37, 0, 1, 200, 64]
-    q, k, v, tables, gt, gl = _paged(lengths, hq, hkv, d, 16, dtype, gpu_device)
+    q, k, v, tables, gt, gl = _paged(lengths, hq, hkv, d, 16, dtype, gpu_device, wide=wide)
     plan = prepare_paged_gqa(q, k, v, gt, gl)
     _check_paged(plan, tables, lengths)
     plan.check_inputs()
@@ -269,8 +272,9 @@ def test_paged_heads(hq, hkv, d, dtype, gpu_device):
     ([1000, 1, 47, 48, 49], 48), ([1500, 3], 1024), ([1024, 1025], 1024), ([9000, 12, 0, 400], 80),
     ([(37 * i) % 150 for i in range(130)], 16)], ids=lambda x: str(x)[:24])
 @pytest.mark.parametrize("order", ["heads", "tokens"])
-def test_paged_lengths(lengths, page, order, gpu_device):
-    q, k, v, tables, gt, gl = _paged(lengths, 8, 2, 128, page, torch.bfloat16, gpu_device, order)
+@pytest.mark.parametrize("wide", WIDE)
+def test_paged_lengths(lengths, page, order, wide, gpu_device):
+    q, k, v, tables, gt, gl = _paged(lengths, 8, 2, 128, page, torch.bfloat16, gpu_device, order, wide=wide)
     plan = prepare_paged_gqa(q, k, v, gt, gl)
     _check_paged(plan, tables, lengths)
     plan.check_inputs()
@@ -282,10 +286,11 @@ def test_paged_long_fp16_d64(gpu_device):
     _check_paged(prepare_paged_gqa(q, k, v, gt, gl, scale=0.25), tables, lengths, 0.25)
 
 
-def test_paged_many_rows(gpu_device):
+@pytest.mark.parametrize("wide", WIDE)
+def test_paged_many_rows(wide, gpu_device):
     """More sequences than a wave has lanes several times over, most of them empty."""
     lengths = [0 if i % 3 else (i * 7) % 60 for i in range(1500)]
-    q, k, v, tables, gt, gl = _paged(lengths, 4, 2, 64, 16, torch.bfloat16, gpu_device)
+    q, k, v, tables, gt, gl = _paged(lengths, 4, 2, 64, 16, torch.bfloat16, gpu_device, wide=wide)
     _check_paged(prepare_paged_gqa(q, k, v, gt, gl), tables, lengths)
 
 
@@ -306,11 +311,22 @@ def test_paged_shared_pages_and_strided_tables(gpu_device):
     plan.check_inputs()
 
 
-def test_paged_non_finite(gpu_device):
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (14, 2, 64), (40, 2, 128)])
+def test_paged_many_sequences(hq, hkv, d, gpu_device):
+    """Enough sequences that they are not all worked on at once."""
+    lengths = [(97 * i) % 400 for i in range(40960 // (hkv * d))]
+    q, k, v, tables, gt, gl = _paged(lengths, hq, hkv, d, 16, torch.bfloat16, gpu_device)
+    plan = prepare_paged_gqa(q, k, v, gt, gl)
+    _check_paged(plan, tables, lengths)
+    plan.check_inputs()
+
+
+@pytest.mark.parametrize("wide", WIDE)
+def test_paged_non_finite(wide, gpu_device):
     """Values that are seen and not finite reach the output, as do NaN keys; a key
     of -inf score drops out; other sequences keep their bits."""
     lengths = [300, 300, 300, 300]
-    q, k, v, tables, gt, gl = _paged(lengths, 8, 2, 128, 16, torch.bfloat16, gpu_device)
+    q, k, v, tables, gt, gl = _paged(lengths, 8, 2, 128, 16, torch.bfloat16, gpu_device, wide=wide)
     plan = prepare_paged_gqa(q, k, v, gt, gl)
     clean = plan.output.clone()
     v[tables[0][7], 0, 3, 100] = float("inf")
@@ -328,11 +344,12 @@ def test_paged_non_finite(gpu_device):
             assert out[2, h].isnan().all()
 
 
-def test_paged_bad_pages_and_lengths(gpu_device):
+@pytest.mark.parametrize("wide", WIDE)
+def test_paged_bad_pages_and_lengths(wide, gpu_device):
     """Page numbers outside the cache are left out, lengths outside the table taken
     as the nearest within; both are reported, the other sequences unchanged."""
     lengths = [60, 33, 100]
-    q, k, v, tables, gt, gl = _paged(lengths, 8, 2, 128, 16, torch.bfloat16, gpu_device)
+    q, k, v, tables, gt, gl = _paged(lengths, 8, 2, 128, 16, torch.bfloat16, gpu_device, wide=wide)
     plan = prepare_paged_gqa(q, k, v, gt, gl)
     clean = plan.output.clone()
     plan.check_inputs()
@@ -384,11 +401,12 @@ def test_paged_offsets_past_32_bits(gpu_device):
         del plan, k, v, kk, vv
 
 
-def test_paged_replays_and_streams(gpu_device):
+@pytest.mark.parametrize("wide", WIDE)
+def test_paged_replays_and_streams(wide, gpu_device):
     """One captured run, replayed on another stream while lengths, tables and
     values change, gives the eager bits; runs repeat their bits."""
     lengths = [1500, 1, 0, 333]
-    q, k, v, tables, gt, gl = _paged(lengths, 32, 8, 128, 16, torch.bfloat16, gpu_device)
+    q, k, v, tables, gt, gl = _paged(lengths, 32, 8, 128, 16, torch.bfloat16, gpu_device, wide=wide)
     k.nan_to_num_(0.5)
     v.nan_to_num_(0.5)
     plan, other = prepare_paged_gqa(q, k, v, gt, gl), prepare_paged_gqa(q, k, v, gt, gl)
