@@ -190,6 +190,15 @@ def _check_scale(scale, d):
     return float(scale)
 
 
+def _fp32_scale(scale, d):
+    """The scale as the kernels use it: a normal fp32 number whose product with
+    log2(e) is one too."""
+    value = ctypes.c_float(_check_scale(scale, d)).value
+    if not 2.0 ** -126 <= value <= 2.0 ** 127:
+        raise ValueError(f"scale must lie in [2^-126, 2^127] (got {scale!r})")
+    return value
+
+
 class _PreparedPlan:
     """A plan of the library with its workspace; ``run()`` enqueues on the
     current stream of q's device."""
@@ -210,7 +219,7 @@ class _PreparedPlan:
         self._fn, self._desc, self._plan, self._device = fn, desc, handle, device
 
     def _stream(self):
-        return ctypes.c_void_p(torch.cuda.current_stream(self._device).cuda_stream)
+        return ctypes.c_void_p(torch.cuda.current_stream(self._device.index).cuda_stream)
 
     def run(self):
         """Enqueue one pass on the current stream; returns the owned output."""
@@ -269,7 +278,7 @@ class PreparedPackedGQA(_PreparedPlan):
         d = N.GqaPackedDesc()
         d.N, d.Hq, d.D = q.shape
         d.S, d.Hkv, d.dtype = starts.shape[0] - 1, k.shape[1], _DTYPES[q.dtype]
-        d.scale = _check_scale(scale, d.D)
+        d.scale = _fp32_scale(scale, d.D)
         d.q_stride, d.k_stride, d.v_stride = (_token_stride(t, n) for t, n in ((q, "q"), (k, "k"), (v, "v")))
         out = _output(out, q)
         check_out_storage(out, [q, k, v, starts])
@@ -314,7 +323,7 @@ class PreparedPagedGQA(_PreparedPlan):
         d = N.GqaPagedDesc()
         d.B, d.Hq, d.D = q.shape
         d.Hkv, d.P, d.page, d.M, d.dtype = hkv, p, page, m, _DTYPES[q.dtype]
-        d.scale = _check_scale(scale, dim)
+        d.scale = _fp32_scale(scale, dim)
         d.q_stride, d.table_stride = _token_stride(q, "q"), _stride(tables, 0, m)
         for t, into in ((k_pages, d.k_strides), (v_pages, d.v_strides)):
             into[0], into[1], into[2] = _stride(t, 0, 8), _stride(t, 1, 8), _stride(t, 2, dim)

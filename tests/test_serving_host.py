@@ -126,7 +126,7 @@ def test_python_refusals():
                 (_rows(6, 128, 4).transpose(1, 2), k, k, starts), (_rows(6, 3, 128), k, k, starts), (q, k, k, starts)]:
         with pytest.raises(ValueError):  # the last: not on a GPU
             prepare_packed_gqa(*bad)
-    for scale in (0.0, -1.0, float("nan"), float("inf")):
+    for scale in (0.0, -1.0, float("nan"), float("inf"), 1e-45, 1e-50, 2e38, 1e39):
         with pytest.raises(ValueError, match="scale"):
             prepare_packed_gqa(q, k, k, starts, scale=scale)
     with pytest.raises(ValueError, match="share storage"):
