@@ -53,8 +53,10 @@ struct GqaPackedArgs {
   int32_t *num_tiles, *tiles, *tile_sums;  // workspace
   // Set by gqa_packed_constants: the group Hq / Hkv; log2 of the XCDs that share a
   // class of KV heads, and a class's heads; ceil(2^32 / G).
-  int G, class_xcds, per_class, listed;
+  int G, class_xcds, per_class;
   uint32_t G_magic;
+  // Set by the launch: entries of the list, 0 without one; CUs of an XCD.
+  int listed, xcd_cus;
 };
 size_t gqa_packed_workspace(int N, int Hq, int Hkv, int S);
 void gqa_packed_bind(GqaPackedArgs *a, void *workspace);

@@ -201,6 +201,16 @@ def test_packed_starts_without_order(count, gpu_device):
         plan.check_inputs()
 
 
+@pytest.mark.parametrize("count,hq,hkv,d", [(80, 40, 1, 64), (40, 16, 1, 128), (90, 24, 2, 128)])
+def test_packed_few_rounds(count, hq, hkv, d, gpu_device):
+    """More tiles than CUs, in a second round of workgroups that is not full."""
+    lengths = [(7 * i) % 20 * (5 if count < 64 else 1) for i in range(count)]
+    q, k, v, starts, on_gpu = _packed(lengths, hq, hkv, d, torch.bfloat16, gpu_device)
+    plan = prepare_packed_gqa(q, k, v, on_gpu)
+    _check_packed(plan, starts)
+    plan.check_inputs()
+
+
 @pytest.mark.parametrize("count", [2100, 5000])
 def test_packed_many_sequences_listed(count, gpu_device):
     """More sequences than the sorting workgroup holds in LDS."""
