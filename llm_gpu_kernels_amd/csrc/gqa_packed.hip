@@ -21,8 +21,15 @@
 // from LDS but issue at most one instruction in four cycles (2.13 ms).
 //
 // K and V come in stages of 32 keys, global -> LDS in whole rows (buffer loads with an
-// LDS destination; keys behind the sequence's end read as zeros), four stages ahead
-// in a ring of five, with one barrier per stage.
+// LDS destination; keys behind the sequence's end read as zeros), three to four
+// stages ahead in a ring of five, with one barrier per stage.
+//
+// Measured, 32 query heads of 128 on 8 KV heads, bf16: one prompt of 16384 tokens 2.0 ms, 1.10
+// PFLOP/s, the matrix cores 57 % busy (1.50 ms with inputs of 0: the card's power
+// bounds the rest; a matrix product of 16384 cubed runs at 1.30 and 1.78 PFLOP/s
+// then); 16 prompts of 65 to 1134 tokens 83 us behind 5 for the list: the start and
+// end of a tile, 5 us with one workgroup left beside it, and the longest tiles;
+// four prompts of up to 48 tokens 6 us: launch and one round of loads.
 #include "common.h"
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"

@@ -23,9 +23,9 @@
 // the P.V product; V comes back transposed with ds_read_b64_tr_b16.
 //
 // Measured, a copy of 2 GiB running at 5.0 TB/s: one sequence of 131072 tokens, 8 KV heads
-// of 128 (537 MB), 97 us and 6.5 us for the join, 5.2 TB/s; 64 sequences of 1 to 8192 (289
-// MB), 60 and 7 us, 4.3 TB/s; by teams, 200 sequences of 16 to 2000, 2 KV heads of 64 (52
-// MB), 14 us.
+// of 128 (537 MB), 96 us, 5.6 TB/s, and 6.4 us for the join; 64 sequences of 1 to 7787 (288
+// MB), 68 us with the join; by teams, 200 sequences of 16 to 1997, 2 KV heads of 64 (39
+// MB), 14.6 us, and one of 700, 8 heads of 128, 8.1 us: launch, table, keys, join.
 #include "common.h"
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"
