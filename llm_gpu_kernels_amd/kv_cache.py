@@ -16,7 +16,7 @@ import ctypes
 import torch
 
 from . import _native as N
-from .attention import _check_int32
+from .attention import _check_int32, _stream_of
 
 __all__ = ["PagedKVCache"]
 
@@ -81,8 +81,7 @@ class PagedKVCache:
         self._desc, self._cache = d, handle
 
     def _stream(self):
-        # By number: the device's name costs 0.8 us more to look up, of a call's 8.
-        return ctypes.c_void_p(torch.cuda.current_stream(self.device.index).cuda_stream)
+        return _stream_of(self.device)
 
     def _token_stride(self, t, name):
         """Token stride of new keys or values (alignment is checked by the library)."""
