@@ -190,6 +190,14 @@ def _check_scale(scale, d):
     return float(scale)
 
 
+def _set_sizes(desc, **sizes):
+    """32-bit fields of a descriptor (ctypes would drop the upper bits silently)."""
+    for name, value in sizes.items():
+        if value >= 2 ** 31:
+            raise ValueError(f"{name} must be below 2^31 (got {value})")
+        setattr(desc, name, value)
+
+
 def _fp32_scale(scale, d):
     """The scale as the kernels use it: a normal fp32 number whose product with
     log2(e) is one too."""
@@ -285,8 +293,8 @@ class PreparedPackedGQA(_PreparedPlan):
             raise ValueError("starts must be an int32 tensor [sequences + 1]")
         _check_int32(starts, "starts", (starts.shape[0],), q.device)
         d = N.GqaPackedDesc()
-        d.N, d.Hq, d.D = q.shape
-        d.S, d.Hkv, d.dtype = starts.shape[0] - 1, k.shape[1], _DTYPES[q.dtype]
+        _set_sizes(d, N=q.shape[0], Hq=q.shape[1], D=q.shape[2], S=starts.shape[0] - 1, Hkv=k.shape[1],
+                   dtype=_DTYPES[q.dtype])
         d.scale = _fp32_scale(scale, d.D)
         d.q_stride, d.k_stride, d.v_stride = (_token_stride(t, n) for t, n in ((q, "q"), (k, "k"), (v, "v")))
         out = _output(out, q)
@@ -330,8 +338,7 @@ class PreparedPagedGQA(_PreparedPlan):
         _check_int32(lengths, "lengths", (b,), q.device)
         p, hkv, page, dim = k_pages.shape
         d = N.GqaPagedDesc()
-        d.B, d.Hq, d.D = q.shape
-        d.Hkv, d.P, d.page, d.M, d.dtype = hkv, p, page, m, _DTYPES[q.dtype]
+        _set_sizes(d, B=b, Hq=q.shape[1], D=dim, Hkv=hkv, P=p, page=page, M=m, dtype=_DTYPES[q.dtype])
         d.scale = _fp32_scale(scale, dim)
         d.q_stride, d.table_stride = _token_stride(q, "q"), _stride(tables, 0, m)
         for t, into in ((k_pages, d.k_strides), (v_pages, d.v_strides)):

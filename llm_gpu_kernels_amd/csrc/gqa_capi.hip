@@ -176,7 +176,9 @@ int validate_paged(const gqa_paged_desc *d) {
   return rc;
 }
 
-size_t paged_workspace(const gqa_paged_desc *d, int cus) { return moe::gqa_paged_workspace(d->B, d->Hq, d->Hkv, d->D, cus); }
+size_t paged_workspace(const gqa_paged_desc *d, int cus) {
+  return moe::gqa_paged_workspace(d->B, d->Hq, d->Hkv, d->D, (int64_t)d->M * d->page, cus);
+}
 
 int need_workspace(const void *workspace, size_t have, size_t need) {
   if (!workspace || !aligned16(workspace) || have < need)

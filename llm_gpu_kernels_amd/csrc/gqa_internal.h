@@ -77,7 +77,7 @@ struct GqaPagedArgs {
                                          // (sequence, block of query heads)
   float *partial;                        // [2 per wave][rows]{m, l, O[D]}
 };
-size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int cus);
+size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int64_t keys, int cus);
 void gqa_paged_bind(GqaPagedArgs *a, void *workspace);
 hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s);
 

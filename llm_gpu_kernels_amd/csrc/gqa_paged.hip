@@ -667,10 +667,12 @@ size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 }  // namespace
 
-// {status words; two words per (sequence, head block); the pieces' states}
-size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int cus) {
+// {status words; two words per (sequence, head block); the pieces' states}; teams
+// have no pieces.
+size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int64_t keys, int cus) {
   const int group = Hq / Hkv, rows = group < kRows ? group : kRows;
   const size_t pairs = (size_t)B * Hkv * ((group + kRows - 1) / kRows);
+  if (team_of(pairs, (keys + kStep - 1) / kStep, waves_of(D, cus))) return 256;
   return 256 + align256(8 * pairs) + (size_t)2 * waves_of(D, cus) * rows * (D + 2) * sizeof(float);
 }
 

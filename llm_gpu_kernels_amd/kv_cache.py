@@ -125,10 +125,12 @@ class PagedKVCache:
         """Write token i's keys and values ([n, kv_heads, head_dim], the heads of
         a token side by side) to ``slots[i]`` of a layer, for every i < n whose
         slot is not -1."""
+        if not isinstance(layer, int) or not 0 <= layer < self.layers:
+            raise ValueError(f"layer must be an int in [0, {self.layers}) (got {layer!r})")
         ks, vs = self._token_stride(k, "k"), self._token_stride(v, "v")
         if k.shape[0] != v.shape[0]:
             raise ValueError("k and v must have the same number of tokens")
-        N.check(N.lib().kv_cache_append(self._cache, int(layer), k.data_ptr(), v.data_ptr(), ks, vs, k.shape[0],
+        N.check(N.lib().kv_cache_append(self._cache, layer, k.data_ptr(), v.data_ptr(), ks, vs, k.shape[0],
                                         self._stream()), "append")
 
     def fork(self, src, dst):

@@ -198,6 +198,32 @@ def test_append_one_token_of_odd_strides(gpu_device):
         assert torch.equal(kv.cpu().view(torch.int16), ours.view(torch.int16))
 
 
+def test_call_refusals(gpu_device):
+    """Arguments that the host can check are refused before anything is enqueued."""
+    p = Pair(gpu_device, 4, 16, 2, 2, 8, heads=2)
+    ok = torch.zeros(8, 2, 64, dtype=torch.bfloat16, device=gpu_device)
+    rows = torch.zeros(2, dtype=torch.int32, device=gpu_device)
+    for layer in (-1, 2, 2 ** 32, 1.0, None):
+        with pytest.raises(ValueError, match="layer"):
+            p.gpu.append(layer, ok, ok)
+    for k in (ok[:7], ok[:, :1], ok.half(), ok.cpu(), ok[:, :, ::2], torch.cat([ok, ok]), ok[0]):
+        with pytest.raises(ValueError):
+            p.gpu.append(0, k, ok)
+    with pytest.raises(ValueError, match="max_tokens"):
+        p.gpu.append(0, torch.cat([ok, ok]), torch.cat([ok, ok]))
+    with pytest.raises(ValueError):
+        p.gpu.append(0, ok.transpose(0, 1).contiguous().transpose(0, 1), ok)
+    for counts, stride in ((rows[:1], 0), (rows.cpu(), 0), (rows, -1), (rows, 5), (rows, 1.0)):
+        with pytest.raises(ValueError):
+            p.gpu.reserve(counts, stride)
+    with pytest.raises(TypeError):
+        p.gpu.reserve(rows.long())
+    for src, dst in ((rows, rows[:1]), (torch.cat([rows, rows]), torch.cat([rows, rows])), (rows[None], rows[None])):
+        with pytest.raises(ValueError):
+            p.gpu.fork(src, dst)
+    assert p.gpu.read_status() == 0 and torch.equal(p.gpu.k.cpu(), p.k) and not p.gpu.refs.any()
+
+
 def test_captured_steps(gpu_device):
     """A captured decode step (reserve and append) replayed on another stream,
     with eager forks and frees between, matches the oracle; so do captured

@@ -131,6 +131,10 @@ def test_python_refusals():
             prepare_packed_gqa(q, k, k, starts, scale=scale)
     with pytest.raises(ValueError, match="share storage"):
         prepare_packed_gqa(q, k, k, starts, out=q)
+    meta = q.to("meta")
+    many = torch.zeros(1, dtype=torch.int32, device="meta").expand(2 ** 32 + 2).clone()
+    with pytest.raises(ValueError, match="S must be below"):
+        prepare_packed_gqa(meta, k.to("meta"), k.to("meta"), many)
     pages, tables, lengths = _rows(9, 2, 16, 128), torch.zeros(6, 3, dtype=torch.int32), torch.zeros(6, dtype=torch.int32)
     with pytest.raises(TypeError):
         prepare_paged_gqa(q, pages, pages, tables.long(), lengths)
@@ -140,6 +144,9 @@ def test_python_refusals():
                 (q, pages, pages, tables, lengths)]:
         with pytest.raises(ValueError):
             prepare_paged_gqa(*bad)
+    huge = pages[:1].to("meta").expand(2 ** 31, 2, 16, 128)
+    with pytest.raises(ValueError, match="P must be below"):
+        prepare_paged_gqa(meta, huge, huge, tables.to("meta"), lengths.to("meta"))
     good = dict(sequences=4, max_pages=8, max_tokens=64)
     with pytest.raises(TypeError):
         PagedKVCache(10, 16, 2, 64, dtype=torch.float32, **good)
