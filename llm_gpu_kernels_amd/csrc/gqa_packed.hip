@@ -129,25 +129,14 @@ __device__ __forceinline__ int quotient(int n, int d, uint32_t magic) {
   return d == 1 ? n : (int)__umulhi((uint32_t)n, magic);
 }
 
-// Bound s of the sequences as given, forced into [0, N].
+// Bound s of the sequences as given, forced into [0, N].  Bounds are taken as the
+// largest so far, so that sequences never overlap and there are no more tiles than
+// the list has room for.
 __device__ __forceinline__ int bound(const GqaPackedArgs &a, int s) { return max(0, min(a.starts[s], a.N)); }
 // Reports bounds that are not what they are taken as.
 __device__ __forceinline__ void check_bounds(const GqaPackedArgs &a, int s, const Rows &q) {
   if (a.starts[s] != q.start || a.starts[s + 1] != q.start + q.len) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
 }
-// Running maximum over the wave's lanes of numbers that are not negative (steps as
-// in wave_scan).  Bounds are taken as the largest so far, so that sequences never
-// overlap and there are no more tiles than the list has room for.
-__device__ __forceinline__ int wave_max_scan(int x) {
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
-  return x;
-}
-
 // The list of all sequences' tiles, those that see the most keys first
 // (the last workgroups to run are short then).  One workgroup sorts them by counting
 // in kClasses classes of equally many stages; the order within a class does not

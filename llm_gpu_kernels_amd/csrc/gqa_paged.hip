@@ -15,7 +15,9 @@
 //     of the keys; whole ones are written at once;
 //   * where even a full table is a few steps per wave, a workgroup takes a
 //     (sequence, head) instead, its waves' states are joined in LDS, and the second
-//     launch falls away (team_of() has the rule);
+//     launch falls away (team_of() has the rule).  Where the table is wider than
+//     that but the lengths are not, the kernel finds out from the lengths and does
+//     the same, and the second launch has nothing to do;
 //   * K and V rows go from HBM to LDS in whole rows (buffer loads with an LDS
 //     destination, a descriptor per 16-key block: a block lies in one page),
 //     permuted within a row so that the operand reads have no bank conflicts.
@@ -26,6 +28,8 @@
 // of 128 (537 MB), 96 us, 5.6 TB/s, and 6.4 us for the join; 64 sequences of 1 to 7787 (288
 // MB), 68 us with the join; by teams, 200 sequences of 16 to 1997, 2 KV heads of 64 (39
 // MB), 14.6 us, and one of 700, 8 heads of 128, 8.1 us: launch, table, keys, join.
+#include <type_traits>
+
 #include "common.h"
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"
@@ -151,9 +155,16 @@ struct Step {
   int page[2], row[2], n[2];  // its 16-key blocks: page, first row, keys (0: none)
 };
 
-// TEAM 0: a range of the flat list per wave.  TEAM > 0: a workgroup of TEAM waves per
-// (sequence, head block), each taking every TEAM-th step, whose states are joined in
-// LDS at the end.
+// The most steps of a wave with which teams are faster than the list, by those that
+// the list gives it (team_of() has figures).
+__host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 20 ? 16 : (int)listed / 2 + 6; }
+
+// TEAM > 0: a workgroup of TEAM waves per (sequence, head block), each taking every
+// TEAM-th step, whose states are joined in LDS at the end.  TEAM 0: a range of the
+// flat list per wave, or teams of the workgroups' waves if the lengths make those
+// faster (tables of 8192 keys, 8 heads of 128: 64 sequences of 128 keys 14.5 us by the list,
+// 9.3 so, 16 of 500 13.7, 10.1, 64 of 1000 48.4, 41.6; what the list loses by
+// looking is 0.3 us).
 template <int D, bool F16, int TEAM>
 __global__ __launch_bounds__(64 * (TEAM ? TEAM : kWaves), TEAM == 8 ? 1 : kWorkgroups<D>)
 void gqa_paged_kernel(GqaPagedArgs a) {
@@ -164,7 +175,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = sgpr(threadIdx.x >> 6);
   const int worker = sgpr(wave * gridDim.x + blockIdx.x), workers = gridDim.x * kWaves;  // few steps: on many CUs
-  constexpr bool kList = TEAM == 0;
+  constexpr int kTeam = TEAM ? TEAM : kWaves;
   const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows, heads = a.Hkv * blocks;
   const int cap = a.M * a.page;
   uint8_t *const kst = smem + wave * kWaveLds<D>, *const vst = kst + kStage<D>, *const qst = vst + kStage<D>;
@@ -188,17 +199,24 @@ void gqa_paged_kernel(GqaPagedArgs a) {
   };
   int b = -1, len = 0, head, s;           // of the next step, with its sequence's length
   int steps, left;                        // of its (sequence, head block), of the wave
-  int per = 1, first = 0;                 // steps of a wave, the wave's first in the list
-  if constexpr (kList) {
-    int sum = 0;
+  int all = 0, per = 1, first = 0;        // steps, those of a wave, the wave's first in the list
+  bool team = TEAM > 0;
+  if constexpr (TEAM == 0) {
+    int sum = 0, most = 0;
     for (;; window += kWave * kWindow) {
       load_lengths();
 #pragma unroll
-      for (int i = 0; i < kWindow; ++i) sum += steps_of(lens[i]);
+      for (int i = 0; i < kWindow; ++i) {
+        sum += steps_of(lens[i]);
+        most = max(most, steps_of(lens[i]));
+      }
       if (window + kWave * kWindow >= a.B) break;
     }
-    const int all = wave_total(sum) * heads;                // < 2^31, checked on the host
+    all = wave_total(sum) * heads;                          // < 2^31, checked on the host
     per = (all + workers - 1) / workers;
+    team = a.B * heads <= (int)gridDim.x && !__builtin_amdgcn_ballot_w64(most > kTeam * most_teamed(per));
+  }
+  if (!team) {
     if ((int64_t)worker * per >= all) return;
     first = worker * per;
     left = min(per, all - first);
@@ -235,6 +253,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
     head = rest / steps;
     s = rest % steps;
   } else {
+    if ((int)blockIdx.x >= a.B * heads) return;
     b = blockIdx.x / heads;
     head = blockIdx.x % heads;
     const int raw = a.lengths[b];
@@ -242,7 +261,9 @@ void gqa_paged_kernel(GqaPagedArgs a) {
     if (raw != len && threadIdx.x == 0) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
     steps = steps_of(len);
     s = wave;
-    left = s < steps ? (steps - s + TEAM - 1) / TEAM : 0;
+    left = s < steps ? (steps - s + kTeam - 1) / kTeam : 0;
+    // For the launch that joins the list's pieces: nothing to do here.
+    if (TEAM == 0 && threadIdx.x == 0) a.pieces[2 * blockIdx.x + 1] = 0;
   }
   // The next sequence that has keys, from `from` on; -1 only if lengths change
   // meanwhile.
@@ -269,268 +290,276 @@ void gqa_paged_kernel(GqaPagedArgs a) {
   const int per_page = a.page / kBlock;
   int page_at = 2 * s / per_page, block_at = 2 * s % per_page;  // of the next step's first block
 
-  // The next step of the range; none left: no keys.
-  auto next_step = [&]() __attribute__((always_inline)) {
-    Step t;
-    t.b = b;
-    t.head = head;
-    t.s = s;
-    t.steps = steps;
-    const int n = left > 0 ? min(kStep, len - kStep * s) : 0;
-    t.n[0] = min(kBlock, n);
-    t.n[1] = max(0, n - kBlock);
-    t.row[0] = block_at * kBlock;
-    const int32_t *const table = a.tables + (int64_t)b * a.table_stride;
-    t.page[0] = n > 0 ? uniform_load(table + page_at) : 0;
-    if (++block_at == per_page) {
-      block_at = 0;
-      ++page_at;
-    }
-    t.row[1] = block_at * kBlock;
-    t.page[1] = n > kBlock ? uniform_load(table + page_at) : 0;
-    if (++block_at == per_page) {
-      block_at = 0;
-      ++page_at;
-    }
-    if constexpr (!kList) {
-      --left;
-      s += TEAM;
-      block_at += 2 * (TEAM - 1);
-      page_at += block_at / per_page;
-      block_at %= per_page;
-    } else if (--left > 0 && ++s == steps) {
-      s = page_at = block_at = 0;
-      if (++head == heads) {
-        head = 0;
-        const int next = next_sequence(b + 1);
-        if (next < 0) {
-          left = 0;
-        } else {
-          b = next;
-          steps = steps_of(len);
+  // Its steps; by teams or by the list (each with code of its own: tests of `team` in the
+  // steps cost the list 1 to 3 %).
+  auto work = [&](auto mode) __attribute__((always_inline)) {
+    constexpr bool kTeams = decltype(mode)::value;
+    // The next step of the range; none left: no keys.
+    auto next_step = [&]() __attribute__((always_inline)) {
+      Step t;
+      t.b = b;
+      t.head = head;
+      t.s = s;
+      t.steps = steps;
+      const int n = left > 0 ? min(kStep, len - kStep * s) : 0;
+      t.n[0] = min(kBlock, n);
+      t.n[1] = max(0, n - kBlock);
+      t.row[0] = block_at * kBlock;
+      const int32_t *const table = a.tables + (int64_t)b * a.table_stride;
+      t.page[0] = n > 0 ? uniform_load(table + page_at) : 0;
+      if (++block_at == per_page) {
+        block_at = 0;
+        ++page_at;
+      }
+      t.row[1] = block_at * kBlock;
+      t.page[1] = n > kBlock ? uniform_load(table + page_at) : 0;
+      if (++block_at == per_page) {
+        block_at = 0;
+        ++page_at;
+      }
+      if constexpr (kTeams) {
+        --left;
+        s += kTeam;
+        block_at += 2 * (kTeam - 1);
+        page_at += block_at / per_page;
+        block_at %= per_page;
+      } else if (--left > 0 && ++s == steps) {
+        s = page_at = block_at = 0;
+        if (++head == heads) {
+          head = 0;
+          const int next = next_sequence(b + 1);
+          if (next < 0) {
+            left = 0;
+          } else {
+            b = next;
+            steps = steps_of(len);
+          }
         }
       }
+      return t;
+    };
+
+    // ---- loads ----
+    // Load j of a block, lane l: 16 bytes of row (64 j + l) / (D / 8), which land
+    // at place (64 j + l) % (D / 8) of that row.
+    uint32_t k_off[kLoads], v_off[kLoads], q_off[kLoads];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int row = (64 * j + lane) / (D / 8), place = lane % (D / 8);
+      k_off[j] = (uint32_t)row * (uint32_t)(2 * a.k_row) + 16 * (place ^ swizzle_k<D>(row));
+      v_off[j] = (uint32_t)row * (uint32_t)(2 * a.v_row) + 16 * (place ^ swizzle_v<D>(row));
+      q_off[j] = (uint32_t)row * (2 * D) + 16 * (place ^ swizzle_k<D>(row));
     }
-    return t;
-  };
-
-  // ---- loads ----
-  // Load j of a block, lane l: 16 bytes of row (64 j + l) / (D / 8), which land
-  // at place (64 j + l) % (D / 8) of that row.
-  uint32_t k_off[kLoads], v_off[kLoads], q_off[kLoads];
+    // Keys of a block that are there: none of a page outside the cache.
+    auto usable = [&](const Step &t, int i) __attribute__((always_inline)) {
+      return (uint32_t)t.page[i] < (uint32_t)a.P ? t.n[i] : 0;
+    };
+    auto issue = [&](const Step &t, const uint16_t *pages, int64_t page_st, int64_t head_st, int64_t row_st,
+                     const uint32_t (&off)[kLoads], uint8_t *stage) __attribute__((always_inline)) {
+      const int64_t head_at = (t.head / blocks) * head_st;
 #pragma unroll
-  for (int j = 0; j < kLoads; ++j) {
-    const int row = (64 * j + lane) / (D / 8), place = lane % (D / 8);
-    k_off[j] = (uint32_t)row * (uint32_t)(2 * a.k_row) + 16 * (place ^ swizzle_k<D>(row));
-    v_off[j] = (uint32_t)row * (uint32_t)(2 * a.v_row) + 16 * (place ^ swizzle_v<D>(row));
-    q_off[j] = (uint32_t)row * (2 * D) + 16 * (place ^ swizzle_k<D>(row));
-  }
-  // Keys of a block that are there: none of a page outside the cache.
-  auto usable = [&](const Step &t, int i) __attribute__((always_inline)) {
-    return (uint32_t)t.page[i] < (uint32_t)a.P ? t.n[i] : 0;
-  };
-  auto issue = [&](const Step &t, const uint16_t *pages, int64_t page_st, int64_t head_st, int64_t row_st,
-                   const uint32_t (&off)[kLoads], uint8_t *stage) __attribute__((always_inline)) {
-    const int64_t head_at = (t.head / blocks) * head_st;
+      for (int i = 0; i < 2; ++i) {
+        const int n = usable(t, i);
+        const uint16_t *const base = pages + (n ? t.page[i] * page_st + head_at + t.row[i] * row_st : 0);
+        const auto rs = buffer(base, n ? (uint32_t)(n - 1) * (uint32_t)(2 * row_st) + 2 * D : 0u);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int n = usable(t, i);
-      const uint16_t *const base = pages + (n ? t.page[i] * page_st + head_at + t.row[i] * row_st : 0);
-      const auto rs = buffer(base, n ? (uint32_t)(n - 1) * (uint32_t)(2 * row_st) + 2 * D : 0u);
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) load_lds16(rs, stage + (i * kLoads + j) * 1024, off[j]);
-    }
-  };
-  auto issue_k = [&](const Step &t) __attribute__((always_inline)) {
-    issue(t, a.k, a.k_page, a.k_head, a.k_row, k_off, kst);
-    asm volatile("" ::: "memory");  // the counted waits rely on the order
-  };
-  auto issue_v = [&](const Step &t) __attribute__((always_inline)) {
-    issue(t, a.v, a.v_page, a.v_head, a.v_row, v_off, vst);
-    asm volatile("" ::: "memory");
-  };
-  auto issue_q = [&](const Step &t) __attribute__((always_inline)) {
-    const int kvh = t.head / blocks, part = t.head % blocks, rows = min(kRows, group - kRows * part);
-    const uint16_t *const base = a.q + t.b * a.q_stride + (int64_t)(kvh * group + kRows * part) * D;
-    const auto rs = buffer(base, (uint32_t)rows * 2 * D);
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) load_lds16(rs, qst + j * 1024, q_off[j]);
-    asm volatile("" ::: "memory");
-  };
-
-  // ---- operand addresses ----
-  uint32_t k_at[kSlices];  // chunk 4 ks + g of row r
-#pragma unroll
-  for (int ks = 0; ks < kSlices; ++ks) k_at[ks] = (uint32_t)(r * 2 * D + 16 * ((4 * ks + g) ^ swizzle_k<D>(r)));
-  const uint32_t k_base = lds_addr(kst);
-  const int v_row = 4 * g + (r >> 2);  // the lane addresses dims 4 (r % 4) .. of this key
-  const uint32_t v_base = lds_addr(vst) + (uint32_t)(v_row * 2 * D + 16 * (((r & 3) >> 1) ^ swizzle_v<D>(v_row)) + 8 * (r & 1));
-
-  // Softmax state of query row r (this lane's keys only in l), base-2 domain; O:
-  // rows 4 g + i, dims 16 dt + r.
-  float m_run = -INFINITY, l_run = 0.f;
-  f32x4 o[kTiles];
-#pragma unroll
-  for (int dt = 0; dt < kTiles; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const float sl2 = a.scale * kLog2e;
-  int piece_from = s, piece_unit = first;  // where the present piece began
-  int unit = first;
-  bool bad_page = false;
-
-  Step cur = next_step(), nx = next_step();
-  issue_q(cur);
-  issue_k(cur);
-  issue_v(cur);
-  while (cur.n[0] > 0) {
-    // K (and Q) have landed once at most V's loads remain.
-    wait_vmcnt<2 * kLoads>();
-    u32x4 kf[2 * kSlices], qf[kSlices];
-    read_kq<D>(k_base, k_at, kf, qf);
-    f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-    for (int ks = 0; ks < kSlices; ++ks)
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) sc[kt] = mfma16x16<F16>(kf[2 * ks + kt], qf[ks], sc[kt]);
-    if (nx.b != cur.b || nx.head != cur.head) issue_q(nx);
-    issue_k(nx);
-    // Lane: keys 16 kt + 4 g + i of query row r.
-    const int n0 = usable(cur, 0), n1 = usable(cur, 1);
-    if (n0 + n1 < kStep) {
-      bad_page |= n0 != cur.n[0] || n1 != cur.n[1];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sc[0][i] = 4 * g + i < n0 ? sc[0][i] : -INFINITY;
-        sc[1][i] = 4 * g + i < n1 ? sc[1][i] : -INFINITY;
+        for (int j = 0; j < kLoads; ++j) load_lds16(rs, stage + (i * kLoads + j) * 1024, off[j]);
       }
-    }
-    const float lmax = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                             fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3]))) * sl2;
-    if (__builtin_amdgcn_ballot_w64(lmax > m_run + kRescaleSlack)) {
-      const float m_new = fmaxf(m_run, quad_max(lmax));
-      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
-      l_run *= alpha;
-      m_run = m_new;
-      float al[4];
+    };
+    auto issue_k = [&](const Step &t) __attribute__((always_inline)) {
+      issue(t, a.k, a.k_page, a.k_head, a.k_row, k_off, kst);
+      asm volatile("" ::: "memory");  // the counted waits rely on the order
+    };
+    auto issue_v = [&](const Step &t) __attribute__((always_inline)) {
+      issue(t, a.v, a.v_page, a.v_head, a.v_row, v_off, vst);
+      asm volatile("" ::: "memory");
+    };
+    auto issue_q = [&](const Step &t) __attribute__((always_inline)) {
+      const int kvh = t.head / blocks, part = t.head % blocks, rows = min(kRows, group - kRows * part);
+      const uint16_t *const base = a.q + t.b * a.q_stride + (int64_t)(kvh * group + kRows * part) * D;
+      const auto rs = buffer(base, (uint32_t)rows * 2 * D);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, 4 * g + i, kWave);
+      for (int j = 0; j < kLoads; ++j) load_lds16(rs, qst + j * 1024, q_off[j]);
+      asm volatile("" ::: "memory");
+    };
+
+    // ---- operand addresses ----
+    uint32_t k_at[kSlices];  // chunk 4 ks + g of row r
+#pragma unroll
+    for (int ks = 0; ks < kSlices; ++ks) k_at[ks] = (uint32_t)(r * 2 * D + 16 * ((4 * ks + g) ^ swizzle_k<D>(r)));
+    const uint32_t k_base = lds_addr(kst);
+    const int v_row = 4 * g + (r >> 2);  // the lane addresses dims 4 (r % 4) .. of this key
+    const uint32_t v_base = lds_addr(vst) + (uint32_t)(v_row * 2 * D + 16 * (((r & 3) >> 1) ^ swizzle_v<D>(v_row)) + 8 * (r & 1));
+
+    // Softmax state of query row r (this lane's keys only in l), base-2 domain; O:
+    // rows 4 g + i, dims 16 dt + r.
+    float m_run = -INFINITY, l_run = 0.f;
+    f32x4 o[kTiles];
+#pragma unroll
+    for (int dt = 0; dt < kTiles; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float sl2 = a.scale * kLog2e;
+    int piece_from = s, piece_unit = first;  // where the present piece began
+    int unit = first;
+    bool bad_page = false;
+
+    Step cur = next_step(), nx = next_step();
+    issue_q(cur);
+    issue_k(cur);
+    issue_v(cur);
+    while (cur.n[0] > 0) {
+      // K (and Q) have landed once at most V's loads remain.
+      wait_vmcnt<2 * kLoads>();
+      u32x4 kf[2 * kSlices], qf[kSlices];
+      read_kq<D>(k_base, k_at, kf, qf);
+      f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int ks = 0; ks < kSlices; ++ks)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) sc[kt] = mfma16x16<F16>(kf[2 * ks + kt], qf[ks], sc[kt]);
+      if (nx.b != cur.b || nx.head != cur.head) issue_q(nx);
+      issue_k(nx);
+      // Lane: keys 16 kt + 4 g + i of query row r.
+      const int n0 = usable(cur, 0), n1 = usable(cur, 1);
+      if (n0 + n1 < kStep) {
+        bad_page |= n0 != cur.n[0] || n1 != cur.n[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[0][i] = 4 * g + i < n0 ? sc[0][i] : -INFINITY;
+          sc[1][i] = 4 * g + i < n1 ? sc[1][i] : -INFINITY;
+        }
+      }
+      const float lmax = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                               fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3]))) * sl2;
+      if (__builtin_amdgcn_ballot_w64(lmax > m_run + kRescaleSlack)) {
+        const float m_new = fmaxf(m_run, quad_max(lmax));
+        const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+        l_run *= alpha;
+        m_run = m_new;
+        float al[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, 4 * g + i, kWave);
+#pragma unroll
+        for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[dt][i] *= al[i];
+      }
+      const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+      float p[2][4];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], sl2, neg_m));
+      l_run += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+      // Probabilities in the type of V: half a step each, against fp32 sums of both.
+      const u32x4 pa = {pack2<F16>(p[0][0], p[0][1]), pack2<F16>(p[0][2], p[0][3]), pack2<F16>(p[1][0], p[1][1]),
+                        pack2<F16>(p[1][2], p[1][3])};
+      // V has landed once at most the next K's loads remain.
+      wait_vmcnt<2 * kLoads>();
+      u32x2 vr[2 * kTiles];
+      read_v<D>(v_base, vr);
+      issue_v(nx);
 #pragma unroll
       for (int dt = 0; dt < kTiles; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[dt][i] *= al[i];
-    }
-    const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
-    float p[2][4];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], sl2, neg_m));
-    l_run += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
-    // Probabilities in the type of V: half a step each, against fp32 sums of both.
-    const u32x4 pa = {pack2<F16>(p[0][0], p[0][1]), pack2<F16>(p[0][2], p[0][3]), pack2<F16>(p[1][0], p[1][1]),
-                      pack2<F16>(p[1][2], p[1][3])};
-    // V has landed once at most the next K's loads remain.
-    wait_vmcnt<2 * kLoads>();
-    u32x2 vr[2 * kTiles];
-    read_v<D>(v_base, vr);
-    issue_v(nx);
-#pragma unroll
-    for (int dt = 0; dt < kTiles; ++dt)
-      o[dt] = mfma16x16<F16>(pa, u32x4{vr[2 * dt][0], vr[2 * dt][1], vr[2 * dt + 1][0], vr[2 * dt + 1][1]}, o[dt]);
+        o[dt] = mfma16x16<F16>(pa, u32x4{vr[2 * dt][0], vr[2 * dt][1], vr[2 * dt + 1][0], vr[2 * dt + 1][1]}, o[dt]);
 
-    // ---- the end of a piece ----
-    const bool pair_ends = cur.s + 1 == cur.steps;
-    if (kList && (pair_ends || nx.n[0] == 0)) {
-      const int kvh = cur.head / blocks, part = cur.head % blocks, rows = min(kRows, group - kRows * part);
-      const int64_t head0 = (int64_t)cur.b * a.Hq + kvh * group + kRows * part;
-      const float l = quad_sum(l_run);
-      const bool whole = pair_ends && piece_from == 0;
-      const int slot = 2 * worker + (piece_unit == first ? 0 : 1);
-      if (piece_from == 0 && lane == 0) {
-        // Pieces of the (sequence, head block): this one, then the first pieces
-        // of the following waves.
-        const int last = (piece_unit + cur.steps - 1) / per;
-        a.pieces[2 * (cur.b * heads + cur.head)] = slot;
-        a.pieces[2 * (cur.b * heads + cur.head) + 1] = whole ? 0 : last - worker + 1;
-      }
-      float L[4], M[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        L[i] = __shfl(l, 4 * g + i, kWave);
-        M[i] = __shfl(m_run, 4 * g + i, kWave);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 4 * g + i;
-        if (row >= rows) continue;
-        if (whole) {
-          const float inv = L[i] == 0.f ? 0.f : 1.0f / L[i];
-          uint16_t *const op = a.out + (head0 + row) * D + r;
-#pragma unroll
-          for (int dt = 0; dt < kTiles; ++dt) op[16 * dt] = (uint16_t)pack2<F16>(o[dt][i] * inv, 0.f);
-        } else {
-          float *const pp = a.partial + ((int64_t)slot * min(group, kRows) + row) * (D + 2);
-          if (r == 0) {
-            pp[0] = M[i];
-            pp[1] = L[i];
-          }
-#pragma unroll
-          for (int dt = 0; dt < kTiles; ++dt) pp[2 + 16 * dt + r] = o[dt][i];
+      // ---- the end of a piece ----
+      const bool pair_ends = cur.s + 1 == cur.steps;
+      if (!kTeams && (pair_ends || nx.n[0] == 0)) {
+        const int kvh = cur.head / blocks, part = cur.head % blocks, rows = min(kRows, group - kRows * part);
+        const int64_t head0 = (int64_t)cur.b * a.Hq + kvh * group + kRows * part;
+        const float l = quad_sum(l_run);
+        const bool whole = pair_ends && piece_from == 0;
+        const int slot = 2 * worker + (piece_unit == first ? 0 : 1);
+        if (piece_from == 0 && lane == 0) {
+          // Pieces of the (sequence, head block): this one, then the first pieces
+          // of the following waves.
+          const int last = (piece_unit + cur.steps - 1) / per;
+          a.pieces[2 * (cur.b * heads + cur.head)] = slot;
+          a.pieces[2 * (cur.b * heads + cur.head) + 1] = whole ? 0 : last - worker + 1;
         }
-      }
-      m_run = -INFINITY;
-      l_run = 0.f;
+        float L[4], M[4];
 #pragma unroll
-      for (int dt = 0; dt < kTiles; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      piece_from = 0;
-      piece_unit = unit + 1;
+        for (int i = 0; i < 4; ++i) {
+          L[i] = __shfl(l, 4 * g + i, kWave);
+          M[i] = __shfl(m_run, 4 * g + i, kWave);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 4 * g + i;
+          if (row >= rows) continue;
+          if (whole) {
+            const float inv = L[i] == 0.f ? 0.f : 1.0f / L[i];
+            uint16_t *const op = a.out + (head0 + row) * D + r;
+#pragma unroll
+            for (int dt = 0; dt < kTiles; ++dt) op[16 * dt] = (uint16_t)pack2<F16>(o[dt][i] * inv, 0.f);
+          } else {
+            float *const pp = a.partial + ((int64_t)slot * min(group, kRows) + row) * (D + 2);
+            if (r == 0) {
+              pp[0] = M[i];
+              pp[1] = L[i];
+            }
+#pragma unroll
+            for (int dt = 0; dt < kTiles; ++dt) pp[2 + 16 * dt + r] = o[dt][i];
+          }
+        }
+        m_run = -INFINITY;
+        l_run = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < kTiles; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        piece_from = 0;
+        piece_unit = unit + 1;
+      }
+      ++unit;
+      cur = nx;
+      nx = next_step();
     }
-    ++unit;
-    cur = nx;
-    nx = next_step();
-  }
-  wait_vmcnt<0>();  // the last (empty) step's loads write LDS
-  if (bad_page && lane == 0) atomicOr(a.status, GQA_STATUS_BAD_PAGE);
+    wait_vmcnt<0>();  // the last (empty) step's loads write LDS
+    if (bad_page && lane == 0) atomicOr(a.status, GQA_STATUS_BAD_PAGE);
 
-  if constexpr (!kList) {
-    // The waves' states, each in its own part of the LDS: O, then m and l per row.
-    const int kvh = head / blocks, part = head % blocks, rows = min(kRows, group - kRows * part);
-    const float l = quad_sum(l_run);
-    float *const mine = (float *)kst;
-    mfma_settle();
-    if (g == 0) {
-      mine[kRows * D + r] = m_run;
-      mine[kRows * D + kRows + r] = l;
+    if constexpr (kTeams) {
+      // The waves' states, each in its own part of the LDS: O, then m and l per row.
+      const int kvh = head / blocks, part = head % blocks, rows = min(kRows, group - kRows * part);
+      const float l = quad_sum(l_run);
+      float *const mine = (float *)kst;
+      mfma_settle();
+      if (g == 0) {
+        mine[kRows * D + r] = m_run;
+        mine[kRows * D + kRows + r] = l;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (4 * g + i < rows) {
+#pragma unroll
+          for (int dt = 0; dt < kTiles; ++dt) mine[(4 * g + i) * D + 16 * dt + r] = pin(o[dt][i]);
+        }
+      __syncthreads();
+      uint32_t *const out = (uint32_t *)(a.out + ((int64_t)b * a.Hq + kvh * group + kRows * part) * D);
+      for (int e = 2 * threadIdx.x; e < rows * D; e += 2 * 64 * kTeam) {
+        const int row = e / D;
+        float m[kTeam], top = -INFINITY, den = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < kTeam; ++w) {
+          m[w] = ((const float *)(smem + w * kWaveLds<D>))[kRows * D + row];
+          top = fmaxf(top, m[w]);
+        }
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < kTeam; ++w) {
+          const float *const x = (const float *)(smem + w * kWaveLds<D>);
+          const float f = __builtin_amdgcn_exp2f(m[w] - ref);
+          const f32x2_t v = *(const f32x2_t *)(x + e);
+          den = __builtin_fmaf(f, x[kRows * D + kRows + row], den);
+          o0 = __builtin_fmaf(f, v[0], o0);
+          o1 = __builtin_fmaf(f, v[1], o1);
+        }
+        const float inv = den == 0.f ? 0.f : 1.0f / den;
+        out[e / 2] = pack2<F16>(o0 * inv, o1 * inv);
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (4 * g + i < rows) {
-#pragma unroll
-        for (int dt = 0; dt < kTiles; ++dt) mine[(4 * g + i) * D + 16 * dt + r] = pin(o[dt][i]);
-      }
-    __syncthreads();
-    uint32_t *const out = (uint32_t *)(a.out + ((int64_t)b * a.Hq + kvh * group + kRows * part) * D);
-    for (int e = 2 * threadIdx.x; e < rows * D; e += 2 * 64 * TEAM) {
-      const int row = e / D;
-      float m[TEAM], top = -INFINITY, den = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll
-      for (int w = 0; w < TEAM; ++w) {
-        m[w] = ((const float *)(smem + w * kWaveLds<D>))[kRows * D + row];
-        top = fmaxf(top, m[w]);
-      }
-      const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int w = 0; w < TEAM; ++w) {
-        const float *const x = (const float *)(smem + w * kWaveLds<D>);
-        const float f = __builtin_amdgcn_exp2f(m[w] - ref);
-        const f32x2_t v = *(const f32x2_t *)(x + e);
-        den = __builtin_fmaf(f, x[kRows * D + kRows + row], den);
-        o0 = __builtin_fmaf(f, v[0], o0);
-        o1 = __builtin_fmaf(f, v[1], o1);
-      }
-      const float inv = den == 0.f ? 0.f : 1.0f / den;
-      out[e / 2] = pack2<F16>(o0 * inv, o1 * inv);
-    }
-  }
+  };
+  if constexpr (TEAM > 0) work(std::true_type());
+  else if (team) work(std::true_type());
+  else work(std::false_type());
 }
 
 // Joins the pieces of a (sequence, head block), in the order of the keys.  A thread
@@ -631,7 +660,7 @@ int waves_of(int D, int cus) { return cus * kWaves * (D == 128 ? kWorkgroups<128
 int team_of(int64_t pairs, int64_t steps, int64_t waves) {
   const int team = 8 * pairs <= waves ? 8 : 4;
   const int64_t listed = (pairs * steps + waves - 1) / waves, teamed = (steps + team - 1) / team;
-  return teamed <= 16 && teamed <= listed / 2 + 6 ? team : 0;
+  return teamed <= most_teamed(listed) ? team : 0;
 }
 
 template <int D, bool F16, int TEAM>

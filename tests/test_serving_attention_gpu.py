@@ -10,7 +10,9 @@ pytestmark = pytest.mark.gpu
 
 HEADS = [(32, 8, 128), (8, 8, 128), (12, 4, 64), (14, 2, 64), (6, 6, 64), (16, 1, 128), (40, 2, 128), (64, 1, 64)]
 TYPES = [torch.bfloat16, torch.float16]
-WIDE = [False, True]  # tables of decode attention
+# Tables of decode attention: just wide enough, wide, wide with a long last sequence.
+# (Three ways in which the work is shared out.)
+WIDE = ["narrow", "wide", "long"]
 
 
 def _assert_close(out, ref, bound, keys, vmax):
@@ -224,13 +226,15 @@ def test_packed_many_sequences_listed(count, gpu_device):
 # ---- paged decode -----------------------------------------------------------------
 
 
-def _paged(lengths, hq, hkv, d, page, dtype, device, order="heads", spare=3, seed=0, wide=False):
+def _paged(lengths, hq, hkv, d, page, dtype, device, order="heads", spare=3, seed=0, wide="narrow"):
     """Pages in a shuffled order; the places behind each sequence's end and the
     spare pages hold NaN, table entries behind the last page an impossible one.
-    Wide tables have room for many more pages (another way to share the work out)."""
+    ``wide``: see WIDE; "long" adds a sequence to ``lengths``."""
+    if wide == "long":
+        lengths.append(1000)
     g = torch.Generator().manual_seed(seed + sum(lengths) + page)
     used = [-(-n // page) for n in lengths]
-    count, width = sum(used) + spare, 1000 if wide else max(used) + 2
+    count, width = sum(used) + spare, max(used) + 2 if wide == "narrow" else 1000
     perm = torch.randperm(count, generator=g).tolist()
     shape = (count, hkv, page, d) if order == "heads" else (count, page, hkv, d)
     kv = [torch.randn(shape, generator=g).to(dtype) for _ in range(2)]
@@ -284,6 +288,7 @@ def test_paged_heads(hq, hkv, d, dtype, wide, gpu_device):
 @pytest.mark.parametrize("order", ["heads", "tokens"])
 @pytest.mark.parametrize("wide", WIDE)
 def test_paged_lengths(lengths, page, order, wide, gpu_device):
+    lengths = list(lengths)
     q, k, v, tables, gt, gl = _paged(lengths, 8, 2, 128, page, torch.bfloat16, gpu_device, order, wide=wide)
     plan = prepare_paged_gqa(q, k, v, gt, gl)
     _check_paged(plan, tables, lengths)
@@ -426,6 +431,7 @@ def test_paged_replays_and_streams(wide, gpu_device):
     with torch.cuda.graph(graph, stream=side):
         plan.run()
     for i, now in enumerate(([1500, 1, 0, 333], [3, 1, 0, 1], [0, 0, 0, 0], [1488, 16, 0, 320], [1, 0, 0, 336])):
+        now = now + lengths[4:]
         gl.copy_(torch.tensor(now, dtype=torch.int32))
         q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(i)))
         side.wait_stream(torch.cuda.current_stream())
