@@ -220,7 +220,7 @@ int gqa_packed_plan_create(gqa_packed_plan **out, const gqa_packed_desc *d) {
   if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");
   p->a = moe::GqaPackedArgs{(const uint16_t *)d->q, (const uint16_t *)d->k, (const uint16_t *)d->v, (uint16_t *)d->out,
                             d->starts, d->q_stride, d->k_stride, d->v_stride, d->N, d->S, d->Hq, d->Hkv, d->D, d->dtype,
-                            scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0, 0, 0};
+                            scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0, 0, 0, 0};
   moe::gqa_packed_bind(&p->a, d->workspace);
   moe::gqa_packed_constants(&p->a);
   p->device = dev;

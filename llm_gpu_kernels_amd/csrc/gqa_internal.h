@@ -55,8 +55,9 @@ struct GqaPackedArgs {
   // class of KV heads, and a class's heads; ceil(2^32 / G).
   int G, class_xcds, per_class;
   uint32_t G_magic;
-  // Set by the launch: entries of the list, 0 without one; CUs of an XCD.
-  int listed, xcd_cus;
+  // Set by the launch: entries of the list, 0 without one; whether tiles are searched
+  // for in the order of their keys; CUs of an XCD.
+  int listed, searched, xcd_cus;
 };
 size_t gqa_packed_workspace(int N, int Hq, int Hkv, int S);
 void gqa_packed_bind(GqaPackedArgs *a, void *workspace);

@@ -328,18 +328,37 @@ __global__ __launch_bounds__(64 * kWaves, kResident<D>) void gqa_packed_kernel(G
   const int in_class = (slot8 << a.class_xcds) + (xcd >> (3 - a.class_xcds)), nth = in_class / a.per_class;
   const int kvh = (xcd & (7 >> a.class_xcds)) + ((in_class - nth * a.per_class) << (3 - a.class_xcds));
   Rows w;
-  if (!a.listed) {  // S <= 64: in the order of the sequences, each one's longest first
+  if (!a.listed) {  // S <= 64
     Rows q = {wave_max_scan(lane < a.S ? bound(a, lane) : 0), 0, 0, 0};
     if (lane < a.S) {
       q.len = max(0, bound(a, lane + 1) - q.start);
       check_bounds(a, lane, q);
     }
-    const int T = (q.len * G + kTileRows - 1) / kTileRows, incl = wave_scan(T);
-    const uint64_t behind = __builtin_amdgcn_ballot_w64(incl > nth);
-    if (!behind) return;
-    const int at = sgpr(__builtin_ctzll(behind));
-    w = Rows{__builtin_amdgcn_readlane(q.start, at), __builtin_amdgcn_readlane(q.len, at),
-             __builtin_amdgcn_readlane(incl, at) - 1 - nth, 0};
+    const int T = (q.len * G + kTileRows - 1) / kTileRows;
+    int at, x;  // the tile's sequence and its number there
+    if (!a.searched) {  // in the order of the sequences, each one's longest first
+      const int incl = wave_scan(T);
+      const uint64_t behind = __builtin_amdgcn_ballot_w64(incl > nth);
+      if (!behind) return;
+      at = sgpr(__builtin_ctzll(behind));
+      x = __builtin_amdgcn_readlane(incl, at) - 1 - nth;
+    } else {
+      // Tiles of the highest number, which see the most keys, first: the largest x of
+      // which more than nth tiles have it or a higher one, two bits at a time.
+      auto from = [&](int lo) __attribute__((always_inline)) { return wave_total(max(0, T - lo)); };
+      if (from(0) <= nth) return;
+      x = 0;
+      for (int by = 1 << ((31 - __builtin_clz(a.N * G / kTileRows + 1)) & ~1); by > 0; by >>= 2) {
+        const int n1 = from(x + by), n2 = from(x + 2 * by), n3 = from(x + 3 * by);
+        x += by * ((n1 > nth) + (n2 > nth) + (n3 > nth));
+      }
+      // Of the sequences that have a tile x, the one with `before` such ones before it.
+      const int before = nth - from(x + 1);
+      const bool has = T > x;
+      const uint64_t have = __builtin_amdgcn_ballot_w64(has);
+      at = sgpr(__builtin_ctzll(__builtin_amdgcn_ballot_w64(has && (int)__popcll(have & lanemask_lt()) == before)));
+    }
+    w = Rows{__builtin_amdgcn_readlane(q.start, at), __builtin_amdgcn_readlane(q.len, at), x, 0};
   } else {
     // Scalar loads: the list does not change while the kernel runs.
     typedef const __attribute__((address_space(4))) int *Uniform;
@@ -611,10 +630,15 @@ hipError_t launch(GqaPackedArgs a, int cus, hipStream_t s) {
   int64_t per_xcd = (tiles * a.per_class + (1 << a.class_xcds) - 1) >> a.class_xcds;
   a.xcd_cus = cus / kXcds;  // a second round that is turned round has to be whole
   if (per_xcd > a.xcd_cus && per_xcd < 2 * a.xcd_cus) per_xcd = 2 * a.xcd_cus;
-  // The order matters once some workgroups start after others; up to 64 sequences a
-  // wave finds its tile by itself (four prompts of up to 48 tokens: 6.5 us, 9.7 with
-  // the list).
-  a.listed = a.S > kWave || (a.S > 1 && per_xcd * kXcds > 4 * cus) ? (int)tiles : 0;
+  // Which tile a workgroup takes.  Up to 64 sequences a wave finds that out by itself: in
+  // the order of the sequences; with the tiles that see the most keys first, 1 us a
+  // workgroup, if CUs have more than one of some length (4 prompts of 900 tokens 45.4, 40.1 us; 32
+  // of 64 10.8, 11.9).  In more rounds than two, and for more sequences, the list,
+  // 5 us and a launch (4 prompts of up to 48 tokens 6.5, 9.7 with it; 50 of 300, D = 64,
+  // 22.7, 26.7; 64 of 20 to 800 248, 236).
+  const bool rounds = per_xcd * kXcds > 2 * kResident<D> * (int64_t)cus;
+  a.listed = a.S > kWave || (a.S > 1 && rounds) ? (int)tiles : 0;
+  a.searched = !a.listed && a.S > 1 && per_xcd > a.xcd_cus && a.N >= 128 * (int64_t)a.S;
   if (a.listed)
     hipLaunchKernelGGL(a.S <= kPlanLds ? gqa_packed_plan<true> : gqa_packed_plan<false>, dim3(1), dim3(kPlanThreads), 0, s,
                        a);

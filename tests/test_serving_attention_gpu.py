@@ -213,6 +213,21 @@ def test_packed_few_rounds(count, hq, hkv, d, gpu_device):
     plan.check_inputs()
 
 
+@pytest.mark.parametrize("lengths,hq,hkv,d", [
+    ([1500, 0, 1100], 32, 8, 128), ([(130 * i) % 700 + 1 for i in range(9)], 32, 8, 128), ([300] * 7, 16, 16, 128),
+    ([(37 * i) % 290 for i in range(64)], 12, 4, 64), ([900, 5, 0, 260], 64, 1, 128), ([0, 1024, 1025, 0], 16, 2, 64)])
+def test_packed_longest_first(lengths, hq, hkv, d, gpu_device):
+    """Up to 64 sequences with somewhat more tiles than CUs, as they are and with rows
+    of no sequence around them, every row in some tile exactly once."""
+    for first, behind in ((0, 0), (3, 40)):
+        q, k, v, starts, on_gpu = _packed(lengths, hq, hkv, d, torch.bfloat16, gpu_device, first=first, behind=behind)
+        out = torch.full_like(q, 7.0).contiguous()
+        plan = prepare_packed_gqa(q, k, v, on_gpu, out)
+        _check_packed(plan, starts)
+        assert (out[:first] == 7).all() and (out[starts[-1]:] == 7).all()
+        plan.check_inputs()
+
+
 @pytest.mark.parametrize("count", [2100, 5000])
 def test_packed_many_sequences_listed(count, gpu_device):
     """More sequences than the sorting workgroup holds in LDS."""
