@@ -343,20 +343,21 @@ __global__ __launch_bounds__(64 * kWaves, kResident<D>) void gqa_packed_kernel(G
       at = sgpr(__builtin_ctzll(behind));
       x = __builtin_amdgcn_readlane(incl, at) - 1 - nth;
     } else {
-      // Tiles of the highest number, which see the most keys, first: the largest x of
-      // which more than nth tiles have it or a higher one, two bits at a time.
-      auto from = [&](int lo) __attribute__((always_inline)) { return wave_total(max(0, T - lo)); };
-      if (from(0) <= nth) return;
-      x = 0;
-      for (int by = 1 << ((31 - __builtin_clz(a.N * G / kTileRows + 1)) & ~1); by > 0; by >>= 2) {
-        const int n1 = from(x + by), n2 = from(x + 2 * by), n3 = from(x + 3 * by);
-        x += by * ((n1 > nth) + (n2 > nth) + (n3 > nth));
-      }
-      // Of the sequences that have a tile x, the one with `before` such ones before it.
-      const int before = nth - from(x + 1);
-      const bool has = T > x;
-      const uint64_t have = __builtin_amdgcn_ballot_w64(has);
-      at = sgpr(__builtin_ctzll(__builtin_amdgcn_ballot_w64(has && (int)__popcll(have & lanemask_lt()) == before)));
+      // Tiles of the highest number, which see the most keys, first.  Tiles numbered
+      // T and up: `above`; the least such T with at most nth of them, `top`, has the
+      // wanted number just below, where every sequence of at least `top` tiles, `some`
+      // in all, has one of each number.
+      int above = 0;
+#pragma unroll 4
+      for (int j = 0; j < a.S; ++j) above += max(0, __builtin_amdgcn_readlane(T, j) - T);
+      constexpr int kMore = 1 << 28;  // than tiles
+      const int top = kMore - __builtin_amdgcn_readlane(wave_max_scan(above <= nth ? kMore - T : 0), kWave - 1);
+      const uint64_t those = __builtin_amdgcn_ballot_w64(T >= top);
+      const int some = (int)__popcll(those);
+      const int rest = nth - __builtin_amdgcn_readlane(above, sgpr(__builtin_ctzll(__builtin_amdgcn_ballot_w64(T == top))));
+      x = top - 1 - rest / some;
+      if (x < 0) return;
+      at = sgpr(__builtin_ctzll(__builtin_amdgcn_ballot_w64(T >= top && (int)__popcll(those & lanemask_lt()) == rest % some)));
     }
     w = Rows{__builtin_amdgcn_readlane(q.start, at), __builtin_amdgcn_readlane(q.len, at), x, 0};
   } else {
@@ -631,11 +632,11 @@ hipError_t launch(GqaPackedArgs a, int cus, hipStream_t s) {
   a.xcd_cus = cus / kXcds;  // a second round that is turned round has to be whole
   if (per_xcd > a.xcd_cus && per_xcd < 2 * a.xcd_cus) per_xcd = 2 * a.xcd_cus;
   // Which tile a workgroup takes.  Up to 64 sequences a wave finds that out by itself: in
-  // the order of the sequences; with the tiles that see the most keys first, 1 us a
-  // workgroup, if CUs have more than one of some length (4 prompts of 900 tokens 45.4, 40.1 us; 32
-  // of 64 10.8, 11.9).  In more rounds than two, and for more sequences, the list,
+  // the order of the sequences; with the tiles that see the most keys first, 0.5 to 1 us
+  // a workgroup, if CUs have more than one of some length (4 prompts of 900 tokens 47.2, 40.7 us;
+  // 32 of 64 10.8, 11.9).  In more rounds than two, and for more sequences, the list,
   // 5 us and a launch (4 prompts of up to 48 tokens 6.5, 9.7 with it; 50 of 300, D = 64,
-  // 22.7, 26.7; 64 of 20 to 800 248, 236).
+  // 24.3, 27.8; 64 of 20 to 800 248, 236).
   const bool rounds = per_xcd * kXcds > 2 * kResident<D> * (int64_t)cus;
   a.listed = a.S > kWave || (a.S > 1 && rounds) ? (int)tiles : 0;
   a.searched = !a.listed && a.S > 1 && per_xcd > a.xcd_cus && a.N >= 128 * (int64_t)a.S;
