@@ -272,6 +272,8 @@ __device__ __forceinline__ void take_rows(const GqaPackedArgs &a, const Rows &w,
     for (int c = 0; c < kPart; ++c) {
       const u32x4 x = *(const u32x4 *)(kp + 8 * c);
 #pragma unroll
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(q[c][i]));  // packed; as floats outside the loop they spill
+#pragma unroll
       for (int i = 0; i < 8; ++i) dot = __builtin_fmaf(element<F16>(q[c], i), element<F16>(x, i), dot);
     }
     const f32x2_t both = halves(dot);
