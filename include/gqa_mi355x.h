@@ -70,8 +70,9 @@ void gqa_seg_plan_destroy(gqa_seg_plan *p);
  * Types bf16 or fp16 (GQA_BF16, GQA_FP16; q, k, v and out alike), head_dim 64
  * or 128, Hq a multiple of Hkv, the group Hq / Hkv at most 64.  Products are
  * summed and softmax statistics held in fp32; probabilities are rounded to the
- * type for the product with V.  Bases 16-byte aligned; strides in elements,
- * multiples of 8.
+ * type for the product with V (half a step; fp16 ones that are less than 2^-25
+ * of their row's largest, 2^-36 of that at most).  Bases 16-byte aligned; strides
+ * in elements, multiples of 8.
  */
 #define GQA_BF16 0
 #define GQA_FP16 1

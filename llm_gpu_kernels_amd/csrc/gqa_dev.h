@@ -11,10 +11,31 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 #define GQA_AS_LDS __attribute__((address_space(3)))
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Running maxima lag the true maxima by at most this much (base-2 exponent), so
-// probabilities stay <= 2^8 and O is rescaled only when a row's maximum grows
-// past it (softmax does not depend on the reference maximum).
+// A row's probabilities are 2^(s - m), s its scores in base 2; softmax does not depend
+// on the reference m, so m may differ from the maximum, and O is rescaled only when a
+// score passes limit(m).
+//   bf16: m is a maximum so far and lags by at most kRescaleSlack: p <= 2^8.
+//   fp16 has five bits of exponent: below 2^-14 p loses bits, below 2^-25 all of them,
+// while the fp32 sum has it whole.  So m lies kF16Bias under a maximum and lags by at
+// most kF16Slack, and the largest p lies in [2^11, 2^15]: those within 2^-25 of it
+// are off by half a step, smaller ones by 2^-36 of it at most.  (With m at a maximum,
+// what many keys add under one that has nearly all of the sum was lost: 18 below it
+// in natural logarithms, most of it.)  No time lost; 13 and 2 cost 5 to 8 % in heads of 64, whose maxima
+// rise by more than 2 here and there.  From 2^20 on a score is itself off by 2^-4 and
+// more, and may pass m by more than limit(m) says: there m is a maximum, and follows
+// every new one.
 constexpr float kRescaleSlack = 8.f;
+constexpr float kF16Bias = 11.f, kF16Slack = 4.f, kF16Exact = 1048576.f;
+template <bool F16>
+__device__ __forceinline__ float reference(float top) {
+  if constexpr (F16) return top - (__builtin_fabsf(top) < kF16Exact ? kF16Bias : 0.f);
+  else return top;
+}
+template <bool F16>
+__device__ __forceinline__ float limit(float m) {
+  if constexpr (F16) return m + (__builtin_fabsf(m) < kF16Exact ? kF16Bias + kF16Slack : 0.f);
+  else return m + kRescaleSlack;
+}
 constexpr int kXcds = 8;
 
 __device__ __forceinline__ int sgpr(int v) { return __builtin_amdgcn_readfirstlane(v); }

@@ -445,6 +445,7 @@ __global__ __launch_bounds__(64 * kWaves, kResident<D>) void gqa_packed_kernel(G
 
   const float sl2 = a.scale * kLog2e;
   float m_run = -INFINITY, l_run = 0.f;  // base-2 domain; l of this lane's keys
+  float m_top = -INFINITY;               // fp16: limit(m_run), kept (two instructions of a stage)
   f32x16 o[kDims], s0, s1;
 #pragma unroll
   for (int db = 0; db < kDims; ++db)
@@ -473,13 +474,14 @@ __global__ __launch_bounds__(64 * kWaves, kResident<D>) void gqa_packed_kernel(G
         mx = fmaxf(mx, s[i]);
       }
     }
-    if (__builtin_amdgcn_ballot_w64(mx * sl2 > m_run + kRescaleSlack)) {
+    if (__builtin_amdgcn_ballot_w64(mx * sl2 > (F16 ? m_top : limit<F16>(m_run)))) {
       mfma_settle();
       const f32x2_t both = halves(mx * sl2);
-      const float m_new = fmaxf(m_run, fmaxf(both[0], both[1]));
+      const float m_new = fmaxf(m_run, reference<F16>(fmaxf(both[0], both[1])));
       const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
       l_run *= alpha;
       m_run = m_new;
+      m_top = limit<F16>(m_new);
 #pragma unroll
       for (int db = 0; db < kDims; ++db)
 #pragma unroll
@@ -490,8 +492,8 @@ __global__ __launch_bounds__(64 * kWaves, kResident<D>) void gqa_packed_kernel(G
     // A: the rest of the next stage's scores beside this one's exponentials.
     u32x4 pb[2];
     float sum0 = 0.f, sum1 = 0.f, p0 = 0.f, p1 = 0.f;
-    // Pair x of probabilities (in the type of V: half a step each, against fp32
-    // sums of both) and of the sums; a pair later than its exponentials.
+    // Pair x of probabilities (in the type of V: half a step each, see reference(),
+    // against fp32 sums of both) and of the sums; a pair later than its exponentials.
     auto take = [&](int x) __attribute__((always_inline)) {
       uint32_t w = pack2<F16>(p0, p1);
       sum0 += p0;

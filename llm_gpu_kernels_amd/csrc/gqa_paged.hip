@@ -394,6 +394,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
     // Softmax state of query row r (this lane's keys only in l), base-2 domain; O:
     // rows 4 g + i, dims 16 dt + r.
     float m_run = -INFINITY, l_run = 0.f;
+    float m_top = -INFINITY;  // fp16: limit(m_run), kept
     f32x4 o[kTiles];
 #pragma unroll
     for (int dt = 0; dt < kTiles; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -430,11 +431,12 @@ void gqa_paged_kernel(GqaPagedArgs a) {
       }
       const float lmax = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                                fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3]))) * sl2;
-      if (__builtin_amdgcn_ballot_w64(lmax > m_run + kRescaleSlack)) {
-        const float m_new = fmaxf(m_run, quad_max(lmax));
+      if (__builtin_amdgcn_ballot_w64(lmax > (F16 ? m_top : limit<F16>(m_run)))) {
+        const float m_new = fmaxf(m_run, reference<F16>(quad_max(lmax)));
         const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
         l_run *= alpha;
         m_run = m_new;
+        m_top = limit<F16>(m_new);
         float al[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, 4 * g + i, kWave);
@@ -450,7 +452,8 @@ void gqa_paged_kernel(GqaPagedArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], sl2, neg_m));
       l_run += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
-      // Probabilities in the type of V: half a step each, against fp32 sums of both.
+      // Probabilities in the type of V: half a step each, see reference(), against fp32
+      // sums of both.
       const u32x4 pa = {pack2<F16>(p[0][0], p[0][1]), pack2<F16>(p[0][2], p[0][3]), pack2<F16>(p[1][0], p[1][1]),
                         pack2<F16>(p[1][2], p[1][3])};
       // V has landed once at most the next K's loads remain.
@@ -502,7 +505,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
             for (int dt = 0; dt < kTiles; ++dt) pp[2 + 16 * dt + r] = o[dt][i];
           }
         }
-        m_run = -INFINITY;
+        m_run = m_top = -INFINITY;
         l_run = 0.f;
 #pragma unroll
         for (int dt = 0; dt < kTiles; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};

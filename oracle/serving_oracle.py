@@ -58,9 +58,9 @@ def tolerance(ref, bound, dtype, keys, vmax):
     rows of up to 128 elements are off by at most 130 * 2^-24 * sum |q k| * scale
     < 2^-13, probabilities by that and by the exp2 and the sums in fp32: 2^-12 of
     the bound covers them.  fp16 probabilities below 2^-14 are off by 2^-25 each
-    against the largest one of at least 1."""
+    against the largest one of at least 2^11, so by 2^-36 of the sum at most."""
     u = torch.finfo(dtype).eps / 2
-    small = keys * 2.0 ** -25 * vmax if dtype == torch.float16 else 0.0
+    small = keys * 2.0 ** -36 * vmax if dtype == torch.float16 else 0.0
     return bound * (u + u * u + 2.0 ** -12) + ref.abs() * u + small
 
 
