@@ -181,7 +181,8 @@ void gqa_paged_kernel(GqaPagedArgs a) {
   uint8_t *const kst = smem + wave * kWaveLds<D>, *const vst = kst + kStage<D>, *const qst = vst + kStage<D>;
 
   // ---- the wave's range of the flat list, or its first step ----
-  auto steps_of = [](int keys) __attribute__((always_inline)) { return (keys + kStep - 1) / kStep; };
+  // (Unsigned: lengths go up to 2^31 - 16.)
+  auto steps_of = [](int keys) __attribute__((always_inline)) { return (int)(((uint32_t)keys + kStep - 1) / kStep); };
   // Lengths of 64 kWindow sequences from `window` on: i-th of a lane at 64 i + lane.
   int window = 0, lens[kWindow];
   auto load_lengths = [&]() __attribute__((always_inline)) {

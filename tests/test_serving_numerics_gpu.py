@@ -4,7 +4,7 @@ tolerances as in oracle/serving_oracle.py, tolerance()."""
 import pytest
 import torch
 
-from llm_gpu_kernels_amd import prepare_packed_gqa, prepare_paged_gqa
+from llm_gpu_kernels_amd import _native as N, prepare_packed_gqa, prepare_paged_gqa
 from oracle import serving_oracle as S
 
 pytestmark = pytest.mark.gpu
@@ -101,3 +101,27 @@ def test_large_scores(negative, q0, dtype, gpu_device):
         paged = prepare_paged_gqa(q[:rows].to(gpu_device), *pages, tables.to(gpu_device),
                                   torch.tensor(lengths, dtype=torch.int32, device=gpu_device))
         _assert_rows(paged.output, q, k, v, lambda r: lengths[r], range(rows))
+
+
+def test_paged_longest(gpu_device):
+    """As many keys as a table may name, 2^31 - 16, all of one page.  Keys of 0 give
+    every key the same probability, a power of two, and the waves' sums of values
+    of 0 to 3 are whole numbers below 2^24 times that; joining up to 4096 of them
+    is off by 2^-12 of the sum at most, less than half a step of bf16, which holds the
+    mean itself."""
+    page, width = 16, (1 << 27) - 1
+    g = torch.Generator().manual_seed(6)
+    v = torch.randint(0, 4, (1, 1, page, 64), generator=g).to(torch.bfloat16).to(gpu_device)
+    q = torch.ones(1, 1, 64, dtype=torch.bfloat16, device=gpu_device)
+    tables = torch.zeros(1, width, dtype=torch.int32, device=gpu_device)
+    lengths = torch.tensor([40], dtype=torch.int32, device=gpu_device)
+    plan = prepare_paged_gqa(q, torch.zeros_like(v), v, tables, lengths)
+    plan.check_inputs()
+    mean = v[0, 0].float().mean(0).to(torch.bfloat16)
+    for n in (32, page * width - 32, page * width - 16, page * width):
+        lengths.fill_(n)
+        assert torch.equal(plan.run()[0, 0], mean), n
+        plan.check_inputs()
+    lengths.fill_(2 ** 31 - 1)      # past the table: taken as all of it
+    assert torch.equal(plan.run()[0, 0], mean)
+    assert plan.read_status() == N.GQA_STATUS_BAD_BOUNDS
