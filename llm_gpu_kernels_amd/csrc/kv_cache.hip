@@ -20,7 +20,8 @@ constexpr int kWaves = kPlanThreads / kWave;
 constexpr int kScanPages = 8;       // pages of a thread per scanned chunk
 static_assert(KV_MAX_SEQUENCES <= kPlanThreads, "a thread per row");
 
-__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+// (Unsigned: a row's tokens go up to 2^31 - 1, a page's up to 1024.)
+__device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((uint32_t)a + b - 1u) / (uint32_t)b); }
 
 // Exclusive sums over the workgroup's threads of two numbers and of a flag, and the
 // totals.

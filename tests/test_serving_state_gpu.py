@@ -1,0 +1,31 @@
+"""Device state of plans and caches that a program reads or wrote wrongly:
+status words beside other streams, tables that name free pages, the largest
+lengths (MI355X only)."""
+import pytest
+import torch
+
+from llm_gpu_kernels_amd import PagedKVCache, _native as N
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(values, device):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+def test_largest_row_of_a_cache(gpu_device):
+    """A row whose length in tokens, rounded up to pages, passes 2^31."""
+    page, width = 1008, 2130440                           # page * width + page - 1 > 2^31
+    c = PagedKVCache(4, page, 1, 64, sequences=2, max_pages=width, max_tokens=16, device=gpu_device)
+    c.tables[0] = 1
+    c.lengths[0] = page * width
+    c.refs[1] = width
+    c.fork(_i32([0], gpu_device), _i32([1], gpu_device))
+    assert c.lengths.tolist() == [page * width] * 2 and c.refs.tolist() == [0, 2 * width, 0, 0]
+    assert (c.tables == 1).all()
+    c.reserve(_i32([1, 0], gpu_device))
+    assert c.read_status() == N.KV_STATUS_TOO_LONG
+    c.compact()
+    assert (c.tables == 0).all() and c.refs.tolist() == [2 * width, 0, 0, 0]
+    c.free(_i32([0, 1], gpu_device))
+    assert c.read_status() == 0 and not c.refs.any() and not c.lengths.any() and (c.tables == -1).all()
