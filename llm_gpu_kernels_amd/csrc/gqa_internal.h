@@ -82,7 +82,7 @@ size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int64_t keys, int cus)
 void gqa_paged_bind(GqaPagedArgs *a, void *workspace);
 hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s);
 
-// Synchronises `s`, reads a status word and enqueues its clearing.
+// Synchronises `s`, reads a status word and clears the bits that it had.
 hipError_t read_and_clear_status(uint32_t *status, uint32_t *flags, hipStream_t s);
 
 }  // namespace moe

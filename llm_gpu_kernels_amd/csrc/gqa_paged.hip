@@ -647,7 +647,7 @@ __global__ __launch_bounds__(kMergeThreads) void gqa_paged_merge(GqaPagedArgs a,
   if (live) *op = pack2<F16>(st.o[0] * inv, st.o[1] * inv);
 }
 
-__global__ void clear_word(uint32_t *w) { *w = 0; }
+__global__ void clear_bits(uint32_t *w, uint32_t bits) { atomicAnd(w, ~bits); }
 
 int waves_of(int D, int cus) { return cus * kWaves * (D == 128 ? kWorkgroups<128> : kWorkgroups<64>); }
 
@@ -723,12 +723,15 @@ hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s) {
   return a.dtype == GQA_FP16 ? launch<64, true>(a, cus, s) : launch<64, false>(a, cus, s);
 }
 
+// Clears the bits that it returns, no others, and is done with that on return: a bit
+// that work on another stream latches meanwhile is in this reading or in the next.
 hipError_t read_and_clear_status(uint32_t *status, uint32_t *flags, hipStream_t s) {
   hipError_t e = hipStreamSynchronize(s);
   if (e == hipSuccess) e = hipMemcpy(flags, status, sizeof(uint32_t), hipMemcpyDeviceToHost);
   if (e == hipSuccess && *flags) {
-    hipLaunchKernelGGL(clear_word, dim3(1), dim3(1), 0, s, status);
+    hipLaunchKernelGGL(clear_bits, dim3(1), dim3(1), 0, s, status, *flags);
     e = hipGetLastError();
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
   }
   return e;
 }

@@ -4,13 +4,48 @@ lengths (MI355X only)."""
 import pytest
 import torch
 
-from llm_gpu_kernels_amd import PagedKVCache, _native as N
+from llm_gpu_kernels_amd import PagedKVCache, _native as N, prepare_paged_gqa
 
 pytestmark = pytest.mark.gpu
 
 
 def _i32(values, device):
     return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+def test_status_beside_another_stream(gpu_device):
+    """A bit that a run on another stream latches while the word is read is in this
+    reading or in the next."""
+    q = torch.zeros(1, 1, 64, dtype=torch.float16, device=gpu_device)
+    pages = torch.zeros(1, 1, 16, 64, dtype=torch.float16, device=gpu_device)
+    tables, lengths = _i32([[0]], gpu_device), _i32([16], gpu_device)
+    plan = prepare_paged_gqa(q, pages, pages, tables, lengths)
+    side = torch.cuda.Stream(device=gpu_device)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    torch.cuda._sleep(1000)
+    start.record()
+    torch.cuda._sleep(1000000)
+    end.record()
+    torch.cuda.synchronize()
+    per_us = 1000000 / (start.elapsed_time(end) * 1e3)
+    lost = []
+    for i in range(300):
+        tables.fill_(7)
+        plan.run()                                    # latches the page
+        tables.fill_(0)
+        lengths.fill_(17)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(max(1, int(i * 0.2 * per_us)))
+            plan.run()                                # latches the length, 0 to 60 us later
+        flags = plan.read_status()
+        side.synchronize()
+        flags |= plan.read_status()
+        if flags != N.GQA_STATUS_BAD_PAGE | N.GQA_STATUS_BAD_BOUNDS:
+            lost.append(i)
+        lengths.fill_(16)
+    assert not lost
+    assert plan.read_status() == 0
 
 
 def test_largest_row_of_a_cache(gpu_device):
