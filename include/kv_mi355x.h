@@ -39,7 +39,8 @@ extern "C" {
 #define KV_STATUS_TOO_LONG 8u     /* a row would pass max_pages: nothing done           */
 #define KV_STATUS_BAD_COUNT 16u   /* a count negative, above the stride, or more than
                                      max_tokens in all: nothing done                    */
-#define KV_STATUS_BAD_STATE 32u   /* a length or page number out of range was found     */
+#define KV_STATUS_BAD_STATE 32u   /* a length or page number out of range was found; by
+                                     compact also a free page behind those in use       */
 
 #define KV_MAX_SEQUENCES 1024
 #define KV_MAX_PAGES (1 << 20)

@@ -408,7 +408,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_compact_plan(KvState s) {
   __syncthreads();
   for (int i = threadIdx.x; i < movers; i += kPlanThreads) {
     const int a = s.move_src[i], b = s.move_dst[i];
-    s.moved_to[a] = b;
+    s.move_of[a] = i;
     s.refs[b] = s.refs[a];
     s.refs[a] = 0;
   }
@@ -424,15 +424,16 @@ __global__ __launch_bounds__(kWideThreads) void kv_compact_finish(KvState s, int
     copy_moves(s, blockIdx.x - row_blocks, gridDim.x - row_blocks);
     return;
   }
-  const int U = (int)s.status[1];
+  const int U = (int)s.status[1], moves = *s.num_moves;
   for (int row = blockIdx.x; row < s.sequences; row += row_blocks) {
     const int n = row_pages(s, row);
     int32_t *const table = s.tables + (int64_t)row * s.max_pages;
     for (int c = threadIdx.x; c < n; c += kWideThreads) {
       const int p = table[c];
       if (p >= 0 && p < U) continue;
-      const int to = p >= U && p < s.pages ? s.moved_to[p] : -1;
-      if (to >= 0 && to < U) table[c] = to;
+      // move_of holds what earlier calls left for pages that did not move in this one.
+      const uint32_t i = p >= U && p < s.pages ? (uint32_t)s.move_of[p] : ~0u;
+      if (i < (uint32_t)moves && s.move_src[i] == p) table[c] = s.move_dst[i];
       else atomicOr(s.status, KV_STATUS_BAD_STATE);
     }
   }
@@ -454,7 +455,7 @@ void kv_bind_workspace(KvState *s, void *workspace) {
   s->move_src = (int32_t *)(w + 256);
   s->move_dst = (int32_t *)(w + 256 + each);
   s->list = (int32_t *)(w + 256 + 2 * each);
-  s->moved_to = (int32_t *)(w + 256 + 3 * each);
+  s->move_of = (int32_t *)(w + 256 + 3 * each);
 }
 
 hipError_t launch_kv_reserve(const KvState &s, const int32_t *counts, int stride, hipStream_t st) {

@@ -14,9 +14,9 @@ struct KvState {
   int64_t *slots;
   uint32_t *status;
   // Scratch: the count of moves, the workgroups of a fork that have finished (0
-  // between calls), the moves' source and target pages, the
-  // pages of a reserve (or of a compaction) in order, and where a moved page went.
-  int32_t *num_moves, *arrived, *move_src, *move_dst, *list, *moved_to;
+  // between calls), the moves' source and target pages, the pages of a reserve in
+  // order, and the number of a moved page's move.
+  int32_t *num_moves, *arrived, *move_src, *move_dst, *list, *move_of;
 };
 
 size_t kv_workspace_bytes(int pages);

@@ -48,6 +48,30 @@ def test_status_beside_another_stream(gpu_device):
     assert plan.read_status() == 0
 
 
+@pytest.mark.parametrize("earlier", [False, True])
+def test_compact_finds_free_pages_in_tables(earlier, gpu_device):
+    """A table that names a free page behind those in use: reported, and left as it is
+    instead of led to another row's page, whatever an earlier compaction moved."""
+    c = PagedKVCache(20, 16, 1, 64, sequences=4, max_pages=4, max_tokens=256, device=gpu_device)
+    c.reserve(_i32([64, 64, 64, 0], gpu_device))          # pages 0 to 11
+    if earlier:
+        c.free(_i32([0], gpu_device))
+        c.compact()                                       # 8 to 11 go to 0 to 3
+        assert c.tables[2].tolist() == [0, 1, 2, 3]
+    for page in (9, 11, 12, 19):
+        if not earlier and page < 12:
+            continue
+        before = c.tables.clone()
+        c.tables[1, 2] = page
+        c.compact()
+        assert c.read_status() == N.KV_STATUS_BAD_STATE
+        assert c.tables[1, 2].item() == page
+        c.tables[1, 2] = before[1, 2]
+        assert torch.equal(c.tables, before)
+    c.compact()
+    assert c.read_status() == 0
+
+
 def test_largest_row_of_a_cache(gpu_device):
     """A row whose length in tokens, rounded up to pages, passes 2^31."""
     page, width = 1008, 2130440                           # page * width + page - 1 > 2^31
