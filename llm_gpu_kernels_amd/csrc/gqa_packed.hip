@@ -60,7 +60,6 @@ __device__ __forceinline__ int swizzle_v(int row) { return D == 128 ? 4 * (row &
 // further).  As inline
 // assembly (it has no output register): the compiler would make every later LDS
 // read wait for all such loads in flight; the kernel waits with exact counts.
-// (Nothing else in this kernel uses m0.)
 template <int N>
 __device__ __forceinline__ void load_lds(u32x4 rsrc, uint32_t dst, const uint32_t (&off)[N]) {
   static_assert(N == 1 || N == 2, "loads of a wave");
@@ -70,12 +69,12 @@ __device__ __forceinline__ void load_lds(u32x4 rsrc, uint32_t dst, const uint32_
         "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
         :
         : "s"(dst), "v"(off[0]), "v"(off[1]), "s"(rsrc)
-        : "memory", "scc");
+        : "memory", "scc", "m0");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(dst), "v"(off[0]), "s"(rsrc)
-                 : "memory");
+                 : "memory", "m0");
 }
 __device__ __forceinline__ u32x4 buffer_words(const void *base, uint32_t bytes) {
   const uint64_t b = sgpr64((uint64_t)base);
