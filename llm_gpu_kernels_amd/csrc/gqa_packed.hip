@@ -34,6 +34,7 @@
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"
 #include "gqa_internal.h"
+#include "launch.h"
 
 namespace moe {
 
@@ -627,9 +628,8 @@ template <int D, bool F16>
 hipError_t launch(GqaPackedArgs a, int cus, hipStream_t s) {
   auto k = gqa_packed_kernel<D, F16>;
   constexpr int lds = kRing * 2 * kStageKeys * D * 2;
-  static const bool attr = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds) ==
-                           hipSuccess;
-  if (!attr) return hipErrorInvalidValue;
+  static std::atomic<uint64_t> allowed{0};
+  if (const hipError_t e = allow_lds((const void *)k, lds, &allowed)) return e;
   const int64_t tiles = max_tiles(a.N, a.G, a.S);
   int64_t per_xcd = (tiles * a.per_class + (1 << a.class_xcds) - 1) >> a.class_xcds;
   a.xcd_cus = cus / kXcds;  // a second round that is turned round has to be whole

@@ -34,6 +34,7 @@
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"
 #include "gqa_internal.h"
+#include "launch.h"
 
 namespace moe {
 
@@ -671,9 +672,8 @@ template <int D, bool F16, int TEAM>
 hipError_t launch_kernel(const GqaPagedArgs &a, int grid, hipStream_t s) {
   auto k = gqa_paged_kernel<D, F16, TEAM>;
   constexpr int waves = TEAM ? TEAM : kWaves, lds = waves * kWaveLds<D>;
-  static const bool attr = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds) ==
-                           hipSuccess;
-  if (!attr) return hipErrorInvalidValue;
+  static std::atomic<uint64_t> allowed{0};
+  if (const hipError_t e = allow_lds((const void *)k, lds, &allowed)) return e;
   hipLaunchKernelGGL(k, dim3(grid), dim3(64 * waves), lds, s, a);
   return hipGetLastError();
 }

@@ -25,6 +25,7 @@
 
 #include "common.h"
 #include "gqa_internal.h"
+#include "launch.h"
 
 namespace moe {
 
@@ -450,9 +451,8 @@ template <int G>
 hipError_t launch_g(const GqaArgs &a, int nsplit, hipStream_t s) {
   auto k = gqa_prefill_kernel<G>;
   constexpr int lds = kSlots * kStageBytes;
-  static const bool attr = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds) ==
-                           hipSuccess;
-  if (!attr) return hipErrorInvalidValue;
+  static std::atomic<uint64_t> allowed{0};
+  if (const hipError_t e = allow_lds((const void *)k, lds, &allowed)) return e;
   const int qt = 32 * (kMfmaWaves / G), nqb = (a.T + qt - 1) / qt;
   hipLaunchKernelGGL(k, dim3(nqb * a.Hkv * nsplit), dim3(kThreads), lds, s, a, nqb, nsplit);
   return hipGetLastError();

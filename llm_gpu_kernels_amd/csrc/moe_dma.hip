@@ -28,6 +28,7 @@
 // task's token rows behind the current unit's MFMAs.  Rounding as in
 // moe_stream.hip.
 #include "common.h"
+#include "launch.h"
 #include "moe_internal.h"
 #include "moe_route_dev.h"
 
@@ -670,10 +671,8 @@ hipError_t launch_one(const ExpertArgs &a, int num_cus, hipStream_t s, const Rou
   using C = DmaCfg<KIND, MT, PLAN>;
   auto k = dma_kernel<KIND, MT, SPU, PLAN>;
   const size_t lds = C::LDS;
-  static const bool attr = hipFuncSetAttribute((const void *)k,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)lds) == hipSuccess;
-  if (!attr) return hipErrorInvalidValue;
+  static std::atomic<uint64_t> allowed{0};
+  if (const hipError_t e = allow_lds((const void *)k, (int)lds, &allowed)) return e;
   RouteArgs none{};
   if (num_cus >= 4096) return hipErrorInvalidValue;  // finish_units packs the grid size in 12 bits
   hipLaunchKernelGGL(k, dim3(num_cus > 0 ? num_cus : 1), dim3(kThreads), lds, s, a, ra ? *ra : none);

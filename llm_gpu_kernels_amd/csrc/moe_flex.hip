@@ -27,6 +27,7 @@
 // and 64-row tasks): columns up to K = 384 / 768 / 1536 for 16 / 32 / 64-row
 // tasks, K beyond.
 #include "common.h"
+#include "launch.h"
 #include "moe_internal.h"
 
 namespace moe {
@@ -252,10 +253,8 @@ hipError_t launch_mt(const ExpertArgs &a, int task_capacity, hipStream_t s) {
   if (grid <= 0) return hipSuccess;
   const size_t lds = (size_t)kWaves * 2 * MT * kWave * sizeof(f32x4);
   auto k = flex_kernel<KIND, MT, W4, true>;
-  static const bool attr = hipFuncSetAttribute((const void *)k,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)lds) == hipSuccess;
-  if (!attr) return hipErrorInvalidValue;
+  static std::atomic<uint64_t> allowed{0};
+  if (const hipError_t e = allow_lds((const void *)k, (int)lds, &allowed)) return e;
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(kThreads), lds, s, a);
   return hipGetLastError();
 }

@@ -32,6 +32,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "launch.h"
 #include "moe_internal.h"
 #include "moe_route_dev.h"
 
@@ -474,10 +475,10 @@ hipError_t launch_one(const ExpertArgs &a, int units_bound, int num_cus, hipStre
                       const RouteArgs *ra = nullptr) {
   auto k = stream_kernel<KIND, MT, SPW, W4, FOLD, PLAN>;
   const size_t lds = stream_lds<KIND, MT, SPW, W4, FOLD>(PLAN);
+  static std::atomic<uint64_t> allowed{0};
+  if (const hipError_t e = allow_lds((const void *)k, (int)lds, &allowed)) return e;
   static int per_cu = [&] {
     int n = 1;
-    (void)hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize,
-                              (int)kMaxLds);
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, (const void *)k, kThreads, lds) !=
             hipSuccess || n < 1)
       n = 1;

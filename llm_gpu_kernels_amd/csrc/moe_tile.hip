@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "launch.h"
 #include "moe_internal.h"
 
 #define MOE_CONST __attribute__((address_space(4)))
@@ -691,11 +692,8 @@ template <int KIND, int NBM, bool W4>
 hipError_t launch_nbm(const ExpertArgs &a, int max_rows, int num_cus, hipStream_t s) {
   auto k = tile_kernel<KIND, NBM, W4>;
   const size_t lds = (size_t)Ring<NBM, W4>::kBytes;
-  static bool attr = [&] {
-    return hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)lds) == hipSuccess;
-  }();
-  if (!attr) return hipErrorInvalidValue;
+  static std::atomic<uint64_t> allowed{0};
+  if (const hipError_t e = allow_lds((const void *)k, (int)lds, &allowed)) return e;
   hipLaunchKernelGGL(k, dim3(num_cus), dim3(kThreads), lds, s, a, max_rows);
   return hipGetLastError();
 }
