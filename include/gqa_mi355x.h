@@ -71,8 +71,11 @@ void gqa_seg_plan_destroy(gqa_seg_plan *p);
  * or 128, Hq a multiple of Hkv, the group Hq / Hkv at most 64.  Products are
  * summed and softmax statistics held in fp32; probabilities are rounded to the
  * type for the product with V (half a step; fp16 ones that are less than 2^-25
- * of their row's largest, 2^-36 of that at most).  Bases 16-byte aligned; strides
- * in elements, multiples of 8.
+ * of their row's largest, 2^-36 of that at most).  Scores (scale q . k) from
+ * 2^26 on in magnitude (bf16: 2^30) may come out as NaN or zeros: fp32 has no
+ * bits left for their differences.  Bases 16-byte aligned; strides in elements,
+ * multiples of 8.  Runs of plans that share a workspace, or of one plan, must be in
+ * stream order.
  */
 #define GQA_BF16 0
 #define GQA_FP16 1
@@ -131,8 +134,7 @@ typedef struct gqa_paged_desc {
   size_t workspace_bytes;
 } gqa_paged_desc;
 typedef struct gqa_paged_plan gqa_paged_plan;
-/* Status words and the partial states of a run; plans that share a workspace
- * must run in stream order. */
+/* Status words and the partial states of a run. */
 int gqa_paged_workspace_bytes(const gqa_paged_desc *d, size_t *bytes);
 int gqa_paged_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d);
 int gqa_paged_plan_run(gqa_paged_plan *p, void *stream);

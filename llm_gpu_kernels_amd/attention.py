@@ -221,7 +221,7 @@ def _stream_of(device):
 
 class _PreparedPlan:
     """A plan of the library with its workspace; ``run()`` enqueues on the
-    current stream of q's device."""
+    current stream of q's device.  Runs of one plan must be in stream order."""
 
     _prefix = ""
 

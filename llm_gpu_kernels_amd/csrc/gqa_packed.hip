@@ -15,19 +15,20 @@
 // with the operands of each read from LDS one phase ahead.  A lane holds sixteen
 // scores of one query (the partner lane l ^ 32 the other sixteen), so the online
 // softmax is lane-local and P is the B operand of O^T as it lies.
-//   Measured before: one workgroup of eight such waves per CU (16384 tokens 2.08
-// against 2.05 ms, 16 ragged prompts 114 against 100 us: nothing runs beside its
-// start and end), and four waves of 64 rows, one per SIMD, that read half as much
-// from LDS but issue at most one instruction in four cycles (2.13 ms).
+//   Measured before, each against two workgroups of four waves as they were then: one
+// workgroup of eight such waves per CU (16384 tokens 2.08 against 2.05 ms, 16 ragged
+// prompts 114 against 100 us: nothing runs beside its start and end), and four waves
+// of 64 rows, one per SIMD, that read half as much from LDS but issue at most one
+// instruction in four cycles (2.13 ms).
 //
 // K and V come in stages of 32 keys, global -> LDS in whole rows (buffer loads with an
 // LDS destination; keys behind the sequence's end read as zeros), three to four
 // stages ahead in a ring of five, with one barrier per stage.
 //
-// Measured, 32 query heads of 128 on 8 KV heads, bf16: one prompt of 16384 tokens 2.0 ms, 1.10
-// PFLOP/s, the matrix cores 57 % busy (1.50 ms with inputs of 0: the card's power
-// bounds the rest; a matrix product of 16384 cubed runs at 1.30 and 1.78 PFLOP/s
-// then); 16 prompts of 65 to 1134 tokens 83 us behind 5 for the list: the start and
+// Measured, 32 query heads of 128 on 8 KV heads, bf16: one prompt of 16384 tokens 2.0 to
+// 2.15 ms by card, 1.02 to 1.10 PFLOP/s, the matrix cores 58 % busy (1.48 ms with
+// inputs of 0: the card's power bounds the rest; a matrix product of 16384 cubed runs
+// at 1.31 PFLOP/s, with inputs of 0 at 1.77); 16 prompts of 65 to 1134 tokens 83 us behind 5 for the list: the start and
 // end of a tile, 5 us with one workgroup left beside it, and the longest tiles;
 // four prompts of up to 48 tokens 6 us: launch and one round of loads.
 #include "common.h"

@@ -163,7 +163,7 @@ __host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 20
 // TEAM > 0: a workgroup of TEAM waves per (sequence, head block), each taking every
 // TEAM-th step, whose states are joined in LDS at the end.  TEAM 0: a range of the
 // flat list per wave, or teams of the workgroups' waves if the lengths make those
-// faster (tables of 8192 keys, 8 heads of 128: 64 sequences of 128 keys 14.5 us by the list,
+// faster and one grid has a workgroup for every pair, of rows of length 0 too (tables of 8192 keys, 8 heads of 128: 64 sequences of 128 keys 14.5 us by the list,
 // 9.3 so, 16 of 500 13.7, 10.1, 64 of 1000 48.4, 41.6; what the list loses by
 // looking is 0.3 us).
 template <int D, bool F16, int TEAM>
@@ -657,11 +657,11 @@ int waves_of(int D, int cus) { return cus * kWaves * (D == 128 ? kWorkgroups<128
 // of its sequence, however long it is.  So: eight waves if all teams then run at
 // once, else four (short prologues overlap; 2048 teams, lengths 1..512: 42 us, by
 // eight 53); and a team only if one with a full table has at most 16 steps a wave, and
-// not many more than half of what the list would give a wave.  Heads of 128, all of
-// one length, list and team: 8 x 128 keys 9.2, 4.7 us; 128 x 512 keys 14.0, 7.8; 128 x
-// 2048 keys 28, 22; 2048 of 1..1024 keys 98, 80; one sequence of 2048 keys among
-// 15 of 40: 13.0, 13.7.  Left to the list: 8 x 2048 keys 10.1, 13.6; 8 x 4096 keys
-// 11.8, 22.5.
+// not many more than half of what the list would give a wave.  By the list and by teams, 8
+// heads of 128, so 8 pairs a sequence: 8 pairs of 128 keys 9.2, 4.7 us; 128 of 512 keys 14.0,
+// 7.8; 128 of 2048 keys 28, 22; 2048 of 1..1024 keys 98, 80; 128, 8 of 2048 keys and the
+// others of 40, 13.0, 13.7.  Left to the list: 8 of 2048 keys 10.1, 13.6; 8 of 4096
+// keys 11.8, 22.5.
 int team_of(int64_t pairs, int64_t steps, int64_t waves) {
   const int team = 8 * pairs <= waves ? 8 : 4;
   const int64_t listed = (pairs * steps + waves - 1) / waves, teamed = (steps + team - 1) / team;

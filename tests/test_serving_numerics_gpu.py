@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 TYPES = [torch.bfloat16, torch.float16]
 
 
-def _assert_rows(out, q, k, v, keys_of_row, rows):
+def _assert_rows(out, q, k, v, keys_of_row, rows, scale=None):
     """Rows ``rows`` of ``out`` [rows, Hq, D]; row r sees its first
     keys_of_row(r) keys of k, v [n, Hkv, D].  tolerance() takes the outputs'
     rounding as relative; fp16 ones below 2^-14 are multiples of 2^-24, so off by
@@ -21,7 +21,7 @@ def _assert_rows(out, q, k, v, keys_of_row, rows):
     vmax = v.float().abs().max().item()
     for r in rows:
         n = keys_of_row(r)
-        ref, bound = S.attention_rows(q[r].cpu(), k[:n].cpu(), v[:n].cpu())
+        ref, bound = S.attention_rows(q[r].cpu(), k[:n].cpu(), v[:n].cpu(), scale)
         off = (out[r].double().cpu() - ref).abs()
         worst = (off / (S.tolerance(ref, bound, out.dtype, n, vmax) + step)).max().item()
         assert worst <= 1.0, (r, worst)
@@ -74,12 +74,7 @@ def test_paged_sink(nats, n, width, hq, hkv, d, dtype, gpu_device):
     plan.check_inputs()
 
 
-@pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("q0", [1.0, 64.0, 720.0, 2300.0, 4096.0, 16384.0, 61440.0])
-@pytest.mark.parametrize("negative", [False, True])
-def test_large_scores(negative, q0, dtype, gpu_device):
-    """Scores from hundreds to tens of millions, their differences far from 1: the keys
-    of the largest one share the probability equally."""
+def _check_large(q0, scale, negative, dtype, device):
     n, d, page = 640, 64, 16
     g = torch.Generator().manual_seed(5)
     q, k, v = torch.zeros(n, 2, d), torch.zeros(n, 1, d), torch.randn(n, 1, d, generator=g)
@@ -89,18 +84,36 @@ def test_large_scores(negative, q0, dtype, gpu_device):
     if negative:
         k = -k
     q, k, v = (t.to(dtype) for t in (q, k, v))
-    starts = torch.tensor([0, n], dtype=torch.int32, device=gpu_device)
-    packed = prepare_packed_gqa(q.to(gpu_device), k.to(gpu_device), v.to(gpu_device), starts)
-    _assert_rows(packed.output, q, k, v, lambda r: r + 1, range(0, n, 37))
+    starts = torch.tensor([0, n], dtype=torch.int32, device=device)
+    packed = prepare_packed_gqa(q.to(device), k.to(device), v.to(device), starts, scale=scale)
+    _assert_rows(packed.output, q, k, v, lambda r: r + 1, range(0, n, 37), scale)
     lengths = list(range(1, n + 1, 37))
     rows = len(lengths)
-    pages = [t.view(n // page, page, 1, d).transpose(1, 2).contiguous().to(gpu_device) for t in (k, v)]
+    pages = [t.view(n // page, page, 1, d).transpose(1, 2).contiguous().to(device) for t in (k, v)]
     for width in (n // page, 20000):
         tables = torch.full((rows, width), -1, dtype=torch.int32)
         tables[:, :n // page] = torch.arange(n // page)
-        paged = prepare_paged_gqa(q[:rows].to(gpu_device), *pages, tables.to(gpu_device),
-                                  torch.tensor(lengths, dtype=torch.int32, device=gpu_device))
-        _assert_rows(paged.output, q, k, v, lambda r: lengths[r], range(rows))
+        paged = prepare_paged_gqa(q[:rows].to(device), *pages, tables.to(device),
+                                  torch.tensor(lengths, dtype=torch.int32, device=device), scale=scale)
+        _assert_rows(paged.output, q, k, v, lambda r: lengths[r], range(rows), scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("q0", [1.0, 64.0, 720.0, 2300.0, 4096.0, 16384.0, 61440.0])
+@pytest.mark.parametrize("negative", [False, True])
+def test_large_scores(negative, q0, dtype, gpu_device):
+    """Scores from hundreds to tens of millions, their differences far from 1: the keys
+    of the largest one share the probability equally."""
+    _check_large(q0, None, negative, dtype, gpu_device)
+
+
+@pytest.mark.parametrize("dtype,scale", [(torch.bfloat16, 5.75), (torch.float16, 0.36)])
+@pytest.mark.parametrize("negative", [False, True])
+def test_largest_scores(negative, dtype, scale, gpu_device):
+    """The same just below 2^30 (fp16: 2^26), where they are documented to end."""
+    assert 0.99 * 2 ** (30 if dtype == torch.bfloat16 else 26) < 61440 * (2048 + 16 * 61) * scale < 2 ** (
+        30 if dtype == torch.bfloat16 else 26)
+    _check_large(61440.0, scale, negative, dtype, gpu_device)
 
 
 def test_paged_longest(gpu_device):
