@@ -20,10 +20,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 // most kF16Slack, and the largest p lies in [2^11, 2^15]: those within 2^-25 of it
 // are off by half a step, smaller ones by 2^-36 of it at most.  (With m at a maximum,
 // what many keys add under one that has nearly all of the sum was lost: 18 below it
-// in natural logarithms, most of it.)  No time lost; 13 and 2 cost 5 to 8 % in heads of 64, whose maxima
-// rise by more than 2 here and there.  From 2^20 on a score is itself off by 2^-4 and
-// more, and may pass m by more than limit(m) says: there m is a maximum, and follows
-// every new one.
+// in natural logarithms, most of it.)  That costs no time; 13 and 2 cost 5 to 8 % with
+// heads of 64, since maxima rise by more than 2 here and there.  From 2^20 on a score is
+// itself off by 2^-4 and more, and may pass m by more than limit(m) says: there m is a
+// maximum, and follows every new one.
 constexpr float kRescaleSlack = 8.f;
 constexpr float kF16Bias = 11.f, kF16Slack = 4.f, kF16Exact = 1048576.f;
 template <bool F16>

@@ -28,9 +28,10 @@
 // Measured, 32 query heads of 128 on 8 KV heads, bf16: one prompt of 16384 tokens 2.0 to
 // 2.15 ms by card, 1.02 to 1.10 PFLOP/s, the matrix cores 58 % busy (1.48 ms with
 // inputs of 0: the card's power bounds the rest; a matrix product of 16384 cubed runs
-// at 1.31 PFLOP/s, with inputs of 0 at 1.77); 16 prompts of 65 to 1134 tokens 83 us behind 5 for the list: the start and
-// end of a tile, 5 us with one workgroup left beside it, and the longest tiles;
-// four prompts of up to 48 tokens 6 us: launch and one round of loads.
+// at 1.31 PFLOP/s, with inputs of 0 at 1.77); 16 prompts of 65 to 1134 tokens 83 us
+// behind 5 for the list: the start and end of a tile, 5 us with one workgroup left
+// beside it, and the longest tiles; four prompts of up to 48 tokens 6 us: launch and
+// one round of loads.
 #include "common.h"
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"

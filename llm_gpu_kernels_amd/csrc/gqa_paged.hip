@@ -163,7 +163,8 @@ __host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 20
 // TEAM > 0: a workgroup of TEAM waves per (sequence, head block), each taking every
 // TEAM-th step, whose states are joined in LDS at the end.  TEAM 0: a range of the
 // flat list per wave, or teams of the workgroups' waves if the lengths make those
-// faster and one grid has a workgroup for every pair, of rows of length 0 too (tables of 8192 keys, 8 heads of 128: 64 sequences of 128 keys 14.5 us by the list,
+// faster and one grid has a workgroup for every pair, of rows of length 0 too
+// (tables of 8192 keys, 8 heads of 128: 64 sequences of 128 keys 14.5 us by the list,
 // 9.3 so, 16 of 500 13.7, 10.1, 64 of 1000 48.4, 41.6; what the list loses by
 // looking is 0.3 us).
 template <int D, bool F16, int TEAM>
