@@ -191,9 +191,14 @@ def _tables(lengths, page, pages, width, seed):
 
 
 def _slots(case, seed):
-    """A slot for every token, without order, and the pages they are drawn from."""
-    pages = -(-case["N"] // case["page"]) + 2
-    return random.Random(int(seed) + 1).sample(range(pages * case["page"]), case["N"]), pages
+    """A slot for every token, and the pages they are in: a chunk's tokens fill pages
+    one after the other, those of a step belong to as many sequences."""
+    page, n, rng = case["page"], case["N"], random.Random(int(seed) + 1)
+    pages = -(-n // page) + 2
+    order = rng.sample(range(pages), pages)
+    if n <= 256 and case["kind"] != "store":
+        return rng.sample(range(pages * page), n), pages, order
+    return [order[i // page] * page + i % page for i in range(n)], pages, order
 
 
 def _values(case, seed, pages):
@@ -293,7 +298,7 @@ def prepare(case, seed):
         q, k, v, positions, inv_freq, weights = _rope_inputs(case, seed)
         cache = None
         if case["store"] != "rows":
-            slots, pages = _slots(case, seed)
+            slots, pages, _ = _slots(case, seed)
             cache = _cache(case, pages, pages, 1, case["N"], None if case["store"] == "pages" else case["store"])
             cache.slots.copy_(torch.tensor(slots, device="cuda"))
         if own:
@@ -304,11 +309,7 @@ def prepare(case, seed):
         return dict(state, q=q, k=k, v=v, positions=positions, inv_freq=inv_freq, weights=weights, cache=cache)
     if kind in ("append", "store"):
         k, v = _rows(case, _generator(seed), [case["Hkv"]] * 2)
-        slots, pages = _slots(case, seed)
-        if kind == "store":  # the tokens of one row, in order
-            order = list(range(pages))
-            random.Random(int(seed) + 1).shuffle(order)
-            slots = [order[i // case["page"]] * case["page"] + i % case["page"] for i in range(case["N"])]
+        slots, pages, order = _slots(case, seed)
         cache = _cache(case, pages, pages, 1, case["N"], case["storage"])
         cache.slots.copy_(torch.tensor(slots, device="cuda"))
         state.update(cache=cache, k=k, v=v)
@@ -637,7 +638,7 @@ def _exact_rope(case, seed):
     q, k = one(q, weights[0]), one(k, weights[1])
     if case["store"] == "rows":
         return dict(q=q, k=k)
-    slots, pages = _slots(case, seed)
+    slots, pages, _ = _slots(case, seed)
     storage = None if case["store"] == "pages" else case["store"]
     (k, ks), (v, vs) = (_exact_pages(x, case, slots, pages, storage) for x in (k, v))
     return dict(q=q, k=k, v=v, **({} if storage is None else dict(k_scales=ks, v_scales=vs)))
@@ -657,7 +658,7 @@ def exact(case, seed):
         k, v = _rows(case, _generator(seed), [case["Hkv"]] * 2)
         if kind == "store":
             return dict(zip("kv", (_exact_values(*_exact_round(x, case["storage"], case["dtype"])) for x in (k, v))))
-        slots, pages = _slots(case, seed)
+        slots, pages, _ = _slots(case, seed)
         (k, ks), (v, vs) = (_exact_pages(x, case, slots, pages, case["storage"]) for x in (k, v))
         return dict(k=k, v=v, k_scales=ks, v_scales=vs)
     group, page = case["Hq"] // case["Hkv"] if "Hq" in case else 0, case["page"]
