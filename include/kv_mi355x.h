@@ -8,7 +8,8 @@
  * owned by the caller, 0 or a negative MOE_E* code, message in
  * moe_last_error().  No counterpart in the reference.
  *
- * k, v     [layers, pages, kv_heads, page_size, head_dim] of 16-bit elements
+ * k, v     [layers, pages, kv_heads, page_size, head_dim] of 16-bit elements, or
+ *          microscaled ones of 8 or 4 bits (KV_STORAGE_*)
  * tables   [sequences, max_pages] int32: the pages of each row in order, -1
  *          behind the last one
  * lengths  [sequences] int32: tokens of each row (0: the row is empty)
@@ -38,7 +39,8 @@ extern "C" {
 #define KV_STATUS_OUT_OF_PAGES 4u /* fewer free pages than reserve needs: nothing done */
 #define KV_STATUS_TOO_LONG 8u     /* a row would pass max_pages: nothing done           */
 #define KV_STATUS_BAD_COUNT 16u   /* a count negative, above the stride, or more than
-                                     max_tokens in all: nothing done                    */
+                                     max_tokens in all: nothing done; a gather's starts
+                                     that do not ascend within [0, tokens]              */
 #define KV_STATUS_BAD_STATE 32u   /* a length or page number out of range was found; by
                                      compact also a free page behind those in use       */
 
@@ -59,9 +61,29 @@ typedef struct kv_cache_desc {
 
 typedef struct kv_cache kv_cache;
 
+/*
+ * How a cache holds its keys and values.  Microscaled: 32 neighbouring elements of a
+ * row, e4m3 (8 bits) or e2m1 (4 bits, two in a byte, the earlier in the low half), stand
+ * for element * 2^(scale - 127); k and v then hold head_dim or head_dim / 2 bytes a row,
+ * and k_scales, v_scales [layers, pages, kv_heads, head_dim / 32, page_size] bytes.
+ */
+#define KV_STORAGE_16BIT 0
+#define KV_STORAGE_MXFP8 1
+#define KV_STORAGE_MXFP4 2
+#define KV_TOKENS_BF16 0
+#define KV_TOKENS_FP16 1
+
 int kv_cache_workspace_bytes(const kv_cache_desc *d, size_t *bytes);
 /* Validate the descriptor and bind its pointers on the current device. */
 int kv_cache_create(kv_cache **out, const kv_cache_desc *d);
+/* The same with a storage (KV_STORAGE_*) and the tokens' type (KV_TOKENS_*), which append
+ * takes and gather gives; k_scales and v_scales (16-byte aligned, zeroed once) are NULL
+ * with KV_STORAGE_16BIT.  append rounds to nearest even under the smallest scale with which
+ * all 32 are in range, 2^-117 at least and at most 2^119 (mxfp8) or 2^125 (mxfp4), with
+ * fp16 tokens 2^7 or 2^13, where larger magnitudes saturate; 32 among which an infinity or
+ * a NaN is read back as NaN. */
+int kv_cache_create_stored(kv_cache **out, const kv_cache_desc *d, int32_t storage, int32_t tokens, void *k_scales,
+                           void *v_scales);
 
 /*
  * Room for counts[s] more tokens in every row s (int32 [sequences]).  Pages are
@@ -79,6 +101,14 @@ int kv_cache_reserve(kv_cache *c, const int32_t *counts, int32_t stride, void *s
  * the cache are left out.  n <= max_tokens. */
 int kv_cache_append(kv_cache *c, int32_t layer, const void *k, const void *v, int64_t k_stride, int64_t v_stride,
                     int32_t n, void *stream);
+/* The first starts[i+1] - starts[i] tokens of row rows[i] (int32 [n], n <= sequences;
+ * fewer if the row is shorter, none if it is negative) read back from a layer to the rows
+ * starts[i].. of k and v ([tokens, kv_heads, head_dim], strides as for append), in the
+ * tokens' type.  starts: int32 [n + 1], ascending within [0, tokens] (else a status, and
+ * some rows may be left out).  Other rows of k and v are left as they were.  k and v share
+ * no memory with each other or the cache. */
+int kv_cache_gather(kv_cache *c, int32_t layer, const int32_t *rows, const int32_t *starts, int32_t n, void *k, void *v,
+                    int64_t k_stride, int64_t v_stride, int32_t tokens, void *stream);
 /* dst[i] becomes a second holder of the pages of src[i] (int32 [n], n <=
  * sequences): rows as they are before the call; dst[i] must be empty.  A pair with
  * a negative row is left out. */

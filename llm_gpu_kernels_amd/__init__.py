@@ -12,6 +12,7 @@ from .moe import (FrozenMoEPolicy, GemmConfig, PreparedMoE, PreparedRoutedMoE, p
 from .attention import (PreparedPackedGQA, PreparedPagedGQA, PreparedSegmentedGQA, prepare_cuda_gqa_compact,
                         prepare_packed_gqa, prepare_paged_gqa, prepare_segmented_gqa)
 from .kv_cache import PagedKVCache
+from .rotary import PreparedQKNormRope, prepare_qk_norm_rope
 from .weight_quant import (PackedGateUp, RepackedGateUp, TiledGateUp, dequantize_tiled,
                            quantize_gate_up, repack_gate_up, restore_v1_layout, tile_gate_up)
 
@@ -21,5 +22,5 @@ __all__ = [
     "prepare_w4_layout_moe", "prepare_w4_moe", "PackedGateUp", "RepackedGateUp", "TiledGateUp",
     "dequantize_tiled", "quantize_gate_up", "repack_gate_up", "restore_v1_layout", "tile_gate_up", "PreparedSegmentedGQA", "prepare_segmented_gqa",
     "prepare_cuda_gqa_compact", "PreparedPackedGQA", "prepare_packed_gqa", "PreparedPagedGQA", "prepare_paged_gqa",
-    "PagedKVCache",
+    "PagedKVCache", "PreparedQKNormRope", "prepare_qk_norm_rope",
 ]

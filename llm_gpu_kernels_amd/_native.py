@@ -77,6 +77,8 @@ class GqaPagedDesc(ctypes.Structure):
 
 KV_STATUS_BAD_ROW, KV_STATUS_NOT_EMPTY, KV_STATUS_OUT_OF_PAGES = 1, 2, 4
 KV_STATUS_TOO_LONG, KV_STATUS_BAD_COUNT, KV_STATUS_BAD_STATE = 8, 16, 32
+KV_STORAGE_16BIT, KV_STORAGE_MXFP8, KV_STORAGE_MXFP4 = 0, 1, 2
+KV_TOKENS_BF16, KV_TOKENS_FP16 = 0, 1
 KV_MAX_SEQUENCES, KV_MAX_PAGES, KV_MAX_TOKENS = 1024, 1 << 20, 1 << 20
 
 
@@ -85,6 +87,13 @@ class KvCacheDesc(ctypes.Structure):
                                        "max_pages", "max_tokens")] + \
                [(n, c_void_p) for n in ("k", "v", "tables", "lengths", "refs", "starts", "slots", "status",
                                         "workspace")] + [("workspace_bytes", c_size_t)]
+
+
+class QkNormRopeDesc(ctypes.Structure):
+    _fields_ = [(n, c_int32) for n in ("N", "Hq", "Hkv", "D", "R", "dtype", "interleaved", "weights_fp32")] + \
+               [(n, c_void_p) for n in ("q", "k", "v", "positions", "inv_freq", "q_weight", "k_weight", "q_out", "k_out")] + \
+               [(n, c_int64) for n in ("q_stride", "k_stride", "v_stride")] + \
+               [("eps", ctypes.c_float), ("layer", c_int32)]
 
 
 # name -> (restype, argtypes); the complete exported ABI of include/*.h.
@@ -124,13 +133,19 @@ SIGNATURES = {
     "gqa_paged_plan_destroy": (None, [c_void_p]),
     "kv_cache_workspace_bytes": (c_int32, [POINTER(KvCacheDesc), POINTER(c_size_t)]),
     "kv_cache_create": (c_int32, [POINTER(c_void_p), POINTER(KvCacheDesc)]),
+    "kv_cache_create_stored": (c_int32, [POINTER(c_void_p), POINTER(KvCacheDesc), c_int32, c_int32, c_void_p, c_void_p]),
     "kv_cache_reserve": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p]),
     "kv_cache_append": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_void_p]),
+    "kv_cache_gather": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int64,
+                                  c_int32, c_void_p]),
     "kv_cache_fork": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
     "kv_cache_free": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p]),
     "kv_cache_compact": (c_int32, [c_void_p, c_void_p]),
     "kv_cache_read_status": (c_int32, [c_void_p, c_void_p, POINTER(c_uint32)]),
     "kv_cache_destroy": (None, [c_void_p]),
+    "qk_norm_rope_create": (c_int32, [POINTER(c_void_p), POINTER(QkNormRopeDesc), c_void_p]),
+    "qk_norm_rope_run": (c_int32, [c_void_p, c_void_p]),
+    "qk_norm_rope_destroy": (None, [c_void_p]),
 }
 
 _LIB = None

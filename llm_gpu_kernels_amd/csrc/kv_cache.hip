@@ -10,6 +10,7 @@
 #include "common.h"
 #include "../../include/kv_mi355x.h"
 #include "kv_internal.h"
+#include "mx_dev.h"
 
 namespace moe {
 
@@ -195,23 +196,25 @@ __global__ __launch_bounds__(kPlanThreads) void kv_reserve_plan(KvState s, const
   }
 }
 
-// Copies the moves' pages in every layer, keys and values, in pieces of kPiece
-// bytes that the workgroups take in turn.  A compaction that moves 269 MB: 107 us,
+// Copies the moves' pages in every layer, keys and values and their scales, in pieces of
+// kPiece bytes that the workgroups take in turn.  A compaction that moves 269 MB: 107 us,
 // 5.0 TB/s read and written.
 constexpr int kPiece = 16384;
 __device__ __forceinline__ void copy_moves(const KvState &s, int block, int blocks) {
   const int n = *s.num_moves;
   if (n == 0) return;
-  const int64_t page_bytes = (int64_t)s.kv_heads * s.page_size * s.head_dim * 2;
-  const int pieces = (int)((page_bytes + kPiece - 1) / kPiece);
-  const int64_t total = (int64_t)n * 2 * s.layers * pieces;
+  const int pieces = (int)((s.page_bytes + kPiece - 1) / kPiece);
+  const int each = pieces + (int)((s.scale_page_bytes + kPiece - 1) / kPiece);
+  const int64_t total = (int64_t)n * 2 * s.layers * each;
   for (int64_t u = block; u < total; u += blocks) {
-    const int piece = (int)(u % pieces);
-    const int64_t rest = u / pieces;
+    int piece = (int)(u % each);
+    const int64_t rest = u / each;
     const int plane = (int)(rest % (2 * s.layers)), m = (int)(rest / (2 * s.layers));
-    uint8_t *const base = (uint8_t *)(plane < s.layers ? s.k : s.v) +
-                          (int64_t)(plane < s.layers ? plane : plane - s.layers) * s.pages * page_bytes +
-                          (int64_t)piece * kPiece;
+    const bool scales = piece >= pieces, keys = plane < s.layers;
+    if (scales) piece -= pieces;
+    const int64_t page_bytes = scales ? s.scale_page_bytes : s.page_bytes;
+    uint8_t *const base = (scales ? (keys ? s.k_scales : s.v_scales) : (uint8_t *)(keys ? s.k : s.v)) +
+                          (int64_t)(keys ? plane : plane - s.layers) * s.pages * page_bytes + (int64_t)piece * kPiece;
     const uint8_t *const from = base + s.move_src[m] * page_bytes;
     uint8_t *const to = base + s.move_dst[m] * page_bytes;
     const int bytes = (int)min((int64_t)kPiece, page_bytes - (int64_t)piece * kPiece);
@@ -274,6 +277,156 @@ __global__ __launch_bounds__(kWideThreads) void kv_append(KvState s, int layer, 
     const int64_t to = plane + ((page * s.kv_heads + head) * s.page_size + row) * s.head_dim + d;
     *(u32x4 *)(s.k + to) = *(const u32x4 *)(k + token * k_stride + c);
     *(u32x4 *)(s.v + to) = *(const u32x4 *)(v + token * v_stride + c);
+  }
+}
+
+// Sixteen values of a thread, half of a block, as elements under the block's scale:
+// fp8 in four words, fp4 in two.  The neighbour lane (l ^ 1) has the other half.
+struct Elements {
+  uint32_t w[4];
+  int scale;
+};
+template <int FMT, bool F16>
+__device__ __forceinline__ Elements quantise16(u32x4 a, u32x4 b) {
+  uint32_t lo = 0, hi = 0;  // largest magnitude by its bits, of the even and the odd values
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    lo = mx::larger(mx::larger(lo, a[i] & 0x7fffu), b[i] & 0x7fffu);
+    hi = mx::larger(mx::larger(hi, a[i] & 0x7fff0000u), b[i] & 0x7fff0000u);
+  }
+  uint32_t top = mx::larger(lo, hi >> 16);
+  top = mx::larger(top, mx::neighbour(top));
+  Elements e;
+  e.scale = mx::scale_byte<FMT, F16>(__float_as_uint(gqa::to_f32<F16>(top)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = i < 2 ? a[2 * i] : b[2 * i - 4], y = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
+    e.w[i] = mx::encode4<FMT>(gqa::to_f32<F16>(x & 0xffffu), gqa::to_f32<F16>(x >> 16), gqa::to_f32<F16>(y & 0xffffu),
+                              gqa::to_f32<F16>(y >> 16), e.scale);
+  }
+  if constexpr (FMT == mx::kFp4) {
+    e.w[0] |= e.w[1] << 16;
+    e.w[1] = e.w[2] | e.w[3] << 16;
+  }
+  return e;
+}
+
+// As kv_append, quantised: a thread has 16 values of a token's keys and of its values.
+template <int FMT, bool F16>
+__global__ __launch_bounds__(kWideThreads) void kv_append_mx(KvState s, int layer, const uint16_t *k, const uint16_t *v,
+                                                            int64_t k_stride, int64_t v_stride, int n) {
+  const int chunks = s.kv_heads * s.head_dim / 16;  // of a token, an even number
+  const int64_t total = (int64_t)n * chunks;
+  const int64_t cells = (int64_t)s.pages * s.page_size, plane = (int64_t)layer * s.pages;
+  // (Both halves of a block run together: total and the grid's threads are even.)
+  for (int64_t u = (int64_t)blockIdx.x * kWideThreads + threadIdx.x; u < total; u += (int64_t)gridDim.x * kWideThreads) {
+    const int token = (int)(u / chunks), c = (int)(u % chunks) * 16;
+    const int64_t slot = s.slots[token];
+    if (slot < 0 || slot >= cells) continue;
+    const int head = c / s.head_dim, d = c % s.head_dim;
+    const int64_t page = slot / s.page_size;
+    const int row = (int)(slot % s.page_size);
+    const int64_t at = (plane + page) * s.kv_heads + head;
+    const int64_t to = (at * s.page_size + row) * mx::row_bytes<FMT>(s.head_dim) + mx::row_bytes<FMT>(d);
+    const int64_t scale_to = (at * (s.head_dim / mx::kBlock) + d / mx::kBlock) * s.page_size + row;
+    const u32x4 *const kp = (const u32x4 *)(k + token * k_stride + c), *const vp = (const u32x4 *)(v + token * v_stride + c);
+    const u32x4 k0 = kp[0], k1 = kp[1], v0 = vp[0], v1 = vp[1];
+    const Elements ke = quantise16<FMT, F16>(k0, k1), ve = quantise16<FMT, F16>(v0, v1);
+    if constexpr (FMT == mx::kFp8) {
+      *(u32x4 *)((uint8_t *)s.k + to) = u32x4{ke.w[0], ke.w[1], ke.w[2], ke.w[3]};
+      *(u32x4 *)((uint8_t *)s.v + to) = u32x4{ve.w[0], ve.w[1], ve.w[2], ve.w[3]};
+    } else {
+      *(u32x2 *)((uint8_t *)s.k + to) = u32x2{ke.w[0], ke.w[1]};
+      *(u32x2 *)((uint8_t *)s.v + to) = u32x2{ve.w[0], ve.w[1]};
+    }
+    if (d % mx::kBlock == 0) {
+      s.k_scales[scale_to] = (uint8_t)ke.scale;
+      s.v_scales[scale_to] = (uint8_t)ve.scale;
+    }
+  }
+}
+
+// Tokens of rows of the cache, read back side by side: row rows[i]'s go to the rows of
+// k and v from starts[i] on.  A workgroup takes kGatherTokens of those; one thread each
+// finds where its token lies, and then all copy 16 values at a time.
+constexpr int kGatherTokens = 16;
+template <int FMT, bool F16>
+__global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, const int32_t *rows, const int32_t *starts,
+                                                         int n, uint16_t *k, uint16_t *v, int64_t k_stride,
+                                                         int64_t v_stride, int tokens) {
+  __shared__ int64_t slots[kGatherTokens];
+  const int first = blockIdx.x * kGatherTokens;
+  if (threadIdx.x < kGatherTokens) {
+    const int t = first + threadIdx.x;
+    int64_t slot = -1;
+    if (t < tokens && t >= starts[0] && t < starts[n]) {
+      int lo = 0, hi = n - 1;  // starts[lo] <= t < starts[hi + 1] throughout
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (starts[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      const int row = rows[lo], j = t - max(starts[lo], 0);
+      if (row >= s.sequences) {
+        atomicOr(s.status, KV_STATUS_BAD_ROW);
+      } else if (row >= 0) {
+        const int len = s.lengths[row];
+        if (len < 0 || len > s.max_pages * s.page_size) {
+          atomicOr(s.status, KV_STATUS_BAD_STATE);
+        } else if (j < len) {
+          const int p = s.tables[(int64_t)row * s.max_pages + j / s.page_size];
+          if (p < 0 || p >= s.pages) atomicOr(s.status, KV_STATUS_BAD_STATE);
+          else slot = (int64_t)p * s.page_size + j % s.page_size;
+        }
+      }
+    }
+    slots[threadIdx.x] = slot;
+  }
+  // Starts that do not ascend within [0, tokens] are reported, once for each of them.
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= n; i += kWideThreads)
+      if (starts[i] < (i ? starts[i - 1] : 0) || starts[i] > tokens) atomicOr(s.status, KV_STATUS_BAD_COUNT);
+  __syncthreads();
+  const int chunks = s.kv_heads * s.head_dim / 16;
+  const int64_t plane = (int64_t)layer * s.pages;
+  for (int u = threadIdx.x; u < chunks * kGatherTokens; u += kWideThreads) {
+    const int nth = u / chunks, c = u % chunks * 16;
+    const int64_t slot = slots[nth];
+    if (slot < 0) continue;
+    const int head = c / s.head_dim, d = c % s.head_dim;
+    const int64_t page = slot / s.page_size, at = (plane + page) * s.kv_heads + head;
+    const int row = (int)(slot % s.page_size);
+    const int64_t from = (at * s.page_size + row) * mx::row_bytes<FMT>(s.head_dim) + mx::row_bytes<FMT>(d);
+    const uint8_t *const kp = (const uint8_t *)s.k + from, *const vp = (const uint8_t *)s.v + from;
+    u32x4 *const ko = (u32x4 *)(k + (int64_t)(first + nth) * k_stride + c);
+    u32x4 *const vo = (u32x4 *)(v + (int64_t)(first + nth) * v_stride + c);
+    u32x4 x[4];
+    if constexpr (FMT == 0) {
+      x[0] = ((const u32x4 *)kp)[0];
+      x[1] = ((const u32x4 *)kp)[1];
+      x[2] = ((const u32x4 *)vp)[0];
+      x[3] = ((const u32x4 *)vp)[1];
+    } else {
+      const int64_t scale_at = (at * (s.head_dim / mx::kBlock) + d / mx::kBlock) * s.page_size + row;
+      const float ks = mx::scale_of(s.k_scales[scale_at]), vs = mx::scale_of(s.v_scales[scale_at]);
+      if constexpr (FMT == mx::kFp8) {
+        const u32x4 kw = *(const u32x4 *)kp, vw = *(const u32x4 *)vp;
+        x[0] = mx::decode8<FMT, F16>(kw[0], kw[1], ks);
+        x[1] = mx::decode8<FMT, F16>(kw[2], kw[3], ks);
+        x[2] = mx::decode8<FMT, F16>(vw[0], vw[1], vs);
+        x[3] = mx::decode8<FMT, F16>(vw[2], vw[3], vs);
+      } else {
+        const u32x2 kw = *(const u32x2 *)kp, vw = *(const u32x2 *)vp;
+        x[0] = mx::decode8<FMT, F16>(kw[0], 0u, ks);
+        x[1] = mx::decode8<FMT, F16>(kw[1], 0u, ks);
+        x[2] = mx::decode8<FMT, F16>(vw[0], 0u, vs);
+        x[3] = mx::decode8<FMT, F16>(vw[1], 0u, vs);
+      }
+    }
+    ko[0] = x[0];
+    ko[1] = x[1];
+    vo[0] = x[2];
+    vo[1] = x[3];
   }
 }
 
@@ -468,10 +621,27 @@ hipError_t launch_kv_reserve(const KvState &s, const int32_t *counts, int stride
 
 hipError_t launch_kv_append(const KvState &s, int layer, const uint16_t *k, const uint16_t *v, int64_t k_stride,
                             int64_t v_stride, int n, hipStream_t st) {
-  const int64_t total = (int64_t)n * (s.kv_heads * s.head_dim / 8);
+  const int64_t total = (int64_t)n * (s.kv_heads * s.head_dim / (s.storage ? 16 : 8));
   const int64_t want = (total + kWideThreads - 1) / kWideThreads;
-  hipLaunchKernelGGL(kv_append, dim3((uint32_t)(want < 65536 ? want : 65536)), dim3(kWideThreads), 0, st, s, layer, k, v,
-                     k_stride, v_stride, n);
+  auto launch = [&](auto *kernel) {
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(want < 65536 ? want : 65536)), dim3(kWideThreads), 0, st, s, layer, k, v,
+                       k_stride, v_stride, n);
+  };
+  if (s.storage == KV_STORAGE_MXFP8) launch(s.f16 ? kv_append_mx<mx::kFp8, true> : kv_append_mx<mx::kFp8, false>);
+  else if (s.storage == KV_STORAGE_MXFP4) launch(s.f16 ? kv_append_mx<mx::kFp4, true> : kv_append_mx<mx::kFp4, false>);
+  else launch(kv_append);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_gather(const KvState &s, int layer, const int32_t *rows, const int32_t *starts, int n, uint16_t *k,
+                            uint16_t *v, int64_t k_stride, int64_t v_stride, int tokens, hipStream_t st) {
+  auto launch = [&](auto *kernel) {
+    hipLaunchKernelGGL(kernel, dim3((tokens + kGatherTokens - 1) / kGatherTokens), dim3(kWideThreads), 0, st, s, layer, rows,
+                       starts, n, k, v, k_stride, v_stride, tokens);
+  };
+  if (s.storage == KV_STORAGE_MXFP8) launch(s.f16 ? kv_gather<mx::kFp8, true> : kv_gather<mx::kFp8, false>);
+  else if (s.storage == KV_STORAGE_MXFP4) launch(s.f16 ? kv_gather<mx::kFp4, true> : kv_gather<mx::kFp4, false>);
+  else launch(kv_gather<0, false>);
   return hipGetLastError();
 }
 

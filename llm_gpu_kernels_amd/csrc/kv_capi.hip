@@ -16,6 +16,13 @@ struct kv_cache {
   int device;
 };
 
+namespace moe {
+const KvState *kv_state(const kv_cache *c, int *device) {
+  *device = c->device;
+  return &c->s;
+}
+}
+
 namespace {
 
 using moe::capi_fail;
@@ -68,6 +75,11 @@ int kv_cache_workspace_bytes(const kv_cache_desc *d, size_t *bytes) {
 }
 
 int kv_cache_create(kv_cache **out, const kv_cache_desc *d) {
+  return kv_cache_create_stored(out, d, KV_STORAGE_16BIT, KV_TOKENS_BF16, nullptr, nullptr);
+}
+
+int kv_cache_create_stored(kv_cache **out, const kv_cache_desc *d, int32_t storage, int32_t tokens, void *k_scales,
+                           void *v_scales) {
   if (!out) return capi_fail(MOE_EINVAL, "null cache pointer");
   *out = nullptr;
   if (const int rc = validate_sizes(d)) return rc;
@@ -75,6 +87,10 @@ int kv_cache_create(kv_cache **out, const kv_cache_desc *d) {
   if (!aligned(d->tables, 4) || !aligned(d->lengths, 4) || !aligned(d->starts, 4) || !aligned(d->status, 4) ||
       !aligned(d->slots, 8) || !aligned(d->refs, 16))
     return capi_fail(MOE_EINVAL, "tables, lengths, starts, status, slots (8-byte) and refs (16-byte aligned) must be given");
+  if (storage < KV_STORAGE_16BIT || storage > KV_STORAGE_MXFP4 || (tokens != KV_TOKENS_BF16 && tokens != KV_TOKENS_FP16))
+    return capi_fail(MOE_EINVAL, "storage must be a KV_STORAGE_* and tokens a KV_TOKENS_* (got %d, %d)", storage, tokens);
+  if (storage != KV_STORAGE_16BIT ? !aligned(k_scales, 16) || !aligned(v_scales, 16) : k_scales || v_scales)
+    return capi_fail(MOE_EINVAL, "k_scales/v_scales must be 16-byte aligned, and null without a microscaled storage");
   const size_t need = moe::kv_workspace_bytes(d->pages);
   if (!aligned(d->workspace, 16) || d->workspace_bytes < need)
     return capi_fail(MOE_ESPACE, "workspace has %zu bytes, needs %zu, 16-byte aligned", d->workspace_bytes, need);
@@ -101,6 +117,13 @@ int kv_cache_create(kv_cache **out, const kv_cache_desc *d) {
   s.starts = d->starts;
   s.slots = d->slots;
   s.status = d->status;
+  s.storage = storage;
+  s.f16 = tokens == KV_TOKENS_FP16;
+  s.k_scales = (uint8_t *)k_scales;
+  s.v_scales = (uint8_t *)v_scales;
+  const int64_t rows = (int64_t)d->kv_heads * d->page_size;
+  s.page_bytes = rows * (storage == KV_STORAGE_16BIT ? 2 * d->head_dim : storage == KV_STORAGE_MXFP8 ? d->head_dim : d->head_dim / 2);
+  s.scale_page_bytes = storage == KV_STORAGE_16BIT ? 0 : rows * (d->head_dim / 32);
   moe::kv_bind_workspace(&s, d->workspace);
   c->device = dev;
   *out = c;
@@ -130,6 +153,26 @@ int kv_cache_append(kv_cache *c, int32_t layer, const void *k, const void *v, in
     return capi_fail(MOE_EINVAL, "token strides must be >= %lld and multiples of 8", (long long)row);
   return on_device(c, "append", [&] {
     return moe::launch_kv_append(c->s, layer, (const uint16_t *)k, (const uint16_t *)v, k_stride, v_stride, n,
+                                 (hipStream_t)stream);
+  });
+}
+
+int kv_cache_gather(kv_cache *c, int32_t layer, const int32_t *rows, const int32_t *starts, int32_t n, void *k, void *v,
+                    int64_t k_stride, int64_t v_stride, int32_t tokens, void *stream) {
+  if (!c) return capi_fail(MOE_EINVAL, "null cache");
+  if (layer < 0 || layer >= c->s.layers)
+    return capi_fail(MOE_EINVAL, "layer must be in [0, %d) (got %d)", c->s.layers, layer);
+  if (n < 0 || n > c->s.sequences)
+    return capi_fail(MOE_EINVAL, "n must be in [0, sequences = %d] (got %d)", c->s.sequences, n);
+  if (tokens < 0) return capi_fail(MOE_EINVAL, "tokens must not be negative (got %d)", tokens);
+  if (n == 0 || tokens == 0) return MOE_OK;
+  if (!aligned(rows, 4) || !aligned(starts, 4)) return capi_fail(MOE_EINVAL, "rows and starts must be given");
+  if (!aligned(k, 16) || !aligned(v, 16)) return capi_fail(MOE_EINVAL, "k/v must be non-null and 16-byte aligned");
+  const int64_t row = (int64_t)c->s.kv_heads * c->s.head_dim;
+  if (k_stride < row || v_stride < row || k_stride % 8 || v_stride % 8)
+    return capi_fail(MOE_EINVAL, "token strides must be >= %lld and multiples of 8", (long long)row);
+  return on_device(c, "gather", [&] {
+    return moe::launch_kv_gather(c->s, layer, rows, starts, n, (uint16_t *)k, (uint16_t *)v, k_stride, v_stride, tokens,
                                  (hipStream_t)stream);
   });
 }

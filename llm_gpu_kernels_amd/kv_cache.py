@@ -20,13 +20,22 @@ from .attention import _check_int32, _stream_of
 
 __all__ = ["PagedKVCache"]
 
+# storage -> the library's number, the elements' type (None: the tokens'), elements per entry
+_STORAGES = {None: (N.KV_STORAGE_16BIT, None, 1), "mxfp8": (N.KV_STORAGE_MXFP8, torch.float8_e4m3fn, 1),
+             "mxfp4": (N.KV_STORAGE_MXFP4, torch.float4_e2m1fn_x2, 2)}
+
 
 class PagedKVCache:
     """Keys and values of up to ``sequences`` rows in ``pages`` pages.
 
     Attributes (tensors on the GPU, updated in place):
 
-    * ``k``, ``v`` [layers, pages, kv_heads, page_size, head_dim];
+    * ``k``, ``v`` [layers, pages, kv_heads, page_size, head_dim]: with ``storage``
+      None of ``dtype``, with "mxfp8" of torch.float8_e4m3fn, with "mxfp4" of
+      torch.float4_e2m1fn_x2 (head_dim / 2 bytes, the earlier element in the low half);
+    * ``k_scales``, ``v_scales`` (None without a storage) torch.float8_e8m0fnu [layers,
+      pages, kv_heads, head_dim / 32, page_size]: element i of a row stands for its value
+      times the row's scale i // 32;
     * ``tables`` int32 [sequences, max_pages]: each row's pages, -1 behind them;
     * ``lengths`` int32 [sequences]: tokens of each row, 0 if it is empty;
     * ``refs`` int32 [pages]: rows that hold the page, 0 if it is free;
@@ -36,14 +45,21 @@ class PagedKVCache:
       counts, as ``prepare_packed_gqa`` takes them;
     * ``used_pages`` int32 [1]: pages in use at the last ``compact``.
 
+    A storage quantises on ``append`` (to nearest even, under the smallest power of two
+    with which the 32 are in range; a block with an infinity or a NaN becomes NaN) and
+    takes 0.52 ("mxfp8") or 0.27 ("mxfp4") of the 16-bit cache's bytes.  ``dtype`` is
+    the type of the tokens that ``append`` takes and ``gather`` gives.
+
     Values that a call on the GPU cannot serve are left out and latch a status
     (``read_status``, ``check_inputs``).
     """
 
     def __init__(self, pages, page_size, kv_heads, head_dim, *, sequences, max_pages, max_tokens, layers=1,
-                 dtype=torch.bfloat16, device="cuda"):
+                 dtype=torch.bfloat16, storage=None, device="cuda"):
         if dtype not in (torch.bfloat16, torch.float16):
             raise TypeError("dtype must be torch.bfloat16 or torch.float16")
+        if storage not in _STORAGES:
+            raise ValueError(f"storage must be None, 'mxfp8' or 'mxfp4' (got {storage!r})")
         device = torch.device(device)
         d = N.KvCacheDesc()
         sizes = dict(pages=pages, page_size=page_size, kv_heads=kv_heads, head_dim=head_dim, layers=layers,
@@ -60,10 +76,17 @@ class PagedKVCache:
             device = torch.device("cuda", torch.cuda.current_device())
         self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
         self.sequences, self.max_pages, self.max_tokens, self.layers = sequences, max_pages, max_tokens, layers
-        self.dtype, self.device = dtype, device
-        shape = (layers, pages, kv_heads, page_size, head_dim)
-        self.k = torch.zeros(shape, dtype=dtype, device=device)
-        self.v = torch.zeros(shape, dtype=dtype, device=device)
+        self.dtype, self.storage, self.device = dtype, storage, device
+        code, element, per_byte = _STORAGES[storage]
+        shape = (layers, pages, kv_heads, page_size, head_dim // per_byte)
+        def zeros(shape, kind):  # (torch fills no elements of four bits)
+            return torch.zeros(shape, dtype=torch.uint8 if element else kind, device=device).view(kind)
+
+        self.k, self.v = zeros(shape, element or dtype), zeros(shape, element or dtype)
+        self.k_scales = self.v_scales = None
+        if storage is not None:
+            shape = (layers, pages, kv_heads, head_dim // 32, page_size)
+            self.k_scales, self.v_scales = zeros(shape, torch.float8_e8m0fnu), zeros(shape, torch.float8_e8m0fnu)
 
         def ints(*size, value=0, kind=torch.int32):
             return torch.full(size, value, dtype=kind, device=device)
@@ -77,7 +100,9 @@ class PagedKVCache:
             setattr(d, name, getattr(self, name).data_ptr())
         d.status, d.workspace_bytes = self._status.data_ptr(), self.workspace.numel()
         with torch.cuda.device(device):
-            N.check(N.lib().kv_cache_create(ctypes.byref(handle), ctypes.byref(d)), "cache")
+            N.check(N.lib().kv_cache_create_stored(
+                ctypes.byref(handle), ctypes.byref(d), code, N.KV_TOKENS_FP16 if dtype == torch.float16 else N.KV_TOKENS_BF16,
+                *(None if t is None else t.data_ptr() for t in (self.k_scales, self.v_scales))), "cache")
         self._desc, self._cache = d, handle
 
     def _stream(self):
@@ -132,6 +157,24 @@ class PagedKVCache:
             raise ValueError("k and v must have the same number of tokens")
         N.check(N.lib().kv_cache_append(self._cache, layer, k.data_ptr(), v.data_ptr(), ks, vs, k.shape[0],
                                         self._stream()), "append")
+
+    def gather(self, layer, rows, starts, k, v):
+        """Read back the first ``starts[i + 1] - starts[i]`` tokens of row ``rows[i]``
+        (int32 [n]; fewer if the row is shorter, none if it is negative) of a layer to
+        the rows ``starts[i]`` and up of ``k`` and ``v`` ([tokens, kv_heads, head_dim] of
+        ``dtype``, the heads of a token side by side), as the keys and values of
+        ``prepare_segmented_gqa`` or ``prepare_packed_gqa`` lie.  ``starts``: int32
+        [n + 1], ascending within [0, tokens].  Other rows of k and v keep what they
+        held; k and v share no memory."""
+        if not isinstance(layer, int) or not 0 <= layer < self.layers:
+            raise ValueError(f"layer must be an int in [0, {self.layers}) (got {layer!r})")
+        rows = self._rows(rows, "rows")
+        _check_int32(starts, "starts", (rows.shape[0] + 1,), self.device)
+        ks, vs = self._token_stride(k, "k"), self._token_stride(v, "v")
+        if k.shape[0] != v.shape[0] or k.shape[0] >= 2 ** 31:
+            raise ValueError("k and v must have the same number of tokens, below 2^31")
+        N.check(N.lib().kv_cache_gather(self._cache, layer, rows.data_ptr(), starts.data_ptr(), rows.shape[0], k.data_ptr(),
+                                        v.data_ptr(), ks, vs, k.shape[0], self._stream()), "gather")
 
     def fork(self, src, dst):
         """Row ``dst[i]``, which must be empty, starts as a copy of row ``src[i]``

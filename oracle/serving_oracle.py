@@ -167,3 +167,72 @@ class Cache:
             for p in t:
                 holders[p] += 1
         assert holders == self.refs
+
+
+# ---- microscaled rows -----------------------------------------------------------
+
+E4M3 = [m * 2.0 ** -9 if e == 0 else (8 + m) * 2.0 ** (e - 10) for e in range(16) for m in range(8)][:-1]
+E2M1 = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+_LAST = {("mxfp8", torch.bfloat16): 119, ("mxfp8", torch.float16): 7, ("mxfp4", torch.bfloat16): 125,
+         ("mxfp4", torch.float16): 13}
+
+
+def mx_quantise(x, storage, dtype):
+    """Rows [..., D] of tokens of a type -> element codes uint8 [..., D] and scale
+    bytes uint8 [..., D / 32], by search over the table of elements."""
+    table = torch.tensor(E4M3 if storage == "mxfp8" else E2M1, dtype=torch.float64)
+    x = x.double().unflatten(-1, (-1, 32))
+    top = x.abs().amax(-1)
+    finite = torch.isfinite(x).all(-1)
+    x = torch.where(finite[..., None], x, 0.0)
+    byte = torch.full(top.shape, 10, dtype=torch.long)
+    for e in range(-116, _LAST[storage, dtype] + 1):  # the next larger scale where this one does not do
+        byte = torch.where(top > float(table[-1]) * 2.0 ** (e - 1), e + 127, byte)
+    y = x / torch.pow(torch.tensor(2.0, dtype=torch.float64), byte - 127)[..., None]
+    a = y.abs().clamp(max=float(table[-1]))
+    low = torch.searchsorted(table, a, right=True) - 1
+    high = (low + 1).clamp(max=len(table) - 1)
+    below, above = a - table[low], table[high] - a
+    code = torch.where((below > above) | ((below == above) & (low % 2 == 1)), high, low)
+    code = torch.where(above == 0, high, code) + torch.signbit(y) * (128 if storage == "mxfp8" else 8)
+    byte = torch.where(finite, byte, 255)
+    return torch.where(finite[..., None], code, 0).flatten(-2).to(torch.uint8), byte.to(torch.uint8)
+
+
+def mx_values(codes, scales, storage):
+    """What codes [..., D] under scale bytes [..., D / 32] stand for, in 64 bits."""
+    table = E4M3 + [math.nan] if storage == "mxfp8" else E2M1
+    table = torch.tensor(table + [-a for a in table], dtype=torch.float64)
+    power = torch.pow(torch.tensor(2.0, dtype=torch.float64), scales.long() - 127)
+    power = torch.where(scales == 255, math.nan, power)
+    return (table[codes.long()].unflatten(-1, (-1, 32)) * power[..., None]).flatten(-2)
+
+
+def mx_pack(codes, storage):
+    """Codes as they lie in a cache: two of four bits in a byte, the earlier low."""
+    return codes if storage == "mxfp8" else codes[..., 0::2] | codes[..., 1::2] << 4
+
+
+def mx_unpack(held, storage):
+    return held if storage == "mxfp8" else torch.stack([held & 15, held >> 4], -1).flatten(-2)
+
+
+# ---- norm and rotation ------------------------------------------------------------
+
+
+def norm_rope(x, positions, inv_freq, weight=None, eps=1e-6, interleaved=False):
+    """x [N, H, D] in 64 bits, pair by pair; also the magnitude of each pair, which
+    bounds what a rotation's roundings can do."""
+    x = x.double()
+    d, half = x.shape[-1], len(inv_freq)
+    if weight is not None:
+        x = x * weight.double() / torch.sqrt((x * x).mean(-1, keepdim=True) + eps)
+    out, size = x.clone(), x.abs()
+    for i in range(half):
+        a = positions.double() * float(inv_freq[i])
+        c, s = a.cos()[:, None], a.sin()[:, None]
+        low, high = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
+        out[..., low] = x[..., low] * c - x[..., high] * s
+        out[..., high] = x[..., high] * c + x[..., low] * s
+        size[..., low] = size[..., high] = x[..., low].abs() + x[..., high].abs()
+    return out, size

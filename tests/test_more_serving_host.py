@@ -1,0 +1,128 @@
+"""Quantised caches, norms and rotation, and attention with shared prefixes without a
+GPU: refusals of the C ABI and of the Python layer, and the oracle's own invariants."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from llm_gpu_kernels_amd import PagedKVCache, _native as N, prepare_qk_norm_rope
+from oracle import serving_oracle as S
+
+BASE = 1 << 20  # an address that is only looked at by the validation
+
+
+def _cache_desc():
+    d = N.KvCacheDesc()
+    d.pages, d.page_size, d.kv_heads, d.head_dim, d.layers = 100, 16, 8, 128, 2
+    d.sequences, d.max_pages, d.max_tokens = 4, 10, 64
+    for name in ("k", "v", "tables", "lengths", "refs", "starts", "slots", "status", "workspace"):
+        setattr(d, name, BASE)
+    d.workspace_bytes = 1 << 30
+    return d
+
+
+@pytest.mark.parametrize("storage,tokens,ks,vs", [(3, 0, BASE, BASE), (-1, 0, None, None), (1, 2, BASE, BASE), (1, 0, None, BASE),
+                                                  (1, 0, BASE, BASE + 8), (2, 1, BASE, None), (0, 0, BASE, BASE)])
+def test_stored_cache_refusals(storage, tokens, ks, vs):
+    handle = ctypes.c_void_p()
+    rc = N.lib().kv_cache_create_stored(ctypes.byref(handle), ctypes.byref(_cache_desc()), storage, tokens, ks, vs)
+    assert rc == N.MOE_EINVAL and not handle.value and N.last_error()
+
+
+def test_gather_null():
+    assert N.lib().kv_cache_gather(None, 0, BASE, BASE, 1, BASE, BASE, 1024, 1024, 5, None) == N.MOE_EINVAL
+
+
+def test_storage_names():
+    good = dict(sequences=4, max_pages=8, max_tokens=64)
+    for storage in ("fp8", "mxfp6", 8, "", torch.float8_e4m3fn):
+        with pytest.raises(ValueError, match="storage"):
+            PagedKVCache(10, 16, 2, 64, storage=storage, **good)
+
+
+def _qk(**kw):
+    d = N.QkNormRopeDesc()
+    d.N, d.Hq, d.Hkv, d.D, d.R = 10, 32, 8, 128, 128
+    for name in ("q", "k", "positions", "inv_freq", "q_weight", "k_weight", "q_out", "k_out"):
+        setattr(d, name, BASE)
+    d.q_stride, d.k_stride, d.v_stride, d.eps = 4096, 1024, 1024, 1e-6
+    for name, value in kw.items():
+        setattr(d, name, value)
+    return d
+
+
+def test_struct_size_matches_header():
+    # 8 int32 + 9 pointers + 3 int64 + float + int32.
+    assert ctypes.sizeof(N.QkNormRopeDesc) == 32 + 72 + 24 + 8
+
+
+@pytest.mark.parametrize("bad", [
+    dict(D=96), dict(D=256), dict(R=0), dict(R=130), dict(R=63), dict(R=-2), dict(dtype=2), dict(N=-1), dict(N=(1 << 28) + 1),
+    dict(Hq=0), dict(Hkv=0), dict(Hq=1 << 20), dict(eps=-1.0), dict(eps=math.nan), dict(eps=math.inf), dict(q=None),
+    dict(k=BASE + 8), dict(v=BASE), dict(positions=None), dict(inv_freq=BASE + 2), dict(q_weight=BASE + 4),
+    dict(k_weight=BASE + 8), dict(q_out=None), dict(k_out=None), dict(k_out=BASE + 8), dict(q_stride=4088),
+    dict(k_stride=1028), dict(q_stride=1 << 41),
+])
+def test_qk_refusals(bad):
+    handle = ctypes.c_void_p()
+    rc = N.lib().qk_norm_rope_create(ctypes.byref(handle), ctypes.byref(_qk(**bad)), None)
+    assert rc == N.MOE_EINVAL and not handle.value and N.last_error()
+
+
+def test_qk_null():
+    handle = ctypes.c_void_p()
+    assert N.lib().qk_norm_rope_run(None, None) == N.MOE_EINVAL
+    assert N.lib().qk_norm_rope_create(ctypes.byref(handle), None, None) == N.MOE_EINVAL
+    assert N.lib().qk_norm_rope_create(None, ctypes.byref(_qk()), None) == N.MOE_EINVAL
+    N.lib().qk_norm_rope_destroy(None)
+
+
+def test_qk_python_refusals():
+    q, k = torch.zeros(6, 4, 128, dtype=torch.bfloat16), torch.zeros(6, 2, 128, dtype=torch.bfloat16)
+    p, f, w = torch.zeros(6, dtype=torch.int32), torch.ones(64), torch.ones(128)
+    for bad in [(q.float(), k, p, f), (q, k, p.long(), f), (q, k, p, f.double()), (q, k, p, f, w.half()),
+                (q, k, p, f, w, w.bfloat16())]:
+        with pytest.raises(TypeError):
+            prepare_qk_norm_rope(*bad)
+    for bad in [(q, k[:5], p, f), (q, k, p[:5], f), (q, k, p, torch.ones(65)), (q, k, p, f[:0]), (q, k, p, f[None]),
+                (q, k.half(), p, f), (q[..., :64], k, p, f), (q, k, p, f, w[:64]), (q, k, p, torch.ones(128)[::2]),
+                (q, k, p, f, None, torch.ones(256)[::2]), (q[:, :, :100], k, p, f), (q, k, p, f)]:  # the last: not on a GPU
+        with pytest.raises(ValueError):
+            prepare_qk_norm_rope(*bad)
+    for eps in (-1e-6, math.nan, math.inf):
+        with pytest.raises(ValueError, match="eps"):
+            prepare_qk_norm_rope(q, k, p, f, eps=eps)
+
+
+@pytest.mark.parametrize("storage", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantised_rows(storage, dtype):
+    """Values are off by half of an element's step, the largest is never cut off where a
+    larger scale is left, quantising the values again changes nothing, and they are
+    numbers of the tokens' type."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(500, 64, generator=g) * torch.exp2(torch.randint(-6, 6, (500, 1), generator=g).float())
+    x = x.to(dtype)
+    codes, scales = S.mx_quantise(x, storage, dtype)
+    values = S.mx_values(codes, scales, storage)
+    scale = torch.exp2(scales.double() - 127).repeat_interleave(32, -1)
+    relative, absolute = (2.0 ** -4, 2.0 ** -10) if storage == "mxfp8" else (2.0 ** -2, 0.25)
+    assert ((values - x.double()).abs() <= torch.maximum(relative * x.double().abs(), absolute * scale)).all()
+    assert torch.equal(values.to(dtype).double(), values)
+    again = S.mx_values(*S.mx_quantise(values.to(dtype), storage, dtype), storage)
+    assert torch.equal(again, values)
+    assert torch.equal(S.mx_unpack(S.mx_pack(codes, storage), storage), codes)
+    if storage == "mxfp8":
+        y = (x.double() / scale).float()
+        assert torch.equal(y.to(torch.float8_e4m3fn).view(torch.uint8) & 127, codes & 127)
+
+
+def test_rotation_keeps_lengths():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(4, 2, 64, generator=g)
+    f = torch.rand(20, generator=g)
+    for interleaved in (False, True):
+        y, _ = S.norm_rope(x, torch.arange(4), f, interleaved=interleaved)
+        assert torch.allclose(y.norm(dim=-1), x.double().norm(dim=-1))
+        assert torch.equal(y[..., 40:], x[..., 40:].double()) and torch.equal(y[0], x[0].double())
