@@ -137,6 +137,24 @@ typedef struct gqa_paged_plan gqa_paged_plan;
 /* Status words and the partial states of a run. */
 int gqa_paged_workspace_bytes(const gqa_paged_desc *d, size_t *bytes);
 int gqa_paged_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d);
+/*
+ * The same over pages of a microscaled cache (kv_mi355x.h): k and v then hold D (MXFP8) or
+ * D / 2 (MXFP4) bytes a row, the rows of a (page, head) side by side; k_strides and
+ * v_strides are in bytes, {page, head, row}, multiples of 16, row D or D / 2.  The scales
+ * of a (page, head), [D / 32, page] bytes, lie together; page and head strides in bytes,
+ * multiples of 16.  Elements are taken in q's type: one whose value is beyond it is an
+ * infinity.  Run, status and destroy as above.
+ */
+#define GQA_STORAGE_16BIT 0
+#define GQA_STORAGE_MXFP8 1
+#define GQA_STORAGE_MXFP4 2
+typedef struct gqa_paged_scales {
+  int32_t storage; /* GQA_STORAGE_MXFP8 or GQA_STORAGE_MXFP4 */
+  const void *k, *v;
+  int64_t k_strides[2], v_strides[2]; /* page, head */
+} gqa_paged_scales;
+int gqa_paged_stored_workspace_bytes(const gqa_paged_desc *d, int32_t storage, size_t *bytes);
+int gqa_paged_stored_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d, const gqa_paged_scales *s);
 int gqa_paged_plan_run(gqa_paged_plan *p, void *stream);
 int gqa_paged_plan_read_status(gqa_paged_plan *p, void *stream, uint32_t *flags);
 void gqa_paged_plan_destroy(gqa_paged_plan *p);

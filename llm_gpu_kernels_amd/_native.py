@@ -57,6 +57,7 @@ class GqaDesc(ctypes.Structure):
 
 
 GQA_BF16, GQA_FP16 = 0, 1
+GQA_STORAGE_16BIT, GQA_STORAGE_MXFP8, GQA_STORAGE_MXFP4 = 0, 1, 2
 GQA_STATUS_BAD_BOUNDS, GQA_STATUS_BAD_PAGE = 1, 2
 
 
@@ -73,6 +74,11 @@ class GqaPagedDesc(ctypes.Structure):
                [("q_stride", c_int64), ("table_stride", c_int64), ("k_strides", c_int64 * 3),
                 ("v_strides", c_int64 * 3), ("scale", ctypes.c_float), ("workspace", c_void_p),
                 ("workspace_bytes", c_size_t)]
+
+
+class GqaPagedScales(ctypes.Structure):
+    _fields_ = [("storage", c_int32), ("k", c_void_p), ("v", c_void_p), ("k_strides", c_int64 * 2),
+                ("v_strides", c_int64 * 2)]
 
 
 KV_STATUS_BAD_ROW, KV_STATUS_NOT_EMPTY, KV_STATUS_OUT_OF_PAGES = 1, 2, 4
@@ -128,6 +134,8 @@ SIGNATURES = {
     "gqa_packed_plan_destroy": (None, [c_void_p]),
     "gqa_paged_workspace_bytes": (c_int32, [POINTER(GqaPagedDesc), POINTER(c_size_t)]),
     "gqa_paged_plan_create": (c_int32, [POINTER(c_void_p), POINTER(GqaPagedDesc)]),
+    "gqa_paged_stored_workspace_bytes": (c_int32, [POINTER(GqaPagedDesc), c_int32, POINTER(c_size_t)]),
+    "gqa_paged_stored_plan_create": (c_int32, [POINTER(c_void_p), POINTER(GqaPagedDesc), POINTER(GqaPagedScales)]),
     "gqa_paged_plan_run": (c_int32, [c_void_p, c_void_p]),
     "gqa_paged_plan_read_status": (c_int32, [c_void_p, c_void_p, POINTER(c_uint32)]),
     "gqa_paged_plan_destroy": (None, [c_void_p]),

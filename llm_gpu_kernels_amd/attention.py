@@ -225,17 +225,19 @@ class _PreparedPlan:
 
     _prefix = ""
 
-    def _create(self, desc, device):
+    def _create(self, desc, device, size=None, create=None):
+        """size, create: calls in the place of the library's workspace_bytes and plan_create."""
         fn = {n: getattr(N.lib(), f"{self._prefix}_{n}") for n in
               ("workspace_bytes", "plan_create", "plan_run", "plan_read_status", "plan_destroy")}
+        size, create = size or fn["workspace_bytes"], create or fn["plan_create"]
         nbytes, handle = ctypes.c_size_t(0), ctypes.c_void_p()
         if device.type != "cuda":
             raise ValueError("q must be on a GPU device")
         with torch.cuda.device(device):
-            N.check(fn["workspace_bytes"](ctypes.byref(desc), ctypes.byref(nbytes)), "prepare")
+            N.check(size(ctypes.byref(desc), ctypes.byref(nbytes)), "prepare")
             self.workspace = torch.zeros(int(nbytes.value), dtype=torch.uint8, device=device)
             desc.workspace, desc.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
-            N.check(fn["plan_create"](ctypes.byref(handle), ctypes.byref(desc)), "prepare")
+            N.check(create(ctypes.byref(handle), ctypes.byref(desc)), "prepare")
         self._fn, self._run, self._desc, self._plan, self._device = fn, fn["plan_run"], desc, handle, device
 
     def run(self):
@@ -319,16 +321,48 @@ def prepare_packed_gqa(q, k, v, starts, out=None, *, scale=None):
     return plan
 
 
+# Elements of a microscaled cache -> the library's storage, elements per entry of a row.
+_STORAGES = {torch.float8_e4m3fn: (N.GQA_STORAGE_MXFP8, 1), torch.float4_e2m1fn_x2: (N.GQA_STORAGE_MXFP4, 2)}
+
+
+def _check_stored(t, scales, name, q):
+    """Pages [P, Hkv, page, D] (or D / 2 entries) of a microscaled cache and their scales
+    [P, Hkv, D / 32, page], rows and scales of a page and head side by side."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in _STORAGES:
+        raise TypeError(f"{name} must be a torch.float8_e4m3fn or torch.float4_e2m1fn_x2 tensor beside scales")
+    if not isinstance(scales, torch.Tensor) or scales.dtype != torch.float8_e8m0fnu:
+        raise TypeError(f"{name}'s scales must be a torch.float8_e8m0fnu tensor")
+    dim = q.shape[2]
+    row = dim // _STORAGES[t.dtype][1]
+    if t.ndim != 4 or t.shape[3] != row or t.device != q.device or scales.device != q.device:
+        raise ValueError(f"{name} must have 4 dimensions, the last of {row}, and be on q's device with its scales")
+    pages, heads, page, _ = t.shape
+    if tuple(scales.shape) != (pages, heads, dim // 32, page):
+        raise ValueError(f"{name}'s scales must have shape {[pages, heads, dim // 32, page]}, got {list(scales.shape)}")
+    for x, inner in ((t, (row, 1)), (scales, (page, 1))):
+        if x.numel() and (_stride(x, 2, inner[0]), _stride(x, 3, 1)) != inner:
+            raise ValueError(f"{name} and its scales must hold a page and head in one piece")
+        if x.numel() and x.data_ptr() % 16:
+            raise ValueError(f"{name} and its scales must be 16-byte aligned")
+
+
 class PreparedPagedGQA(_PreparedPlan):
-    """Owns the output and workspace; binds q, the pages, tables and lengths by
+    """Owns the output and workspace; binds q, the pages, scales, tables and lengths by
     address."""
 
     _prefix = "gqa_paged"
 
-    def __init__(self, q, k_pages, v_pages, tables, lengths, out=None, scale=None):
+    def __init__(self, q, k_pages, v_pages, tables, lengths, out=None, scale=None, k_scales=None, v_scales=None):
         _check_rows(q, "q")
-        _check_rows(k_pages, "k_pages", 4, q)
-        _check_rows(v_pages, "v_pages", 4, q)
+        stored = k_scales is not None or v_scales is not None
+        if stored:
+            _check_stored(k_pages, k_scales, "k_pages", q)
+            _check_stored(v_pages, v_scales, "v_pages", q)
+            if v_pages.dtype != k_pages.dtype:
+                raise TypeError("k_pages and v_pages must have one dtype")
+        else:
+            _check_rows(k_pages, "k_pages", 4, q)
+            _check_rows(v_pages, "v_pages", 4, q)
         if k_pages.shape != v_pages.shape:
             raise ValueError("k_pages and v_pages must have one shape")
         if not isinstance(tables, torch.Tensor) or tables.ndim != 2:
@@ -336,22 +370,33 @@ class PreparedPagedGQA(_PreparedPlan):
         b, m = q.shape[0], tables.shape[1]
         _check_int32(tables, "tables", (b, m), q.device)
         _check_int32(lengths, "lengths", (b,), q.device)
-        p, hkv, page, dim = k_pages.shape
+        p, hkv, page, row = k_pages.shape
+        dim = q.shape[2]
         d = N.GqaPagedDesc()
         _set_sizes(d, B=b, Hq=q.shape[1], D=dim, Hkv=hkv, P=p, page=page, M=m, dtype=_DTYPES[q.dtype])
         d.scale = _fp32_scale(scale, dim)
         d.q_stride, d.table_stride = _token_stride(q, "q"), _stride(tables, 0, m)
+        least = 16 if stored else 8  # any stride will do for a dimension of one entry
         for t, into in ((k_pages, d.k_strides), (v_pages, d.v_strides)):
-            into[0], into[1], into[2] = _stride(t, 0, 8), _stride(t, 1, 8), _stride(t, 2, dim)
+            into[0], into[1], into[2] = _stride(t, 0, least), _stride(t, 1, least), _stride(t, 2, row)
         out = _output(out, q)
-        check_out_storage(out, [q, k_pages, v_pages, tables, lengths])
+        check_out_storage(out, [q, k_pages, v_pages, tables, lengths] + ([k_scales, v_scales] if stored else []))
         self.q, self.k_pages, self.v_pages, self.tables, self.lengths, self.output = (q, k_pages, v_pages, tables,
                                                                                       lengths, out)
+        self.k_scales, self.v_scales = k_scales, v_scales
         d.q, d.k, d.v, d.out, d.tables, d.lengths = (t.data_ptr() for t in (q, k_pages, v_pages, out, tables, lengths))
-        self._create(d, q.device)
+        if not stored:
+            self._create(d, q.device)
+            return
+        s = N.GqaPagedScales()
+        s.storage, s.k, s.v = _STORAGES[k_pages.dtype][0], k_scales.data_ptr(), v_scales.data_ptr()
+        for t, into in ((k_scales, s.k_strides), (v_scales, s.v_strides)):
+            into[0], into[1] = _stride(t, 0, 16), _stride(t, 1, 16)
+        self._create(d, q.device, lambda desc, nbytes: N.lib().gqa_paged_stored_workspace_bytes(desc, s.storage, nbytes),
+                     lambda plan, desc: N.lib().gqa_paged_stored_plan_create(plan, desc, ctypes.byref(s)))
 
 
-def prepare_paged_gqa(q, k_pages, v_pages, tables, lengths, out=None, *, scale=None):
+def prepare_paged_gqa(q, k_pages, v_pages, tables, lengths, out=None, *, scale=None, k_scales=None, v_scales=None):
     """Attention of one new token of each of B sequences over a paged cache.
 
     ``q`` [B, Hq, D], bf16 or fp16, D 64 or 128; ``k_pages`` and ``v_pages``
@@ -361,8 +406,14 @@ def prepare_paged_gqa(q, k_pages, v_pages, tables, lengths, out=None, *, scale=N
     ``j % page`` of page ``tables[b, j // page]``, and all ``lengths[b]`` keys
     are seen, the new token's own among them (``append`` it first).  Length 0
     gives zeros.  Values of all of them may change in place between runs; table
-    entries behind a sequence's last page are not read.  Prepares and runs once;
-    ``run()`` has no host sync and no allocation."""
-    plan = PreparedPagedGQA(q, k_pages, v_pages, tables, lengths, out, scale)
+    entries behind a sequence's last page are not read.
+
+    For a cache with a storage ``k_pages`` and ``v_pages`` are its elements
+    (torch.float8_e4m3fn [P, Hkv, page, D] or torch.float4_e2m1fn_x2 [P, Hkv, page, D / 2])
+    and ``k_scales`` and ``v_scales`` (``cache.k_scales[layer]``) their scales; a page's
+    rows of a head lie side by side.  Elements are taken in q's type: one whose value is
+    beyond it is an infinity.  Prepares and runs once; ``run()`` has no host sync and no
+    allocation."""
+    plan = PreparedPagedGQA(q, k_pages, v_pages, tables, lengths, out, scale, k_scales, v_scales)
     plan.run()
     return plan

@@ -157,9 +157,12 @@ int validate_paged_sizes(const gqa_paged_desc *d) {
   return MOE_OK;
 }
 
-int validate_paged(const gqa_paged_desc *d) {
+// scales: NULL for pages of 16-bit elements.
+int validate_paged(const gqa_paged_desc *d, const gqa_paged_scales *scales) {
   using moe::capi_fail;
   if (const int rc = validate_paged_sizes(d)) return rc;
+  if (scales && scales->storage != GQA_STORAGE_MXFP8 && scales->storage != GQA_STORAGE_MXFP4)
+    return capi_fail(MOE_EINVAL, "storage must be GQA_STORAGE_MXFP8 or GQA_STORAGE_MXFP4 (got %d)", scales->storage);
   if (d->B == 0) return MOE_OK;
   if (!d->q || !d->k || !d->v || !d->out || !aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out))
     return capi_fail(MOE_EINVAL, "q/k/v/out must be non-null and 16-byte aligned");
@@ -167,6 +170,18 @@ int validate_paged(const gqa_paged_desc *d) {
     return capi_fail(MOE_EINVAL, "tables and lengths must be given");
   if (d->table_stride < d->M) return capi_fail(MOE_EINVAL, "table_stride must be at least M = %d", d->M);
   int rc = check_stride("q row stride", d->q_stride, (int64_t)d->Hq * d->D);
+  if (rc) return rc;
+  if (scales) {
+    const int64_t row = scales->storage == GQA_STORAGE_MXFP8 ? d->D : d->D / 2;
+    if (!scales->k || !scales->v || !aligned16(scales->k) || !aligned16(scales->v))
+      return capi_fail(MOE_EINVAL, "scales must be non-null and 16-byte aligned");
+    for (const int64_t *st : {d->k_strides, d->v_strides})
+      if (st[2] != row) return capi_fail(MOE_EINVAL, "the rows of a page and head must lie %lld bytes apart", (long long)row);
+    for (const int64_t *st : {d->k_strides, d->v_strides, scales->k_strides, scales->v_strides})
+      if (st[0] < 16 || st[0] % 16 || st[1] < 16 || st[1] % 16)
+        return capi_fail(MOE_EINVAL, "page and head strides must be positive multiples of 16 bytes");
+    return MOE_OK;
+  }
   for (int kv = 0; !rc && kv < 2; ++kv) {
     const int64_t *st = kv ? d->v_strides : d->k_strides;
     if (st[0] < 8 || st[0] % 8 || st[1] < 8 || st[1] % 8)
@@ -176,8 +191,8 @@ int validate_paged(const gqa_paged_desc *d) {
   return rc;
 }
 
-size_t paged_workspace(const gqa_paged_desc *d, int cus) {
-  return moe::gqa_paged_workspace(d->B, d->Hq, d->Hkv, d->D, (int64_t)d->M * d->page, cus);
+size_t paged_workspace(const gqa_paged_desc *d, int storage, int cus) {
+  return moe::gqa_paged_workspace(d->B, d->Hq, d->Hkv, d->D, storage, (int64_t)d->M * d->page, cus);
 }
 
 int need_workspace(const void *workspace, size_t have, size_t need) {
@@ -244,32 +259,55 @@ int gqa_packed_plan_read_status(gqa_packed_plan *p, void *stream, uint32_t *flag
 void gqa_packed_plan_destroy(gqa_packed_plan *p) { delete p; }
 
 int gqa_paged_workspace_bytes(const gqa_paged_desc *d, size_t *bytes) {
+  return gqa_paged_stored_workspace_bytes(d, GQA_STORAGE_16BIT, bytes);
+}
+
+int gqa_paged_stored_workspace_bytes(const gqa_paged_desc *d, int32_t storage, size_t *bytes) {
   int rc = validate_paged_sizes(d), dev = 0, cus = 0;
+  if (!rc && (storage < GQA_STORAGE_16BIT || storage > GQA_STORAGE_MXFP4))
+    rc = moe::capi_fail(MOE_EINVAL, "unknown storage %d", storage);
   if (!rc && !bytes) rc = moe::capi_fail(MOE_EINVAL, "null bytes");
   if (!rc) rc = device_cus(&dev, &cus);
-  if (!rc) *bytes = paged_workspace(d, cus);
+  if (!rc) *bytes = paged_workspace(d, storage, cus);
   return rc;
 }
 
-int gqa_paged_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d) {
+static int create_paged(gqa_paged_plan **out, const gqa_paged_desc *d, const gqa_paged_scales *scales) {
   if (!out) return moe::capi_fail(MOE_EINVAL, "null plan pointer");
   *out = nullptr;
-  int rc = validate_paged(d), dev = 0, cus = 0;
+  const int storage = scales ? scales->storage : GQA_STORAGE_16BIT;
+  int rc = validate_paged(d, scales), dev = 0, cus = 0;
   if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, 256);
   if (!rc) rc = device_cus(&dev, &cus);
-  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, paged_workspace(d, cus));
+  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, paged_workspace(d, storage, cus));
   if (rc) return rc;
   gqa_paged_plan *p = new (std::nothrow) gqa_paged_plan;
   if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");
   p->a = moe::GqaPagedArgs{(const uint16_t *)d->q, (const uint16_t *)d->k, (const uint16_t *)d->v, (uint16_t *)d->out,
                            d->tables, d->lengths, d->q_stride, d->table_stride, d->k_strides[0], d->k_strides[1],
                            d->k_strides[2], d->v_strides[0], d->v_strides[1], d->v_strides[2], d->B, d->Hq, d->Hkv, d->D,
-                           d->P, d->page, d->M, d->dtype, scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr};
+                           d->P, d->page, d->M, d->dtype, scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr,
+                           storage, nullptr, nullptr, 0, 0, 0, 0};
+  if (scales) {
+    p->a.k_scales = (const uint8_t *)scales->k;
+    p->a.v_scales = (const uint8_t *)scales->v;
+    p->a.ks_page = scales->k_strides[0];
+    p->a.ks_head = scales->k_strides[1];
+    p->a.vs_page = scales->v_strides[0];
+    p->a.vs_head = scales->v_strides[1];
+  }
   moe::gqa_paged_bind(&p->a, d->workspace);
   p->device = dev;
   p->cus = cus;
   *out = p;
   return MOE_OK;
+}
+
+int gqa_paged_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d) { return create_paged(out, d, nullptr); }
+
+int gqa_paged_stored_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d, const gqa_paged_scales *s) {
+  if (!s) return moe::capi_fail(MOE_EINVAL, "null scales");
+  return create_paged(out, d, s);
 }
 
 int gqa_paged_plan_run(gqa_paged_plan *p, void *stream) {

@@ -77,8 +77,13 @@ struct GqaPagedArgs {
   int32_t *pieces;                       // {first slot, pieces (0: none, written at once)} per
                                          // (sequence, block of query heads)
   float *partial;                        // [2 per wave][rows]{m, l, O[D]}
+  // Microscaled pages (GQA_STORAGE_*, 0: 16-bit ones): then the strides of k and v above
+  // are in bytes, as these of their scales.
+  int storage;
+  const uint8_t *k_scales, *v_scales;
+  int64_t ks_page, ks_head, vs_page, vs_head;
 };
-size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int64_t keys, int cus);
+size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int storage, int64_t keys, int cus);
 void gqa_paged_bind(GqaPagedArgs *a, void *workspace);
 hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s);
 
