@@ -159,6 +159,27 @@ int gqa_paged_plan_run(gqa_paged_plan *p, void *stream);
 int gqa_paged_plan_read_status(gqa_paged_plan *p, void *stream, uint32_t *flags);
 void gqa_paged_plan_destroy(gqa_paged_plan *p);
 
+/*
+ * The paged form where groups of sequences start with the same keys: group g is the
+ * sequences starts[g] .. starts[g+1]-1 (int32 [G + 1], ascending within [0, B]; sequences
+ * before starts[0] and from starts[G] on are in none), and the first prefixes[g] keys
+ * (int32 [G]) are the same for all of its members that have keys; they are read once, by
+ * the table of one of them.  All of them that are in whole blocks of 16 keys, within every
+ * such member's length, count; what they hold beyond that each sequence reads by itself.
+ * Every other table entry is the sequence's own, as without groups.  Bounds that do not
+ * ascend within [0, B] are reported (GQA_STATUS_BAD_BOUNDS) and nothing is shared then; so
+ * are negative prefixes, taken as 0.  starts and prefixes lie on the GPU and are read by
+ * every run.  G <= 2^16; desc as for the paged form, with a workspace of
+ * gqa_shared_workspace_bytes().
+ */
+typedef struct gqa_shared_plan gqa_shared_plan;
+int gqa_shared_workspace_bytes(const gqa_paged_desc *d, int32_t G, size_t *bytes);
+int gqa_shared_plan_create(gqa_shared_plan **out, const gqa_paged_desc *d, int32_t G, const int32_t *starts,
+                           const int32_t *prefixes);
+int gqa_shared_plan_run(gqa_shared_plan *p, void *stream);
+int gqa_shared_plan_read_status(gqa_shared_plan *p, void *stream, uint32_t *flags);
+void gqa_shared_plan_destroy(gqa_shared_plan *p);
+
 #ifdef __cplusplus
 }
 #endif

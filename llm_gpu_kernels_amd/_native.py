@@ -139,6 +139,11 @@ SIGNATURES = {
     "gqa_paged_plan_run": (c_int32, [c_void_p, c_void_p]),
     "gqa_paged_plan_read_status": (c_int32, [c_void_p, c_void_p, POINTER(c_uint32)]),
     "gqa_paged_plan_destroy": (None, [c_void_p]),
+    "gqa_shared_workspace_bytes": (c_int32, [POINTER(GqaPagedDesc), c_int32, POINTER(c_size_t)]),
+    "gqa_shared_plan_create": (c_int32, [POINTER(c_void_p), POINTER(GqaPagedDesc), c_int32, c_void_p, c_void_p]),
+    "gqa_shared_plan_run": (c_int32, [c_void_p, c_void_p]),
+    "gqa_shared_plan_read_status": (c_int32, [c_void_p, c_void_p, POINTER(c_uint32)]),
+    "gqa_shared_plan_destroy": (None, [c_void_p]),
     "kv_cache_workspace_bytes": (c_int32, [POINTER(KvCacheDesc), POINTER(c_size_t)]),
     "kv_cache_create": (c_int32, [POINTER(c_void_p), POINTER(KvCacheDesc)]),
     "kv_cache_create_stored": (c_int32, [POINTER(c_void_p), POINTER(KvCacheDesc), c_int32, c_int32, c_void_p, c_void_p]),

@@ -22,7 +22,7 @@ import torch
 from . import _native as N
 
 __all__ = ["PreparedSegmentedGQA", "prepare_segmented_gqa", "prepare_cuda_gqa_compact", "PreparedPackedGQA",
-           "prepare_packed_gqa", "PreparedPagedGQA", "prepare_paged_gqa"]
+           "prepare_packed_gqa", "PreparedPagedGQA", "prepare_paged_gqa", "PreparedSharedGQA", "prepare_shared_gqa"]
 
 
 def _validate(t, name, device, heads):
@@ -360,7 +360,22 @@ class PreparedPagedGQA(_PreparedPlan):
             _check_stored(v_pages, v_scales, "v_pages", q)
             if v_pages.dtype != k_pages.dtype:
                 raise TypeError("k_pages and v_pages must have one dtype")
-        else:
+        d = self._bind(q, k_pages, v_pages, tables, lengths, out, scale, (k_scales, v_scales) if stored else ())
+        self.k_scales, self.v_scales = k_scales, v_scales
+        if not stored:
+            self._create(d, q.device)
+            return
+        s = N.GqaPagedScales()
+        s.storage, s.k, s.v = _STORAGES[k_pages.dtype][0], k_scales.data_ptr(), v_scales.data_ptr()
+        for t, into in ((k_scales, s.k_strides), (v_scales, s.v_strides)):
+            into[0], into[1] = _stride(t, 0, 16), _stride(t, 1, 16)
+        self._create(d, q.device, lambda desc, nbytes: N.lib().gqa_paged_stored_workspace_bytes(desc, s.storage, nbytes),
+                     lambda plan, desc: N.lib().gqa_paged_stored_plan_create(plan, desc, ctypes.byref(s)))
+
+    def _bind(self, q, k_pages, v_pages, tables, lengths, out, scale, more=()):
+        """The descriptor of attention over pages; ``more``: other inputs, and with them
+        elements that have been checked already."""
+        if not more:
             _check_rows(k_pages, "k_pages", 4, q)
             _check_rows(v_pages, "v_pages", 4, q)
         if k_pages.shape != v_pages.shape:
@@ -371,29 +386,19 @@ class PreparedPagedGQA(_PreparedPlan):
         _check_int32(tables, "tables", (b, m), q.device)
         _check_int32(lengths, "lengths", (b,), q.device)
         p, hkv, page, row = k_pages.shape
-        dim = q.shape[2]
         d = N.GqaPagedDesc()
-        _set_sizes(d, B=b, Hq=q.shape[1], D=dim, Hkv=hkv, P=p, page=page, M=m, dtype=_DTYPES[q.dtype])
-        d.scale = _fp32_scale(scale, dim)
+        _set_sizes(d, B=b, Hq=q.shape[1], D=q.shape[2], Hkv=hkv, P=p, page=page, M=m, dtype=_DTYPES[q.dtype])
+        d.scale = _fp32_scale(scale, q.shape[2])
         d.q_stride, d.table_stride = _token_stride(q, "q"), _stride(tables, 0, m)
-        least = 16 if stored else 8  # any stride will do for a dimension of one entry
+        least = 16 if more else 8  # any stride will do for a dimension of one entry
         for t, into in ((k_pages, d.k_strides), (v_pages, d.v_strides)):
             into[0], into[1], into[2] = _stride(t, 0, least), _stride(t, 1, least), _stride(t, 2, row)
         out = _output(out, q)
-        check_out_storage(out, [q, k_pages, v_pages, tables, lengths] + ([k_scales, v_scales] if stored else []))
+        check_out_storage(out, [q, k_pages, v_pages, tables, lengths, *more])
         self.q, self.k_pages, self.v_pages, self.tables, self.lengths, self.output = (q, k_pages, v_pages, tables,
                                                                                       lengths, out)
-        self.k_scales, self.v_scales = k_scales, v_scales
         d.q, d.k, d.v, d.out, d.tables, d.lengths = (t.data_ptr() for t in (q, k_pages, v_pages, out, tables, lengths))
-        if not stored:
-            self._create(d, q.device)
-            return
-        s = N.GqaPagedScales()
-        s.storage, s.k, s.v = _STORAGES[k_pages.dtype][0], k_scales.data_ptr(), v_scales.data_ptr()
-        for t, into in ((k_scales, s.k_strides), (v_scales, s.v_strides)):
-            into[0], into[1] = _stride(t, 0, 16), _stride(t, 1, 16)
-        self._create(d, q.device, lambda desc, nbytes: N.lib().gqa_paged_stored_workspace_bytes(desc, s.storage, nbytes),
-                     lambda plan, desc: N.lib().gqa_paged_stored_plan_create(plan, desc, ctypes.byref(s)))
+        return d
 
 
 def prepare_paged_gqa(q, k_pages, v_pages, tables, lengths, out=None, *, scale=None, k_scales=None, v_scales=None):
@@ -415,5 +420,47 @@ def prepare_paged_gqa(q, k_pages, v_pages, tables, lengths, out=None, *, scale=N
     beyond it is an infinity.  Prepares and runs once; ``run()`` has no host sync and no
     allocation."""
     plan = PreparedPagedGQA(q, k_pages, v_pages, tables, lengths, out, scale, k_scales, v_scales)
+    plan.run()
+    return plan
+
+
+class PreparedSharedGQA(PreparedPagedGQA):
+    """Owns the output and workspace; binds q, the pages, tables, lengths, starts and
+    prefixes by address."""
+
+    _prefix = "gqa_shared"
+
+    def __init__(self, q, k_pages, v_pages, tables, lengths, starts, prefixes, out=None, scale=None):
+        _check_rows(q, "q")
+        d = self._bind(q, k_pages, v_pages, tables, lengths, out, scale)
+        if not isinstance(starts, torch.Tensor) or starts.ndim != 1 or starts.shape[0] < 1:
+            raise ValueError("starts must be an int32 tensor [groups + 1]")
+        groups = starts.shape[0] - 1
+        _check_int32(starts, "starts", (groups + 1,), q.device)
+        _check_int32(prefixes, "prefixes", (groups,), q.device)
+        check_out_storage(self.output, [starts, prefixes])
+        if groups >= 2 ** 31:
+            raise ValueError(f"starts must have below 2^31 entries (got {groups + 1})")
+        self.starts, self.prefixes = starts, prefixes
+        self._create(d, q.device, lambda desc, nbytes: N.lib().gqa_shared_workspace_bytes(desc, groups, nbytes),
+                     lambda plan, desc: N.lib().gqa_shared_plan_create(plan, desc, groups, starts.data_ptr(),
+                                                                       prefixes.data_ptr()))
+
+
+def prepare_shared_gqa(q, k_pages, v_pages, tables, lengths, starts, prefixes, out=None, *, scale=None):
+    """``prepare_paged_gqa`` where groups of sequences start with the same keys.
+
+    Samples of one prompt, started by ``PagedKVCache.fork``, share its pages; their
+    queries then go over them together, and the pages are read once.  ``starts`` int32
+    [G + 1] and ``prefixes`` int32 [G] on the GPU: the sequences ``starts[g]`` to
+    ``starts[g + 1] - 1`` are a group (none may have fewer than two; sequences outside of
+    [starts[0], starts[G]) are in no group), and their first ``prefixes[g]`` keys are the
+    same.  Members of length 0 are left out; of the others the shortest bounds what is
+    shared, in whole blocks of 16 keys.  The table of one member is read for it, every
+    sequence's own for the rest, so the result is that of ``prepare_paged_gqa`` but for
+    the order of sums.  Pages are 16-bit.  Values of all tensors may change in place
+    between runs.  Prepares and runs once; ``run()`` has no host sync and no
+    allocation."""
+    plan = PreparedSharedGQA(q, k_pages, v_pages, tables, lengths, starts, prefixes, out, scale)
     plan.run()
     return plan

@@ -26,6 +26,10 @@ struct gqa_paged_plan {
   moe::GqaPagedArgs a;
   int device, cus;
 };
+struct gqa_shared_plan {
+  moe::GqaSharedArgs a;
+  int device, cus;
+};
 
 struct gqa_seg_plan {
   moe::GqaArgs a;
@@ -191,6 +195,20 @@ int validate_paged(const gqa_paged_desc *d, const gqa_paged_scales *scales) {
   return rc;
 }
 
+// Without what lies in the workspace.
+moe::GqaPagedArgs paged_args(const gqa_paged_desc *d) {
+  return moe::GqaPagedArgs{(const uint16_t *)d->q, (const uint16_t *)d->k, (const uint16_t *)d->v, (uint16_t *)d->out,
+                           d->tables, d->lengths, d->q_stride, d->table_stride, d->k_strides[0], d->k_strides[1],
+                           d->k_strides[2], d->v_strides[0], d->v_strides[1], d->v_strides[2], d->B, d->Hq, d->Hkv, d->D,
+                           d->P, d->page, d->M, d->dtype, scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr,
+                           GQA_STORAGE_16BIT, nullptr, nullptr, 0, 0, 0, 0, nullptr};
+}
+
+int validate_groups(int G) {
+  if (G < 0 || G > (1 << 16)) return moe::capi_fail(MOE_EINVAL, "G must be in [0, 2^16] (got %d)", G);
+  return MOE_OK;
+}
+
 size_t paged_workspace(const gqa_paged_desc *d, int storage, int cus) {
   return moe::gqa_paged_workspace(d->B, d->Hq, d->Hkv, d->D, storage, (int64_t)d->M * d->page, cus);
 }
@@ -283,11 +301,8 @@ static int create_paged(gqa_paged_plan **out, const gqa_paged_desc *d, const gqa
   if (rc) return rc;
   gqa_paged_plan *p = new (std::nothrow) gqa_paged_plan;
   if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");
-  p->a = moe::GqaPagedArgs{(const uint16_t *)d->q, (const uint16_t *)d->k, (const uint16_t *)d->v, (uint16_t *)d->out,
-                           d->tables, d->lengths, d->q_stride, d->table_stride, d->k_strides[0], d->k_strides[1],
-                           d->k_strides[2], d->v_strides[0], d->v_strides[1], d->v_strides[2], d->B, d->Hq, d->Hkv, d->D,
-                           d->P, d->page, d->M, d->dtype, scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr,
-                           storage, nullptr, nullptr, 0, 0, 0, 0};
+  p->a = paged_args(d);
+  p->a.storage = storage;
   if (scales) {
     p->a.k_scales = (const uint8_t *)scales->k;
     p->a.v_scales = (const uint8_t *)scales->v;
@@ -323,6 +338,54 @@ int gqa_paged_plan_read_status(gqa_paged_plan *p, void *stream, uint32_t *flags)
 }
 
 void gqa_paged_plan_destroy(gqa_paged_plan *p) { delete p; }
+
+int gqa_shared_workspace_bytes(const gqa_paged_desc *d, int32_t G, size_t *bytes) {
+  int rc = validate_paged_sizes(d), dev = 0, cus = 0;
+  if (!rc) rc = validate_groups(G);
+  if (!rc && !bytes) rc = moe::capi_fail(MOE_EINVAL, "null bytes");
+  if (!rc) rc = device_cus(&dev, &cus);
+  if (!rc) *bytes = moe::gqa_shared_workspace(d->B, d->Hq, d->Hkv, d->D, G, cus);
+  return rc;
+}
+
+int gqa_shared_plan_create(gqa_shared_plan **out, const gqa_paged_desc *d, int32_t G, const int32_t *starts,
+                           const int32_t *prefixes) {
+  if (!out) return moe::capi_fail(MOE_EINVAL, "null plan pointer");
+  *out = nullptr;
+  int rc = validate_paged(d, nullptr), dev = 0, cus = 0;
+  if (!rc) rc = validate_groups(G);
+  if (!rc && d->B > 0 && (!starts || ((uintptr_t)starts & 3u) || (G > 0 && (!prefixes || ((uintptr_t)prefixes & 3u)))))
+    rc = moe::capi_fail(MOE_EINVAL, "starts and prefixes must be given");
+  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, 256);
+  if (!rc) rc = device_cus(&dev, &cus);
+  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, moe::gqa_shared_workspace(d->B, d->Hq, d->Hkv, d->D, G, cus));
+  if (rc) return rc;
+  gqa_shared_plan *p = new (std::nothrow) gqa_shared_plan();
+  if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");
+  p->a.p = paged_args(d);
+  p->a.starts = starts;
+  p->a.prefixes = prefixes;
+  p->a.G = G;
+  moe::gqa_shared_bind(&p->a, d->workspace, cus);
+  p->device = dev;
+  p->cus = cus;
+  *out = p;
+  return MOE_OK;
+}
+
+int gqa_shared_plan_run(gqa_shared_plan *p, void *stream) {
+  if (!p) return moe::capi_fail(MOE_EINVAL, "null plan");
+  if (p->a.p.B == 0) return MOE_OK;
+  return on_device(p->device, "shared gqa launch", [&] { return moe::launch_gqa_shared(p->a, p->cus, (hipStream_t)stream); });
+}
+
+int gqa_shared_plan_read_status(gqa_shared_plan *p, void *stream, uint32_t *flags) {
+  if (!p || !flags) return moe::capi_fail(MOE_EINVAL, "null plan or flags");
+  return on_device(p->device, "status",
+                   [&] { return moe::read_and_clear_status(p->a.p.status, flags, (hipStream_t)stream); });
+}
+
+void gqa_shared_plan_destroy(gqa_shared_plan *p) { delete p; }
 
 int gqa_seg_workspace_bytes(const gqa_seg_desc *d, size_t *bytes) {
   int dev = 0, cus = 0;

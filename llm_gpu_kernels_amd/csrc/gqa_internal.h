@@ -82,10 +82,30 @@ struct GqaPagedArgs {
   int storage;
   const uint8_t *k_scales, *v_scales;
   int64_t ks_page, ks_head, vs_page, vs_head;
+  const int32_t *skips;                  // [B] keys of each row that are left out (gqa_shared.hip)
 };
 size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int storage, int64_t keys, int cus);
 void gqa_paged_bind(GqaPagedArgs *a, void *workspace);
 hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s);
+
+// The same where groups of sequences start with the same keys (gqa_shared.hip).
+struct GqaSharedArgs {
+  GqaPagedArgs p;                        // 16-bit pages; skips, pieces and partial in the workspace
+  const int32_t *starts, *prefixes;      // [G + 1], [G]
+  int G, rest_waves;
+  int32_t *total;                        // steps of all groups' prefixes
+  int32_t *skips, *group_of;             // [B]: keys that a row's group attends for it; group, -1: none
+  int32_t *first, *source, *steps, *at;  // [G + 1] each: first member, the one whose table is read,
+                                         // steps of the prefix, steps of all before
+  float *heads;                          // [B][Hq]{m, l, O[D]}: a prefix's first piece
+  float *more;                           // [workgroup][kSharedRows]: pieces that others began
+};
+constexpr int kSharedRows = 256;         // query rows of a workgroup
+size_t gqa_shared_workspace(int B, int Hq, int Hkv, int D, int G, int cus);
+void gqa_shared_bind(GqaSharedArgs *a, void *workspace, int cus);
+hipError_t launch_gqa_shared(const GqaSharedArgs &a, int cus, hipStream_t s);
+int gqa_shared_rest_waves(int D, int cus);
+hipError_t launch_gqa_shared_rest(const GqaPagedArgs &a, int cus, hipStream_t s);  // the keys behind (gqa_paged.hip)
 
 // Synchronises `s`, reads a status word and clears the bits that it had.
 hipError_t read_and_clear_status(uint32_t *status, uint32_t *flags, hipStream_t s);

@@ -49,7 +49,6 @@ constexpr int kWaves = 4;
 constexpr int kTileRows = kWaveRows * kWaves;  // of a workgroup
 constexpr int kStageKeys = 32;
 constexpr int kRing = 5;        // stages in LDS
-typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 // Row i of a stage's K (V) tile holds its 16-byte chunk c at place c ^ swizzle(i):
 // sixteen lanes that read one chunk of sixteen K rows, or 32 lanes that read four
@@ -59,56 +58,6 @@ __device__ __forceinline__ int swizzle_k(int row) { return D == 128 ? row & 15 :
 template <int D>
 __device__ __forceinline__ int swizzle_v(int row) { return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
 
-// 16 bytes per lane from a buffer straight into LDS at `dst` + 16 l (load j 1024 j
-// further).  As inline
-// assembly (it has no output register): the compiler would make every later LDS
-// read wait for all such loads in flight; the kernel waits with exact counts.
-template <int N>
-__device__ __forceinline__ void load_lds(u32x4 rsrc, uint32_t dst, const uint32_t (&off)[N]) {
-  static_assert(N == 1 || N == 2, "loads of a wave");
-  if constexpr (N == 2)
-    asm volatile(
-        "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
-        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
-        :
-        : "s"(dst), "v"(off[0]), "v"(off[1]), "s"(rsrc)
-        : "memory", "scc", "m0");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :
-                 : "s"(dst), "v"(off[0]), "s"(rsrc)
-                 : "memory", "m0");
-}
-__device__ __forceinline__ u32x4 buffer_words(const void *base, uint32_t bytes) {
-  const uint64_t b = sgpr64((uint64_t)base);
-  return u32x4{(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, (uint32_t)sgpr((int)bytes), 0x00020000u};
-}
-__device__ __forceinline__ u32x4 lds_b128(uint32_t at) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  return *(const GQA_AS_LDS u32x4 *)at;
-#else
-  return u32x4{at, 0u, 0u, 0u};
-#endif
-}
-__device__ __forceinline__ void lds_write_b64(uint32_t at, u32x2 v) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  *(GQA_AS_LDS u32x2 *)at = v;
-#endif
-}
-// Within each group of 16 lanes, lane 4a + b receives element b of the 8-byte
-// rows addressed by lanes a, a + 4, a + 8, a + 12.
-__device__ __forceinline__ u32x2 lds_tr16(uint32_t at) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((GQA_AS_LDS i16x4 *)at));
-#else
-  return u32x2{at, 0u};
-#endif
-}
-// The value of this lane and of lane l ^ 32, in the same order on both.
-__device__ __forceinline__ f32x2_t halves(float x) {
-  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return f32x2_t{__uint_as_float(h[0]), __uint_as_float(h[1])};
-}
 template <bool F16>
 __device__ __forceinline__ bool not_finite2(uint32_t w) {
   constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;

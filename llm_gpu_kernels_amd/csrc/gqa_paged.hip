@@ -156,11 +156,6 @@ __device__ __forceinline__ void read_v(uint32_t base, u32x2 (&v)[D / 8]) {
   }
 }
 
-// Read by scalar loads: the tables do not change while the kernel runs.
-__device__ __forceinline__ int uniform_load(const int32_t *p) {
-  return *(const __attribute__((address_space(4))) int32_t *)(const __attribute__((address_space(4))) void *)p;
-}
-
 // What a lane holds of a step of a microscaled cache, for each 16-key block: of key r the
 // dims D/4 g.. of K and their scale; of the keys 4 g + i the dims D/16 r.. of V, and the
 // four keys' scales of the block that those are in, a byte each.
@@ -210,7 +205,10 @@ __host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 20
 // (tables of 8192 keys, 8 heads of 128: 64 sequences of 128 keys 14.5 us by the list,
 // 9.3 so, 16 of 500 13.7, 10.1, 64 of 1000 48.4, 41.6; what the list loses by
 // looking is 0.3 us).
-template <int D, bool F16, int TEAM, int FMT>
+//
+// SHARED: the list alone, of every sequence's keys behind the first skips[b] of them (a
+// multiple of 16), and every piece leaves its state: gqa_shared.hip joins them.
+template <int D, bool F16, int TEAM, int FMT, bool SHARED>
 __global__ __launch_bounds__(64 * (TEAM ? TEAM : kWaves), (TEAM == 8 ? (FMT ? 2 : 1) : kWorkgroups<D, FMT>))
 void gqa_paged_kernel(GqaPagedArgs a) {
   constexpr int kSlices = D / 32;               // 32-dim slices of a row
@@ -241,6 +239,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
       const int ok = max(0, min(lens[i], cap));
       if (lens[i] != ok) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
       lens[i] = ok;
+      if constexpr (SHARED) lens[i] = max(0, ok - (window + kWave * i + lane < a.B ? a.skips[window + kWave * i + lane] : 0));
     }
   };
   int b = -1, len = 0, head, s;           // of the next step, with its sequence's length
@@ -260,7 +259,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
     }
     all = wave_total(sum) * heads;                          // < 2^31, checked on the host
     per = (all + workers - 1) / workers;
-    team = a.B * heads <= (int)gridDim.x && !__builtin_amdgcn_ballot_w64(most > kTeam * most_teamed(per));
+    team = !SHARED && a.B * heads <= (int)gridDim.x && !__builtin_amdgcn_ballot_w64(most > kTeam * most_teamed(per));
   }
   if (!team) {
     if ((int64_t)worker * per >= all) return;
@@ -334,7 +333,10 @@ void gqa_paged_kernel(GqaPagedArgs a) {
     }
   };
   const int per_page = a.page / kBlock;
-  int page_at = 2 * s / per_page, block_at = 2 * s % per_page;  // of the next step's first block
+  // Blocks of the next step's sequence before its first step, and the page and the block
+  // there of its next.
+  int skipped = SHARED ? uniform_load(a.skips + b) / kBlock : 0;
+  int page_at = (skipped + 2 * s) / per_page, block_at = (skipped + 2 * s) % per_page;
 
   // Its steps; by teams or by the list (each with code of its own: tests of `team` in the
   // steps cost the list 1 to 3 %).
@@ -379,7 +381,12 @@ void gqa_paged_kernel(GqaPagedArgs a) {
           } else {
             b = next;
             steps = steps_of(len);
+            if constexpr (SHARED) skipped = uniform_load(a.skips + b) / kBlock;
           }
+        }
+        if constexpr (SHARED) {
+          page_at = skipped / per_page;
+          block_at = skipped % per_page;
         }
       }
       return t;
@@ -612,14 +619,15 @@ void gqa_paged_kernel(GqaPagedArgs a) {
         const int kvh = cur.head / blocks, part = cur.head % blocks, rows = min(kRows, group - kRows * part);
         const int64_t head0 = (int64_t)cur.b * a.Hq + kvh * group + kRows * part;
         const float l = quad_sum(l_run);
-        const bool whole = pair_ends && piece_from == 0;
-        const int slot = 2 * worker + (piece_unit == first ? 0 : 1);
+        const bool all_of_it = pair_ends && piece_from == 0, whole = !SHARED && all_of_it;
+        const int slot = SHARED && all_of_it ? 2 * workers + cur.b * heads + cur.head
+                                             : 2 * worker + (piece_unit == first ? 0 : 1);
         if (piece_from == 0 && lane == 0) {
           // Pieces of the (sequence, head block): this one, then the first pieces
           // of the following waves.
           const int last = (piece_unit + cur.steps - 1) / per;
           a.pieces[2 * (cur.b * heads + cur.head)] = slot;
-          a.pieces[2 * (cur.b * heads + cur.head) + 1] = whole ? 0 : last - worker + 1;
+          a.pieces[2 * (cur.b * heads + cur.head) + 1] = whole ? 0 : SHARED && all_of_it ? 1 : last - worker + 1;
         }
         float L[4], M[4];
 #pragma unroll
@@ -816,9 +824,9 @@ int team_of(int64_t pairs, int64_t steps, int64_t waves) {
   return teamed <= most_teamed(listed) ? team : 0;
 }
 
-template <int D, bool F16, int TEAM, int FMT>
+template <int D, bool F16, int TEAM, int FMT, bool SHARED = false>
 hipError_t launch_kernel(const GqaPagedArgs &a, int grid, hipStream_t s) {
-  auto k = gqa_paged_kernel<D, F16, TEAM, FMT>;
+  auto k = gqa_paged_kernel<D, F16, TEAM, FMT, SHARED>;
   constexpr int waves = TEAM ? TEAM : kWaves, lds = waves * kLds<D, FMT>;
   static std::atomic<uint64_t> allowed{0};
   if (const hipError_t e = allow_lds((const void *)k, lds, &allowed)) return e;
@@ -878,6 +886,15 @@ hipError_t launch(const GqaPagedArgs &a, int cus, hipStream_t s) {
 hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s) {
   if (a.D == 128) return a.dtype == GQA_FP16 ? launch<128, true>(a, cus, s) : launch<128, false>(a, cus, s);
   return a.dtype == GQA_FP16 ? launch<64, true>(a, cus, s) : launch<64, false>(a, cus, s);
+}
+
+int gqa_shared_rest_waves(int D, int cus) { return waves_of(D, GQA_STORAGE_16BIT, cus); }
+
+hipError_t launch_gqa_shared_rest(const GqaPagedArgs &a, int cus, hipStream_t s) {
+  const int grid = waves_of(a.D, GQA_STORAGE_16BIT, cus) / kWaves;
+  if (a.D == 128)
+    return a.dtype == GQA_FP16 ? launch_kernel<128, true, 0, 0, true>(a, grid, s) : launch_kernel<128, false, 0, 0, true>(a, grid, s);
+  return a.dtype == GQA_FP16 ? launch_kernel<64, true, 0, 0, true>(a, grid, s) : launch_kernel<64, false, 0, 0, true>(a, grid, s);
 }
 
 // Clears the bits that it returns, no others, and is done with that on return: a bit

@@ -2,11 +2,13 @@
 GPU: refusals of the C ABI and of the Python layer, and the oracle's own invariants."""
 import ctypes
 import math
+from pathlib import Path
 
 import pytest
 import torch
 
-from llm_gpu_kernels_amd import PagedKVCache, _native as N, prepare_qk_norm_rope
+from llm_gpu_kernels_amd import (PagedKVCache, _native as N, prepare_paged_gqa, prepare_qk_norm_rope,
+                                 prepare_shared_gqa)
 from oracle import serving_oracle as S
 
 BASE = 1 << 20  # an address that is only looked at by the validation
@@ -126,3 +128,98 @@ def test_rotation_keeps_lengths():
         y, _ = S.norm_rope(x, torch.arange(4), f, interleaved=interleaved)
         assert torch.allclose(y.norm(dim=-1), x.double().norm(dim=-1))
         assert torch.equal(y[..., 40:], x[..., 40:].double()) and torch.equal(y[0], x[0].double())
+
+
+# ---- attention over quantised pages, and with shared prefixes ---------------------
+
+
+def _paged(**kw):
+    d = N.GqaPagedDesc()
+    d.B, d.Hq, d.Hkv, d.D, d.P, d.page, d.M, d.dtype = 5, 32, 8, 128, 100, 16, 20, N.GQA_BF16
+    d.q = d.k = d.v = d.out = d.tables = d.lengths = d.workspace = BASE
+    d.q_stride, d.table_stride = 4096, 20
+    for st in (d.k_strides, d.v_strides):
+        st[0], st[1], st[2] = 16 * 8 * 128, 16 * 128, 128
+    d.workspace_bytes = 1 << 30
+    for name, value in kw.items():
+        setattr(d, name, (ctypes.c_int64 * 3)(*value) if name.endswith("strides") else value)
+    return d
+
+
+def _scales(**kw):
+    s = N.GqaPagedScales()
+    s.storage, s.k, s.v = N.GQA_STORAGE_MXFP8, BASE, BASE
+    for st in (s.k_strides, s.v_strides):
+        st[0], st[1] = 8 * 64, 64
+    for name, value in kw.items():
+        setattr(s, name, (ctypes.c_int64 * 2)(*value) if name.endswith("strides") else value)
+    return s
+
+
+@pytest.mark.parametrize("desc,scales", [
+    ({}, dict(storage=0)), ({}, dict(storage=3)), ({}, dict(k=None)), ({}, dict(v=BASE + 8)), ({}, dict(k_strides=(512, 60))),
+    ({}, dict(v_strides=(0, 64))), (dict(k_strides=(16384, 2048, 256)), {}), (dict(v_strides=(16384, 2040, 128)), {}),
+    (dict(k_strides=(8, 2048, 128)), {}), ({}, dict(storage=N.GQA_STORAGE_MXFP4)), (dict(D=96), {}), (dict(page=24), {}),
+    (dict(workspace=None), {}), (dict(workspace_bytes=255), {}), (dict(k=BASE + 4), {}), (dict(q_stride=4090), {}),
+])
+def test_stored_attention_refusals(desc, scales):
+    handle = ctypes.c_void_p()
+    rc = N.lib().gqa_paged_stored_plan_create(ctypes.byref(handle), ctypes.byref(_paged(**desc)), ctypes.byref(_scales(**scales)))
+    assert rc in (N.MOE_EINVAL, N.MOE_ESPACE) and not handle.value and N.last_error()
+
+
+@pytest.mark.parametrize("bad,groups,starts,prefixes", [
+    ({}, -1, BASE, BASE), ({}, (1 << 16) + 1, BASE, BASE), ({}, 3, None, BASE), ({}, 3, BASE, None), ({}, 3, BASE + 2, BASE),
+    ({}, 3, BASE, BASE + 1), (dict(D=80), 3, BASE, BASE), (dict(lengths=None), 3, BASE, BASE), (dict(page=8), 3, BASE, BASE),
+    (dict(workspace_bytes=128), 3, BASE, BASE), (dict(k_strides=(16384, 2048, 100)), 3, BASE, BASE),
+])
+def test_shared_refusals(bad, groups, starts, prefixes):
+    handle = ctypes.c_void_p()
+    rc = N.lib().gqa_shared_plan_create(ctypes.byref(handle), ctypes.byref(_paged(**bad)), groups, starts, prefixes)
+    assert rc in (N.MOE_EINVAL, N.MOE_ESPACE) and not handle.value and N.last_error()
+
+
+def test_attention_null_handles():
+    lib, flags, size, handle = N.lib(), ctypes.c_uint32(), ctypes.c_size_t(), ctypes.c_void_p()
+    for rc in (lib.gqa_shared_plan_run(None, None), lib.gqa_shared_plan_read_status(None, None, ctypes.byref(flags)),
+               lib.gqa_paged_stored_plan_create(ctypes.byref(handle), ctypes.byref(_paged()), None),
+               lib.gqa_shared_plan_create(None, ctypes.byref(_paged()), 0, BASE, BASE),
+               lib.gqa_paged_stored_workspace_bytes(ctypes.byref(_paged()), 5, ctypes.byref(size)),
+               lib.gqa_shared_workspace_bytes(ctypes.byref(_paged()), -2, ctypes.byref(size)),
+               lib.gqa_shared_workspace_bytes(ctypes.byref(_paged()), 1, None)):
+        assert rc == N.MOE_EINVAL and N.last_error()
+    lib.gqa_shared_plan_destroy(None)
+    assert ctypes.sizeof(N.GqaPagedScales) == 8 + 16 + 32  # int32 (+pad) + 2 pointers + 4 int64
+
+
+def test_attention_python_refusals():
+    q, pages = torch.zeros(6, 4, 128, dtype=torch.bfloat16), torch.zeros(9, 2, 16, 128, dtype=torch.bfloat16)
+    tables, lengths = torch.zeros(6, 3, dtype=torch.int32), torch.zeros(6, dtype=torch.int32)
+    starts, prefixes = torch.tensor([0, 2, 6], dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for bad in [(starts.long(), prefixes), (starts, prefixes.long()), (starts, None)]:
+        with pytest.raises(TypeError):
+            prepare_shared_gqa(q, pages, pages, tables, lengths, *bad)
+    eight = torch.zeros(9, 2, 16, 128, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    with pytest.raises(TypeError):  # the shared form has 16-bit pages
+        prepare_shared_gqa(q, eight, eight, tables, lengths, starts, prefixes)
+    for bad in [(starts[:0], prefixes), (starts[None], prefixes), (starts, prefixes[:1]), (starts[:2], prefixes),
+                (None, prefixes), (starts, prefixes)]:  # the last: not on a GPU
+        with pytest.raises(ValueError):
+            prepare_shared_gqa(q, pages, pages, tables, lengths, *bad)
+    with pytest.raises(ValueError, match="scale"):
+        prepare_shared_gqa(q, pages, pages, tables, lengths, starts, prefixes, scale=-1.0)
+    with pytest.raises(ValueError, match="share storage"):
+        prepare_shared_gqa(q, pages, pages, tables, lengths, starts, prefixes, out=q)
+    scales = torch.zeros(9, 2, 4, 16, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    with pytest.raises(TypeError):
+        prepare_paged_gqa(q, pages, pages, tables, lengths, k_scales=scales, v_scales=scales)
+    with pytest.raises(TypeError):
+        prepare_paged_gqa(q, eight, eight, tables, lengths, k_scales=scales)
+    with pytest.raises(ValueError):  # not on a GPU
+        prepare_paged_gqa(q, eight, eight, tables, lengths, k_scales=scales, v_scales=scales)
+
+
+def test_shared_attention_asks_for_its_lds():
+    """Through allow_lds(), as every kernel with more than 64 KiB."""
+    text = (Path(N.__file__).parent / "csrc" / "gqa_shared.hip").read_text()
+    assert "allow_lds((const void *)prefix, kPrefixLds<D>, &allowed)" in text
