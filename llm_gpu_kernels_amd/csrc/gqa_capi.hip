@@ -182,8 +182,8 @@ int validate_paged(const gqa_paged_desc *d, const gqa_paged_scales *scales) {
     for (const int64_t *st : {d->k_strides, d->v_strides})
       if (st[2] != row) return capi_fail(MOE_EINVAL, "the rows of a page and head must lie %lld bytes apart", (long long)row);
     for (const int64_t *st : {d->k_strides, d->v_strides, scales->k_strides, scales->v_strides})
-      if (st[0] < 16 || st[0] % 16 || st[1] < 16 || st[1] % 16)
-        return capi_fail(MOE_EINVAL, "page and head strides must be positive multiples of 16 bytes");
+      if (st[0] < 16 || st[0] % 16 || st[1] < 16 || st[1] % 16 || st[0] >= 1LL << 31)
+        return capi_fail(MOE_EINVAL, "page and head strides must be positive multiples of 16 bytes, page strides below 2^31");
     return MOE_OK;
   }
   for (int kv = 0; !rc && kv < 2; ++kv) {
@@ -210,7 +210,9 @@ int validate_groups(int G) {
 }
 
 size_t paged_workspace(const gqa_paged_desc *d, int storage, int cus) {
-  return moe::gqa_paged_workspace(d->B, d->Hq, d->Hkv, d->D, storage, (int64_t)d->M * d->page, cus);
+  const int64_t keys = (int64_t)d->M * d->page;
+  return storage == GQA_STORAGE_16BIT ? moe::gqa_paged_workspace(d->B, d->Hq, d->Hkv, d->D, keys, cus)
+                                      : moe::gqa_mx_workspace(d->B, d->Hq, d->Hkv, d->D, storage, keys, cus);
 }
 
 int need_workspace(const void *workspace, size_t have, size_t need) {
@@ -328,7 +330,10 @@ int gqa_paged_stored_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d, 
 int gqa_paged_plan_run(gqa_paged_plan *p, void *stream) {
   if (!p) return moe::capi_fail(MOE_EINVAL, "null plan");
   if (p->a.B == 0) return MOE_OK;
-  return on_device(p->device, "paged gqa launch", [&] { return moe::launch_gqa_paged(p->a, p->cus, (hipStream_t)stream); });
+  return on_device(p->device, "paged gqa launch", [&] {
+    return p->a.storage == GQA_STORAGE_16BIT ? moe::launch_gqa_paged(p->a, p->cus, (hipStream_t)stream)
+                                             : moe::launch_gqa_mx(p->a, p->cus, (hipStream_t)stream);
+  });
 }
 
 int gqa_paged_plan_read_status(gqa_paged_plan *p, void *stream, uint32_t *flags) {

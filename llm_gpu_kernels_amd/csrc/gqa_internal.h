@@ -84,9 +84,15 @@ struct GqaPagedArgs {
   int64_t ks_page, ks_head, vs_page, vs_head;
   const int32_t *skips;                  // [B] keys of each row that are left out (gqa_shared.hip)
 };
-size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int storage, int64_t keys, int cus);
+size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int64_t keys, int cus);
 void gqa_paged_bind(GqaPagedArgs *a, void *workspace);
 hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s);
+// Joins the pieces of each (sequence, block of query heads): the first in slot
+// pieces[2 i], the j-th in slot 2 (pieces[2 i] / 2 + j).
+hipError_t launch_gqa_paged_merge(const GqaPagedArgs &a, int cus, hipStream_t s);
+// Over microscaled pages (gqa_mx.hip); the workspace is bound as above.
+size_t gqa_mx_workspace(int B, int Hq, int Hkv, int D, int storage, int64_t keys, int cus);
+hipError_t launch_gqa_mx(const GqaPagedArgs &a, int cus, hipStream_t s);
 
 // The same where groups of sequences start with the same keys (gqa_shared.hip).
 struct GqaSharedArgs {

@@ -24,13 +24,6 @@
 // Scores are computed transposed, S^T = K Q^T, so they land in the A layout of
 // the P.V product; V comes back transposed with ds_read_b64_tr_b16.
 //
-// A microscaled cache (FMT > 0) needs no LDS for K and V: which 8 of a slice's dims are
-// multiplied together is free as long as K and Q agree, so a lane has a quarter of a
-// key's row, D/4 dims under one scale, and which dims are a tile of O is free too, so
-// it has D/16 neighbouring dims of its eight values' rows.  Both go from HBM to
-// registers, are converted there, exactly, by single instructions that apply the
-// scale, and the bytes of two values are put side by side.
-//
 // Measured, a copy of 2 GiB running at 5.0 TB/s: one sequence of 131072 tokens, 8 KV heads
 // of 128 (537 MB), 96 us, 5.6 TB/s, and 6.4 us for the join; 64 sequences of 1 to 7787 (288
 // MB), 68 us with the join; by teams, 200 sequences of 16 to 1997, 2 KV heads of 64 (39
@@ -42,7 +35,6 @@
 #include "gqa_dev.h"
 #include "gqa_internal.h"
 #include "launch.h"
-#include "mx_dev.h"
 
 namespace moe {
 
@@ -62,12 +54,7 @@ constexpr int kWindow = 4;      // sequences per lane whose lengths a wave holds
 // sixteen (eight) different bank groups.
 template <int D> constexpr int kStage = kStep * D * 2;
 template <int D> constexpr int kWaveLds = 5 * kStage<D> / 2;
-template <int D> constexpr int kStateLds = (kRows * D + 2 * kRows) * 4;  // a wave's state, for a team's join
-template <int D, int FMT> constexpr int kLds = FMT ? kStateLds<D> : kWaveLds<D>;
-// Per CU.  Without stages in LDS registers bound it: 168 for three waves a SIMD, 128 for
-// four.
-template <int D, int FMT>
-constexpr int kWorkgroups = FMT ? (D == 128 ? 3 : 4) : 160 * 1024 / (kWaves * kWaveLds<D>);
+template <int D> constexpr int kWorkgroups = 160 * 1024 / (kWaves * kWaveLds<D>);  // per CU
 template <int D>
 __device__ __forceinline__ int swizzle_k(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
 template <int D>
@@ -156,36 +143,6 @@ __device__ __forceinline__ void read_v(uint32_t base, u32x2 (&v)[D / 8]) {
   }
 }
 
-// What a lane holds of a step of a microscaled cache, for each 16-key block: of key r the
-// dims D/4 g.. of K and their scale; of the keys 4 g + i the dims D/16 r.. of V, and the
-// four keys' scales of the block that those are in, a byte each.
-template <int D, int FMT>
-struct MxStep {
-  static constexpr int kKeyWords = mx::row_bytes<FMT>(D) / 16, kValueBytes = mx::row_bytes<FMT>(D) / 16;
-  static constexpr int kValueWords = kValueBytes > 4 ? 2 : 1;
-  uint32_t k[2][kKeyWords], k_scale[2];
-  uint32_t v[2][4][kValueWords], v_scales[2];
-};
-template <int D>
-struct MxStep<D, 0> {};
-template <int N>
-__device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t (&w)[N]) {
-  if constexpr (N == 8) {
-    const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0), b = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 16, 0, 0);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = i < 4 ? a[i] : b[i - 4];
-  } else if constexpr (N == 4) {
-    const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = a[i];
-  } else {
-    static_assert(N == 2, "words of a lane");
-    const u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 0);
-    w[0] = a[0];
-    w[1] = a[1];
-  }
-}
-
 // A step: up to 32 keys of one (sequence, head block).  All fields are the same
 // in every lane.
 struct Step {
@@ -208,8 +165,8 @@ __host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 20
 //
 // SHARED: the list alone, of every sequence's keys behind the first skips[b] of them (a
 // multiple of 16), and every piece leaves its state: gqa_shared.hip joins them.
-template <int D, bool F16, int TEAM, int FMT, bool SHARED>
-__global__ __launch_bounds__(64 * (TEAM ? TEAM : kWaves), (TEAM == 8 ? (FMT ? 2 : 1) : kWorkgroups<D, FMT>))
+template <int D, bool F16, int TEAM, bool SHARED>
+__global__ __launch_bounds__(64 * (TEAM ? TEAM : kWaves), TEAM == 8 ? 1 : kWorkgroups<D>)
 void gqa_paged_kernel(GqaPagedArgs a) {
   constexpr int kSlices = D / 32;               // 32-dim slices of a row
   constexpr int kTiles = D / 16;                // 16-dim tiles of O
@@ -221,7 +178,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
   constexpr int kTeam = TEAM ? TEAM : kWaves;
   const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows, heads = a.Hkv * blocks;
   const int cap = a.M * a.page;
-  uint8_t *const kst = smem + wave * kLds<D, FMT>, *const vst = kst + kStage<D>, *const qst = vst + kStage<D>;
+  uint8_t *const kst = smem + wave * kWaveLds<D>, *const vst = kst + kStage<D>, *const qst = vst + kStage<D>;
 
   // ---- the wave's range of the flat list, or its first step ----
   // (Unsigned: lengths go up to 2^31 - 16.)
@@ -419,63 +376,21 @@ void gqa_paged_kernel(GqaPagedArgs a) {
         for (int j = 0; j < kLoads; ++j) load_lds16(rs, stage + (i * kLoads + j) * 1024, off[j]);
       }
     };
-    // Microscaled: strides are in bytes, a (page, head)'s rows and scales side by side.
-    using Mx = MxStep<D, FMT>;
-    constexpr uint32_t kRowBytes = (uint32_t)mx::row_bytes<FMT>(D);
-    Mx mxs;
-    u32x4 qf[kSlices];
     auto issue_k = [&](const Step &t) __attribute__((always_inline)) {
-      if constexpr (FMT == 0) {
-        issue(t, a.k, a.k_page, a.k_head, a.k_row, k_off, kst);
-        asm volatile("" ::: "memory");  // the counted waits rely on the order
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int n = usable(t, i), kvh = t.head / blocks;
-          const uint8_t *const base = (const uint8_t *)a.k + (n ? t.page[i] * a.k_page + kvh * a.k_head + t.row[i] * (int)kRowBytes : 0);
-          load_words(buffer(base, (uint32_t)n * kRowBytes), (uint32_t)r * kRowBytes + (uint32_t)g * (kRowBytes / 4), mxs.k[i]);
-          const uint8_t *const scales = a.k_scales + (n ? t.page[i] * a.ks_page + kvh * a.ks_head + t.row[i] : 0);
-          mxs.k_scale[i] = __builtin_amdgcn_raw_buffer_load_b8(buffer(scales, n ? (uint32_t)(D / mx::kBlock * a.page - t.row[i]) : 0u),
-                                                               (uint32_t)(g * (D / 4) / mx::kBlock * a.page + r), 0, 0);
-        }
-      }
+      issue(t, a.k, a.k_page, a.k_head, a.k_row, k_off, kst);
+      asm volatile("" ::: "memory");  // the counted waits rely on the order
     };
     auto issue_v = [&](const Step &t) __attribute__((always_inline)) {
-      if constexpr (FMT == 0) {
-        issue(t, a.v, a.v_page, a.v_head, a.v_row, v_off, vst);
-        asm volatile("" ::: "memory");
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int n = usable(t, i), kvh = t.head / blocks;
-          const uint8_t *const base = (const uint8_t *)a.v + (n ? t.page[i] * a.v_page + kvh * a.v_head + t.row[i] * (int)kRowBytes : 0);
-          const auto rs = buffer(base, (uint32_t)n * kRowBytes);
-          const uint32_t off = (uint32_t)(4 * g) * kRowBytes + (uint32_t)r * Mx::kValueBytes;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (Mx::kValueBytes == 8) load_words(rs, off + j * kRowBytes, mxs.v[i][j]);
-            else if constexpr (Mx::kValueBytes == 4) mxs.v[i][j][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off + j * kRowBytes, 0, 0);
-            else mxs.v[i][j][0] = __builtin_amdgcn_raw_buffer_load_b16(rs, off + j * kRowBytes, 0, 0);
-          }
-          const uint8_t *const scales = a.v_scales + (n ? t.page[i] * a.vs_page + kvh * a.vs_head + t.row[i] : 0);
-          mxs.v_scales[i] = __builtin_amdgcn_raw_buffer_load_b32(buffer(scales, n ? (uint32_t)(D / mx::kBlock * a.page - t.row[i]) : 0u),
-                                                                 (uint32_t)(r * (D / 16) / mx::kBlock * a.page + 4 * g), 0, 0);
-        }
-      }
+      issue(t, a.v, a.v_page, a.v_head, a.v_row, v_off, vst);
+      asm volatile("" ::: "memory");
     };
     auto issue_q = [&](const Step &t) __attribute__((always_inline)) {
       const int kvh = t.head / blocks, part = t.head % blocks, rows = min(kRows, group - kRows * part);
       const uint16_t *const base = a.q + t.b * a.q_stride + (int64_t)(kvh * group + kRows * part) * D;
       const auto rs = buffer(base, (uint32_t)rows * 2 * D);
-      if constexpr (FMT == 0) {
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) load_lds16(rs, qst + j * 1024, q_off[j]);
-        asm volatile("" ::: "memory");
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < kSlices; ++ks)
-          qf[ks] = __builtin_amdgcn_raw_buffer_load_b128(rs, (uint32_t)(r * 2 * D + g * (D / 2) + 16 * ks), 0, 0);
-      }
+      for (int j = 0; j < kLoads; ++j) load_lds16(rs, qst + j * 1024, q_off[j]);
+      asm volatile("" ::: "memory");
     };
 
     // ---- operand addresses ----
@@ -487,8 +402,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
     const uint32_t v_base = lds_addr(vst) + (uint32_t)(v_row * 2 * D + 16 * (((r & 3) >> 1) ^ swizzle_v<D>(v_row)) + 8 * (r & 1));
 
     // Softmax state of query row r (this lane's keys only in l), base-2 domain; O:
-    // rows 4 g + i, dims dim_of(dt).
-    auto dim_of = [&](int dt) __attribute__((always_inline)) { return FMT == 0 ? 16 * dt + r : kTiles * r + dt; };
+    // rows 4 g + i, dims 16 dt + r.
     float m_run = -INFINITY, l_run = 0.f;
     float m_top = -INFINITY;  // fp16: limit(m_run), kept
     f32x4 o[kTiles];
@@ -504,22 +418,10 @@ void gqa_paged_kernel(GqaPagedArgs a) {
     issue_k(cur);
     issue_v(cur);
     while (cur.n[0] > 0) {
-      u32x4 kf[2 * kSlices];
-      if constexpr (FMT == 0) {
-        // K (and Q) have landed once at most V's loads remain.
-        wait_vmcnt<2 * kLoads>();
-        read_kq<D>(k_base, k_at, kf, qf);
-      } else {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          const float scale = mx::scale_of(mxs.k_scale[kt]);
-#pragma unroll
-          for (int ks = 0; ks < kSlices; ++ks) {
-            if constexpr (FMT == mx::kFp8) kf[2 * ks + kt] = mx::decode8<FMT, F16>(mxs.k[kt][2 * ks], mxs.k[kt][2 * ks + 1], scale);
-            else kf[2 * ks + kt] = mx::decode8<FMT, F16>(mxs.k[kt][ks], 0u, scale);
-          }
-        }
-      }
+      // K (and Q) have landed once at most V's loads remain.
+      wait_vmcnt<2 * kLoads>();
+      u32x4 kf[2 * kSlices], qf[kSlices];
+      read_kq<D>(k_base, k_at, kf, qf);
       f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int ks = 0; ks < kSlices; ++ks)
@@ -535,14 +437,6 @@ void gqa_paged_kernel(GqaPagedArgs a) {
         for (int i = 0; i < 4; ++i) {
           sc[0][i] = 4 * g + i < n0 ? sc[0][i] : -INFINITY;
           sc[1][i] = 4 * g + i < n1 ? sc[1][i] : -INFINITY;
-        }
-        if constexpr (FMT > 0) {
-          // Keys that are not there are 0; so are their scales, whatever the page holds.
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int left_keys = min(max((i ? n1 : n0) - 4 * g, 0), 4);
-            mxs.v_scales[i] &= left_keys == 4 ? ~0u : (1u << 8 * left_keys) - 1u;
-          }
         }
       }
       const float lmax = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
@@ -572,46 +466,14 @@ void gqa_paged_kernel(GqaPagedArgs a) {
       // sums of both.
       const u32x4 pa = {pack2<F16>(p[0][0], p[0][1]), pack2<F16>(p[0][2], p[0][3]), pack2<F16>(p[1][0], p[1][1]),
                         pack2<F16>(p[1][2], p[1][3])};
-      if constexpr (FMT == 0) {
-        // V has landed once at most the next K's loads remain.
-        wait_vmcnt<2 * kLoads>();
-        u32x2 vr[2 * kTiles];
-        read_v<D>(v_base, vr);
-        issue_v(nx);
+      // V has landed once at most the next K's loads remain.
+      wait_vmcnt<2 * kLoads>();
+      u32x2 vr[2 * kTiles];
+      read_v<D>(v_base, vr);
+      issue_v(nx);
 #pragma unroll
-        for (int dt = 0; dt < kTiles; ++dt)
-          o[dt] = mfma16x16<F16>(pa, u32x4{vr[2 * dt][0], vr[2 * dt][1], vr[2 * dt + 1][0], vr[2 * dt + 1][1]}, o[dt]);
-      } else {
-        // Two tiles at a time: neighbouring dims 2 p and 2 p + 1 of the lane's eight keys, two
-        // keys of a dim side by side.
-        auto tiles = [&](auto pair) __attribute__((always_inline)) {
-          constexpr int P = decltype(pair)::value;
-          u32x4 even, odd;
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              uint32_t x[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float scale = mx::scale_of(mxs.v_scales[i] >> 8 * (2 * j + e) & 0xffu);
-                if constexpr (FMT == mx::kFp8) x[e] = mx::decode2<FMT, F16, P & 1>(mxs.v[i][2 * j + e][P / 2], scale);
-                else x[e] = mx::decode2<FMT, F16, P>(mxs.v[i][2 * j + e][0], scale);
-              }
-              even[2 * i + j] = __builtin_amdgcn_perm(x[1], x[0], 0x05040100u);
-              odd[2 * i + j] = __builtin_amdgcn_perm(x[1], x[0], 0x07060302u);
-            }
-          o[2 * P] = mfma16x16<F16>(pa, even, o[2 * P]);
-          o[2 * P + 1] = mfma16x16<F16>(pa, odd, o[2 * P + 1]);
-        };
-        tiles(std::integral_constant<int, 0>());
-        tiles(std::integral_constant<int, 1>());
-        if constexpr (D == 128) {
-          tiles(std::integral_constant<int, 2>());
-          tiles(std::integral_constant<int, 3>());
-        }
-        issue_v(nx);
-      }
+      for (int dt = 0; dt < kTiles; ++dt)
+        o[dt] = mfma16x16<F16>(pa, u32x4{vr[2 * dt][0], vr[2 * dt][1], vr[2 * dt + 1][0], vr[2 * dt + 1][1]}, o[dt]);
 
       // ---- the end of a piece ----
       const bool pair_ends = cur.s + 1 == cur.steps;
@@ -641,15 +503,9 @@ void gqa_paged_kernel(GqaPagedArgs a) {
           if (row >= rows) continue;
           if (whole) {
             const float inv = L[i] == 0.f ? 0.f : 1.0f / L[i];
-            if constexpr (FMT == 0) {
-              uint16_t *const op = a.out + (head0 + row) * D + r;
+            uint16_t *const op = a.out + (head0 + row) * D + r;
 #pragma unroll
-              for (int dt = 0; dt < kTiles; ++dt) op[16 * dt] = (uint16_t)pack2<F16>(o[dt][i] * inv, 0.f);
-            } else {
-              uint32_t *const op = (uint32_t *)(a.out + (head0 + row) * D + kTiles * r);
-#pragma unroll
-              for (int dt = 0; dt < kTiles; dt += 2) op[dt / 2] = pack2<F16>(o[dt][i] * inv, o[dt + 1][i] * inv);
-            }
+            for (int dt = 0; dt < kTiles; ++dt) op[16 * dt] = (uint16_t)pack2<F16>(o[dt][i] * inv, 0.f);
           } else {
             float *const pp = a.partial + ((int64_t)slot * min(group, kRows) + row) * (D + 2);
             if (r == 0) {
@@ -657,7 +513,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
               pp[1] = L[i];
             }
 #pragma unroll
-            for (int dt = 0; dt < kTiles; ++dt) pp[2 + dim_of(dt)] = o[dt][i];
+            for (int dt = 0; dt < kTiles; ++dt) pp[2 + 16 * dt + r] = o[dt][i];
           }
         }
         m_run = m_top = -INFINITY;
@@ -671,7 +527,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
       cur = nx;
       nx = next_step();
     }
-    if constexpr (FMT == 0) wait_vmcnt<0>();  // the last (empty) step's loads write LDS
+    wait_vmcnt<0>();  // the last (empty) step's loads write LDS
     if (bad_page && lane == 0) atomicOr(a.status, GQA_STATUS_BAD_PAGE);
 
     if constexpr (kTeams) {
@@ -688,7 +544,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
       for (int i = 0; i < 4; ++i)
         if (4 * g + i < rows) {
 #pragma unroll
-          for (int dt = 0; dt < kTiles; ++dt) mine[(4 * g + i) * D + dim_of(dt)] = pin(o[dt][i]);
+          for (int dt = 0; dt < kTiles; ++dt) mine[(4 * g + i) * D + 16 * dt + r] = pin(o[dt][i]);
         }
       __syncthreads();
       uint32_t *const out = (uint32_t *)(a.out + ((int64_t)b * a.Hq + kvh * group + kRows * part) * D);
@@ -697,13 +553,13 @@ void gqa_paged_kernel(GqaPagedArgs a) {
         float m[kTeam], top = -INFINITY, den = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll
         for (int w = 0; w < kTeam; ++w) {
-          m[w] = ((const float *)(smem + w * kLds<D, FMT>))[kRows * D + row];
+          m[w] = ((const float *)(smem + w * kWaveLds<D>))[kRows * D + row];
           top = fmaxf(top, m[w]);
         }
         const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int w = 0; w < kTeam; ++w) {
-          const float *const x = (const float *)(smem + w * kLds<D, FMT>);
+          const float *const x = (const float *)(smem + w * kWaveLds<D>);
           const float f = __builtin_amdgcn_exp2f(m[w] - ref);
           const f32x2_t v = *(const f32x2_t *)(x + e);
           den = __builtin_fmaf(f, x[kRows * D + kRows + row], den);
@@ -803,10 +659,7 @@ __global__ __launch_bounds__(kMergeThreads) void gqa_paged_merge(GqaPagedArgs a,
 
 __global__ void clear_bits(uint32_t *w, uint32_t bits) { atomicAnd(w, ~bits); }
 
-int waves_of(int D, int storage, int cus) {
-  if (storage) return cus * kWaves * (D == 128 ? kWorkgroups<128, 1> : kWorkgroups<64, 1>);
-  return cus * kWaves * (D == 128 ? kWorkgroups<128, 0> : kWorkgroups<64, 0>);
-}
+int waves_of(int D, int cus) { return cus * kWaves * (D == 128 ? kWorkgroups<128> : kWorkgroups<64>); }
 
 // Waves of a workgroup per (sequence, head block), or 0 for the list and its merge,
 // by the steps of a full table.  A team needs no second launch (4 to 7 us), but has all
@@ -824,45 +677,50 @@ int team_of(int64_t pairs, int64_t steps, int64_t waves) {
   return teamed <= most_teamed(listed) ? team : 0;
 }
 
-template <int D, bool F16, int TEAM, int FMT, bool SHARED = false>
+template <int D, bool F16, int TEAM, bool SHARED = false>
 hipError_t launch_kernel(const GqaPagedArgs &a, int grid, hipStream_t s) {
-  auto k = gqa_paged_kernel<D, F16, TEAM, FMT, SHARED>;
-  constexpr int waves = TEAM ? TEAM : kWaves, lds = waves * kLds<D, FMT>;
+  auto k = gqa_paged_kernel<D, F16, TEAM, SHARED>;
+  constexpr int waves = TEAM ? TEAM : kWaves, lds = waves * kWaveLds<D>;
   static std::atomic<uint64_t> allowed{0};
   if (const hipError_t e = allow_lds((const void *)k, lds, &allowed)) return e;
   hipLaunchKernelGGL(k, dim3(grid), dim3(64 * waves), lds, s, a);
   return hipGetLastError();
 }
 
-template <int D, bool F16, int FMT>
+template <int D, bool F16>
 hipError_t launch(const GqaPagedArgs &a, int cus, hipStream_t s) {
   const int group = a.Hq / a.Hkv, heads = a.Hkv * ((group + kRows - 1) / kRows), pairs = a.B * heads;
-  const int team = team_of(pairs, ((int64_t)a.M * a.page + kStep - 1) / kStep, waves_of(D, FMT, cus));
-  if (team == 8) return launch_kernel<D, F16, 8, FMT>(a, pairs, s);
-  if (team == 4) return launch_kernel<D, F16, 4, FMT>(a, pairs, s);
-  const hipError_t e = launch_kernel<D, F16, 0, FMT>(a, cus * kWorkgroups<D, FMT>, s);
-  if (e != hipSuccess) return e;
-  // Threads per piece in a merge workgroup: all of a (sequence, head block), two
-  // elements each; fewer, and pieces shared out over groups, while that leaves CUs
-  // without a workgroup.
-  const int need = min(group, kRows) * D / 2;
-  int chunk = kMergeThreads;
-  while (chunk > 16 && (chunk >= 2 * need || (int64_t)pairs * ((need + chunk - 1) / chunk) < cus)) chunk /= 2;
-  hipLaunchKernelGGL(gqa_paged_merge<F16>, dim3(pairs, (need + chunk - 1) / chunk), dim3(kMergeThreads), 0, s, a, chunk);
-  return hipGetLastError();
+  const int team = team_of(pairs, ((int64_t)a.M * a.page + kStep - 1) / kStep, waves_of(D, cus));
+  if (team == 8) return launch_kernel<D, F16, 8>(a, pairs, s);
+  if (team == 4) return launch_kernel<D, F16, 4>(a, pairs, s);
+  if (const hipError_t e = launch_kernel<D, F16, 0>(a, cus * kWorkgroups<D>, s)) return e;
+  return launch_gqa_paged_merge(a, cus, s);
 }
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 }  // namespace
 
+hipError_t launch_gqa_paged_merge(const GqaPagedArgs &a, int cus, hipStream_t s) {
+  const int group = a.Hq / a.Hkv, D = a.D, pairs = a.B * a.Hkv * ((group + kRows - 1) / kRows);
+  // Threads per piece in a merge workgroup: all of a (sequence, head block), two
+  // elements each; fewer, and pieces shared out over groups, while that leaves CUs
+  // without a workgroup.
+  const int need = min(group, kRows) * D / 2;
+  int chunk = kMergeThreads;
+  while (chunk > 16 && (chunk >= 2 * need || (int64_t)pairs * ((need + chunk - 1) / chunk) < cus)) chunk /= 2;
+  hipLaunchKernelGGL(a.dtype == GQA_FP16 ? gqa_paged_merge<true> : gqa_paged_merge<false>,
+                     dim3(pairs, (need + chunk - 1) / chunk), dim3(kMergeThreads), 0, s, a, chunk);
+  return hipGetLastError();
+}
+
 // {status words; two words per (sequence, head block); the pieces' states}; teams
 // have no pieces.
-size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int storage, int64_t keys, int cus) {
+size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int64_t keys, int cus) {
   const int group = Hq / Hkv, rows = group < kRows ? group : kRows;
   const size_t pairs = (size_t)B * Hkv * ((group + kRows - 1) / kRows);
-  if (team_of(pairs, (keys + kStep - 1) / kStep, waves_of(D, storage, cus))) return 256;
-  return 256 + align256(8 * pairs) + (size_t)2 * waves_of(D, storage, cus) * rows * (D + 2) * sizeof(float);
+  if (team_of(pairs, (keys + kStep - 1) / kStep, waves_of(D, cus))) return 256;
+  return 256 + align256(8 * pairs) + (size_t)2 * waves_of(D, cus) * rows * (D + 2) * sizeof(float);
 }
 
 void gqa_paged_bind(GqaPagedArgs *a, void *workspace) {
@@ -874,27 +732,17 @@ void gqa_paged_bind(GqaPagedArgs *a, void *workspace) {
   a->partial = (float *)(w + 256 + align256(8 * pairs));
 }
 
-namespace {
-template <int D, bool F16>
-hipError_t launch(const GqaPagedArgs &a, int cus, hipStream_t s) {
-  if (a.storage == GQA_STORAGE_MXFP8) return launch<D, F16, mx::kFp8>(a, cus, s);
-  if (a.storage == GQA_STORAGE_MXFP4) return launch<D, F16, mx::kFp4>(a, cus, s);
-  return launch<D, F16, 0>(a, cus, s);
-}
-}  // namespace
-
 hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s) {
   if (a.D == 128) return a.dtype == GQA_FP16 ? launch<128, true>(a, cus, s) : launch<128, false>(a, cus, s);
   return a.dtype == GQA_FP16 ? launch<64, true>(a, cus, s) : launch<64, false>(a, cus, s);
 }
 
-int gqa_shared_rest_waves(int D, int cus) { return waves_of(D, GQA_STORAGE_16BIT, cus); }
+int gqa_shared_rest_waves(int D, int cus) { return waves_of(D, cus); }
 
 hipError_t launch_gqa_shared_rest(const GqaPagedArgs &a, int cus, hipStream_t s) {
-  const int grid = waves_of(a.D, GQA_STORAGE_16BIT, cus) / kWaves;
-  if (a.D == 128)
-    return a.dtype == GQA_FP16 ? launch_kernel<128, true, 0, 0, true>(a, grid, s) : launch_kernel<128, false, 0, 0, true>(a, grid, s);
-  return a.dtype == GQA_FP16 ? launch_kernel<64, true, 0, 0, true>(a, grid, s) : launch_kernel<64, false, 0, 0, true>(a, grid, s);
+  const int grid = waves_of(a.D, cus) / kWaves;
+  if (a.D == 128) return a.dtype == GQA_FP16 ? launch_kernel<128, true, 0, true>(a, grid, s) : launch_kernel<128, false, 0, true>(a, grid, s);
+  return a.dtype == GQA_FP16 ? launch_kernel<64, true, 0, true>(a, grid, s) : launch_kernel<64, false, 0, true>(a, grid, s);
 }
 
 // Clears the bits that it returns, no others, and is done with that on return: a bit
