@@ -169,7 +169,7 @@ void gqa_paged_plan_destroy(gqa_paged_plan *p);
  * Every other table entry is the sequence's own, as without groups.  Bounds that do not
  * ascend within [0, B] are reported (GQA_STATUS_BAD_BOUNDS) and nothing is shared then; so
  * are negative prefixes, taken as 0.  starts and prefixes lie on the GPU and are read by
- * every run.  G <= 2^16; desc as for the paged form, with a workspace of
+ * every run.  G <= 1024; desc as for the paged form, with a workspace of
  * gqa_shared_workspace_bytes().
  */
 typedef struct gqa_shared_plan gqa_shared_plan;

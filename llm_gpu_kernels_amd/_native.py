@@ -43,7 +43,7 @@ class MoeLayout(ctypes.Structure):
 
 STATIC_WORKSPACE_BYTES = 16 << 20  # MOE_STATIC_WORKSPACE_BYTES
 
-GQA_MAX_SEGMENTS = 4
+GQA_MAX_SEGMENTS, GQA_MAX_GROUPS = 4, 1024
 
 
 class GqaDesc(ctypes.Structure):

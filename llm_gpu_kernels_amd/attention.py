@@ -439,8 +439,8 @@ class PreparedSharedGQA(PreparedPagedGQA):
         _check_int32(starts, "starts", (groups + 1,), q.device)
         _check_int32(prefixes, "prefixes", (groups,), q.device)
         check_out_storage(self.output, [starts, prefixes])
-        if groups >= 2 ** 31:
-            raise ValueError(f"starts must have below 2^31 entries (got {groups + 1})")
+        if groups > N.GQA_MAX_GROUPS:
+            raise ValueError(f"starts must have at most {N.GQA_MAX_GROUPS + 1} entries (got {groups + 1})")
         self.starts, self.prefixes = starts, prefixes
         self._create(d, q.device, lambda desc, nbytes: N.lib().gqa_shared_workspace_bytes(desc, groups, nbytes),
                      lambda plan, desc: N.lib().gqa_shared_plan_create(plan, desc, groups, starts.data_ptr(),
@@ -452,7 +452,7 @@ def prepare_shared_gqa(q, k_pages, v_pages, tables, lengths, starts, prefixes, o
 
     Samples of one prompt, started by ``PagedKVCache.fork``, share its pages; their
     queries then go over them together, and the pages are read once.  ``starts`` int32
-    [G + 1] and ``prefixes`` int32 [G] on the GPU: the sequences ``starts[g]`` to
+    [G + 1] and ``prefixes`` int32 [G] on the GPU, G up to 1024: the sequences ``starts[g]`` to
     ``starts[g + 1] - 1`` are a group (none may have fewer than two; sequences outside of
     [starts[0], starts[G]) are in no group), and their first ``prefixes[g]`` keys are the
     same.  Members of length 0 are left out; of the others the shortest bounds what is

@@ -201,11 +201,11 @@ moe::GqaPagedArgs paged_args(const gqa_paged_desc *d) {
                            d->tables, d->lengths, d->q_stride, d->table_stride, d->k_strides[0], d->k_strides[1],
                            d->k_strides[2], d->v_strides[0], d->v_strides[1], d->v_strides[2], d->B, d->Hq, d->Hkv, d->D,
                            d->P, d->page, d->M, d->dtype, scale_or_default(d->scale, d->D), nullptr, nullptr, nullptr,
-                           GQA_STORAGE_16BIT, nullptr, nullptr, 0, 0, 0, 0, nullptr};
+                           GQA_STORAGE_16BIT, nullptr, nullptr, 0, 0, 0, 0, {}};
 }
 
 int validate_groups(int G) {
-  if (G < 0 || G > (1 << 16)) return moe::capi_fail(MOE_EINVAL, "G must be in [0, 2^16] (got %d)", G);
+  if (G < 0 || G > moe::kMaxGroups) return moe::capi_fail(MOE_EINVAL, "G must be in [0, %d] (got %d)", moe::kMaxGroups, G);
   return MOE_OK;
 }
 
@@ -370,8 +370,7 @@ int gqa_shared_plan_create(gqa_shared_plan **out, const gqa_paged_desc *d, int32
   p->a.p = paged_args(d);
   p->a.starts = starts;
   p->a.prefixes = prefixes;
-  p->a.G = G;
-  moe::gqa_shared_bind(&p->a, d->workspace, cus);
+  moe::gqa_shared_bind(&p->a, G, d->workspace, cus);
   p->device = dev;
   p->cus = cus;
   *out = p;

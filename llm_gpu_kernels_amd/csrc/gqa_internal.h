@@ -64,6 +64,24 @@ void gqa_packed_bind(GqaPackedArgs *a, void *workspace);
 void gqa_packed_constants(GqaPackedArgs *a);
 hipError_t launch_gqa_packed(const GqaPackedArgs &a, int cus, hipStream_t s);
 
+constexpr int kSharedRows = 128;         // query rows of a workgroup over a prefix
+constexpr int kMaxGroups = 1024;
+// What gqa_shared.hip plans for a run, and the states of its prefixes.
+struct GqaSharedState {
+  int G;
+  int32_t *header;                       // {units, workgroups for them}
+  // [G][16]: {units before, steps of a chunk, first member, query rows of a KV head, member
+  // whose table is read, keys, tiles, rows of a tile, chunks, units before but each (KV
+  // head, tile)'s first}.  A unit: a KV head's tile of rows over a chunk of the steps, in the
+  // order (KV head, chunk, tile).
+  int32_t *groups;
+  // [B][8]: {keys that its group attends for it, chunks, tiles, rows of a tile, its first row
+  // in the group, units before but each (KV head, tile)'s first}.
+  int32_t *rows;
+  float *heads;                          // [B][Hq]{m, l, O[D]}: of a prefix's first chunk
+  float *more;                           // [unit but each first][kSharedRows]: of the others
+};
+
 // One new token per sequence over a paged cache (gqa_paged.hip).
 struct GqaPagedArgs {
   const uint16_t *q, *k, *v;             // q [B, Hq, D]; k, v: pages
@@ -82,7 +100,7 @@ struct GqaPagedArgs {
   int storage;
   const uint8_t *k_scales, *v_scales;
   int64_t ks_page, ks_head, vs_page, vs_head;
-  const int32_t *skips;                  // [B] keys of each row that are left out (gqa_shared.hip)
+  GqaSharedState shared;
 };
 size_t gqa_paged_workspace(int B, int Hq, int Hkv, int D, int64_t keys, int cus);
 void gqa_paged_bind(GqaPagedArgs *a, void *workspace);
@@ -94,24 +112,18 @@ hipError_t launch_gqa_paged_merge(const GqaPagedArgs &a, int cus, hipStream_t s)
 size_t gqa_mx_workspace(int B, int Hq, int Hkv, int D, int storage, int64_t keys, int cus);
 hipError_t launch_gqa_mx(const GqaPagedArgs &a, int cus, hipStream_t s);
 
-// The same where groups of sequences start with the same keys (gqa_shared.hip).
+// The same where groups of sequences start with the same keys (gqa_shared.hip): 16-bit
+// pages, and the lists and states in the workspace.
 struct GqaSharedArgs {
-  GqaPagedArgs p;                        // 16-bit pages; skips, pieces and partial in the workspace
+  GqaPagedArgs p;
   const int32_t *starts, *prefixes;      // [G + 1], [G]
-  int G, rest_waves;
-  int32_t *total;                        // steps of all groups' prefixes
-  int32_t *skips, *group_of;             // [B]: keys that a row's group attends for it; group, -1: none
-  int32_t *first, *source, *steps, *at;  // [G + 1] each: first member, the one whose table is read,
-                                         // steps of the prefix, steps of all before
-  float *heads;                          // [B][Hq]{m, l, O[D]}: a prefix's first piece
-  float *more;                           // [workgroup][kSharedRows]: pieces that others began
 };
-constexpr int kSharedRows = 256;         // query rows of a workgroup
 size_t gqa_shared_workspace(int B, int Hq, int Hkv, int D, int G, int cus);
-void gqa_shared_bind(GqaSharedArgs *a, void *workspace, int cus);
+void gqa_shared_bind(GqaSharedArgs *a, int G, void *workspace, int cus);
 hipError_t launch_gqa_shared(const GqaSharedArgs &a, int cus, hipStream_t s);
-int gqa_shared_rest_waves(int D, int cus);
-hipError_t launch_gqa_shared_rest(const GqaPagedArgs &a, int cus, hipStream_t s);  // the keys behind (gqa_paged.hip)
+// Of gqa_paged.hip: workgroups of four waves, and the launch over the planned work.
+int gqa_shared_workgroups(int D, int cus);
+hipError_t launch_gqa_shared_work(const GqaPagedArgs &a, int cus, hipStream_t s);
 
 // Synchronises `s`, reads a status word and clears the bits that it had.
 hipError_t read_and_clear_status(uint32_t *status, uint32_t *flags, hipStream_t s);

@@ -34,6 +34,7 @@
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"
 #include "gqa_internal.h"
+#include "gqa_prefix_dev.h"
 #include "launch.h"
 
 namespace moe {
@@ -55,6 +56,8 @@ constexpr int kWindow = 4;      // sequences per lane whose lengths a wave holds
 template <int D> constexpr int kStage = kStep * D * 2;
 template <int D> constexpr int kWaveLds = 5 * kStage<D> / 2;
 template <int D> constexpr int kWorkgroups = 160 * 1024 / (kWaves * kWaveLds<D>);  // per CU
+// Over prefixes too: 134 registers a lane with heads of 64.
+template <int D> constexpr int kSharedGroups = D == 128 ? 2 : 3;
 template <int D>
 __device__ __forceinline__ int swizzle_k(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
 template <int D>
@@ -163,10 +166,10 @@ __host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 20
 // 9.3 so, 16 of 500 13.7, 10.1, 64 of 1000 48.4, 41.6; what the list loses by
 // looking is 0.3 us).
 //
-// SHARED: the list alone, of every sequence's keys behind the first skips[b] of them (a
-// multiple of 16), and every piece leaves its state: gqa_shared.hip joins them.
+// SHARED: the first workgroups go over prefixes that groups of sequences share (gqa_shared.hip
+// plans that), the others by the list over the keys behind; every piece leaves its state.
 template <int D, bool F16, int TEAM, bool SHARED>
-__global__ __launch_bounds__(64 * (TEAM ? TEAM : kWaves), TEAM == 8 ? 1 : kWorkgroups<D>)
+__global__ __launch_bounds__(64 * (TEAM ? TEAM : kWaves), (TEAM == 8 ? 1 : SHARED ? kSharedGroups<D> : kWorkgroups<D>))
 void gqa_paged_kernel(GqaPagedArgs a) {
   constexpr int kSlices = D / 32;               // 32-dim slices of a row
   constexpr int kTiles = D / 16;                // 16-dim tiles of O
@@ -174,7 +177,16 @@ void gqa_paged_kernel(GqaPagedArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = sgpr(threadIdx.x >> 6);
-  const int worker = sgpr(wave * gridDim.x + blockIdx.x), workers = gridDim.x * kWaves;  // few steps: on many CUs
+  int before_list = 0;  // workgroups that the list has not
+  if constexpr (SHARED) {
+    before_list = uniform_load(a.shared.header + 1);
+    if ((int)blockIdx.x < before_list) {
+      shared::prefix<D, F16>(a, smem);
+      return;
+    }
+  }
+  const int listed = SHARED ? (int)gridDim.x - before_list : gridDim.x;
+  const int worker = sgpr(wave * listed + (int)blockIdx.x - before_list), workers = listed * kWaves;  // few steps: on many CUs
   constexpr int kTeam = TEAM ? TEAM : kWaves;
   const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows, heads = a.Hkv * blocks;
   const int cap = a.M * a.page;
@@ -196,7 +208,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
       const int ok = max(0, min(lens[i], cap));
       if (lens[i] != ok) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
       lens[i] = ok;
-      if constexpr (SHARED) lens[i] = max(0, ok - (window + kWave * i + lane < a.B ? a.skips[window + kWave * i + lane] : 0));
+      if constexpr (SHARED) lens[i] = max(0, ok - (window + kWave * i + lane < a.B ? a.shared.rows[8 * (window + kWave * i + lane)] : 0));
     }
   };
   int b = -1, len = 0, head, s;           // of the next step, with its sequence's length
@@ -292,7 +304,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
   const int per_page = a.page / kBlock;
   // Blocks of the next step's sequence before its first step, and the page and the block
   // there of its next.
-  int skipped = SHARED ? uniform_load(a.skips + b) / kBlock : 0;
+  int skipped = SHARED ? uniform_load(a.shared.rows + 8 * b) / kBlock : 0;
   int page_at = (skipped + 2 * s) / per_page, block_at = (skipped + 2 * s) % per_page;
 
   // Its steps; by teams or by the list (each with code of its own: tests of `team` in the
@@ -338,7 +350,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
           } else {
             b = next;
             steps = steps_of(len);
-            if constexpr (SHARED) skipped = uniform_load(a.skips + b) / kBlock;
+            if constexpr (SHARED) skipped = uniform_load(a.shared.rows + 8 * b) / kBlock;
           }
         }
         if constexpr (SHARED) {
@@ -482,7 +494,7 @@ void gqa_paged_kernel(GqaPagedArgs a) {
         const int64_t head0 = (int64_t)cur.b * a.Hq + kvh * group + kRows * part;
         const float l = quad_sum(l_run);
         const bool all_of_it = pair_ends && piece_from == 0, whole = !SHARED && all_of_it;
-        const int slot = SHARED && all_of_it ? 2 * workers + cur.b * heads + cur.head
+        const int slot = SHARED && all_of_it ? 2 * (int)gridDim.x * kWaves + cur.b * heads + cur.head
                                              : 2 * worker + (piece_unit == first ? 0 : 1);
         if (piece_from == 0 && lane == 0) {
           // Pieces of the (sequence, head block): this one, then the first pieces
@@ -737,10 +749,13 @@ hipError_t launch_gqa_paged(const GqaPagedArgs &a, int cus, hipStream_t s) {
   return a.dtype == GQA_FP16 ? launch<64, true>(a, cus, s) : launch<64, false>(a, cus, s);
 }
 
-int gqa_shared_rest_waves(int D, int cus) { return waves_of(D, cus); }
+int gqa_shared_workgroups(int D, int cus) { return cus * (D == 128 ? kSharedGroups<128> : kSharedGroups<64>); }
 
-hipError_t launch_gqa_shared_rest(const GqaPagedArgs &a, int cus, hipStream_t s) {
-  const int grid = waves_of(a.D, cus) / kWaves;
+hipError_t launch_gqa_shared_work(const GqaPagedArgs &a, int cus, hipStream_t s) {
+  static_assert(kWaves == shared::kWaves && kWaves * kWaveLds<128> >= shared::kRing * 2 * shared::kTile<128> &&
+                    kWaves * kWaveLds<64> >= shared::kRing * 2 * shared::kTile<64>,
+                "the stages of a prefix have their place");
+  const int grid = gqa_shared_workgroups(a.D, cus);
   if (a.D == 128) return a.dtype == GQA_FP16 ? launch_kernel<128, true, 0, true>(a, grid, s) : launch_kernel<128, false, 0, true>(a, grid, s);
   return a.dtype == GQA_FP16 ? launch_kernel<64, true, 0, true>(a, grid, s) : launch_kernel<64, false, 0, true>(a, grid, s);
 }
