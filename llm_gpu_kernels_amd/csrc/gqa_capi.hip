@@ -27,7 +27,7 @@ struct gqa_paged_plan {
   int device, cus;
 };
 struct gqa_shared_plan {
-  moe::GqaSharedArgs a;
+  moe::GqaPagedArgs a;
   int device, cus;
 };
 
@@ -367,10 +367,8 @@ int gqa_shared_plan_create(gqa_shared_plan **out, const gqa_paged_desc *d, int32
   if (rc) return rc;
   gqa_shared_plan *p = new (std::nothrow) gqa_shared_plan();
   if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");
-  p->a.p = paged_args(d);
-  p->a.starts = starts;
-  p->a.prefixes = prefixes;
-  moe::gqa_shared_bind(&p->a, G, d->workspace, cus);
+  p->a = paged_args(d);
+  moe::gqa_shared_bind(&p->a, G, starts, prefixes, d->workspace, cus);
   p->device = dev;
   p->cus = cus;
   *out = p;
@@ -379,14 +377,14 @@ int gqa_shared_plan_create(gqa_shared_plan **out, const gqa_paged_desc *d, int32
 
 int gqa_shared_plan_run(gqa_shared_plan *p, void *stream) {
   if (!p) return moe::capi_fail(MOE_EINVAL, "null plan");
-  if (p->a.p.B == 0) return MOE_OK;
+  if (p->a.B == 0) return MOE_OK;
   return on_device(p->device, "shared gqa launch", [&] { return moe::launch_gqa_shared(p->a, p->cus, (hipStream_t)stream); });
 }
 
 int gqa_shared_plan_read_status(gqa_shared_plan *p, void *stream, uint32_t *flags) {
   if (!p || !flags) return moe::capi_fail(MOE_EINVAL, "null plan or flags");
   return on_device(p->device, "status",
-                   [&] { return moe::read_and_clear_status(p->a.p.status, flags, (hipStream_t)stream); });
+                   [&] { return moe::read_and_clear_status(p->a.status, flags, (hipStream_t)stream); });
 }
 
 void gqa_shared_plan_destroy(gqa_shared_plan *p) { delete p; }

@@ -69,6 +69,8 @@ constexpr int kMaxGroups = 1024;
 // What gqa_shared.hip plans for a run, and the states of its prefixes.
 struct GqaSharedState {
   int G;
+  int local;                             // every workgroup of the work plans by itself
+  const int32_t *starts, *prefixes;      // [G + 1], [G]
   int32_t *header;                       // {units, workgroups for them}
   // [G][16]: {units before, steps of a chunk, first member, query rows of a KV head, member
   // whose table is read, keys, tiles, rows of a tile, chunks, units before but each (KV
@@ -112,18 +114,17 @@ hipError_t launch_gqa_paged_merge(const GqaPagedArgs &a, int cus, hipStream_t s)
 size_t gqa_mx_workspace(int B, int Hq, int Hkv, int D, int storage, int64_t keys, int cus);
 hipError_t launch_gqa_mx(const GqaPagedArgs &a, int cus, hipStream_t s);
 
-// The same where groups of sequences start with the same keys (gqa_shared.hip): 16-bit
-// pages, and the lists and states in the workspace.
-struct GqaSharedArgs {
-  GqaPagedArgs p;
-  const int32_t *starts, *prefixes;      // [G + 1], [G]
-};
+// The same where groups of sequences start with the same keys (gqa_shared.hip), of 16-bit
+// pages: with a.shared.
 size_t gqa_shared_workspace(int B, int Hq, int Hkv, int D, int G, int cus);
-void gqa_shared_bind(GqaSharedArgs *a, int G, void *workspace, int cus);
-hipError_t launch_gqa_shared(const GqaSharedArgs &a, int cus, hipStream_t s);
+void gqa_shared_bind(GqaPagedArgs *a, int G, const int32_t *starts, const int32_t *prefixes, void *workspace, int cus);
+hipError_t launch_gqa_shared(const GqaPagedArgs &a, int cus, hipStream_t s);
 // Of gqa_paged.hip: workgroups of four waves, and the launch over the planned work.
 int gqa_shared_workgroups(int D, int cus);
 hipError_t launch_gqa_shared_work(const GqaPagedArgs &a, int cus, hipStream_t s);
+// Whether every row is worked on by itself, and that.
+bool gqa_shared_by_rows(const GqaPagedArgs &a, int cus);
+hipError_t launch_gqa_shared_rows(const GqaPagedArgs &a, hipStream_t s);
 
 // Synchronises `s`, reads a status word and clears the bits that it had.
 hipError_t read_and_clear_status(uint32_t *status, uint32_t *flags, hipStream_t s);

@@ -168,6 +168,7 @@ __host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 20
 //
 // SHARED: the first workgroups go over prefixes that groups of sequences share (gqa_shared.hip
 // plans that), the others by the list over the keys behind; every piece leaves its state.
+// With TEAM all rows by themselves.
 template <int D, bool F16, int TEAM, bool SHARED>
 __global__ __launch_bounds__(64 * (TEAM ? TEAM : kWaves), (TEAM == 8 ? 1 : SHARED ? kSharedGroups<D> : kWorkgroups<D>))
 void gqa_paged_kernel(GqaPagedArgs a) {
@@ -178,12 +179,20 @@ void gqa_paged_kernel(GqaPagedArgs a) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = sgpr(threadIdx.x >> 6);
   int before_list = 0;  // workgroups that the list has not
-  if constexpr (SHARED) {
-    before_list = uniform_load(a.shared.header + 1);
+  int skips[kWindow] = {0, 0, 0, 0};  // SHARED: keys left out of the window's sequences
+  if constexpr (SHARED && TEAM > 0) {
+    if (blockIdx.x == 0) shared::check_groups(a);
+  }
+  if constexpr (SHARED && TEAM == 0) {
+    static_assert(kWindow == 4 && kWaves == shared::kWaves, "a plan's rows");
+    const shared::Plan plan = a.shared.local ? shared::plan_here(a, smem) : shared::plan_there(a);
+    before_list = plan.workgroups;
     if ((int)blockIdx.x < before_list) {
-      shared::prefix<D, F16>(a, smem);
+      shared::prefix<D, F16>(a, plan, smem);
       return;
     }
+#pragma unroll
+    for (int i = 0; i < kWindow; ++i) skips[i] = plan.skips[i];
   }
   const int listed = SHARED ? (int)gridDim.x - before_list : gridDim.x;
   const int worker = sgpr(wave * listed + (int)blockIdx.x - before_list), workers = listed * kWaves;  // few steps: on many CUs
@@ -208,7 +217,11 @@ void gqa_paged_kernel(GqaPagedArgs a) {
       const int ok = max(0, min(lens[i], cap));
       if (lens[i] != ok) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
       lens[i] = ok;
-      if constexpr (SHARED) lens[i] = max(0, ok - (window + kWave * i + lane < a.B ? a.shared.rows[8 * (window + kWave * i + lane)] : 0));
+      if constexpr (SHARED) {
+        const int at = window + kWave * i + lane;
+        if (!a.shared.local) skips[i] = at < a.B ? a.shared.rows[8 * at] : 0;
+        lens[i] = max(0, ok - skips[i]);
+      }
     }
   };
   int b = -1, len = 0, head, s;           // of the next step, with its sequence's length
@@ -304,7 +317,15 @@ void gqa_paged_kernel(GqaPagedArgs a) {
   const int per_page = a.page / kBlock;
   // Blocks of the next step's sequence before its first step, and the page and the block
   // there of its next.
-  int skipped = SHARED ? uniform_load(a.shared.rows + 8 * b) / kBlock : 0;
+  auto skipped_of = [&](int row) __attribute__((always_inline)) {
+    int skip = 0;
+#pragma unroll
+    for (int i = 0; i < kWindow; ++i)
+      if (row - window >= kWave * i && row - window < kWave * (i + 1)) skip = __builtin_amdgcn_readlane(skips[i], row - window - kWave * i);
+    return skip / kBlock;
+  };
+  constexpr bool kSkips = SHARED && TEAM == 0;
+  int skipped = kSkips ? skipped_of(b) : 0;
   int page_at = (skipped + 2 * s) / per_page, block_at = (skipped + 2 * s) % per_page;
 
   // Its steps; by teams or by the list (each with code of its own: tests of `team` in the
@@ -350,10 +371,10 @@ void gqa_paged_kernel(GqaPagedArgs a) {
           } else {
             b = next;
             steps = steps_of(len);
-            if constexpr (SHARED) skipped = uniform_load(a.shared.rows + 8 * b) / kBlock;
+            if constexpr (kSkips) skipped = skipped_of(b);
           }
         }
-        if constexpr (SHARED) {
+        if constexpr (kSkips) {
           page_at = skipped / per_page;
           block_at = skipped % per_page;
         }
@@ -758,6 +779,21 @@ hipError_t launch_gqa_shared_work(const GqaPagedArgs &a, int cus, hipStream_t s)
   const int grid = gqa_shared_workgroups(a.D, cus);
   if (a.D == 128) return a.dtype == GQA_FP16 ? launch_kernel<128, true, 0, true>(a, grid, s) : launch_kernel<128, false, 0, true>(a, grid, s);
   return a.dtype == GQA_FP16 ? launch_kernel<64, true, 0, true>(a, grid, s) : launch_kernel<64, false, 0, true>(a, grid, s);
+}
+
+// Where even a full table is a few steps for each of eight waves per (sequence, head block),
+// and those all run at once, the pages that rows share come from the L2 and one launch
+// beats the two: 8 and 32 rows with a prefix of 1500 keys, tables of 1616, 8 heads of 128,
+// 12.0 and 12.7 us, by groups 19.2 and 25.3.  Beyond, 128 rows of 1000 to 1200 keys 29.4, by groups
+// 26.5; 8 of 4000 20.2, 21.9; 40 groups of 4 rows of 2000 201, 91.
+bool gqa_shared_by_rows(const GqaPagedArgs &a, int cus) {
+  const int group = a.Hq / a.Hkv, pairs = a.B * a.Hkv * ((group + kRows - 1) / kRows);
+  return team_of(pairs, ((int64_t)a.M * a.page + kStep - 1) / kStep, waves_of(a.D, cus)) == 8;
+}
+hipError_t launch_gqa_shared_rows(const GqaPagedArgs &a, hipStream_t s) {
+  const int group = a.Hq / a.Hkv, pairs = a.B * a.Hkv * ((group + kRows - 1) / kRows);
+  if (a.D == 128) return a.dtype == GQA_FP16 ? launch_kernel<128, true, 8, true>(a, pairs, s) : launch_kernel<128, false, 8, true>(a, pairs, s);
+  return a.dtype == GQA_FP16 ? launch_kernel<64, true, 8, true>(a, pairs, s) : launch_kernel<64, false, 8, true>(a, pairs, s);
 }
 
 // Clears the bits that it returns, no others, and is done with that on return: a bit

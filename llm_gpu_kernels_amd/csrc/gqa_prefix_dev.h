@@ -38,11 +38,167 @@ __device__ __forceinline__ int swizzle_v(int row) { return D == 128 ? 4 * (row &
 constexpr int kRing = 5;                                 // stages of 32 keys in LDS
 template <int D> constexpr int kTile = kStep * D * 2;   // bytes of a stage's K (or V)
 
+// A group's work; a lane of a wave has one.  A unit: a KV head's tile of rows over a chunk of
+// the steps, in the order (KV head, chunk, tile).
+struct Group {
+  int before, chunk_steps, first, rows;     // units before, steps of a chunk, first member, query rows
+  int source, keys, tiles, tile_rows;       // member whose table is read, keys that are shared
+  int chunks, more;                         // units before but each (KV head, tile)'s first
+};
+// The plan of a run: units, the workgroups for them, the groups of the wave's lanes and the
+// keys that a group attends for the rows 64 i + lane.
+struct Plan {
+  int units, workgroups;
+  Group group;
+  int skips[4];
+};
+constexpr int kLocalRows = 64 * kWaves, kLocalGroups = kWave;
+
+// Length of a row as the paged kernels take it.
+__device__ __forceinline__ int length_of(const GqaPagedArgs &p, int b) { return max(0, min(p.lengths[b], p.M * p.page)); }
+__device__ __forceinline__ int steps_of(int keys) { return (int)(((uint32_t)keys + kStep - 1) / kStep); }
+
+// What a group of `rows` query rows of a KV head and `live` members with keys shares: the
+// multiple of 16 keys up to its prefix and its shortest member, if there are two of those.
+__device__ __forceinline__ void share(Group *g, int wanted, int least, int live) {
+  g->keys = live < 2 ? 0 : max(0, min(wanted, least)) / kBlock * kBlock;
+  g->tiles = g->keys ? (g->rows + kSharedRows - 1) / kSharedRows : 0;
+  const int blocks = (g->rows + 31) / 32;
+  g->tile_rows = g->tiles ? (blocks + g->tiles - 1) / g->tiles * 32 : 32;
+}
+// Workgroups for the prefixes, of all, by steps: those are as many bytes in either part, and
+// the four waves of the list's have a step each in flight, as the others have four stages.
+__device__ __forceinline__ int share_of(int64_t shared, int64_t listed, int workgroups) {
+  if (shared == 0) return 0;
+  const int n = (int)((shared * workgroups + (shared + listed) / 2) / (shared + listed));
+  return max(1, min(n, listed ? workgroups - 1 : workgroups));
+}
+// Steps of a chunk: the fewest with which the units are not more than the workgroups, of
+// kSizes from the average up to three times that.  If none is (there are more groups than
+// that), the average, and a workgroup has several units.
+constexpr int kLeastSteps = 2;  // one costs more in states than it gains
+constexpr int kSizes = 16;
+__device__ __forceinline__ int chunk_size(int64_t shared, int n, int i) {
+  const int even = n ? max(kLeastSteps, (int)((shared + n - 1) / n)) : 1;
+  return even + (int)((int64_t)even * i / 8);
+}
+__device__ __forceinline__ void cut(Group *g, int size) {
+  const int steps = steps_of(g->keys);
+  g->chunks = (steps + size - 1) / size;
+  g->chunk_steps = g->chunks ? (steps + g->chunks - 1) / g->chunks : 1;
+}
+
+// The plan by one workgroup of four waves for itself: up to 64 groups and 256 rows.  Bounds
+// that do not ascend within [0, B]: nothing is shared.  Workgroup 0 reports and leaves
+// what the join needs of each row.
+__device__ __forceinline__ Plan plan_here(const GqaPagedArgs &p, uint8_t *smem) {
+  struct Lds {
+    int starts[kLocalGroups + 1], least[kLocalGroups], live[kLocalGroups], source[kLocalGroups], keys[kLocalGroups];
+    int skips[kLocalRows], fits[kSizes], rest, wrong;
+  };
+  Lds *const lds = (Lds *)smem;
+  const GqaSharedState &st = p.shared;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per_head = p.Hq / p.Hkv, G = st.G;
+  const int raw = tid < p.B ? p.lengths[tid] : 0, len = max(0, min(raw, p.M * p.page));
+  const int wanted = lane < G ? st.prefixes[lane] : 0;
+  if (tid <= G) lds->starts[tid] = st.starts[tid];
+  if (tid < G) {
+    lds->least[tid] = lds->source[tid] = 0x7fffffff;
+    lds->live[tid] = 0;
+  }
+  if (tid == 0) lds->rest = lds->wrong = 0;
+  __syncthreads();
+  // (__syncthreads_or() has LDS of its own, and with it one workgroup per CU less.)
+  if (tid <= G && (lds->starts[tid] < 0 || lds->starts[tid] > p.B || (tid > 0 && lds->starts[tid] < lds->starts[tid - 1]))) lds->wrong = 1;
+  __syncthreads();
+  const bool bad = lds->wrong != 0;
+  if (blockIdx.x == 0 && ((bad && tid == 0) || wanted < 0)) atomicOr(p.status, GQA_STATUS_BAD_BOUNDS);
+  int g = -1;  // the row's group
+  if (!bad && G > 0 && tid < p.B && tid >= lds->starts[0] && tid < lds->starts[G]) {
+    int hi = G - 1;
+    g = 0;
+    while (g < hi) {
+      const int mid = (g + hi + 1) >> 1;
+      if (lds->starts[mid] <= tid) g = mid;
+      else hi = mid - 1;
+    }
+  }
+  if (g >= 0 && len > 0) {
+    atomicMin(lds->least + g, len);
+    atomicMin(lds->source + g, tid);
+    atomicAdd(lds->live + g, 1);
+  }
+  __syncthreads();
+  Plan plan = {};
+  Group &mine = plan.group;  // every wave has all groups
+  mine.before = 0x7fffffff;
+  if (lane < G) {
+    mine.first = bad ? 0 : lds->starts[lane];
+    mine.rows = bad ? 0 : (lds->starts[lane + 1] - mine.first) * per_head;
+    share(&mine, wanted, lds->least[lane], lds->live[lane]);
+    mine.source = mine.keys ? lds->source[lane] : 0;
+    if (wave == 0) lds->keys[lane] = mine.keys;
+  }
+  __syncthreads();
+  const int skip = g >= 0 && len > 0 ? lds->keys[g] : 0;
+  lds->skips[tid] = skip;
+  const int rest = wave_total(steps_of(len - skip));
+  if (lane == 0) atomicAdd(&lds->rest, rest);
+  const int heads_units = mine.tiles * p.Hkv;  // of a chunk
+  const int64_t shared = wave_total(steps_of(mine.keys) * heads_units);  // below 2^30, checked on the host
+  __syncthreads();
+  plan.workgroups = share_of(shared, (int64_t)lds->rest * p.Hkv * ((per_head + 15) / 16), gridDim.x);
+  for (int i = wave; i < kSizes; i += kWaves) {
+    const int size = chunk_size(shared, plan.workgroups, i);
+    const int units = wave_total(heads_units * ((steps_of(mine.keys) + size - 1) / size));
+    if (lane == 0) lds->fits[i] = units <= plan.workgroups;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) plan.skips[i] = lds->skips[kWave * i + lane];
+  __syncthreads();
+  const uint64_t fit = __builtin_amdgcn_ballot_w64(lane < kSizes && lds->fits[lane & (kSizes - 1)]);
+  cut(&mine, chunk_size(shared, plan.workgroups, fit ? sgpr(__builtin_ctzll(fit)) : 0));
+  const int units = mine.chunks * heads_units, extra = max(0, units - heads_units);
+  const int incl = wave_scan(units);
+  if (lane < G) mine.before = incl - units;
+  mine.more = wave_scan(extra) - extra;
+  plan.units = __builtin_amdgcn_readlane(incl, 63);
+  if (blockIdx.x == 0) {
+    const int from = max(g, 0);  // all lanes take part in the exchange
+    const int chunks = __shfl(mine.chunks, from, kWave), tiles = __shfl(mine.tiles, from, kWave);
+    const int tile_rows = __shfl(mine.tile_rows, from, kWave), first = __shfl(mine.first, from, kWave);
+    const int more = __shfl(mine.more, from, kWave);
+    if (tid < p.B) {
+      int32_t *const rec = st.rows + 8 * tid;
+      *(int4 *)rec = make_int4(skip, chunks, tiles, tile_rows);
+      *(int2 *)(rec + 4) = make_int2((tid - first) * per_head, more);
+    }
+  }
+  __syncthreads();  // the LDS is the work's from here
+  return plan;
+}
+// Reports bounds and prefixes, for a launch that does without a plan: by one workgroup.
+__device__ __forceinline__ void check_groups(const GqaPagedArgs &p) {
+  const GqaSharedState &st = p.shared;
+  for (int g = threadIdx.x; g <= st.G; g += blockDim.x) {
+    const int at = st.starts[g];
+    if (at < 0 || at > p.B || (g > 0 && at < st.starts[g - 1]) || (g < st.G && st.prefixes[g] < 0))
+      atomicOr(p.status, GQA_STATUS_BAD_BOUNDS);
+  }
+}
+// The plan as gqa_shared_plan() left it.
+__device__ __forceinline__ Plan plan_there(const GqaPagedArgs &p) {
+  Plan plan = {};
+  plan.units = uniform_load(p.shared.header);
+  plan.workgroups = uniform_load(p.shared.header + 1);
+  return plan;
+}
+
 // Keys that every row of a group sees, in pages; the loop is the packed kernel's, where its
 // overlaps and operand layouts are explained.  A workgroup has up to 128 query rows of a
 // group and KV head (row = member * G + head), 32 per wave.
 template <int D, bool F16>
-__device__ __forceinline__ void prefix(const GqaPagedArgs &p, uint8_t *smem) {
+__device__ __forceinline__ void prefix(const GqaPagedArgs &p, const Plan &plan, uint8_t *smem) {
   constexpr int kSteps = D / 16;                        // QK MFMAs per stage
   constexpr int kDims = D / 32;                         // 32-dim tiles of O
   constexpr int kChunks = D / 8;                        // 16-byte chunks of a row
@@ -52,7 +208,7 @@ __device__ __forceinline__ void prefix(const GqaPagedArgs &p, uint8_t *smem) {
   const int wave = sgpr(threadIdx.x >> 6);
   const int group = p.Hq / p.Hkv, per_page = p.page / kBlock;
   // Neighbouring units, whose rows see the same keys, on one XCD, which has them in its L2.
-  const int units = uniform_load(a.header), workgroups = uniform_load(a.header + 1);
+  const int units = plan.units, workgroups = plan.workgroups;
   const int xcd = blockIdx.x % kXcds, first_unit = xcd * (workgroups / kXcds) + min(xcd, workgroups % kXcds) + (int)blockIdx.x / kXcds;
   const uint32_t lds0 = lds_addr(smem);
   const float sl2 = p.scale * kLog2e;
@@ -75,25 +231,34 @@ __device__ __forceinline__ void prefix(const GqaPagedArgs &p, uint8_t *smem) {
   const uint32_t v_at = (uint32_t)(kTile<D> + v_key * 2 * D + 16 * (v_chunk ^ swizzle_v<D>(v_key)) + 8 * (lane & 1));
 
   for (int u = first_unit; u < units; u += workgroups) {
-    // The last group with at most u units before it has some: a chunk of 64 groups, then a
-    // lane for each.
-    int lo = 0, hi = (a.G - 1) / kWave;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (uniform_load(a.groups + 16 * kWave * mid) <= u) lo = mid;
-      else hi = mid - 1;
+    // The last group with at most u units before it has some: a lane for each of 64.
+    Group of = plan.group;
+    if (!a.local) {
+      int lo = 0, hi = (a.G - 1) / kWave;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (uniform_load(a.groups + 16 * kWave * mid) <= u) lo = mid;
+        else hi = mid - 1;
+      }
+      of.before = 0x7fffffff;
+      if (kWave * lo + lane < a.G) {
+        const int32_t *const rec = a.groups + 16 * (kWave * lo + lane);
+        const int4 x = *(const int4 *)rec, y = *(const int4 *)(rec + 4);
+        const int2 z = *(const int2 *)(rec + 8);
+        of = Group{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y};
+      }
     }
-    const int at_lane = kWave * lo + lane < a.G ? a.groups[16 * (kWave * lo + lane)] : 0x7fffffff;
-    const int g = kWave * lo + (int)__popcll(__builtin_amdgcn_ballot_w64(at_lane <= u)) - 1;
-    const int32_t *const rec = a.groups + 16 * g;
-    const int before = uniform_load(rec), chunk_steps = uniform_load(rec + 1), first = uniform_load(rec + 2);
-    const int rows = uniform_load(rec + 3), source = uniform_load(rec + 4), keys = uniform_load(rec + 5);
-    const int tiles = uniform_load(rec + 6), tile_rows = uniform_load(rec + 7), chunks = uniform_load(rec + 8);
+    const int g = sgpr((int)__popcll(__builtin_amdgcn_ballot_w64(of.before <= u)) - 1);
+    const int before = __builtin_amdgcn_readlane(of.before, g), chunk_steps = __builtin_amdgcn_readlane(of.chunk_steps, g);
+    const int first = __builtin_amdgcn_readlane(of.first, g), rows = __builtin_amdgcn_readlane(of.rows, g);
+    const int source = __builtin_amdgcn_readlane(of.source, g), keys = __builtin_amdgcn_readlane(of.keys, g);
+    const int tiles = __builtin_amdgcn_readlane(of.tiles, g), tile_rows = __builtin_amdgcn_readlane(of.tile_rows, g);
+    const int chunks = __builtin_amdgcn_readlane(of.chunks, g), more = __builtin_amdgcn_readlane(of.more, g);
     const int rest = (u - before) / tiles, tile = u - before - rest * tiles, kvh = rest / chunks, chunk = rest - kvh * chunks;
     const int s0 = chunk * chunk_steps, stages = min(chunk_steps, (keys + kStep - 1) / kStep - s0);
     const int row0 = tile * tile_rows + kWaveRows * wave;
     const bool own = kWaveRows * wave < tile_rows && row0 < rows;
-    const int more_at = uniform_load(rec + 9) + (kvh * (chunks - 1) + chunk - 1) * tiles + tile;  // chunk > 0
+    const int more_at = more + (kvh * (chunks - 1) + chunk - 1) * tiles + tile;  // chunk > 0
 
     // ---- loads ----
     const int32_t *const table = p.tables + (int64_t)source * p.table_stride;

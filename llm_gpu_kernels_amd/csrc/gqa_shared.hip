@@ -1,6 +1,9 @@
 // Attention of one new token per sequence over a paged cache, where groups of sequences
 // start with the same keys (samples of one prompt, users of one instruction), on gfx950.
 //
+// Tables that are wide for the rows are worked on in two launches; of narrow ones
+// every row goes by itself (gqa_shared_by_rows() has the rule).
+//
 // softmax(q K^T) V over a prefix and the rest of a row's keys is joined from the two
 // parts' (max, sum, O), so a prefix is read once for all rows of its group: up to 128
 // query rows (the members' heads of one KV head) are one workgroup's, 32 per wave, and K
@@ -8,9 +11,10 @@
 // hundreds the matrix cores.  The keys behind the prefix are worked on as
 // gqa_paged.hip works on whole rows.
 //
-//   plan    one workgroup: the keys that each group shares, and how they are cut into
-//           chunks, so that the units of work, (group, KV head, chunk, up to 128 rows), are
-//           as many as the workgroups for them;
+//   plan    the keys that each group shares, and how they are cut into chunks, so that the
+//           units of work, (group, KV head, chunk, up to 128 rows), are as many as the
+//           workgroups for them.  Up to 64 groups and 256 sequences every workgroup finds
+//           that out by itself, else one does before;
 //   work    one launch for both parts, which fill the chip together: a unit per workgroup
 //           of the first ones; gqa_paged.hip's list of steps over the keys behind, a range
 //           per wave of the others.  Every piece leaves its states;
@@ -19,39 +23,32 @@
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"
 #include "gqa_internal.h"
+#include "gqa_prefix_dev.h"
 
 namespace moe {
 
 using namespace gqa;
+using shared::length_of;
+using shared::steps_of;
 
 namespace {
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / kWave;
-constexpr int kStep = 32, kBlock = 16;
 constexpr int kRows = 16;       // query heads of a piece of the rest
-constexpr int kMergeThreads = 256, kBatch = 8;
+constexpr int kMergeThreads = 256, kBatch = 16;
 
-// Row length as the paged kernels take it.
-__device__ __forceinline__ int length_of(const GqaPagedArgs &p, int b) { return max(0, min(p.lengths[b], p.M * p.page)); }
-
-// What each group shares: the multiple of 16 keys up to its prefix, and up to the shortest
-// of its members that have keys, if there are two of those.  Bounds that do not ascend
-// within [0, B]: nothing is shared, and every row is attended by itself.
 // A thread per group, and one per row of the batch.
 static_assert(kMaxGroups <= kPlanThreads, "a thread per group");
-constexpr int kLeastSteps = 4;  // of a chunk: fewer cost more in states than they gain
-__global__ __launch_bounds__(kPlanThreads) void gqa_shared_plan(GqaSharedArgs a, int workgroups) {
+__global__ __launch_bounds__(kPlanThreads) void gqa_shared_plan(GqaPagedArgs p, int workgroups) {
   __shared__ int starts[kMaxGroups + 1], least[kMaxGroups], live[kMaxGroups], source[kMaxGroups];
-  __shared__ int keys_of[kMaxGroups], steps_lds[kMaxGroups], per_chunk[kMaxGroups];  // units of a chunk
-  __shared__ int chunks_lds[kMaxGroups], more_lds[kMaxGroups], sums[2][kPlanWaves], fits[kPlanWaves];
+  __shared__ shared::Group groups[kMaxGroups];
+  __shared__ int sums[2][kPlanWaves], fits[kPlanWaves];
   __shared__ unsigned long long shared_steps, rest_steps;
-  const GqaPagedArgs &p = a.p;
+  static_assert(kPlanWaves == shared::kSizes, "a wave per size");
   const GqaSharedState &st = p.shared;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per_head = p.Hq / p.Hkv, G = st.G;
-  const auto steps_of = [](int keys) { return (int)(((uint32_t)keys + kStep - 1) / kStep); };
-  const int len0 = tid < p.B ? length_of(p, tid) : 0;  // of the thread's first row
-  for (int g = tid; g <= G; g += kPlanThreads) starts[g] = a.starts[g];
-  const int wanted = tid < G ? a.prefixes[tid] : 0;
+  for (int g = tid; g <= G; g += kPlanThreads) starts[g] = st.starts[g];
+  const int wanted = tid < G ? st.prefixes[tid] : 0;
   if (tid < G) {
     least[tid] = source[tid] = 0x7fffffff;
     live[tid] = 0;
@@ -62,7 +59,6 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_shared_plan(GqaSharedArgs a,
   for (int g = tid; g <= G; g += kPlanThreads) wrong |= starts[g] < 0 || starts[g] > p.B || (g > 0 && starts[g] < starts[g - 1]);
   const bool bad = __syncthreads_or(wrong);
   if ((bad && tid == 0) || wanted < 0) atomicOr(p.status, GQA_STATUS_BAD_BOUNDS);
-
   // The group of a row; -1: none.
   auto group_of = [&](int b) {
     if (bad || G == 0 || b < starts[0] || b >= starts[G]) return -1;
@@ -74,73 +70,63 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_shared_plan(GqaSharedArgs a,
     }
     return lo;
   };
-  const int group0 = tid < p.B ? group_of(tid) : -1;
   for (int b = tid; b < p.B; b += kPlanThreads) {
-    const int g = b == tid ? group0 : group_of(b), len = b == tid ? len0 : length_of(p, b);
+    const int g = group_of(b), len = length_of(p, b);
     if (g < 0 || len == 0) continue;
     atomicMin(least + g, len);
     atomicMin(source + g, b);
     atomicAdd(live + g, 1);
   }
   __syncthreads();
-  int rows = 0, tiles = 0, steps = 0;
+  shared::Group mine = {};
   if (tid < G) {
-    const int keys = live[tid] < 2 ? 0 : max(0, min(wanted, least[tid])) / kBlock * kBlock;
-    rows = bad ? 0 : (starts[tid + 1] - starts[tid]) * per_head;
-    tiles = keys ? (rows + kSharedRows - 1) / kSharedRows : 0;
-    steps = steps_of(keys);
-    keys_of[tid] = keys;
-    steps_lds[tid] = steps;
-    per_chunk[tid] = tiles * p.Hkv;
-    if (steps) atomicAdd(&shared_steps, (unsigned long long)steps * tiles * p.Hkv);
+    mine.first = bad ? 0 : starts[tid];
+    mine.rows = bad ? 0 : (starts[tid + 1] - mine.first) * per_head;
+    shared::share(&mine, wanted, least[tid], live[tid]);
+    mine.source = mine.keys ? source[tid] : 0;
+    groups[tid] = mine;
+    if (mine.keys) atomicAdd(&shared_steps, (unsigned long long)steps_of(mine.keys) * mine.tiles * p.Hkv);
   }
   __syncthreads();
   unsigned long long rest = 0;  // steps of the keys that no group has
   for (int b = tid; b < p.B; b += kPlanThreads) {
-    const int g = b == tid ? group0 : group_of(b), len = b == tid ? len0 : length_of(p, b);
-    rest += steps_of(len - (g >= 0 && len > 0 ? keys_of[g] : 0));
+    const int g = group_of(b), len = length_of(p, b);
+    rest += steps_of(len - (g >= 0 && len > 0 ? groups[g].keys : 0));
   }
   if (rest) atomicAdd(&rest_steps, rest);
   __syncthreads();
-  // Workgroups by steps, which are as many bytes in either part; the four waves of the
-  // list's have a step each in flight, as the others have four stages.
-  const int64_t shared = (int64_t)shared_steps, listed = (int64_t)rest_steps * p.Hkv * ((per_head + kRows - 1) / kRows);
-  int n = shared ? (int)((shared * workgroups + (shared + listed) / 2) / (shared + listed)) : 0;
-  if (shared) n = max(1, min(n, listed ? workgroups - 1 : workgroups));
-  // Steps of a chunk: the fewest with which the units are not more than the workgroups, of
-  // sixteen sizes from one to three times the average; a wave tries each.
-  const int even = n ? max(kLeastSteps, (int)((shared + n - 1) / n)) : 1;
-  auto size = [&](int w) { return even + (int)((int64_t)even * w / 8); };
+  const int64_t all_shared = (int64_t)shared_steps;
+  const int n = shared::share_of(all_shared, (int64_t)rest_steps * p.Hkv * ((per_head + kRows - 1) / kRows), workgroups);
+  const int size = shared::chunk_size(all_shared, n, wave);
   int units = 0;
-  for (int g = lane; g < G; g += kWave) units += per_chunk[g] * ((steps_lds[g] + size(wave) - 1) / size(wave));
+  for (int g = lane; g < G; g += kWave) units += groups[g].tiles * p.Hkv * ((steps_of(groups[g].keys) + size - 1) / size);
   units = wave_total(units);
   if (lane == 0) fits[wave] = units <= n;
   __syncthreads();
   int chosen = 0;
-  while (chosen < kPlanWaves - 1 && !fits[chosen]) ++chosen;
-  if (!fits[chosen]) chosen = 0;  // more groups than that: several units for a workgroup
-  const int chunks = steps ? (steps + size(chosen) - 1) / size(chosen) : 0;
-  const int mine = chunks * tiles * p.Hkv, extra = chunks ? mine - tiles * p.Hkv : 0;
-  const int incl = wave_scan(mine), incl_extra = wave_scan(extra);
+  while (chosen < kPlanWaves && !fits[chosen]) ++chosen;
+  shared::cut(&mine, shared::chunk_size(all_shared, n, chosen < kPlanWaves ? chosen : 0));
+  const int per_chunk = mine.tiles * p.Hkv, own = mine.chunks * per_chunk, extra = max(0, own - per_chunk);
+  const int incl = wave_scan(own), incl_extra = wave_scan(extra);
   if (lane == kWave - 1) {
     sums[0][wave] = incl;
     sums[1][wave] = incl_extra;
   }
   __syncthreads();
-  int before = incl - mine, more = incl_extra - extra, all = 0;
+  mine.before = incl - own;
+  mine.more = incl_extra - extra;
+  int all = 0;
   for (int w = 0; w < kPlanWaves; ++w) {
-    before += w < wave ? sums[0][w] : 0;
-    more += w < wave ? sums[1][w] : 0;
+    mine.before += w < wave ? sums[0][w] : 0;
+    mine.more += w < wave ? sums[1][w] : 0;
     all += sums[0][w];
   }
   if (tid < G) {
-    chunks_lds[tid] = chunks;
-    more_lds[tid] = more;
-    const int blocks = (rows + 31) / 32, tile_rows = tiles ? (blocks + tiles - 1) / tiles * 32 : 32;
+    groups[tid] = mine;
     int32_t *const rec = st.groups + 16 * tid;
-    *(int4 *)rec = make_int4(before, chunks ? (steps + chunks - 1) / chunks : 1, bad ? 0 : starts[tid], rows);
-    *(int4 *)(rec + 4) = make_int4(live[tid] ? source[tid] : 0, keys_of[tid], tiles, tile_rows);
-    *(int2 *)(rec + 8) = make_int2(chunks, more);
+    *(int4 *)rec = make_int4(mine.before, mine.chunk_steps, mine.first, mine.rows);
+    *(int4 *)(rec + 4) = make_int4(mine.source, mine.keys, mine.tiles, mine.tile_rows);
+    *(int2 *)(rec + 8) = make_int2(mine.chunks, mine.more);
   }
   if (tid == 0) {
     st.header[0] = all;
@@ -148,15 +134,11 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_shared_plan(GqaSharedArgs a,
   }
   __syncthreads();
   for (int b = tid; b < p.B; b += kPlanThreads) {
-    const int g = b == tid ? group0 : group_of(b), len = b == tid ? len0 : length_of(p, b);
+    const int g = group_of(b);
+    const shared::Group x = groups[max(g, 0)];
     int32_t *const rec = st.rows + 8 * b;
-    if (g < 0 || len == 0 || keys_of[g] == 0) {
-      rec[0] = 0;
-      continue;
-    }
-    const int all_rows = (starts[g + 1] - starts[g]) * per_head, t = per_chunk[g] / p.Hkv, blocks = (all_rows + 31) / 32;
-    *(int4 *)rec = make_int4(keys_of[g], chunks_lds[g], t, (blocks + t - 1) / t * 32);
-    *(int2 *)(rec + 4) = make_int2((b - starts[g]) * per_head, more_lds[g]);
+    *(int4 *)rec = make_int4(g >= 0 && length_of(p, b) > 0 ? x.keys : 0, x.chunks, x.tiles, x.tile_rows);
+    *(int2 *)(rec + 4) = make_int2((b - x.first) * per_head, x.more);
   }
 }
 
@@ -275,20 +257,21 @@ Layout layout_of(int B, int Hq, int Hkv, int D, int G, int cus) {
 
 size_t gqa_shared_workspace(int B, int Hq, int Hkv, int D, int G, int cus) { return layout_of(B, Hq, Hkv, D, G, cus).bytes; }
 
-void gqa_shared_bind(GqaSharedArgs *a, int G, void *workspace, int cus) {
+void gqa_shared_bind(GqaPagedArgs *a, int G, const int32_t *starts, const int32_t *prefixes, void *workspace, int cus) {
   uint8_t *const w = (uint8_t *)workspace;
-  GqaPagedArgs &p = a->p;
-  const Layout l = layout_of(p.B, p.Hq, p.Hkv, p.D, G, cus);
-  p.status = (uint32_t *)w;
-  p.pieces = (int32_t *)(w + l.pieces);
-  p.partial = (float *)(w + l.partial);
-  p.shared = GqaSharedState{G, (int32_t *)(w + l.header), (int32_t *)(w + l.groups), (int32_t *)(w + l.rows),
-                            (float *)(w + l.heads), (float *)(w + l.more)};
+  const Layout l = layout_of(a->B, a->Hq, a->Hkv, a->D, G, cus);
+  a->status = (uint32_t *)w;
+  a->pieces = (int32_t *)(w + l.pieces);
+  a->partial = (float *)(w + l.partial);
+  a->shared = GqaSharedState{G, G <= shared::kLocalGroups && a->B <= shared::kLocalRows, starts, prefixes,
+                             (int32_t *)(w + l.header), (int32_t *)(w + l.groups), (int32_t *)(w + l.rows),
+                             (float *)(w + l.heads), (float *)(w + l.more)};
 }
 
-hipError_t launch_gqa_shared(const GqaSharedArgs &a, int cus, hipStream_t s) {
-  const GqaPagedArgs &p = a.p;
-  hipLaunchKernelGGL(gqa_shared_plan, dim3(1), dim3(kPlanThreads), 0, s, a, gqa_shared_workgroups(p.D, cus));
+hipError_t launch_gqa_shared(const GqaPagedArgs &p, int cus, hipStream_t s) {
+  if (gqa_shared_by_rows(p, cus)) return launch_gqa_shared_rows(p, s);
+  if (!p.shared.local)
+    hipLaunchKernelGGL(gqa_shared_plan, dim3(1), dim3(kPlanThreads), 0, s, p, gqa_shared_workgroups(p.D, cus));
   if (const hipError_t e = launch_gqa_shared_work(p, cus, s)) return e;
   const int group = p.Hq / p.Hkv, pairs = p.B * p.Hkv * ((group + kRows - 1) / kRows), need = (group < kRows ? group : kRows) * p.D / 2;
   int chunk = kMergeThreads;

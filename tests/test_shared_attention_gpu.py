@@ -25,13 +25,22 @@ def _assert_close(out, ref, bound, keys, vmax):
     assert worst <= 1.0, worst
 
 
+@pytest.fixture(autouse=True, params=["narrow", "wide"])
+def tables(request, monkeypatch):
+    """Tables just wide enough, of which small ones are worked on row by row, and wide
+    ones, whose groups are worked on together."""
+    monkeypatch.setattr(Groups, "least_width", 1 if request.param == "narrow" else 1000)
+
+
 class Groups:
     """Groups as (prefix, lengths of the members), sequences of no group before and behind
     them.  Whole pages of a prefix are held once, the rest of it by every member; places
     behind each sequence's end hold NaN, table entries behind the last page an impossible
     number."""
 
-    def __init__(self, groups, hq, hkv, d, page, dtype, device, before=(), behind=(), order="heads", fill=None):
+    least_width = 1
+
+    def __init__(self, groups, hq, hkv, d, page, dtype, device, before=(), behind=(), order="heads"):
         self.device = device
         self.lengths = list(before) + [n for _, members in groups for n in members] + list(behind)
         g = torch.Generator().manual_seed(sum(self.lengths) + page + hq)
@@ -52,7 +61,7 @@ class Groups:
         shape = (count, hkv, page, d)
         kv = [torch.randn(shape, generator=g) for _ in range(2)]
         kv = [t.to(dtype) for t in kv]
-        width = max([len(x) for x in plans] + [1]) + 2
+        width = max([len(x) for x in plans] + [self.least_width]) + 2
         self.tables = [[perm[i] for i in x] + [1 << 29] * (width - len(x)) for x in plans]
         heads_of = {}
         for b, (n, o) in enumerate(zip(self.lengths, owner)):
@@ -274,7 +283,7 @@ def test_forked_samples(gpu_device):
     """Prompts forked into samples that grow by tokens of their own."""
     g = torch.Generator().manual_seed(4)
     hq, hkv, d, page = 8, 2, 128, 16
-    c = PagedKVCache(200, page, hkv, d, sequences=9, max_pages=30, max_tokens=400, device=gpu_device)
+    c = PagedKVCache(200, page, hkv, d, sequences=9, max_pages=30 * Groups.least_width, max_tokens=400, device=gpu_device)
     counts = [150, 0, 0, 0, 77, 0, 0, 20, 0]
     c.reserve(_i32(counts, gpu_device))
     rows = torch.randn(400, 2 * hkv, d, generator=g).to(torch.bfloat16).to(gpu_device)
