@@ -312,20 +312,19 @@ __device__ __forceinline__ Elements quantise16(u32x4 a, u32x4 b) {
 }
 
 // As kv_append, quantised: a thread has 16 values of a token's keys and of its values.
+constexpr int kAppendTokens = 4;  // of a workgroup
 template <int FMT, bool F16>
 __global__ __launch_bounds__(kWideThreads) void kv_append_mx(KvState s, int layer, const uint16_t *k, const uint16_t *v,
                                                             int64_t k_stride, int64_t v_stride, int n) {
-  const int chunks = s.kv_heads * s.head_dim / 16;  // of a token, an even number
-  const int64_t total = (int64_t)n * chunks;
+  const int chunks = s.kv_heads * s.head_dim / 16;  // of a token, an even number: both halves of a block run together
   const int64_t cells = (int64_t)s.pages * s.page_size, plane = (int64_t)layer * s.pages;
-  // (Both halves of a block run together: total and the grid's threads are even.)
-  for (int64_t u = (int64_t)blockIdx.x * kWideThreads + threadIdx.x; u < total; u += (int64_t)gridDim.x * kWideThreads) {
-    const int token = (int)(u / chunks), c = (int)(u % chunks) * 16;
+  for (int u = threadIdx.x; u < kAppendTokens * chunks; u += kWideThreads) {
+    const int nth = u / chunks, c = (u - nth * chunks) * 16, token = blockIdx.x * kAppendTokens + nth;
+    if (token >= n) continue;
     const int64_t slot = s.slots[token];
     if (slot < 0 || slot >= cells) continue;
     const int head = c / s.head_dim, d = c % s.head_dim;
-    const int64_t page = slot / s.page_size;
-    const int row = (int)(slot % s.page_size);
+    const int page = (int)slot / s.page_size, row = (int)slot - page * s.page_size;  // (slot < 2^30)
     const int64_t at = (plane + page) * s.kv_heads + head;
     const int64_t to = (at * s.page_size + row) * mx::row_bytes<FMT>(s.head_dim) + mx::row_bytes<FMT>(d);
     const int64_t scale_to = (at * (s.head_dim / mx::kBlock) + d / mx::kBlock) * s.page_size + row;
@@ -348,17 +347,17 @@ __global__ __launch_bounds__(kWideThreads) void kv_append_mx(KvState s, int laye
 
 // Tokens of rows of the cache, read back side by side: row rows[i]'s go to the rows of
 // k and v from starts[i] on.  A workgroup takes kGatherTokens of those; one thread each
-// finds where its token lies, and then all copy 16 values at a time.
-constexpr int kGatherTokens = 16;
+// finds where its token lies, and then all copy 8 values at a time.
+constexpr int kGatherTokens = 8;
 template <int FMT, bool F16>
 __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, const int32_t *rows, const int32_t *starts,
                                                          int n, uint16_t *k, uint16_t *v, int64_t k_stride,
                                                          int64_t v_stride, int tokens) {
-  __shared__ int64_t slots[kGatherTokens];
+  __shared__ int slots[kGatherTokens];  // below 2^30
   const int first = blockIdx.x * kGatherTokens;
   if (threadIdx.x < kGatherTokens) {
     const int t = first + threadIdx.x;
-    int64_t slot = -1;
+    int slot = -1;
     if (t < tokens && t >= starts[0] && t < starts[n]) {
       int lo = 0, hi = n - 1;  // starts[lo] <= t < starts[hi + 1] throughout
       while (lo < hi) {
@@ -376,7 +375,7 @@ __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, 
         } else if (j < len) {
           const int p = s.tables[(int64_t)row * s.max_pages + j / s.page_size];
           if (p < 0 || p >= s.pages) atomicOr(s.status, KV_STATUS_BAD_STATE);
-          else slot = (int64_t)p * s.page_size + j % s.page_size;
+          else slot = p * s.page_size + j % s.page_size;
         }
       }
     }
@@ -387,46 +386,36 @@ __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, 
     for (int i = threadIdx.x; i <= n; i += kWideThreads)
       if (starts[i] < (i ? starts[i - 1] : 0) || starts[i] > tokens) atomicOr(s.status, KV_STATUS_BAD_COUNT);
   __syncthreads();
-  const int chunks = s.kv_heads * s.head_dim / 16;
+  const int chunks = s.kv_heads * s.head_dim / 8;
   const int64_t plane = (int64_t)layer * s.pages;
+#pragma unroll 2
   for (int u = threadIdx.x; u < chunks * kGatherTokens; u += kWideThreads) {
-    const int nth = u / chunks, c = u % chunks * 16;
-    const int64_t slot = slots[nth];
+    const int nth = u / chunks, c = (u - nth * chunks) * 8;
+    const int slot = slots[nth];
     if (slot < 0) continue;
-    const int head = c / s.head_dim, d = c % s.head_dim;
-    const int64_t page = slot / s.page_size, at = (plane + page) * s.kv_heads + head;
-    const int row = (int)(slot % s.page_size);
+    const int head = c / s.head_dim, d = c - head * s.head_dim;
+    const int page = slot / s.page_size, row = slot - page * s.page_size;
+    const int64_t at = (plane + page) * s.kv_heads + head;
     const int64_t from = (at * s.page_size + row) * mx::row_bytes<FMT>(s.head_dim) + mx::row_bytes<FMT>(d);
     const uint8_t *const kp = (const uint8_t *)s.k + from, *const vp = (const uint8_t *)s.v + from;
-    u32x4 *const ko = (u32x4 *)(k + (int64_t)(first + nth) * k_stride + c);
-    u32x4 *const vo = (u32x4 *)(v + (int64_t)(first + nth) * v_stride + c);
-    u32x4 x[4];
+    u32x4 x, y;
     if constexpr (FMT == 0) {
-      x[0] = ((const u32x4 *)kp)[0];
-      x[1] = ((const u32x4 *)kp)[1];
-      x[2] = ((const u32x4 *)vp)[0];
-      x[3] = ((const u32x4 *)vp)[1];
+      x = *(const u32x4 *)kp;
+      y = *(const u32x4 *)vp;
     } else {
       const int64_t scale_at = (at * (s.head_dim / mx::kBlock) + d / mx::kBlock) * s.page_size + row;
       const float ks = mx::scale_of(s.k_scales[scale_at]), vs = mx::scale_of(s.v_scales[scale_at]);
       if constexpr (FMT == mx::kFp8) {
-        const u32x4 kw = *(const u32x4 *)kp, vw = *(const u32x4 *)vp;
-        x[0] = mx::decode8<FMT, F16>(kw[0], kw[1], ks);
-        x[1] = mx::decode8<FMT, F16>(kw[2], kw[3], ks);
-        x[2] = mx::decode8<FMT, F16>(vw[0], vw[1], vs);
-        x[3] = mx::decode8<FMT, F16>(vw[2], vw[3], vs);
-      } else {
         const u32x2 kw = *(const u32x2 *)kp, vw = *(const u32x2 *)vp;
-        x[0] = mx::decode8<FMT, F16>(kw[0], 0u, ks);
-        x[1] = mx::decode8<FMT, F16>(kw[1], 0u, ks);
-        x[2] = mx::decode8<FMT, F16>(vw[0], 0u, vs);
-        x[3] = mx::decode8<FMT, F16>(vw[1], 0u, vs);
+        x = mx::decode8<FMT, F16>(kw[0], kw[1], ks);
+        y = mx::decode8<FMT, F16>(vw[0], vw[1], vs);
+      } else {
+        x = mx::decode8<FMT, F16>(*(const uint32_t *)kp, 0u, ks);
+        y = mx::decode8<FMT, F16>(*(const uint32_t *)vp, 0u, vs);
       }
     }
-    ko[0] = x[0];
-    ko[1] = x[1];
-    vo[0] = x[2];
-    vo[1] = x[3];
+    *(u32x4 *)(k + (int64_t)(first + nth) * k_stride + c) = x;
+    *(u32x4 *)(v + (int64_t)(first + nth) * v_stride + c) = y;
   }
 }
 
@@ -621,11 +610,11 @@ hipError_t launch_kv_reserve(const KvState &s, const int32_t *counts, int stride
 
 hipError_t launch_kv_append(const KvState &s, int layer, const uint16_t *k, const uint16_t *v, int64_t k_stride,
                             int64_t v_stride, int n, hipStream_t st) {
-  const int64_t total = (int64_t)n * (s.kv_heads * s.head_dim / (s.storage ? 16 : 8));
-  const int64_t want = (total + kWideThreads - 1) / kWideThreads;
+  const int64_t total = (int64_t)n * (s.kv_heads * s.head_dim / 8);
+  const int64_t want = s.storage ? (n + kAppendTokens - 1) / kAppendTokens : (total + kWideThreads - 1) / kWideThreads;
   auto launch = [&](auto *kernel) {
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(want < 65536 ? want : 65536)), dim3(kWideThreads), 0, st, s, layer, k, v,
-                       k_stride, v_stride, n);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(s.storage || want < 65536 ? want : 65536)), dim3(kWideThreads), 0, st, s, layer,
+                       k, v, k_stride, v_stride, n);
   };
   if (s.storage == KV_STORAGE_MXFP8) launch(s.f16 ? kv_append_mx<mx::kFp8, true> : kv_append_mx<mx::kFp8, false>);
   else if (s.storage == KV_STORAGE_MXFP4) launch(s.f16 ? kv_append_mx<mx::kFp4, true> : kv_append_mx<mx::kFp4, false>);

@@ -2,10 +2,12 @@
 // with the keys and values written to a cache (include/qk_mi355x.h has the formulas).
 //
 // Every byte is read and written once, so HBM bounds it; per element there are a few
-// operations.  A workgroup has one token: its first wave computes the token's R/2 sines
-// and cosines into LDS (the angle in 64 bits, in turns, so that far positions lose
-// nothing, then half turns in fp32), and a head row is the work of D/8 lanes, 16 bytes
-// each on either side.  Rows are independent: no barrier but the one for the angles.
+// operations.  A wave has one token, or some of its heads: each lane computes one of the
+// R/2 angles (in 64 bits, in turns, so that far positions lose nothing, then half turns
+// in fp32), and takes from LDS the cosines and sines that its eight elements of every row
+// meet.  A row is the work of D/8 lanes, 16 bytes each on either side; the sum of squares and
+// the elements R/2 further come by lane exchanges within vector instructions.  No
+// workgroup's waves wait for each other.
 #include "common.h"
 #include "gqa_dev.h"
 #include "mx_dev.h"
@@ -16,23 +18,36 @@ namespace moe {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
 
-// How a lane finds the partner of an element: kHalves, R/2 dims away in whole groups of
-// eight; kNeighbours, in the lane; kAny, R/2 dims away.
-constexpr int kHalves = 0, kNeighbours = 1, kAny = 2;
+// How a lane finds the partners of its elements: kNeighbours, in the lane; 1, 2, 4 or 8, so
+// many lanes on (R/2 = 8 times that); kAny, R/2 elements on, through LDS.
+constexpr int kNeighbours = 0, kAny = 16;
 
 __device__ __forceinline__ void angle(int position, float freq, float *c, float *s) {
   const double turns = (double)position * (double)freq * 0.15915494309189533577;
   sincospif(2.f * (float)(turns - rint(turns)), s, c);
 }
 
-// Sum over the D/8 lanes of a row, the same on each.
+template <int CTRL, int BANKS = 0xf>
+__device__ __forceinline__ float dpp(float old, float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(x), CTRL, 0xf, BANKS, false));
+}
+// The value of lane l ^ N of a row of sixteen lanes.
+template <int N>
+__device__ __forceinline__ float partner(float x) {
+  if constexpr (N == 1) return dpp<0xb1>(x, x);        // quad_perm 1 0 3 2
+  else if constexpr (N == 2) return dpp<0x4e>(x, x);   // quad_perm 2 3 0 1
+  else if constexpr (N == 4) return dpp<0x114, 0xa>(dpp<0x104, 0x5>(x, x), x);  // row_shl:4, row_shr:4
+  else return dpp<0x128>(x, x);                        // row_ror:8
+}
+// Sum over the D/8 lanes of a row, in the same order on each.
 template <int D>
 __device__ __forceinline__ float row_sum(float x) {
-#pragma unroll
-  for (int o = 1; o < D / 8; o *= 2) x += __shfl_xor(x, o, kWave);
-  return x;
+  if constexpr (D == 128) x += dpp<0x140>(x, x);  // row_mirror: lane 15 - l
+  x += dpp<0x141>(x, x);                          // row_half_mirror: 7 - l
+  x += partner<1>(x);
+  return x + partner<2>(x);
 }
 
 // Eight values of a lane, a quarter of a block, to a cache row under the block's scale.
@@ -50,113 +65,135 @@ __device__ __forceinline__ void put8(uint8_t *to, uint8_t *scale_to, const float
   if (first) *scale_to = (uint8_t)byte;
 }
 
-// FMT: how the cache holds its rows (0: 16 bits, or no cache).
+// FMT: how the cache holds its rows (0: 16 bits, or no cache).  A token's rows of kRows heads
+// are `passes` of them; `parts` waves have a token, `each` passes of them one.
 template <int D, bool F16, int PAIRS, int FMT>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope(QkArgs a, int passes) {
-  constexpr int kLanes = D / 8, kRows = kThreads / kLanes;  // lanes of a row, rows at a time
-  __shared__ __attribute__((aligned(16))) float cosines[D / 2], sines[D / 2];
-  __shared__ __attribute__((aligned(16))) float turned[PAIRS == kNeighbours ? 1 : kRows][D];
-  const int t = blockIdx.x, c = threadIdx.x % kLanes, mine = threadIdx.x / kLanes;
+__global__ __launch_bounds__(kThreads) void qk_norm_rope(QkArgs a, int parts, int each) {
+  constexpr int kLanes = D / 8, kRows = kWave / kLanes;  // lanes of a row, rows at a time
+  __shared__ __attribute__((aligned(16))) float turn[kWaves][2][kWave];
+  __shared__ __attribute__((aligned(16))) float lds_rows[kWaves][PAIRS == kAny ? kRows : 1][PAIRS == kAny ? D : 4];
+  const int lane = threadIdx.x & 63, wave = gqa::sgpr(threadIdx.x >> 6), c = lane % kLanes, nth = lane / kLanes;
+  const int64_t unit = (int64_t)blockIdx.x * kWaves + wave;
+  const int t = gqa::sgpr((int)(unit / parts)), part = gqa::sgpr((int)(unit - (int64_t)t * parts));
+  if (t >= a.N) return;
   const int half = a.R / 2, rows = a.Hq + a.Hkv + (a.cached ? a.Hkv : 0);
-  const int from = blockIdx.y * passes * kRows;
-  int64_t slot = -1;
+  const int from = part * each * kRows, to = min(rows, from + each * kRows);
+  const uint16_t *const qp = a.q + t * a.q_stride, *const kp = a.k + t * a.k_stride, *const vp = a.v + t * a.v_stride;
+  // The lane's elements of the row h, which is a query's, a key's or a value's.
+  auto load = [&](int h) __attribute__((always_inline)) {
+    u32x4 x = {0u, 0u, 0u, 0u};
+    if (h < to) {
+      const uint16_t *const p = h < a.Hq ? qp + (int64_t)h * D : h < a.Hq + a.Hkv ? kp + (int64_t)(h - a.Hq) * D
+                                                                                : vp + (int64_t)(h - a.Hq - a.Hkv) * D;
+      x = *(const u32x4 *)(p + 8 * c);
+    }
+    return x;
+  };
+  u32x4 next = load(from + nth);
+  // The token's page and row there; -1: none.  (A cache has at most 2^30 places.)
+  int page = -1, page_row = 0;
   if (a.cached) {
-    slot = a.cache.slots[t];
-    if (slot >= (int64_t)a.cache.pages * a.cache.page_size) slot = -1;
+    const int64_t slot = a.cache.slots[t];
+    const bool in = slot >= 0 && slot < (int64_t)a.cache.pages * a.cache.page_size;
+    const int place = gqa::sgpr(in ? (int)slot : -1);
+    page = place < 0 ? -1 : place / a.cache.page_size;
+    page_row = place - page * a.cache.page_size;
   }
-  if ((int)threadIdx.x < half) angle(a.positions[t], a.inv_freq[threadIdx.x], cosines + threadIdx.x, sines + threadIdx.x);
-  __syncthreads();
-  for (int pass = 0; pass < passes; ++pass) {
-    const int h = from + pass * kRows + mine;
-    // Lanes without a row go along: rows are whole groups of lanes, and the others of a
-    // wave shuffle with them.
-    const bool live = h < rows, query = h < a.Hq, key = !query && h < a.Hq + a.Hkv;
-    const int head = query ? h : key ? h - a.Hq : h - a.Hq - a.Hkv;
-    const uint16_t *const x = (query ? a.q + t * a.q_stride : key ? a.k + t * a.k_stride : a.v + t * a.v_stride);
-    u32x4 raw = {0u, 0u, 0u, 0u};
-    if (live) raw = *(const u32x4 *)(x + (int64_t)head * D + 8 * c);
+  float wq[8], wk[8];
+  auto weights = [&](const void *w, float (&x)[8]) __attribute__((always_inline)) {
+    if (!w) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = 1.f;
+    } else if (a.weights_fp32) {
+      const f32x4 lo = ((const f32x4 *)w)[2 * c], hi = ((const f32x4 *)w)[2 * c + 1];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = i < 4 ? lo[i] : hi[i - 4];
+    } else {
+      const u32x4 r = ((const u32x4 *)w)[c];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = gqa::to_f32<F16>(i & 1 ? r[i / 2] >> 16 : r[i / 2] & 0xffffu);
+    }
+  };
+  weights(a.q_weight, wq);
+  weights(a.k_weight, wk);
+  if (lane < half) angle(a.positions[t], a.inv_freq[lane], &turn[wave][0][lane], &turn[wave][1][lane]);
+  __builtin_amdgcn_wave_barrier();  // a wave's LDS operations are in order
+  // Of element 8 c + i: the cosine, the sine with its sign, and where its partner lies.
+  // Neighbours: of the pair 4 c + i.
+  float cs[8], sn[8];
+#pragma unroll
+  for (int i = 0; i < (PAIRS == kNeighbours ? 4 : 8); ++i) {
+    const int d = 8 * c + i, p = PAIRS == kNeighbours ? 4 * c + i : d < half ? d : d - half;
+    cs[i] = turn[wave][0][min(p, half - 1)];
+    sn[i] = turn[wave][1][min(p, half - 1)];
+    if (PAIRS != kNeighbours && d < half) sn[i] = -sn[i];
+  }
+  for (int h0 = from; h0 < to; h0 += kRows) {
+    const int h = h0 + nth;
+    const u32x4 raw = next;
+    next = load(h + kRows);
+    // Lanes without a row go along: the others of the wave exchange with them.
+    const bool live = h < to, query = h < a.Hq, key = !query && h < a.Hq + a.Hkv;
     float y[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       y[2 * i] = gqa::to_f32<F16>(raw[i] & 0xffffu);
       y[2 * i + 1] = gqa::to_f32<F16>(raw[i] >> 16);
     }
-    const void *const weight = query ? a.q_weight : key ? a.k_weight : nullptr;
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(y[i], y[i], sum);
     sum = row_sum<D>(sum);
-    if (weight) {
-      const float scale = 1.0f / sqrtf(sum * (1.0f / D) + a.eps);
-      float w[8];
-      if (a.weights_fp32) {
-        const f32x4 w0 = ((const f32x4 *)weight)[2 * c], w1 = ((const f32x4 *)weight)[2 * c + 1];
+    if (query ? a.q_weight != nullptr : key && a.k_weight != nullptr) {
+      const float scale = rsqrtf(sum * (1.0f / D) + a.eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = i < 4 ? w0[i] : w1[i - 4];
-      } else {
-        const u32x4 wr = ((const u32x4 *)weight)[c];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = gqa::to_f32<F16>(i & 1 ? wr[i / 2] >> 16 : wr[i / 2] & 0xffffu);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * scale * w[i];
+      for (int i = 0; i < 8; ++i) y[i] = y[i] * scale * (query ? wq[i] : wk[i]);
     }
     if constexpr (PAIRS == kNeighbours) {
       if (query || key) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int p = 4 * c + i;
-          if (p >= half) continue;
-          const float cs = cosines[p], sn = sines[p], l = y[2 * i], u = y[2 * i + 1];
-          y[2 * i] = l * cs - u * sn;
-          y[2 * i + 1] = u * cs + l * sn;
+          const float l = y[2 * i], u = y[2 * i + 1];
+          const bool turns = 4 * c + i < half;
+          y[2 * i] = turns ? l * cs[i] - u * sn[i] : l;
+          y[2 * i + 1] = turns ? u * cs[i] + l * sn[i] : u;
         }
       }
-    } else {
-      // The row's lanes are in one wave and in step: what they write they can read.
-      float *const row = turned[mine];
+    } else if constexpr (PAIRS == kAny) {
+      float *const row = lds_rows[wave][nth];
 #pragma unroll
       for (int i = 0; i < 8; ++i) row[8 * c + i] = y[i];
       __builtin_amdgcn_wave_barrier();
       if (query || key) {
-        if constexpr (PAIRS == kHalves) {
-          if (8 * c < a.R) {
-            const bool low = 8 * c < half;
-            const int p = low ? 8 * c : 8 * c - half, other = low ? 8 * c + half : p;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float cs = cosines[p + i], sn = sines[p + i], z = row[other + i];
-              y[i] = low ? y[i] * cs - z * sn : y[i] * cs + z * sn;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int d = 8 * c + i;
-            if (d >= a.R) continue;
-            const bool low = d < half;
-            const int p = low ? d : d - half;
-            const float z = row[low ? d + half : p];
-            y[i] = low ? y[i] * cosines[p] - z * sines[p] : y[i] * cosines[p] + z * sines[p];
-          }
+        for (int i = 0; i < 8; ++i) {
+          const int d = 8 * c + i;
+          if (d < a.R) y[i] = y[i] * cs[i] + row[d < half ? d + half : d - half] * sn[i];
         }
       }
-      __builtin_amdgcn_wave_barrier();  // read before the next pass writes
+      __builtin_amdgcn_wave_barrier();  // read before the next rows are written
+    } else {
+      float z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] = partner<PAIRS>(y[i]);
+      if ((query || key) && c < 2 * PAIRS) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * cs[i] + z[i] * sn[i];
+      }
     }
     const u32x4 out = {gqa::pack2<F16>(y[0], y[1]), gqa::pack2<F16>(y[2], y[3]), gqa::pack2<F16>(y[4], y[5]),
                        gqa::pack2<F16>(y[6], y[7])};
-    if (live && query) *(u32x4 *)(a.q_out + ((int64_t)t * a.Hq + head) * D + 8 * c) = out;
-    if (live && key && a.k_out) *(u32x4 *)(a.k_out + ((int64_t)t * a.Hkv + head) * D + 8 * c) = out;
-    if (live && !query && slot >= 0) {
+    if (live && query) *(u32x4 *)(a.q_out + ((int64_t)t * a.Hq + h) * D + 8 * c) = out;
+    if (live && key && a.k_out) *(u32x4 *)(a.k_out + ((int64_t)t * a.Hkv + h - a.Hq) * D + 8 * c) = out;
+    if (live && !query && page >= 0) {
       const KvState &s = a.cache;
-      const int64_t at = ((int64_t)a.layer * s.pages + slot / s.page_size) * a.Hkv + head;
-      const int row = (int)(slot % s.page_size);
-      uint8_t *const to = (uint8_t *)(key ? s.k : s.v) + (at * s.page_size + row) * mx::row_bytes<FMT>(D) + mx::row_bytes<FMT>(8 * c);
+      const int64_t at = ((int64_t)a.layer * s.pages + page) * a.Hkv + (key ? h - a.Hq : h - a.Hq - a.Hkv);
+      uint8_t *const to_row = (uint8_t *)(key ? s.k : s.v) + (at * s.page_size + page_row) * mx::row_bytes<FMT>(D) + mx::row_bytes<FMT>(8 * c);
       if constexpr (FMT == 0)
         // Values are copied: their bits stay, a NaN's too.
-        *(u32x4 *)to = key ? out : raw;
+        *(u32x4 *)to_row = key ? out : raw;
       else
-        put8<FMT, F16>(to, (key ? s.k_scales : s.v_scales) + (at * (D / mx::kBlock) + c / 4) * s.page_size + row, y,
+        put8<FMT, F16>(to_row, (key ? s.k_scales : s.v_scales) + (at * (D / mx::kBlock) + c / 4) * s.page_size + page_row, y,
                        c % 4 == 0);
     }
   }
@@ -164,15 +201,23 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope(QkArgs a, int passes) {
 
 template <int D, bool F16, int FMT>
 hipError_t launch(const QkArgs &a, int cus, hipStream_t s) {
-  constexpr int kRows = kThreads / (D / 8);
-  const int rows = a.Hq + a.Hkv + (a.cached ? a.Hkv : 0), all = (rows + kRows - 1) / kRows;
-  // A workgroup for every pass where those have a place on the chip at once (eight a CU),
-  // else one for all of a token's, which computes its angles once.
-  const int passes = (int64_t)a.N * all <= 8 * cus ? 1 : all;
-  const dim3 grid(a.N, (all + passes - 1) / passes);
-  if (a.interleaved) hipLaunchKernelGGL((qk_norm_rope<D, F16, kNeighbours, FMT>), grid, dim3(kThreads), 0, s, a, passes);
-  else if (a.R % 16 == 0) hipLaunchKernelGGL((qk_norm_rope<D, F16, kHalves, FMT>), grid, dim3(kThreads), 0, s, a, passes);
-  else hipLaunchKernelGGL((qk_norm_rope<D, F16, kAny, FMT>), grid, dim3(kThreads), 0, s, a, passes);
+  constexpr int kRows = kWave / (D / 8);
+  const int rows = a.Hq + a.Hkv + (a.cached ? a.Hkv : 0), passes = (rows + kRows - 1) / kRows;
+  // A token's passes are shared out over waves, each of which computes its angles: while all
+  // waves run at once (24 a CU; 1000 tokens of 32 + 8 heads of 128: 6.8 us, 8.0 with three times as
+  // many), and in two where they do not any more (8191 tokens: 38.6, in one 42.2, in five 40.3).
+  const int64_t places = 20 * (int64_t)cus;
+  const int most = a.N > places ? 2 : (int)(places / a.N), each = (passes + most - 1) / most;
+  const int parts = (passes + each - 1) / each;
+  const uint32_t grid = (uint32_t)(((int64_t)a.N * parts + kWaves - 1) / kWaves);
+  auto go = [&](auto *kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0, s, a, parts, each); };
+  const int lanes = a.R / 16;
+  if (a.interleaved) go(qk_norm_rope<D, F16, kNeighbours, FMT>);
+  else if (a.R % 16 || (lanes & (lanes - 1))) go(qk_norm_rope<D, F16, kAny, FMT>);
+  else if (lanes == 1) go(qk_norm_rope<D, F16, 1, FMT>);
+  else if (lanes == 2) go(qk_norm_rope<D, F16, 2, FMT>);
+  else if (lanes == 4) go(qk_norm_rope<D, F16, 4, FMT>);
+  else go(qk_norm_rope<D, F16, D == 128 ? 8 : 4, FMT>);
   return hipGetLastError();
 }
 
