@@ -35,10 +35,9 @@ namespace {
 constexpr int kBlock = 16;   // keys that lie in one page
 constexpr int kRows = 16;    // query rows of an MFMA
 constexpr int kWindow = 4;   // sequences per lane whose lengths a wave holds
-#ifndef KG
-#define KG 2
-#endif
-constexpr int kGroups = KG;
+// Workgroups of four waves per CU: 256 registers a lane.  (With three, 168, some spill: one
+// sequence of 131072 keys, four bits, 44.3 us, with two 37.4.)
+constexpr int kGroups = 2;
 
 // 16-key blocks of a step: a step is 64 bytes of K and of V per lane.
 template <int D, int FMT> constexpr int kBlocks = 2 * 128 / mx::row_bytes<FMT>(D);
@@ -86,14 +85,17 @@ struct Segment {
 };
 // Places of a pair in the list besides its steps: what its start and end cost, in steps
 // of a wave.
-#ifndef KOVER
-#define KOVER 6
-#endif
-constexpr int kOverhead = KOVER;
+// (64 sequences of 1 to 7787 keys, eight bits: with 2 34.6 us, 6 25.7, 12 26.6; without, 78.)
+constexpr int kOverhead = 6;
 
-// Steps a wave of a workgroup with a whole (sequence, head) may have, by those that the
-// list would give it.
-__host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 20 ? 16 : (int)listed / 2 + 6; }
+// Steps that a wave of a workgroup with a whole (sequence, head) may have, by those that the
+// list would give it.  A team has one launch and nothing to join, but all of its sequence.
+// By teams and by the list, 8 KV heads of 128, eight bits: one sequence of 128 keys 5.4,
+// 10.9 us; of 700 9.2, 11.2; of 1500 13.8, 11.7; of 2048 16.6, 12.0; 16 of 512 8.4, 13.8; of 2048
+// 17.7, 20.8; of 4096 36.0, 35.7; 64 of 700 20.4, 22.5; of 2048 52.9, 55.2; 256 of 1 to 1024 28.2,
+// 34.3.  Four bits (steps of 64 keys): one of 1500 10.6, 11.9; of 2048 12.6, 12.4; 16 of 2048
+// 14.7, 18.5; of 4096 23.5, 23.9.
+__host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 8 ? 17 : 2 * (int)listed + 2; }
 
 // LISTED: ranges of the list; otherwise a (sequence, head block) per workgroup.  TEAM
 // waves.
