@@ -263,47 +263,48 @@ __device__ __forceinline__ void prefix(const GqaPagedArgs &p, const Plan &plan, 
     // ---- loads ----
     const int32_t *const table = p.tables + (int64_t)source * p.table_stride;
     const uint16_t *const k_head = p.k + kvh * p.k_head, *const v_head = p.v + kvh * p.v_head;
-    // The next stage's blocks: place in the table, block there, page, which is loaded a stage
-    // ahead, and whether it is within the keys.
-    int at[2], in[2], page[2], loaded = 0;
-    auto find = [&]() __attribute__((always_inline)) {
+    // Pages and rows of the unit's next 128 blocks of 16 keys, from `base` on: lane l has blocks
+    // l and 64 + l; a block that is not there: row -1.  (Scalar loads stage by stage made every
+    // wait for operands from LDS wait for them too.)
+    int base = 2 * s0, pages[2], rows_at[2], loaded = 0;
+    auto look_up = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        page[i] = (2 * (s0 + loaded) + i) * kBlock < keys ? uniform_load(table + at[i]) : 0x7fffffff;
+      for (int i = 0; i < 2; ++i) {
+        const int blk = base + kWave * i + lane, at = blk / per_page;
+        const bool in = blk * kBlock < keys && blk < 2 * (s0 + stages);
+        const int page = in ? table[at] : 0;
+        const bool ok = (uint32_t)page < (uint32_t)p.P;
+        bad_page |= in && !ok;
+        pages[i] = ok ? page : 0;
+        rows_at[i] = in && ok ? (blk - at * per_page) * kBlock : -1;
+      }
     };
-    at[0] = 2 * s0 / per_page;
-    in[0] = 2 * s0 - at[0] * per_page;
-    at[1] = in[0] + 1 == per_page ? at[0] + 1 : at[0];
-    in[1] = in[0] + 1 == per_page ? 0 : in[0] + 1;
-    find();
+    look_up();
     // Blocks of the stages in flight that are there, two bits each, the last loaded lowest.
     uint32_t there = 0, load_slot = lds0 + wave * kLoads * 1024;
     auto issue = [&]() __attribute__((always_inline)) {
-      uint32_t bits = 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        bits |= (uint32_t)page[i] < (uint32_t)p.P ? 1u << i : 0u;
-        bad_page |= (uint32_t)page[i] >= (uint32_t)p.P && (2 * (s0 + loaded) + i) * kBlock < keys;
+      int at = 2 * (s0 + loaded) - base;
+      if (at == 2 * kWave) {
+        base += at;
+        at = 0;
+        look_up();
       }
-      there = there << 2 | bits;
-      const bool mine = bits >> block & 1u;
-      const int64_t my_page = mine ? (block ? page[1] : page[0]) : 0, my_row = (block ? in[1] : in[0]) * kBlock;
+      int row[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        row[i] = at < kWave ? __builtin_amdgcn_readlane(rows_at[0], at + i) : __builtin_amdgcn_readlane(rows_at[1], at + i - kWave);
+      const int my_page = at < kWave ? __builtin_amdgcn_readlane(pages[0], at + block)
+                                     : __builtin_amdgcn_readlane(pages[1], at + block - kWave);
+      const int my_row = block ? row[1] : row[0];
+      there = there << 2 | (row[0] >= 0 ? 1u : 0u) | (row[1] >= 0 ? 2u : 0u);
+      const bool mine = my_row >= 0;
+      const int64_t from_row = mine ? my_row : 0;
       const uint32_t slot = sgpr((int)load_slot);
-      load_lds(buffer_words(k_head + my_page * p.k_page + my_row * p.k_row, mine ? k_bytes : 0u), slot, k_off);
-      load_lds(buffer_words(v_head + my_page * p.v_page + my_row * p.v_row, mine ? v_bytes : 0u), slot + kTile<D>, v_off);
+      load_lds(buffer_words(k_head + my_page * p.k_page + from_row * p.k_row, mine ? k_bytes : 0u), slot, k_off);
+      load_lds(buffer_words(v_head + my_page * p.v_page + from_row * p.v_row, mine ? v_bytes : 0u), slot + kTile<D>, v_off);
       load_slot = load_slot + 2 * kTile<D> >= lds0 + kRing * 2 * kTile<D> ? load_slot - (kRing - 1) * 2 * kTile<D>
                                                                           : load_slot + 2 * kTile<D>;
       ++loaded;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {  // a stage on: two blocks, a page has one at least
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (++in[i] == per_page) {
-            in[i] = 0;
-            ++at[i];
-          }
-      }
-      find();
     };
     // In step st of the loop: stage st + 2 is there for every wave, and every wave is
     // done with stage st - 1, whose slot takes the next one.
@@ -490,7 +491,7 @@ __device__ __forceinline__ void prefix(const GqaPagedArgs &p, const Plan &plan, 
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   }
-  if (bad_page && threadIdx.x == 0) atomicOr(p.status, GQA_STATUS_BAD_PAGE);
+  if (__builtin_amdgcn_ballot_w64(bad_page) && threadIdx.x == 0) atomicOr(p.status, GQA_STATUS_BAD_PAGE);
 }
 
 }  // namespace shared
