@@ -47,6 +47,7 @@ extern "C" {
 #define KV_MAX_SEQUENCES 1024
 #define KV_MAX_PAGES (1 << 20)
 #define KV_MAX_TOKENS (1 << 20)
+#define KV_MAX_GATHER_TOKENS (1 << 26)
 
 typedef struct kv_cache_desc {
   int32_t pages, page_size, kv_heads, head_dim, layers;
@@ -105,8 +106,8 @@ int kv_cache_append(kv_cache *c, int32_t layer, const void *k, const void *v, in
  * fewer if the row is shorter, none if it is negative) read back from a layer to the rows
  * starts[i].. of k and v ([tokens, kv_heads, head_dim], strides as for append), in the
  * tokens' type.  starts: int32 [n + 1], ascending within [0, tokens] (else a status, and
- * some rows may be left out).  Other rows of k and v are left as they were.  k and v share
- * no memory with each other or the cache. */
+ * some rows may be left out); tokens <= KV_MAX_GATHER_TOKENS.  Other rows of k and v are
+ * left as they were.  k and v share no memory with each other or the cache. */
 int kv_cache_gather(kv_cache *c, int32_t layer, const int32_t *rows, const int32_t *starts, int32_t n, void *k, void *v,
                     int64_t k_stride, int64_t v_stride, int32_t tokens, void *stream);
 /* dst[i] becomes a second holder of the pages of src[i] (int32 [n], n <=

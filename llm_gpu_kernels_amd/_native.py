@@ -86,6 +86,7 @@ KV_STATUS_TOO_LONG, KV_STATUS_BAD_COUNT, KV_STATUS_BAD_STATE = 8, 16, 32
 KV_STORAGE_16BIT, KV_STORAGE_MXFP8, KV_STORAGE_MXFP4 = 0, 1, 2
 KV_TOKENS_BF16, KV_TOKENS_FP16 = 0, 1
 KV_MAX_SEQUENCES, KV_MAX_PAGES, KV_MAX_TOKENS = 1024, 1 << 20, 1 << 20
+KV_MAX_GATHER_TOKENS = 1 << 26
 
 
 class KvCacheDesc(ctypes.Structure):

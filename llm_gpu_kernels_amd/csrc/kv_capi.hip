@@ -164,7 +164,8 @@ int kv_cache_gather(kv_cache *c, int32_t layer, const int32_t *rows, const int32
     return capi_fail(MOE_EINVAL, "layer must be in [0, %d) (got %d)", c->s.layers, layer);
   if (n < 0 || n > c->s.sequences)
     return capi_fail(MOE_EINVAL, "n must be in [0, sequences = %d] (got %d)", c->s.sequences, n);
-  if (tokens < 0) return capi_fail(MOE_EINVAL, "tokens must not be negative (got %d)", tokens);
+  if (tokens < 0 || tokens > KV_MAX_GATHER_TOKENS)
+    return capi_fail(MOE_EINVAL, "tokens must be in [0, %d] (got %d)", KV_MAX_GATHER_TOKENS, tokens);
   if (n == 0 || tokens == 0) return MOE_OK;
   if (!aligned(rows, 4) || !aligned(starts, 4)) return capi_fail(MOE_EINVAL, "rows and starts must be given");
   if (!aligned(k, 16) || !aligned(v, 16)) return capi_fail(MOE_EINVAL, "k/v must be non-null and 16-byte aligned");

@@ -164,15 +164,15 @@ class PagedKVCache:
         the rows ``starts[i]`` and up of ``k`` and ``v`` ([tokens, kv_heads, head_dim] of
         ``dtype``, the heads of a token side by side), as the keys and values of
         ``prepare_segmented_gqa`` or ``prepare_packed_gqa`` lie.  ``starts``: int32
-        [n + 1], ascending within [0, tokens].  Other rows of k and v keep what they
-        held; k and v share no memory."""
+        [n + 1], ascending within [0, tokens], tokens at most 2^26.  Other rows of k and v
+        keep what they held; k and v share no memory."""
         if not isinstance(layer, int) or not 0 <= layer < self.layers:
             raise ValueError(f"layer must be an int in [0, {self.layers}) (got {layer!r})")
         rows = self._rows(rows, "rows")
         _check_int32(starts, "starts", (rows.shape[0] + 1,), self.device)
         ks, vs = self._token_stride(k, "k"), self._token_stride(v, "v")
-        if k.shape[0] != v.shape[0] or k.shape[0] >= 2 ** 31:
-            raise ValueError("k and v must have the same number of tokens, below 2^31")
+        if k.shape[0] != v.shape[0] or k.shape[0] > N.KV_MAX_GATHER_TOKENS:
+            raise ValueError(f"k and v must have the same number of tokens, at most {N.KV_MAX_GATHER_TOKENS}")
         N.check(N.lib().kv_cache_gather(self._cache, layer, rows.data_ptr(), starts.data_ptr(), rows.shape[0], k.data_ptr(),
                                         v.data_ptr(), ks, vs, k.shape[0], self._stream()), "gather")
 

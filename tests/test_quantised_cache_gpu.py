@@ -197,6 +197,19 @@ def test_gather_nothing(gpu_device):
     c.check_inputs()
 
 
+def test_gather_more_tokens_than_a_grid(gpu_device):
+    """Refused before anything is launched."""
+    c = _cache(gpu_device, "mxfp8")
+    k = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device=gpu_device)
+    rows, starts, many = _i32([0], gpu_device), _i32([0, 1], gpu_device), N.KV_MAX_GATHER_TOKENS + 1
+    with pytest.raises(ValueError, match="tokens"):
+        c.gather(0, rows, starts, k.expand(many, 2, 64), k.expand(many, 2, 64))
+    for tokens in (many, 2 ** 31 - 1, -1):
+        assert N.lib().kv_cache_gather(c._cache, 0, rows.data_ptr(), starts.data_ptr(), 1, k.data_ptr(), k.data_ptr(), 128,
+                                       128, tokens, None) == N.MOE_EINVAL
+    c.check_inputs()
+
+
 @pytest.mark.parametrize("what,status", [("page", N.KV_STATUS_BAD_STATE), ("length", N.KV_STATUS_BAD_STATE),
                                          ("row", N.KV_STATUS_BAD_ROW), ("starts", N.KV_STATUS_BAD_COUNT),
                                          ("behind", N.KV_STATUS_BAD_COUNT), ("negative", N.KV_STATUS_BAD_COUNT)])
