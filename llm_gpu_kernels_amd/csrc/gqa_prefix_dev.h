@@ -70,7 +70,7 @@ __device__ __forceinline__ void share(Group *g, int wanted, int least, int live)
 // the four waves of the list's have a step each in flight, as the others have four stages.
 __device__ __forceinline__ int share_of(int64_t shared, int64_t listed, int workgroups) {
   if (shared == 0) return 0;
-  const int n = (int)((shared * workgroups + (shared + listed) / 2) / (shared + listed));
+  const int n = (int)((float)workgroups * ((float)shared / (float)(shared + listed)) + 0.5f);
   return max(1, min(n, listed ? workgroups - 1 : workgroups));
 }
 // Steps of a chunk: the fewest with which the units are not more than the workgroups, of
@@ -78,14 +78,14 @@ __device__ __forceinline__ int share_of(int64_t shared, int64_t listed, int work
 // that), the average, and a workgroup has several units.
 constexpr int kLeastSteps = 2;  // one costs more in states than it gains
 constexpr int kSizes = 16;
-__device__ __forceinline__ int chunk_size(int64_t shared, int n, int i) {
-  const int even = n ? max(kLeastSteps, (int)((shared + n - 1) / n)) : 1;
-  return even + (int)((int64_t)even * i / 8);
+__device__ __forceinline__ int chunk_size(int64_t shared, int n, int i) {  // shared < 2^30, checked on the host
+  const int even = n ? max(kLeastSteps, (int)(((uint32_t)shared + (uint32_t)n - 1u) / (uint32_t)n)) : 1;
+  return even + (int)((int64_t)even * i >> 3);
 }
 __device__ __forceinline__ void cut(Group *g, int size) {
-  const int steps = steps_of(g->keys);
-  g->chunks = (steps + size - 1) / size;
-  g->chunk_steps = g->chunks ? (steps + g->chunks - 1) / g->chunks : 1;
+  const uint32_t steps = (uint32_t)steps_of(g->keys), chunks = (steps + (uint32_t)size - 1u) / (uint32_t)size;
+  g->chunks = (int)chunks;
+  g->chunk_steps = chunks ? (int)((steps + chunks - 1u) / chunks) : 1;
 }
 
 // The plan by one workgroup of four waves for itself: up to 64 groups and 256 rows.  Bounds
@@ -110,11 +110,8 @@ __device__ __forceinline__ Plan plan_here(const GqaPagedArgs &p, uint8_t *smem) 
   __syncthreads();
   // (__syncthreads_or() has LDS of its own, and with it one workgroup per CU less.)
   if (tid <= G && (lds->starts[tid] < 0 || lds->starts[tid] > p.B || (tid > 0 && lds->starts[tid] < lds->starts[tid - 1]))) lds->wrong = 1;
-  __syncthreads();
-  const bool bad = lds->wrong != 0;
-  if (blockIdx.x == 0 && ((bad && tid == 0) || wanted < 0)) atomicOr(p.status, GQA_STATUS_BAD_BOUNDS);
-  int g = -1;  // the row's group
-  if (!bad && G > 0 && tid < p.B && tid >= lds->starts[0] && tid < lds->starts[G]) {
+  int g = -1;  // the row's group, if no bound is wrong
+  if (G > 0 && tid < p.B && tid >= lds->starts[0] && tid < lds->starts[G]) {
     int hi = G - 1;
     g = 0;
     while (g < hi) {
@@ -129,13 +126,16 @@ __device__ __forceinline__ Plan plan_here(const GqaPagedArgs &p, uint8_t *smem) 
     atomicAdd(lds->live + g, 1);
   }
   __syncthreads();
+  const bool bad = lds->wrong != 0;
+  if (bad) g = -1;
+  if (blockIdx.x == 0 && ((bad && tid == 0) || wanted < 0)) atomicOr(p.status, GQA_STATUS_BAD_BOUNDS);
   Plan plan = {};
   Group &mine = plan.group;  // every wave has all groups
   mine.before = 0x7fffffff;
   if (lane < G) {
     mine.first = bad ? 0 : lds->starts[lane];
     mine.rows = bad ? 0 : (lds->starts[lane + 1] - mine.first) * per_head;
-    share(&mine, wanted, lds->least[lane], lds->live[lane]);
+    share(&mine, wanted, lds->least[lane], bad ? 0 : lds->live[lane]);
     mine.source = mine.keys ? lds->source[lane] : 0;
     if (wave == 0) lds->keys[lane] = mine.keys;
   }
@@ -145,13 +145,20 @@ __device__ __forceinline__ Plan plan_here(const GqaPagedArgs &p, uint8_t *smem) 
   const int rest = wave_total(steps_of(len - skip));
   if (lane == 0) atomicAdd(&lds->rest, rest);
   const int heads_units = mine.tiles * p.Hkv;  // of a chunk
-  const int64_t shared = wave_total(steps_of(mine.keys) * heads_units);  // below 2^30, checked on the host
+  const int64_t shared = wave_total(steps_of(mine.keys) * heads_units);
   __syncthreads();
   plan.workgroups = share_of(shared, (int64_t)lds->rest * p.Hkv * ((per_head + 15) / 16), gridDim.x);
-  for (int i = wave; i < kSizes; i += kWaves) {
-    const int size = chunk_size(shared, plan.workgroups, i);
-    const int units = wave_total(heads_units * ((steps_of(mine.keys) + size - 1) / size));
-    if (lane == 0) lds->fits[i] = units <= plan.workgroups;
+  constexpr int kOwn = kSizes / kWaves;  // sizes of a wave
+  int units_of[kOwn];
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const int size = chunk_size(shared, plan.workgroups, kOwn * wave + i);
+    units_of[i] = heads_units * (int)(((uint32_t)steps_of(mine.keys) + (uint32_t)size - 1u) / (uint32_t)size);
+  }
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    units_of[i] = wave_total(units_of[i]);
+    if (lane == 0) lds->fits[kOwn * wave + i] = units_of[i] <= plan.workgroups;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) plan.skips[i] = lds->skips[kWave * i + lane];
