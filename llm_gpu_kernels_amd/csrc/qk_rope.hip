@@ -8,6 +8,11 @@
 // meet.  A row is the work of D/8 lanes, 16 bytes each on either side; the sum of squares and
 // the elements R/2 further come by lane exchanges within vector instructions.  No
 // workgroup's waves wait for each other.
+//
+// Measured, a copy of 2 GiB running at 5.1 TB/s: 8191 tokens of 32 + 8 heads of 128 (168 MB)
+// 38.8 us, 4.3 TB/s (a workgroup per token, its rows in LDS: 51); 2500 of 12 + 4 heads of 64
+// with their cache in eight bits 7.3; 16 tokens 3.6, the launch, a load and a chain of some
+// hundred instructions.
 #include "common.h"
 #include "gqa_dev.h"
 #include "mx_dev.h"
