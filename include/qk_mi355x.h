@@ -23,6 +23,8 @@ extern "C" {
  *   out = y, but for i < R/2, with the angle a = positions[t] inv_freq[i],
  *     (out_l, out_h) = (y_l cos a - y_h sin a, y_h cos a + y_l sin a),
  *     (l, h) = (i, i + R/2), or (2 i, 2 i + 1) with interleaved.
+ * The sum of squares is an fp32 number too: past its range y is 0, and below it, with eps
+ * 0, not finite.
  * bf16 or fp16 (KV_TOKENS_*), D 64 or 128, R even up to D; bases 16-byte aligned, the heads
  * of a token side by side, token strides in elements, multiples of 8.
  *

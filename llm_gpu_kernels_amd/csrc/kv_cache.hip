@@ -323,6 +323,8 @@ __global__ __launch_bounds__(kWideThreads) void kv_append_mx(KvState s, int laye
   for (int u = threadIdx.x; u < kAppendTokens * chunks; u += kWideThreads) {
     const int nth = u / chunks, c = (u - nth * chunks) * 16, token = blockIdx.x * kAppendTokens + nth;
     if (token >= n) continue;
+    const u32x4 *const kp = (const u32x4 *)(k + token * k_stride + c), *const vp = (const u32x4 *)(v + token * v_stride + c);
+    const u32x4 k0 = kp[0], k1 = kp[1], v0 = vp[0], v1 = vp[1];  // beside the slot, not behind it
     const int64_t slot = s.slots[token];
     if (slot < 0 || slot >= cells) continue;
     const int head = c / s.head_dim, d = c % s.head_dim;
@@ -330,8 +332,6 @@ __global__ __launch_bounds__(kWideThreads) void kv_append_mx(KvState s, int laye
     const int64_t at = (plane + page) * s.kv_heads + head;
     const int64_t to = (at * s.page_size + row) * mx::row_bytes<FMT>(s.head_dim) + mx::row_bytes<FMT>(d);
     const int64_t scale_to = (at * (s.head_dim / mx::kBlock) + d / mx::kBlock) * s.page_size + row;
-    const u32x4 *const kp = (const u32x4 *)(k + token * k_stride + c), *const vp = (const u32x4 *)(v + token * v_stride + c);
-    const u32x4 k0 = kp[0], k1 = kp[1], v0 = vp[0], v1 = vp[1];
     const Elements ke = quantise16<FMT, F16>(k0, k1), ve = quantise16<FMT, F16>(v0, v1);
     if constexpr (FMT == mx::kFp8) {
       *(u32x4 *)((uint8_t *)s.k + to) = u32x4{ke.w[0], ke.w[1], ke.w[2], ke.w[3]};
@@ -351,8 +351,9 @@ __global__ __launch_bounds__(kWideThreads) void kv_append_mx(KvState s, int laye
 // k and v from starts[i] on.  A workgroup takes kGatherTokens of those; one thread each
 // finds where its token lies, and then all copy 8 values at a time: stores of whole lines.
 // HBM, two thirds of it writes: 31000 tokens of 8 heads of 128 in eight bits (193 MB) 44.6 us,
-// 4.3 TB/s (16 values at a time 49.7; four tokens a workgroup 46.2); 4000 in four bits 8.4, the
-// chain of three dependent loads before the first element.
+// 4.3 TB/s (16 values at a time 49.7; four tokens a workgroup 46.2; non-temporal stores 32.6, but
+// attention of 64 queries over 6 rows of 3000 so read back 139 instead of 109); 4000 in four bits
+// 8.4, the chain of three dependent loads before the first element.
 constexpr int kGatherTokens = 8;
 template <int FMT, bool F16>
 __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, const int32_t *rows, const int32_t *starts,
@@ -374,11 +375,12 @@ __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, 
       if (row >= s.sequences) {
         atomicOr(s.status, KV_STATUS_BAD_ROW);
       } else if (row >= 0) {
-        const int len = s.lengths[row];
-        if (len < 0 || len > s.max_pages * s.page_size) {
+        // The page beside the length, not behind it.
+        const int cap = s.max_pages * s.page_size, len = s.lengths[row];
+        const int p = j < cap ? s.tables[(int64_t)row * s.max_pages + j / s.page_size] : -1;
+        if (len < 0 || len > cap) {
           atomicOr(s.status, KV_STATUS_BAD_STATE);
         } else if (j < len) {
-          const int p = s.tables[(int64_t)row * s.max_pages + j / s.page_size];
           if (p < 0 || p >= s.pages) atomicOr(s.status, KV_STATUS_BAD_STATE);
           else slot = p * s.page_size + j % s.page_size;
         }
@@ -386,8 +388,8 @@ __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, 
     }
     slots[threadIdx.x] = slot;
   }
-  // Starts that do not ascend within [0, tokens] are reported, once for each of them.
-  if (blockIdx.x == 0)
+  // Starts that do not ascend within [0, tokens] are reported.
+  if (blockIdx.x == gridDim.x - 1)
     for (int i = threadIdx.x; i <= n; i += kWideThreads)
       if (starts[i] < (i ? starts[i - 1] : 0) || starts[i] > tokens) atomicOr(s.status, KV_STATUS_BAD_COUNT);
   __syncthreads();
