@@ -104,10 +104,20 @@ constexpr int kOverhead = 6;
 // 14.7, 18.5; of 4096 23.5, 23.9.
 __host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 8 ? 17 : 2 * (int)listed + 2; }
 
-// LISTED: ranges of the list; otherwise a (sequence, head block) per workgroup.  TEAM
-// waves.
+// What the host divides for the kernel: query heads per KV head, blocks of up to 16 of them, and
+// the logarithm of a page's blocks of keys (-1: not a power of two).
+struct Shape {
+  int group, blocks, page_shift;
+};
+
+// LISTED: ranges of the list; otherwise a (sequence, head block) per workgroup, of a grid
+// (block of query heads, KV head, sequence).  TEAM waves.
+//
+// A call with a few steps is as long as its first pass over the code, whose instructions come
+// from the L2: what a team does not need is not compiled into it, and its arguments are read
+// at once, not line by line where they are used.
 template <int D, bool F16, int FMT, int TEAM, bool LISTED>
-__global__ __launch_bounds__(64 * TEAM, (TEAM == 8 ? 2 : kGroups)) void gqa_mx_kernel(GqaPagedArgs a) {
+__global__ __launch_bounds__(64 * TEAM, (TEAM == 8 ? 2 : kGroups)) void gqa_mx_kernel(GqaPagedArgs a, Shape shape) {
   constexpr int kSlices = D / 32, kTiles = D / 16;
   constexpr int kN = kBlocks<D, FMT>, kKeys = kStep<D, FMT>;
   constexpr uint32_t kRowBytes = (uint32_t)mx::row_bytes<FMT>(D);
@@ -115,8 +125,12 @@ __global__ __launch_bounds__(64 * TEAM, (TEAM == 8 ? 2 : kGroups)) void gqa_mx_k
   extern __shared__ __attribute__((aligned(16))) float states[];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = sgpr(threadIdx.x >> 6);
-  const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows, heads = a.Hkv * blocks;
-  const int cap = a.M * a.page, per_page = a.page / kBlock;
+  if constexpr (!LISTED)
+    asm volatile("" ::"s"(a.q), "s"(a.k), "s"(a.v), "s"(a.out), "s"(a.tables), "s"(a.lengths), "s"(a.k_page), "s"(a.k_head),
+                 "s"(a.v_page), "s"(a.v_head), "s"(a.M), "s"(a.scale), "s"(a.k_scales), "s"(a.ks_page), "s"(a.vs_page),
+                 "s"(shape.group));
+  const int group = shape.group, blocks = shape.blocks, heads = a.Hkv * blocks;
+  const int cap = a.M * a.page;
   auto steps_of = [](int keys) __attribute__((always_inline)) { return (int)(((uint32_t)keys + kKeys - 1) / kKeys); };
 
   // ---- the workgroup's range, and its first segment ----
@@ -196,10 +210,12 @@ __global__ __launch_bounds__(64 * TEAM, (TEAM == 8 ? 2 : kGroups)) void gqa_mx_k
     }
   }
   if (paired) {
-    if ((int)blockIdx.x >= a.B * heads) return;
-    const int b = blockIdx.x / heads, head = blockIdx.x % heads, raw = a.lengths[b], len = sgpr(max(0, min(raw, cap)));
+    if (LISTED && (int)blockIdx.x >= a.B * heads) return;
+    const int b = LISTED ? blockIdx.x / heads : blockIdx.z, head = blockIdx.x - b * heads;
+    const int kvh = LISTED ? head / blocks : blockIdx.y, part = LISTED ? head - kvh * blocks : blockIdx.x;
+    const int raw = a.lengths[b], len = sgpr(max(0, min(raw, cap)));
     if (raw != len && threadIdx.x == 0) atomicOr(a.status, GQA_STATUS_BAD_BOUNDS);
-    seg = Segment{b, head / blocks, head % blocks, len, steps_of(len), 0, 0, steps_of(len)};
+    seg = Segment{b, kvh, part, len, steps_of(len), 0, 0, steps_of(len)};
     // For the launch that joins the list's pieces: nothing to do here.
     if (LISTED && threadIdx.x == 0) a.pieces[2 * blockIdx.x + 1] = 0;
   }
@@ -256,12 +272,13 @@ __global__ __launch_bounds__(64 * TEAM, (TEAM == 8 ? 2 : kGroups)) void gqa_mx_k
     int page, row;
   };
   auto look_up = [&](const Segment &x, int t) __attribute__((always_inline)) {
-    const int blk = kN * (t + TEAM * (lane / kN)) + lane % kN, at = blk / per_page;
-    const bool in = kBlock * blk < x.len;
+    const int blk = kN * (t + TEAM * (lane / kN)) + lane % kN;
+    const int at = __builtin_expect(shape.page_shift >= 0, 1) ? blk >> shape.page_shift : blk / (a.page / kBlock);
+    const bool in = (uint32_t)(kBlock * blk) < (uint32_t)x.len;  // (a window may go past 2^31 keys)
     const int page = in ? a.tables[(int64_t)x.b * a.table_stride + at] : 0;
     const bool ok = (uint32_t)page < (uint32_t)a.P;
     bad_page |= !ok;
-    return Window{ok ? page : 0, in && ok ? (blk - at * per_page) * kBlock : -1};
+    return Window{ok ? page : 0, in && ok ? blk * kBlock - at * a.page : -1};
   };
   // The nth step of a window, step t of the segment: the keys of its blocks that are there
   // (a byte each) into n, what they hold into raw.  Blocks that are not there are read from
@@ -407,12 +424,16 @@ __global__ __launch_bounds__(64 * TEAM, (TEAM == 8 ? 2 : kGroups)) void gqa_mx_k
   R cur, nxt;
   uint64_t n_cur = 0, n_nxt = 0;
   bool ahead = false;  // cur holds the wave's first step of the segment
-  Window win = look_up(seg, seg.s + wave), win_next;
+  Window win = look_up(seg, seg.s + wave), win_next = {};
   issue_q(seg);
   const int rows_most = min(group, kRows), stride = rows_most * D + 2 * kRows;  // floats of a wave's state
   for (int nth = 0;; ++nth) {
-    const Segment next = next_segment(seg);
-    win_next = look_up(next, next.s + wave);
+    Segment next = seg;
+    next.s = next.e = 0;
+    if constexpr (LISTED) {
+      next = next_segment(seg);
+      win_next = look_up(next, next.s + wave);
+    }
     m_run = m_top = -INFINITY;
     l_run = 0.f;
 #pragma unroll
@@ -522,19 +543,21 @@ template <int D, bool F16, int FMT>
 hipError_t launch(const GqaPagedArgs &a, int cus, hipStream_t s) {
   const int group = a.Hq / a.Hkv, rows = group < kRows ? group : kRows, pairs = a.B * a.Hkv * ((group + kRows - 1) / kRows);
   const int team = team_of(pairs, ((int64_t)a.M * a.page + kStep<D, FMT> - 1) / kStep<D, FMT>, cus);
+  const int blocks = (group + kRows - 1) / kRows, per_page = a.page / kBlock;
+  const Shape shape = {group, blocks, per_page & (per_page - 1) ? -1 : __builtin_ctz(per_page)};
   const int lds = (team == 8 ? 8 : 4) * (rows * D + 2 * kRows) * (int)sizeof(float);  // at most 66 KiB
   if (team == 8) {
     auto wide = gqa_mx_kernel<D, F16, FMT, 8, false>;
     static std::atomic<uint64_t> allowed{0};
     if (const hipError_t e = allow_lds((const void *)wide, 8 * (kRows * D + 2 * kRows) * (int)sizeof(float), &allowed)) return e;
-    hipLaunchKernelGGL(wide, dim3(pairs), dim3(512), lds, s, a);
+    hipLaunchKernelGGL(wide, dim3(blocks, a.Hkv, a.B), dim3(512), lds, s, a, shape);
     return hipGetLastError();
   }
   if (team == 4) {
-    hipLaunchKernelGGL((gqa_mx_kernel<D, F16, FMT, 4, false>), dim3(pairs), dim3(256), lds, s, a);
+    hipLaunchKernelGGL((gqa_mx_kernel<D, F16, FMT, 4, false>), dim3(blocks, a.Hkv, a.B), dim3(256), lds, s, a, shape);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL((gqa_mx_kernel<D, F16, FMT, 4, true>), dim3(cus * kGroups), dim3(256), lds, s, a);
+  hipLaunchKernelGGL((gqa_mx_kernel<D, F16, FMT, 4, true>), dim3(cus * kGroups), dim3(256), lds, s, a, shape);
   if (const hipError_t e = hipGetLastError()) return e;
   return launch_gqa_paged_merge(a, cus, s);
 }
