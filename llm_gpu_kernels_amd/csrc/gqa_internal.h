@@ -82,6 +82,8 @@ struct GqaSharedState {
   int32_t *rows;
   float *heads;                          // [B][Hq]{m, l, O[D]}: of a prefix's first chunk
   float *more;                           // [unit but each first][kSharedRows]: of the others
+  int group;                             // query heads per KV head
+  int page_shift;                        // log2 of a page's blocks of 16 keys; -1: no power of two
 };
 
 // One new token per sequence over a paged cache (gqa_paged.hip).

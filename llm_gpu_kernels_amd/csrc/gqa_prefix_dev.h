@@ -98,7 +98,7 @@ __device__ __forceinline__ Plan plan_here(const GqaPagedArgs &p, uint8_t *smem) 
   };
   Lds *const lds = (Lds *)smem;
   const GqaSharedState &st = p.shared;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per_head = p.Hq / p.Hkv, G = st.G;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per_head = st.group, G = st.G;
   const int raw = tid < p.B ? p.lengths[tid] : 0, len = max(0, min(raw, p.M * p.page));
   const int wanted = lane < G ? st.prefixes[lane] : 0;
   if (tid <= G) lds->starts[tid] = st.starts[tid];
@@ -213,7 +213,7 @@ __device__ __forceinline__ void prefix(const GqaPagedArgs &p, const Plan &plan, 
   const GqaSharedState &a = p.shared;
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const int wave = sgpr(threadIdx.x >> 6);
-  const int group = p.Hq / p.Hkv, per_page = p.page / kBlock;
+  const int group = a.group;
   // Neighbouring units, whose rows see the same keys, on one XCD, which has them in its L2.
   const int units = plan.units, workgroups = plan.workgroups;
   const int xcd = blockIdx.x % kXcds, first_unit = xcd * (workgroups / kXcds) + min(xcd, workgroups % kXcds) + (int)blockIdx.x / kXcds;
@@ -277,13 +277,14 @@ __device__ __forceinline__ void prefix(const GqaPagedArgs &p, const Plan &plan, 
     auto look_up = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int blk = base + kWave * i + lane, at = blk / per_page;
+        const int blk = base + kWave * i + lane;
+        const int at = blk / (p.page / kBlock);
         const bool in = blk * kBlock < keys && blk < 2 * (s0 + stages);
         const int page = in ? table[at] : 0;
         const bool ok = (uint32_t)page < (uint32_t)p.P;
         bad_page |= in && !ok;
         pages[i] = ok ? page : 0;
-        rows_at[i] = in && ok ? (blk - at * per_page) * kBlock : -1;
+        rows_at[i] = in && ok ? blk * kBlock - at * p.page : -1;
       }
     };
     look_up();

@@ -268,12 +268,14 @@ size_t gqa_shared_workspace(int B, int Hq, int Hkv, int D, int G, int cus) { ret
 void gqa_shared_bind(GqaPagedArgs *a, int G, const int32_t *starts, const int32_t *prefixes, void *workspace, int cus) {
   uint8_t *const w = (uint8_t *)workspace;
   const Layout l = layout_of(a->B, a->Hq, a->Hkv, a->D, G, cus);
+  const int per_page = a->page / 16;
   a->status = (uint32_t *)w;
   a->pieces = (int32_t *)(w + l.pieces);
   a->partial = (float *)(w + l.partial);
   a->shared = GqaSharedState{G, G <= shared::kLocalGroups && a->B <= shared::kLocalRows, starts, prefixes,
                              (int32_t *)(w + l.header), (int32_t *)(w + l.groups), (int32_t *)(w + l.rows),
-                             (float *)(w + l.heads), (float *)(w + l.more)};
+                             (float *)(w + l.heads), (float *)(w + l.more), a->Hq / a->Hkv,
+                             per_page & (per_page - 1) ? -1 : __builtin_ctz(per_page)};
 }
 
 hipError_t launch_gqa_shared(const GqaPagedArgs &p, int cus, hipStream_t s) {
