@@ -327,7 +327,7 @@ __global__ __launch_bounds__(kWideThreads) void kv_append_mx(KvState s, int laye
     const u32x4 k0 = kp[0], k1 = kp[1], v0 = vp[0], v1 = vp[1];  // beside the slot, not behind it
     const int64_t slot = s.slots[token];
     if (slot < 0 || slot >= cells) continue;
-    const int head = c / s.head_dim, d = c % s.head_dim;
+    const int head = c >> (s.head_dim == 128 ? 7 : 6), d = c & (s.head_dim - 1);
     const int page = (int)slot / s.page_size, row = (int)slot - page * s.page_size;  // (slot < 2^30)
     const int64_t at = (plane + page) * s.kv_heads + head;
     const int64_t to = (at * s.page_size + row) * mx::row_bytes<FMT>(s.head_dim) + mx::row_bytes<FMT>(d);
@@ -359,11 +359,11 @@ template <int FMT, bool F16>
 __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, const int32_t *rows, const int32_t *starts,
                                                          int n, uint16_t *k, uint16_t *v, int64_t k_stride,
                                                          int64_t v_stride, int tokens) {
-  __shared__ int slots[kGatherTokens];  // below 2^30
+  __shared__ int pages[kGatherTokens], rows_at[kGatherTokens];  // -1: none; the row in the page
   const int first = blockIdx.x * kGatherTokens;
   if (threadIdx.x < kGatherTokens) {
     const int t = first + threadIdx.x;
-    int slot = -1;
+    int page = -1, page_row = 0;
     if (t < tokens && t >= starts[0] && t < starts[n]) {
       int lo = 0, hi = n - 1;  // starts[lo] <= t < starts[hi + 1] throughout
       while (lo < hi) {
@@ -382,26 +382,25 @@ __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, 
           atomicOr(s.status, KV_STATUS_BAD_STATE);
         } else if (j < len) {
           if (p < 0 || p >= s.pages) atomicOr(s.status, KV_STATUS_BAD_STATE);
-          else slot = p * s.page_size + j % s.page_size;
+          else page = p, page_row = j % s.page_size;
         }
       }
     }
-    slots[threadIdx.x] = slot;
+    pages[threadIdx.x] = page;
+    rows_at[threadIdx.x] = page_row;
   }
   // Starts that do not ascend within [0, tokens] are reported.
   if (blockIdx.x == gridDim.x - 1)
     for (int i = threadIdx.x; i <= n; i += kWideThreads)
       if (starts[i] < (i ? starts[i - 1] : 0) || starts[i] > tokens) atomicOr(s.status, KV_STATUS_BAD_COUNT);
   __syncthreads();
-  const int chunks = s.kv_heads * s.head_dim / 8;
+  const int chunks = s.kv_heads * s.head_dim / 8, half = s.head_dim == 128 ? 7 : 6;  // half: log2 head_dim
   const int64_t plane = (int64_t)layer * s.pages;
 #pragma unroll 2
   for (int u = threadIdx.x; u < chunks * kGatherTokens; u += kWideThreads) {
-    const int nth = u / chunks, c = (u - nth * chunks) * 8;
-    const int slot = slots[nth];
-    if (slot < 0) continue;
-    const int head = c / s.head_dim, d = c - head * s.head_dim;
-    const int page = slot / s.page_size, row = slot - page * s.page_size;
+    const int nth = u / chunks, c = (u - nth * chunks) * 8, page = pages[nth], row = rows_at[nth];
+    if (page < 0) continue;
+    const int head = c >> half, d = c & (s.head_dim - 1);
     const int64_t at = (plane + page) * s.kv_heads + head;
     const int64_t from = (at * s.page_size + row) * mx::row_bytes<FMT>(s.head_dim) + mx::row_bytes<FMT>(d);
     const uint8_t *const kp = (const uint8_t *)s.k + from, *const vp = (const uint8_t *)s.v + from;

@@ -10,9 +10,9 @@
 // workgroup's waves wait for each other.
 //
 // Measured, a copy of 2 GiB running at 5.1 TB/s: 8191 tokens of 32 + 8 heads of 128 (168 MB)
-// 38.8 us, 4.3 TB/s (a workgroup per token, its rows in LDS: 51); 2500 of 12 + 4 heads of 64
-// with their cache in eight bits 7.3; 16 tokens 3.6, the launch, a load and a chain of some
-// hundred instructions.  (Non-temporal stores: 32.3, and the attention that reads the rows loses 8.)
+// 33.8 us, 5.0 TB/s (a workgroup per token, its rows in LDS: 51; arguments, positions and weights
+// loaded where they are used: 38.8); 2500 of 12 + 4 heads of 64 with their cache in eight bits
+// 7.3; 16 tokens 3.6, the launch, a load and a chain of some hundred instructions.
 #include "common.h"
 #include "gqa_dev.h"
 #include "mx_dev.h"
@@ -77,9 +77,13 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope(QkArgs a, int parts, in
   constexpr int kLanes = D / 8, kRows = kWave / kLanes;  // lanes of a row, rows at a time
   __shared__ __attribute__((aligned(16))) float turn[kWaves][2][kWave];
   __shared__ __attribute__((aligned(16))) float lds_rows[kWaves][PAIRS == kAny ? kRows : 1][PAIRS == kAny ? D : 4];
+  // The arguments at once, not line by line where they are used: a token takes no longer than that.
+  asm volatile("" ::"s"(a.N), "s"(a.Hkv), "s"(a.R), "s"(a.weights_fp32), "s"(a.q), "s"(a.k), "s"(a.v), "s"(a.positions),
+               "s"(a.inv_freq), "s"(a.q_weight), "s"(a.k_weight), "s"(a.q_out), "s"(a.k_out), "s"(a.q_stride), "s"(a.k_stride),
+               "s"(a.v_stride), "s"(a.eps), "s"(a.cache.slots), "s"(parts), "s"(each));
   const int lane = threadIdx.x & 63, wave = gqa::sgpr(threadIdx.x >> 6), c = lane % kLanes, nth = lane / kLanes;
-  const int64_t unit = (int64_t)blockIdx.x * kWaves + wave;
-  const int t = gqa::sgpr((int)(unit / parts)), part = gqa::sgpr((int)(unit - (int64_t)t * parts));
+  const uint32_t unit = blockIdx.x * kWaves + wave;  // below 2^27
+  const int t = gqa::sgpr((int)(unit / (uint32_t)parts)), part = gqa::sgpr((int)(unit - (uint32_t)(t * parts)));
   if (t >= a.N) return;
   const int half = a.R / 2, rows = a.Hq + a.Hkv + (a.cached ? a.Hkv : 0);
   const int from = part * each * kRows, to = min(rows, from + each * kRows);
@@ -94,7 +98,18 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope(QkArgs a, int parts, in
     }
     return x;
   };
+  // Everything that is needed before the first row is loaded before the first wait.
+  const int position = a.positions[t];
+  const float freq = a.inv_freq[min(lane, half - 1)];
   u32x4 next = load(from + nth);
+  u32x4 raw_q[2] = {}, raw_k[2] = {};
+  auto fetch = [&](const void *w, u32x4 (&x)[2]) __attribute__((always_inline)) {
+    if (!w) return;
+    x[0] = ((const u32x4 *)w)[a.weights_fp32 ? 2 * c : c];
+    if (a.weights_fp32) x[1] = ((const u32x4 *)w)[2 * c + 1];
+  };
+  fetch(a.q_weight, raw_q);
+  fetch(a.k_weight, raw_k);
   // The token's page and row there; -1: none.  (A cache has at most 2^30 places.)
   int page = -1, page_row = 0;
   if (a.cached) {
@@ -105,23 +120,14 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope(QkArgs a, int parts, in
     page_row = place - page * a.cache.page_size;
   }
   float wq[8], wk[8];
-  auto weights = [&](const void *w, float (&x)[8]) __attribute__((always_inline)) {
-    if (!w) {
+  if (lane < half) angle(position, freq, &turn[wave][0][lane], &turn[wave][1][lane]);
+  auto weights = [&](const u32x4 (&r)[2], float (&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 1.f;
-    } else if (a.weights_fp32) {
-      const f32x4 lo = ((const f32x4 *)w)[2 * c], hi = ((const f32x4 *)w)[2 * c + 1];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = i < 4 ? lo[i] : hi[i - 4];
-    } else {
-      const u32x4 r = ((const u32x4 *)w)[c];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = gqa::to_f32<F16>(i & 1 ? r[i / 2] >> 16 : r[i / 2] & 0xffffu);
-    }
+    for (int i = 0; i < 8; ++i)
+      x[i] = a.weights_fp32 ? __uint_as_float(r[i / 4][i % 4]) : gqa::to_f32<F16>(i & 1 ? r[0][i / 2] >> 16 : r[0][i / 2] & 0xffffu);
   };
-  weights(a.q_weight, wq);
-  weights(a.k_weight, wk);
-  if (lane < half) angle(a.positions[t], a.inv_freq[lane], &turn[wave][0][lane], &turn[wave][1][lane]);
+  weights(raw_q, wq);
+  weights(raw_k, wk);
   __builtin_amdgcn_wave_barrier();  // a wave's LDS operations are in order
   // Of element 8 c + i: the cosine, the sine with its sign, and where its partner lies.
   // Neighbours: of the pair 4 c + i.
@@ -209,8 +215,9 @@ hipError_t launch(const QkArgs &a, int cus, hipStream_t s) {
   constexpr int kRows = kWave / (D / 8);
   const int rows = a.Hq + a.Hkv + (a.cached ? a.Hkv : 0), passes = (rows + kRows - 1) / kRows;
   // A token's passes are shared out over waves, each of which computes its angles: while all
-  // waves run at once (24 a CU; 1000 tokens of 32 + 8 heads of 128: 6.8 us, 8.0 with three times as
-  // many), and in two where they do not any more (8191 tokens: 38.6, in one 42.2, in five 40.3).
+  // waves run at once (24 a CU; 1000 tokens of 32 + 8 heads of 128: 6.4 us, 7.5 with twice as many,
+  // 6.8 with 12 a CU), and in two where they do not any more (8191 tokens: 33.8, in one 37.5, in three
+  // 34.1).
   const int64_t places = 20 * (int64_t)cus;
   const int most = a.N > places ? 2 : (int)(places / a.N), each = (passes + most - 1) / most;
   const int parts = (passes + each - 1) / each;
