@@ -123,12 +123,19 @@ class PagedKVCache:
             raise ValueError(f"{name} must have inner strides ({dim}, 1)")
         return s0 if shape[0] > 1 else heads * dim
 
+    def _ints(self, t, name, size):
+        # The usual case first: with a few tokens a call is as long as its checks.
+        if not (type(t) is torch.Tensor and t.dtype is torch.int32 and t.shape == (size,) and t.device == self.device
+                and t.is_contiguous()):
+            _check_int32(t, name, (size,), self.device)
+
     def _rows(self, t, name):
         if not isinstance(t, torch.Tensor) or t.ndim != 1:
             raise ValueError(f"{name} must be an int32 tensor [n]")
-        _check_int32(t, name, (t.shape[0],), self.device)
-        if t.shape[0] > self.sequences:
-            raise ValueError(f"{name} must name at most {self.sequences} rows (got {t.shape[0]})")
+        n = t.shape[0]
+        self._ints(t, name, n)
+        if n > self.sequences:
+            raise ValueError(f"{name} must name at most {self.sequences} rows (got {n})")
         return t
 
     def reserve(self, counts, stride=0):
@@ -168,13 +175,13 @@ class PagedKVCache:
         keep what they held; k and v share no memory."""
         if not isinstance(layer, int) or not 0 <= layer < self.layers:
             raise ValueError(f"layer must be an int in [0, {self.layers}) (got {layer!r})")
-        rows = self._rows(rows, "rows")
-        _check_int32(starts, "starts", (rows.shape[0] + 1,), self.device)
-        ks, vs = self._token_stride(k, "k"), self._token_stride(v, "v")
-        if k.shape[0] != v.shape[0] or k.shape[0] > N.KV_MAX_GATHER_TOKENS:
+        n = self._rows(rows, "rows").shape[0]
+        self._ints(starts, "starts", n + 1)
+        ks, vs, tokens = self._token_stride(k, "k"), self._token_stride(v, "v"), k.shape[0]
+        if tokens != v.shape[0] or tokens > N.KV_MAX_GATHER_TOKENS:
             raise ValueError(f"k and v must have the same number of tokens, at most {N.KV_MAX_GATHER_TOKENS}")
-        N.check(N.lib().kv_cache_gather(self._cache, layer, rows.data_ptr(), starts.data_ptr(), rows.shape[0], k.data_ptr(),
-                                        v.data_ptr(), ks, vs, k.shape[0], self._stream()), "gather")
+        N.check(N.lib().kv_cache_gather(self._cache, layer, rows.data_ptr(), starts.data_ptr(), n, k.data_ptr(),
+                                        v.data_ptr(), ks, vs, tokens, self._stream()), "gather")
 
     def fork(self, src, dst):
         """Row ``dst[i]``, which must be empty, starts as a copy of row ``src[i]``
