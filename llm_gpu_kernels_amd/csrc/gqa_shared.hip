@@ -162,7 +162,7 @@ template <bool F16>
 __global__ __launch_bounds__(kMergeThreads) void gqa_shared_join(GqaPagedArgs p, int chunk) {
   __shared__ State states[kMergeThreads];
   const GqaSharedState &a = p.shared;
-  const int group = p.Hq / p.Hkv, blocks = (group + kRows - 1) / kRows, heads = p.Hkv * blocks;
+  const int group = a.group, blocks = (group + kRows - 1) / kRows, heads = p.Hkv * blocks;
   const int b = blockIdx.x / heads, head = blockIdx.x % heads, kvh = head / blocks, part = head % blocks;
   const int rows = min(kRows, group - kRows * part), per_slot = min(group, kRows), groups = kMergeThreads / chunk;
   const int e = 2 * (blockIdx.y * chunk + threadIdx.x % chunk), mine = threadIdx.x / chunk;  // element, group
@@ -171,16 +171,17 @@ __global__ __launch_bounds__(kMergeThreads) void gqa_shared_join(GqaPagedArgs p,
   const int row = live ? e >> half : 0, d = e & (p.D - 1), qh = kvh * group + kRows * part + row;
   const int64_t record = p.D + 2;
 
+  // (All at once: a launch of small loads is as long as its chain of them.)
   const int32_t *const rec = a.rows + 8 * b;
-  const int skip = uniform_load(rec), len = length_of(p, b);
-  const int slot = p.pieces[2 * blockIdx.x], left = p.pieces[2 * blockIdx.x + 1];
+  const int skip = uniform_load(rec), of_chunks = uniform_load(rec + 1), tiles = uniform_load(rec + 2);
+  const int tile_rows = uniform_load(rec + 3), first_row = uniform_load(rec + 4), more = uniform_load(rec + 5);
+  const int len = length_of(p, b), slot = p.pieces[2 * blockIdx.x], left = p.pieces[2 * blockIdx.x + 1];
   int chunks = 0;
   int64_t at = 0, apart = 0;  // of the second chunk's record, between two chunks'
   if (skip > 0) {
-    chunks = uniform_load(rec + 1);
-    const int tiles = uniform_load(rec + 2), tile_rows = uniform_load(rec + 3);
-    const int place = uniform_load(rec + 4) + kRows * part + row, tile = place / tile_rows;
-    at = ((int64_t)(uniform_load(rec + 5) + kvh * (chunks - 1) * tiles + tile) * kSharedRows + place - tile * tile_rows) * record;
+    chunks = of_chunks;
+    const int place = first_row + kRows * part + row, tile = place / tile_rows;
+    at = ((int64_t)(more + kvh * (chunks - 1) * tiles + tile) * kSharedRows + place - tile * tile_rows) * record;
     apart = (int64_t)tiles * kSharedRows * record;
   }
   const int n = chunks + (len > skip ? left : 0);
