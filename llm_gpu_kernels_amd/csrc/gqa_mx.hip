@@ -19,9 +19,9 @@
 // (sequence, head), and the second launch falls away.
 //
 // Measured, 32 query and 8 KV heads of 128, a copy of 2 GiB running at 5.1 TB/s, the join
-// among it: 64 sequences of 1 to 7027 keys in eight bits (88 MB) 25.7 us, the main kernel
-// 20.9 and the join 5.0; one of 131072 in four bits (143 MB) 37.9, 33.4 and 5.3; one of
-// 700 in eight bits, a team, 9.2: launch, table, three dependent steps a wave, join in LDS.
+// among it: 64 sequences of 1 to 7027 keys in eight bits (88 MB) 25.5 us, the main kernel
+// 20.6 and the join 5.1; one of 131072 in four bits (143 MB) 37.6, 33.0 and 5.3; one of
+// 700 in eight bits, a team, 8.7: launch, table, three dependent steps a wave, join in LDS.
 // (The join by the last workgroup to arrive, in the same launch: 24.8 and 43.0, and counters
 // that have to outlive a run.)
 #include <type_traits>
@@ -97,11 +97,11 @@ constexpr int kOverhead = 6;
 
 // Steps that a wave of a workgroup with a whole (sequence, head) may have, by those that the
 // list would give it.  A team has one launch and nothing to join, but all of its sequence.
-// By teams and by the list, 8 KV heads of 128, eight bits: one sequence of 128 keys 5.4,
-// 10.9 us; of 700 9.2, 11.2; of 1500 13.8, 11.7; of 2048 16.6, 12.0; 16 of 512 8.4, 13.8; of 2048
-// 17.7, 20.8; of 4096 36.0, 35.7; 64 of 700 20.4, 22.5; of 2048 52.9, 55.2; 256 of 1 to 1024 28.2,
-// 34.3.  Four bits (steps of 64 keys): one of 1500 10.6, 11.9; of 2048 12.6, 12.4; 16 of 2048
-// 14.7, 18.5; of 4096 23.5, 23.9.
+// By teams and by the list, 8 KV heads of 128, eight bits: one sequence of 128 keys 4.4,
+// 10.0 us; of 700 8.7, 10.5; of 1500 13.2, 11.2; of 2048 16.0, 11.4; 16 of 512 7.8, 13.3; of 2048
+// 17.3, 20.5; of 4096 35.5, 35.4; 64 of 700 19.6, 22.0; of 2048 52.4, 55.1; 256 of 1 to 1024 27.9,
+// 33.8.  Four bits (steps of 64 keys): one of 1500 9.9, 11.1; of 2048 11.8, 11.6; 16 of 2048
+// 13.6, 18.1; of 4096 22.5, 23.4.
 __host__ __device__ inline int most_teamed(int64_t listed) { return listed >= 8 ? 17 : 2 * (int)listed + 2; }
 
 // What the host divides for the kernel: query heads per KV head, blocks of up to 16 of them, and
@@ -115,7 +115,7 @@ struct Shape {
 //
 // A call with a few steps is as long as its first pass over the code, whose instructions come
 // from the L2: what a team does not need is not compiled into it, and its arguments are read
-// at once, not line by line where they are used.
+// at once, not line by line where they are used (700 keys 9.2 to 8.7 us, 128 5.4 to 4.4).
 template <int D, bool F16, int FMT, int TEAM, bool LISTED>
 __global__ __launch_bounds__(64 * TEAM, (TEAM == 8 ? 2 : kGroups)) void gqa_mx_kernel(GqaPagedArgs a, Shape shape) {
   constexpr int kSlices = D / 32, kTiles = D / 16;

@@ -22,11 +22,11 @@
 //
 // Measured, 32 query and 8 KV heads of 128, a copy of 2 GiB running at 5.1 TB/s: four groups
 // of 22 to 40 sequences, prefixes of 4995 to 11383 keys, up to 600 keys of their own (186 MB)
-// 63.4 us (by gqa_paged.hip 593), of which the plan 4 and the join 7; the prefixes alone 59,
+// 63.2 us (by gqa_paged.hip 593), of which the plan 4 and the join 7; the prefixes alone 59,
 // the rest alone 36.  The loads alone and the products alone take 9 in 10 of that each, the
 // states 5: a stage of two tiles on a CU takes 1.07, the packed kernel's 1.0, and tiles of less
 // than 128 rows leave SIMDs without work.  Eight sequences with one prefix of 1500 keys, row
-// by row, 11.9.
+// by row, 11.7.
 #include "common.h"
 #include "../../include/gqa_mi355x.h"
 #include "gqa_dev.h"

@@ -350,10 +350,10 @@ __global__ __launch_bounds__(kWideThreads) void kv_append_mx(KvState s, int laye
 // Tokens of rows of the cache, read back side by side: row rows[i]'s go to the rows of
 // k and v from starts[i] on.  A workgroup takes kGatherTokens of those; one thread each
 // finds where its token lies, and then all copy 8 values at a time: stores of whole lines.
-// HBM, two thirds of it writes: 31000 tokens of 8 heads of 128 in eight bits (193 MB) 44.6 us,
-// 4.3 TB/s (16 values at a time 49.7; four tokens a workgroup 46.2; non-temporal stores 32.6, but
+// HBM, two thirds of it writes: 31000 tokens of 8 heads of 128 in eight bits (193 MB) 43.6 us,
+// 4.4 TB/s (16 values at a time 49.7; four tokens a workgroup 46.2; non-temporal stores 32.6, but
 // attention of 64 queries over 6 rows of 3000 so read back 139 instead of 109); 4000 in four bits
-// 8.4, the chain of three dependent loads before the first element.
+// 7.5, the chain of three dependent loads before the first element.
 constexpr int kGatherTokens = 8;
 template <int FMT, bool F16>
 __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, const int32_t *rows, const int32_t *starts,
