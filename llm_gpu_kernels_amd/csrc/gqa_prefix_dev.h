@@ -262,7 +262,7 @@ __device__ __forceinline__ void prefix(const GqaPagedArgs &p, const Plan &plan, 
     const int tiles = __builtin_amdgcn_readlane(of.tiles, g), tile_rows = __builtin_amdgcn_readlane(of.tile_rows, g);
     const int chunks = __builtin_amdgcn_readlane(of.chunks, g), more = __builtin_amdgcn_readlane(of.more, g);
     const int rest = (u - before) / tiles, tile = u - before - rest * tiles, kvh = rest / chunks, chunk = rest - kvh * chunks;
-    const int s0 = chunk * chunk_steps, stages = min(chunk_steps, (keys + kStep - 1) / kStep - s0);
+    const int s0 = chunk * chunk_steps, stages = min(chunk_steps, steps_of(keys) - s0);
     const int row0 = tile * tile_rows + kWaveRows * wave;
     const bool own = kWaveRows * wave < tile_rows && row0 < rows;
     const int more_at = more + (kvh * (chunks - 1) + chunk - 1) * tiles + tile;  // chunk > 0

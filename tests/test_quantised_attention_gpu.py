@@ -195,6 +195,24 @@ def test_offsets_past_32_bits(storage, gpu_device):
 
 
 @pytest.mark.parametrize("storage", STORAGES)
+def test_keys_up_to_2_31(storage, gpu_device):
+    """The longest sequence that a call allows, of one page over and over: attention over its 16
+    keys.  2048 waves take its 2^27 blocks, two at a time, so a sum of a wave has 2^15 terms and
+    is off by 2^15 * 2^-24 of its magnitudes at most: the denominator by 2^-9 of itself, O by 2^-9
+    of the bound, and the join of 1024 pieces by 2^-13 of both."""
+    p = Pages([16], 1, 1, 64, 16, torch.bfloat16, storage, gpu_device)
+    k, ks, v, vs = p.gpu
+    pages = 2 ** 27 - 1
+    tables = torch.full((1, pages), p.tables[0][0], dtype=torch.int32, device=gpu_device)
+    lengths = torch.tensor([16 * pages], dtype=torch.int32, device=gpu_device)
+    plan = prepare_paged_gqa(p.q, k, v, tables, lengths, k_scales=ks, v_scales=vs)
+    plan.check_inputs()
+    ref, bound = p.reference()
+    off, tol = (plan.output.double().cpu() - ref).abs(), S.tolerance(ref, bound, torch.bfloat16, 16, 6.0)
+    assert (off <= tol + bound * (2.0 ** -8 + 2.0 ** -12)).all()
+
+
+@pytest.mark.parametrize("storage", STORAGES)
 def test_two_streams_and_a_graph(storage, gpu_device):
     """Two plans at once on streams of their own, one of them captured and replayed."""
     a = Pages([700, 33, 2000], 8, 2, 128, 16, torch.bfloat16, storage, gpu_device)

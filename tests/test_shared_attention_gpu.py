@@ -252,6 +252,25 @@ def test_offsets_past_32_bits(gpu_device):
     x.check(plan)
 
 
+def test_keys_up_to_2_31(gpu_device):
+    """The longest sequences that a call allows, of one page over and over: attention over its
+    16 keys, but that the second sequence lacks the last page's last 5.  A workgroup has some 2^17
+    stages of the prefix, so its denominators are off by 2^17 * 2^-24 of themselves, and O, of two
+    products a stage, by 2^-6 of the bound; the 5 keys are 2^-28 of all."""
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(1, 1, 16, 64, generator=g).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(2, 4, 64, generator=g).to(torch.bfloat16)
+    pages = 2 ** 27 - 1
+    tables = torch.zeros(2, pages, dtype=torch.int32, device=gpu_device)
+    lengths = _i32([16 * pages, 16 * pages - 5], gpu_device)
+    plan = prepare_shared_gqa(q.to(gpu_device), k.to(gpu_device), v.to(gpu_device), tables, lengths, _i32([0, 2], gpu_device),
+                              _i32([2 ** 31 - 1], gpu_device))
+    plan.check_inputs()
+    ref, bound = S.paged_attention(q, k, v, [[0], [0]], [16, 16])
+    off, tol = (plan.output.double().cpu() - ref).abs(), S.tolerance(ref, bound, torch.bfloat16, 16, 6.0)
+    assert (off <= tol + bound * (2.0 ** -6 + 2.0 ** -7 + 2.0 ** -12)).all()
+
+
 def test_two_streams_and_a_graph(gpu_device):
     a = Groups([(640, [700, 650, 2000])], 8, 2, 128, 16, torch.bfloat16, gpu_device, behind=[50])
     b = Groups([(64, [70, 80, 90]), (96, [99, 100])], 8, 2, 128, 16, torch.bfloat16, gpu_device)
