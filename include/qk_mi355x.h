@@ -25,8 +25,8 @@ extern "C" {
  *     (l, h) = (i, i + R/2), or (2 i, 2 i + 1) with interleaved.
  * The sum of squares is an fp32 number too: past its range y is 0, and below it, with eps
  * 0, not finite.
- * bf16 or fp16 (KV_TOKENS_*), D 64 or 128, R even up to D; bases 16-byte aligned, the heads
- * of a token side by side, token strides in elements, multiples of 8.
+ * bf16 or fp16 (KV_TOKENS_*), D 64 or 128, R even up to D, N up to 2^24; bases 16-byte
+ * aligned, the heads of a token side by side, token strides in elements, multiples of 8.
  *
  * q_out [N, Hq, D] and k_out [N, Hkv, D] are contiguous and share no memory with an input.
  * With a cache, token t's keys, so treated, and its values v [N, Hkv, D], as they are, go

@@ -59,7 +59,7 @@ def test_struct_size_matches_header():
 
 
 @pytest.mark.parametrize("bad", [
-    dict(D=96), dict(D=256), dict(R=0), dict(R=130), dict(R=63), dict(R=-2), dict(dtype=2), dict(N=-1), dict(N=(1 << 25) + 1),
+    dict(D=96), dict(D=256), dict(R=0), dict(R=130), dict(R=63), dict(R=-2), dict(dtype=2), dict(N=-1), dict(N=(1 << 24) + 1),
     dict(Hq=0), dict(Hkv=0), dict(Hq=1 << 20), dict(eps=-1.0), dict(eps=math.nan), dict(eps=math.inf), dict(q=None),
     dict(k=BASE + 8), dict(v=BASE), dict(positions=None), dict(inv_freq=BASE + 2), dict(q_weight=BASE + 4),
     dict(k_weight=BASE + 8), dict(q_out=None), dict(k_out=None), dict(k_out=BASE + 8), dict(q_stride=4088),
