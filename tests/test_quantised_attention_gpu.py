@@ -194,6 +194,30 @@ def test_offsets_past_32_bits(storage, gpu_device):
     p.check(plan)
 
 
+def test_most_sequences_and_heads(gpu_device):
+    """As many as a call allows, 2^16 of each: the last ones are attended too."""
+    p = Pages([20], 1, 1, 64, 16, torch.bfloat16, "mxfp4", gpu_device)
+    k, ks, v, vs = p.gpu
+    many, rows = 2 ** 16, [0, 1, 30000, 2 ** 16 - 1]
+    lengths = torch.zeros(many, dtype=torch.int32, device=gpu_device)
+    lengths[rows] = 20
+    plan = prepare_paged_gqa(p.q.expand(many, 1, 64).contiguous(), k, v, p.gt.expand(many, -1).contiguous(), lengths, k_scales=ks,
+                             v_scales=vs)
+    plan.check_inputs()
+    ref, bound = p.reference()
+    for row in rows:
+        _assert_close(plan.output[row:row + 1], ref, bound, 20, 6.0)
+    plan.output[rows] = 0
+    assert (plan.output == 0).all()
+    k, ks, v, vs = (t.view(torch.uint8)[p.tables[0][0]][None].expand(1, many, -1, -1).contiguous().view(t.dtype) for t in p.gpu)
+    plan = prepare_paged_gqa(p.q.expand(1, many, 64).contiguous(), k, v, torch.zeros_like(p.gt[:, :1]), torch.full_like(p.gl, 16),
+                             k_scales=ks, v_scales=vs)
+    plan.check_inputs()
+    ref, bound = S.paged_attention(p.q.cpu(), *p.values, [p.tables[0][:1]], [16])
+    _assert_close(plan.output[:, -1:], ref, bound, 16, 6.0)
+    assert (plan.output == plan.output[:, :1]).all()
+
+
 @pytest.mark.parametrize("storage", STORAGES)
 def test_keys_up_to_2_31(storage, gpu_device):
     """The longest sequence that a call allows, of one page over and over: attention over its 16
