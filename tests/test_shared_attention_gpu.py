@@ -152,6 +152,14 @@ def test_many_sequences(gpu_device):
     x.check(x.plan())
 
 
+@pytest.mark.parametrize("groups,members,behind", [(64, 4, 0), (64, 4, 1), (65, 3, 0), (1024, 2, 3)])
+def test_many_groups(groups, members, behind, gpu_device):
+    """About and past what every workgroup plans by itself, and as many as a call allows."""
+    x = Groups([(33 + i % 20, [40 + (i + 7 * j) % 30 for j in range(members)]) for i in range(groups)], 2, 1, 64, 16,
+               torch.bfloat16, gpu_device, behind=[50] * behind)
+    x.check(x.plan())
+
+
 def test_every_prefix_length(gpu_device):
     """One set of tensors, starts and prefixes changed between runs."""
     x = Groups([(160, [161 + 3 * i for i in range(12)])], 8, 2, 128, 16, torch.bfloat16, gpu_device, before=[40], behind=[50])
