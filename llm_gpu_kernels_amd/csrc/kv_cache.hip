@@ -348,10 +348,10 @@ __global__ __launch_bounds__(kWideThreads) void kv_append_mx(KvState s, int laye
 }
 
 // Tokens of rows of the cache, read back side by side: row rows[i]'s go to the rows of
-// k and v from starts[i] on.  A workgroup takes kGatherTokens of those; one thread each
-// finds where its token lies, and then all copy 8 values at a time: stores of whole lines.
-// HBM, two thirds of it writes: 31000 tokens of 8 heads of 128 in eight bits (193 MB) 43.6 us,
-// 4.4 TB/s (16 values at a time 49.7; four tokens a workgroup 46.2; non-temporal stores 32.6, but
+// k and v from starts[i] on.  A workgroup takes kGatherTokens of those, finds where each token
+// lies, and then all threads copy 8 values at a time: stores of whole lines.
+// HBM, two thirds of it writes: 31000 tokens of 8 heads of 128 in eight bits (193 MB) 42.3 us,
+// 4.6 TB/s (16 values at a time 49.7; four tokens a workgroup 46.2; non-temporal stores 32.6, but
 // attention of 64 queries over 6 rows of 3000 so read back 139 instead of 109); 4000 in four bits
 // 7.5, the chain of three dependent loads before the first element.
 constexpr int kGatherTokens = 8;
@@ -359,35 +359,41 @@ template <int FMT, bool F16>
 __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, const int32_t *rows, const int32_t *starts,
                                                          int n, uint16_t *k, uint16_t *v, int64_t k_stride,
                                                          int64_t v_stride, int tokens) {
-  __shared__ int pages[kGatherTokens], rows_at[kGatherTokens];  // -1: none; the row in the page
-  const int first = blockIdx.x * kGatherTokens;
-  if (threadIdx.x < kGatherTokens) {
-    const int t = first + threadIdx.x;
-    int page = -1, page_row = 0;
-    if (t < tokens && t >= starts[0] && t < starts[n]) {
-      int lo = 0, hi = n - 1;  // starts[lo] <= t < starts[hi + 1] throughout
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (starts[mid] <= t) lo = mid;
-        else hi = mid - 1;
-      }
-      const int row = rows[lo], j = t - max(starts[lo], 0);
-      if (row >= s.sequences) {
-        atomicOr(s.status, KV_STATUS_BAD_ROW);
-      } else if (row >= 0) {
-        // The page beside the length, not behind it.
-        const int cap = s.max_pages * s.page_size, len = s.lengths[row];
-        const int p = j < cap ? s.tables[(int64_t)row * s.max_pages + j / s.page_size] : -1;
-        if (len < 0 || len > cap) {
-          atomicOr(s.status, KV_STATUS_BAD_STATE);
-        } else if (j < len) {
-          if (p < 0 || p >= s.pages) atomicOr(s.status, KV_STATUS_BAD_STATE);
-          else page = p, page_row = j % s.page_size;
+  __shared__ int2 places[kGatherTokens];  // {page, row there}; page -1: none
+  const int first = blockIdx.x * kGatherTokens, lane = threadIdx.x & 63;
+  if (threadIdx.x < kGatherTokens) places[threadIdx.x] = make_int2(-1, 0);
+  // The waves look through 64 of rows[] each; a lane below kGatherTokens takes the token of its
+  // number if the wave finds it.  (A search by halves was a load behind another for each.)
+  int row = -1, from = 0;
+  for (int base = gqa::sgpr(threadIdx.x - lane); base < n; base += kWideThreads) {
+    const int i = base + lane, begin = i < n ? starts[i] : 0, end = i < n ? starts[i + 1] : 0, r = i < n ? rows[i] : -1;
+#pragma unroll
+    for (int q = 0; q < kGatherTokens; ++q) {
+      const uint64_t in = __builtin_amdgcn_ballot_w64(begin <= first + q && first + q < end);
+      if (in) {
+        const int at = __builtin_ctzll(in), its_row = __builtin_amdgcn_readlane(r, at), its_begin = __builtin_amdgcn_readlane(begin, at);
+        if (lane == q) {
+          row = its_row;
+          from = max(its_begin, 0);
         }
       }
     }
-    pages[threadIdx.x] = page;
-    rows_at[threadIdx.x] = page_row;
+  }
+  __syncthreads();
+  if (row >= 0 && first + lane < tokens) {
+    if (row >= s.sequences) {
+      atomicOr(s.status, KV_STATUS_BAD_ROW);
+    } else {
+      // The page beside the length, not behind it.
+      const int j = first + lane - from, cap = s.max_pages * s.page_size, len = s.lengths[row];
+      const int p = j < cap ? s.tables[(int64_t)row * s.max_pages + j / s.page_size] : -1;
+      if (len < 0 || len > cap) {
+        atomicOr(s.status, KV_STATUS_BAD_STATE);
+      } else if (j < len) {
+        if (p < 0 || p >= s.pages) atomicOr(s.status, KV_STATUS_BAD_STATE);
+        else places[lane] = make_int2(p, j % s.page_size);
+      }
+    }
   }
   // Starts that do not ascend within [0, tokens] are reported.
   if (blockIdx.x == gridDim.x - 1)
@@ -398,7 +404,7 @@ __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, 
   const int64_t plane = (int64_t)layer * s.pages;
 #pragma unroll 2
   for (int u = threadIdx.x; u < chunks * kGatherTokens; u += kWideThreads) {
-    const int nth = u / chunks, c = (u - nth * chunks) * 8, page = pages[nth], row = rows_at[nth];
+    const int nth = u / chunks, c = (u - nth * chunks) * 8, page = places[nth].x, row = places[nth].y;
     if (page < 0) continue;
     const int head = c >> half, d = c & (s.head_dim - 1);
     const int64_t at = (plane + page) * s.kv_heads + head;
