@@ -318,6 +318,9 @@ constexpr int kAppendTokens = 4;  // of a workgroup
 template <int FMT, bool F16>
 __global__ __launch_bounds__(kWideThreads) void kv_append_mx(KvState s, int layer, const uint16_t *k, const uint16_t *v,
                                                             int64_t k_stride, int64_t v_stride, int n) {
+  // The arguments at once, not line by line where they are used: 0.1 us.
+  asm volatile("" ::"s"(s.k), "s"(s.v), "s"(s.slots), "s"(s.k_scales), "s"(s.v_scales), "s"(s.pages), "s"(s.kv_heads),
+               "s"(s.page_size), "s"(s.head_dim), "s"(k), "s"(v), "s"(k_stride), "s"(v_stride), "s"(n), "s"(layer));
   const int chunks = s.kv_heads * s.head_dim / 16;  // of a token, an even number: both halves of a block run together
   const int64_t cells = (int64_t)s.pages * s.page_size, plane = (int64_t)layer * s.pages;
   for (int u = threadIdx.x; u < kAppendTokens * chunks; u += kWideThreads) {
@@ -359,6 +362,10 @@ template <int FMT, bool F16>
 __global__ __launch_bounds__(kWideThreads) void kv_gather(KvState s, int layer, const int32_t *rows, const int32_t *starts,
                                                          int n, uint16_t *k, uint16_t *v, int64_t k_stride,
                                                          int64_t v_stride, int tokens) {
+  // As in kv_append_mx: 0.2 us.
+  asm volatile("" ::"s"(s.k), "s"(s.v), "s"(s.tables), "s"(s.lengths), "s"(s.k_scales), "s"(s.v_scales), "s"(s.pages),
+               "s"(s.kv_heads), "s"(s.page_size), "s"(s.head_dim), "s"(s.max_pages), "s"(k), "s"(v), "s"(k_stride),
+               "s"(v_stride), "s"(n), "s"(layer), "s"(rows), "s"(starts));
   __shared__ int2 places[kGatherTokens];  // {page, row there}; page -1: none
   const int first = blockIdx.x * kGatherTokens, lane = threadIdx.x & 63;
   if (threadIdx.x < kGatherTokens) places[threadIdx.x] = make_int2(-1, 0);
