@@ -89,8 +89,9 @@ __device__ __forceinline__ void cut(Group *g, int size) {
 }
 
 // The plan by one workgroup of four waves for itself: up to 64 groups and 256 rows.  Bounds
-// that do not ascend within [0, B]: nothing is shared.  Workgroup 0 reports and leaves
-// what the join needs of each row.
+// that do not ascend within [0, B]: nothing is shared.  Workgroup 0 reports those, negative
+// prefixes and lengths out of range (the list reports lengths too, but has no workgroup where
+// no key lies behind a prefix) and leaves what the join needs of each row.
 __device__ __forceinline__ Plan plan_here(const GqaPagedArgs &p, uint8_t *smem) {
   struct Lds {
     int starts[kLocalGroups + 1], least[kLocalGroups], live[kLocalGroups], source[kLocalGroups], keys[kLocalGroups];
@@ -128,7 +129,7 @@ __device__ __forceinline__ Plan plan_here(const GqaPagedArgs &p, uint8_t *smem) 
   __syncthreads();
   const bool bad = lds->wrong != 0;
   if (bad) g = -1;
-  if (blockIdx.x == 0 && ((bad && tid == 0) || wanted < 0)) atomicOr(p.status, GQA_STATUS_BAD_BOUNDS);
+  if (blockIdx.x == 0 && ((bad && tid == 0) || wanted < 0 || raw != len)) atomicOr(p.status, GQA_STATUS_BAD_BOUNDS);
   Plan plan = {};
   Group &mine = plan.group;  // every wave has all groups
   mine.before = 0x7fffffff;

@@ -80,6 +80,8 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_shared_plan(GqaPagedArgs p, 
   };
   for (int b = tid; b < p.B; b += kPlanThreads) {
     const int g = group_of(b), len = length_of(p, b);
+    // Here, since where no key lies behind a prefix the list has no workgroup that would.
+    if (p.lengths[b] != len) atomicOr(p.status, GQA_STATUS_BAD_BOUNDS);
     if (g < 0 || len == 0) continue;
     atomicMin(least + g, len);
     atomicMin(source + g, b);

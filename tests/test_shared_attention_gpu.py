@@ -346,3 +346,47 @@ def test_nothing_to_do(gpu_device):
     x.gl.zero_()
     plan = x.plan()
     assert (plan.run() == 0).all() and plan.read_status() == 0
+
+
+@pytest.mark.parametrize("lengths,kept", [([64, 64, -3], [64, 64, 0]), ([-2 ** 31, 64, 64], [0, 64, 64]),
+                                          ([-1, -2, -3], [0, 0, 0]), (["past"] * 3, ["table"] * 3),
+                                          ([2 ** 31 - 1, "table", "past"], ["table"] * 3)], ids=str)
+@pytest.mark.parametrize("groups,members", [(1, 3), (65, 3), (1, 258)], ids=["here", "groups", "rows"])
+def test_bad_lengths_without_keys_behind_a_prefix(groups, members, lengths, kept, gpu_device):
+    """Lengths out of range are reported where every key is one of a prefix too, planned by each
+    workgroup and (more than 64 groups or 256 sequences) by a launch before, and are worked on as
+    if they were at the limit that they pass."""
+    g = torch.Generator().manual_seed(groups + members)
+    page, hq, hkv, d, width = 16, 2, 1, 64, 4 if Groups.least_width == 1 else 600
+    table = page * width
+    numbers = {"past": table + 1, "table": table}
+    lengths, kept = ([numbers.get(n, n) for n in x] for x in (lengths, kept))
+    # The bad group last, its third length that of all members behind; the others of 32 keys.
+    before = (groups - 1) * members
+    lengths = [32] * before + lengths + lengths[2:] * (members - 3)
+    kept = [32] * before + kept + kept[2:] * (members - 3)
+    rows = [[j % 40 for j in range(width)]] * len(lengths)  # 40 pages over and over
+    k, v = (torch.randn(40, hkv, page, d, generator=g).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(len(lengths), hq, d, generator=g).to(torch.bfloat16)
+    starts, prefixes = [i * members for i in range(groups + 1)], [32] * (groups - 1) + [table]
+    args = [q.to(gpu_device), k.to(gpu_device), v.to(gpu_device), _i32(rows, gpu_device)]
+    good = prepare_shared_gqa(*args, _i32(kept, gpu_device), _i32(starts, gpu_device), _i32(prefixes, gpu_device))
+    assert good.read_status() == 0
+    plan = prepare_shared_gqa(*args, _i32(lengths, gpu_device), _i32(starts, gpu_device), _i32(prefixes, gpu_device))
+    for _ in range(2):
+        assert plan.read_status() == N.GQA_STATUS_BAD_BOUNDS and plan.read_status() == 0
+        assert torch.equal(plan.output, good.output)
+        plan.run()
+    ref, bound = S.paged_attention(q, k, v, rows, kept)
+    _assert_close(good.output, ref, bound, table, 6.0)
+
+
+def test_prefixes_longer_than_every_member(gpu_device):
+    """Prefixes past the shortest member, up to the largest number: it bounds what is shared."""
+    x = Groups([(160, [161 + 3 * i for i in range(12)])], 8, 2, 128, 16, torch.bfloat16, gpu_device, before=[40], behind=[50])
+    plan = x.plan()
+    for prefix in (161, 176, 10 ** 6, 2 ** 31 - 1):
+        x.gp[0] = prefix
+        plan.output.zero_()
+        plan.run()
+        x.check(plan)
