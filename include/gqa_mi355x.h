@@ -142,10 +142,11 @@ int gqa_paged_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d);
  * D / 2 (MXFP4) bytes a row, the rows of a (page, head) side by side; k_strides and
  * v_strides are in bytes, {page, head, row}, multiples of 16, row D or D / 2.  The scales
  * of a (page, head), [D / 32, page] bytes, lie together; page and head strides in bytes,
- * multiples of 16.  Page strides are below 2^31.  Elements are taken in q's type: one
- * whose value is beyond it is an infinity, one whose value is below its normal numbers is
- * off by its smallest such number at most (append writes none of either for tokens of q's
- * type).  Run, status and destroy as above.
+ * multiples of 16.  Page strides are below 2^31.  Elements are taken in q's type, to
+ * nearest even: one whose value is beyond it is an infinity, one between its smallest
+ * numbers (multiples of 2^-24 in fp16) is off by half of the smallest.  What append writes
+ * for tokens of q's type are numbers of that type; what the norm and rotation write for
+ * fp16 (qk_mi355x.h) may lie between them.  Run, status and destroy as above.
  */
 #define GQA_STORAGE_16BIT 0
 #define GQA_STORAGE_MXFP8 1

@@ -82,7 +82,7 @@ int kv_cache_create(kv_cache **out, const kv_cache_desc *d);
  * with KV_STORAGE_16BIT.  append rounds to nearest even under the smallest scale with which
  * all 32 are in range, 2^-117 at least and at most 2^119 (mxfp8) or 2^125 (mxfp4), with
  * fp16 tokens 2^7 or 2^13, where larger magnitudes saturate; 32 among which an infinity or
- * a NaN is read back as NaN. */
+ * a NaN is read back as NaN.  What it writes are numbers of the tokens' type. */
 int kv_cache_create_stored(kv_cache **out, const kv_cache_desc *d, int32_t storage, int32_t tokens, void *k_scales,
                            void *v_scales);
 
@@ -105,7 +105,8 @@ int kv_cache_append(kv_cache *c, int32_t layer, const void *k, const void *v, in
 /* The first starts[i+1] - starts[i] tokens of row rows[i] (int32 [n], n <= sequences;
  * fewer if the row is shorter, none if it is negative) read back from a layer to the rows
  * starts[i].. of k and v ([tokens, kv_heads, head_dim], strides as for append), in the
- * tokens' type.  starts: int32 [n + 1], ascending within [0, tokens] (else a status, and
+ * tokens' type, to nearest even where that does not hold them (no case of what append
+ * wrote).  starts: int32 [n + 1], ascending within [0, tokens] (else a status, and
  * some rows may be left out); tokens <= KV_MAX_GATHER_TOKENS.  Other rows of k and v are
  * left as they were.  k and v share no memory with each other or the cache. */
 int kv_cache_gather(kv_cache *c, int32_t layer, const int32_t *rows, const int32_t *starts, int32_t n, void *k, void *v,

@@ -31,7 +31,9 @@ extern "C" {
  * q_out [N, Hq, D] and k_out [N, Hkv, D] are contiguous and share no memory with an input.
  * With a cache, token t's keys, so treated, and its values v [N, Hkv, D], as they are, go
  * to slots[t] of `layer` (slots outside the cache are left out), quantised if the cache is,
- * from fp32; k_out may then be NULL.
+ * from fp32; k_out may then be NULL.  Keys so quantised need not be numbers of the type: fp16
+ * ends at 2^-24, and elements of 32 keys up to 448 * 2^-16 (MXFP8) or 6 * 2^-24 (MXFP4) go
+ * below.  Read back and attention take those to nearest, off by 2^-25 at most.
  */
 typedef struct qk_norm_rope_desc {
   int32_t N, Hq, Hkv, D, R, dtype;

@@ -9,8 +9,8 @@
 //     dims, and their scales;
 //   * which dims make a tile of O is free too: a lane takes D/16 neighbouring dims of its
 //     eight values' rows;
-//   * elements are converted exactly to q's type by single instructions that apply the
-//     scale, and the 16-bit halves of two values are put side by side.
+//   * elements are converted to q's type (exactly where it holds them) by single instructions
+//     that apply the scale, and the 16-bit halves of two values are put side by side.
 // The work is one flat list of steps, (sequence, KV head, step), cut into equal ranges, one
 // per workgroup; in a range its four waves take the steps of a (sequence, head) in turn
 // and join their states in LDS where it ends.  A (sequence, head) that a range's end

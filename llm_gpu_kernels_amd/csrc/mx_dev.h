@@ -11,7 +11,12 @@
 // an infinity or a NaN reads back as NaN.
 //
 // gfx950 converts both ways in single instructions, to nearest even; its decoders
-// apply the scale exactly, since no product needs more bits than 16-bit types have.
+// apply the scale exactly where the 16-bit type holds the product, which has 4 or 2 bits.
+// It does for all that is made of bf16 tokens, and of fp16 ones: those are multiples of 2^-24,
+// and so is one that is rounded to 4 or 2 bits or to an element's step above 2^-24.  Keys that
+// are quantised from fp32 under scales below 2^-15 (fp8) or 2^-23 (fp4) may lie between
+// fp16's smallest numbers: decoded to nearest even, off by 2^-25 (every element under every
+// scale is tested).
 #pragma once
 
 #include "common.h"

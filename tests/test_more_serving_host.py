@@ -119,6 +119,22 @@ def test_quantised_rows(storage, dtype):
         assert torch.equal(y.to(torch.float8_e4m3fn).view(torch.uint8) & 127, codes & 127)
 
 
+@pytest.mark.parametrize("storage", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantised_tokens_are_numbers_of_their_type(storage, dtype):
+    """Every finite token, the smallest too, beside some powers of two as the largest of its
+    block."""
+    x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = x[torch.isfinite(x)]
+    for e in range(-24, 16, 3) if dtype == torch.float16 else (-133, -120, -100, -10, 0, 60, 127):
+        top = torch.tensor(2.0, dtype=torch.float64).pow(e)
+        y = x[x.double().abs() <= top]
+        y = torch.cat([y, torch.zeros(-len(y) % 31, dtype=dtype)]).view(-1, 31)
+        rows = torch.cat([y, top.to(dtype).expand(len(y), 1)], 1)
+        values = S.mx_values(*S.mx_quantise(rows, storage, dtype), storage)
+        assert torch.equal(values.to(dtype).double(), values)
+
+
 def test_rotation_keeps_lengths():
     g = torch.Generator().manual_seed(1)
     x = torch.randn(4, 2, 64, generator=g)

@@ -234,3 +234,36 @@ def test_refusals_with_a_cache(gpu_device):
     prepare_qk_norm_rope(q, k, positions, inv_freq, q_out=q_out, k_out=k_out)
     with pytest.raises(ValueError, match="overlap"):
         prepare_qk_norm_rope(q, k, positions, inv_freq, q_out=q_out, k_out=flat[128:128 + k.numel()].view(k.shape))
+
+
+@pytest.mark.parametrize("storage", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("down", [20, 24])
+def test_small_fp16_keys_into_a_cache(down, interleaved, storage, gpu_device):
+    """Keys quantised from fp32 below what fp16 holds: as near as the others in the cache, and
+    read back to the nearest fp16 number.  Elements of four bits lie between fp16's numbers only
+    where the largest of 32 is at most 6 * 2^-24 = 0.375 * 2^-20, so not among normed keys
+    times 2^-20 and more."""
+    n, hkv, d = 90, 2, 64
+    q, k, v, positions, inv_freq, _ = _inputs(n, 4, hkv, d, d, torch.float16, gpu_device, fused=False)
+    g = torch.Generator().manual_seed(8)
+    weight = 2.0 ** -down * (1 + torch.rand(d, generator=g))
+    c, slots = _cached(gpu_device, torch.float16, storage, n, hkv, d)
+    slots = list(range(n))
+    c.slots[:n] = torch.arange(n, device=gpu_device)
+    prepare_qk_norm_rope(q, k, positions, inv_freq, None, weight.to(gpu_device), interleaved=interleaved, v=v, cache=c, layer=1)
+    keys, b = _held(c, c.k, c.k_scales, slots, 1)
+    scale = torch.pow(torch.tensor(2.0, dtype=torch.float64), b.long() - 127).repeat_interleave(32, -1)
+    relative, absolute = (2.0 ** -4, 2.0 ** -10) if storage == "mxfp8" else (2.0 ** -2, 0.25)
+    _near(keys, k, positions, inv_freq, weight, interleaved=interleaved,
+          step=lambda ref: torch.maximum(relative * ref.abs(), absolute * scale))
+    off = (keys.half().double() - keys).abs()
+    top = keys.abs().unflatten(-1, (-1, 32)).amax(-1)
+    small = top <= (448 * 2.0 ** -16 if storage == "mxfp8" else 6 * 2.0 ** -24)  # what the type may not hold
+    assert small.any() == (storage == "mxfp8" or down == 24) and (off <= 2.0 ** -25).all()
+    assert (off > 0).any() == small.any() and (off.unflatten(-1, (-1, 32)).amax(-1)[~small] == 0).all()
+    c.tables[0, :c.pages], c.lengths[0] = torch.arange(c.pages, dtype=torch.int32, device=gpu_device), n
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    at = [torch.tensor(x, dtype=torch.int32, device=gpu_device) for x in ([0], [0, n])]
+    c.gather(1, *at, ko, vo)
+    assert torch.equal(ko.cpu(), keys.half())

@@ -361,3 +361,28 @@ def test_serving_steps(hq, hkv, d, dtype, storage, gpu_device):
     c.compact()
     held(1, 4, lengths)
     c.check_inputs()
+
+
+@pytest.mark.parametrize("wide", WIDE)
+@pytest.mark.parametrize("storage", STORAGES)
+def test_elements_between_the_smallest_fp16_numbers(storage, wide, gpu_device):
+    """Keys and values that fp16 does not hold: attention over them to nearest even.  Large
+    queries give scores as of N(0, 1) rows; an output below 2^-14 is off by 2^-25 instead of
+    by half a step of its own."""
+    p = Pages([300, 77, 1], 8, 2, 128, 16, torch.float16, storage, gpu_device, wide=wide)
+    down = 20 if storage == "mxfp8" else 24  # powers of two
+    lost = 0
+    for i in (0, 1):
+        s = p.gpu[2 * i + 1].view(torch.uint8)
+        s.copy_(torch.where(s == 255, s, s - down))
+        x = p.values[i] * 2.0 ** -down
+        p.values[i] = x.half().double()
+        lost += int((p.values[i] != x).sum())
+    assert lost > 0
+    p.q *= 2.0 ** 12
+    scale = 128 ** -0.5 * 2.0 ** (down - 12)
+    plan = p.plan(scale=scale)
+    ref, bound = p.reference(scale)
+    tol = S.tolerance(ref, bound, torch.float16, max(p.lengths), p.values[1].abs().max().item()) + 2.0 ** -25
+    assert ((plan.output.double().cpu() - ref).abs() <= tol).all()
+    plan.check_inputs()

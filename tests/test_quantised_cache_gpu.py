@@ -333,3 +333,44 @@ def test_offsets_past_32_bits(storage, gpu_device):
         want = S.mx_values(*S.mx_quantise(x.cpu(), storage, x.dtype), storage).to(x.dtype)
         assert torch.equal(out[500:].cpu(), want) and (out[:500] == 0).all()
     c.check_inputs()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("storage", STORAGES)
+def test_gather_every_element_under_every_scale(storage, dtype, gpu_device):
+    """In the tokens' type to nearest even: what that holds exactly, fp16 between its smallest
+    numbers too, beyond its largest an infinity."""
+    n = 1020
+    c = _cache(gpu_device, storage, dtype, pages=2, page=1024, heads=1, sequences=1, max_pages=2, max_tokens=n, layers=1)
+    codes = torch.arange(n * 64).view(n, 64) % (256 if storage == "mxfp8" else 16)
+    scales = torch.arange(n) // 4  # 0 to 254
+    held = S.mx_pack(codes.to(torch.uint8), storage)
+    for t, s in ((c.k, c.k_scales), (c.v, c.v_scales)):
+        t.view(torch.uint8)[0, 1, 0, :n] = held.to(gpu_device)
+        s.view(torch.uint8)[0, 1, 0, :, :n] = scales.to(torch.uint8).expand(2, n).to(gpu_device)
+    c.tables[0, 0], c.lengths[0] = 1, n
+    k, v = (torch.zeros(n, 1, 64, dtype=dtype, device=gpu_device) for _ in range(2))
+    c.gather(0, _i32([0], gpu_device), _i32([0, n], gpu_device), k, v)
+    values = S.mx_values(codes, scales[:, None].expand(n, 2), storage)
+    want = values.to(dtype)
+    assert not torch.equal(want.double().nan_to_num(0), values.nan_to_num(0))  # some do not fit
+    for out in (k, v):
+        out = out[:, 0].cpu()
+        assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(0), want.nan_to_num(0))
+
+
+@pytest.mark.parametrize("storage", STORAGES)
+def test_small_fp16_tokens_read_back(storage, gpu_device):
+    """What append writes of tokens down to fp16's smallest is read back without another rounding."""
+    g = torch.Generator().manual_seed(6)
+    c = _cache(gpu_device, storage, torch.float16)
+    e = torch.randint(-24, -8, (2, 150, 2, 2, 1), generator=g).double()
+    x = torch.randn(2, 150, 2, 2, 32, generator=g, dtype=torch.float64) * torch.pow(torch.tensor(2.0, dtype=torch.float64), e)
+    k, v = x.flatten(-2).half().to(gpu_device)
+    c.slots[:150] = torch.arange(150, device=gpu_device)
+    c.append(0, k, v)
+    c.tables[0, :10], c.lengths[0] = _i32(list(range(10)), gpu_device), 150
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    c.gather(0, _i32([0], gpu_device), _i32([0, 150], gpu_device), ko, vo)
+    for out, x in ((ko, k), (vo, v)):
+        assert torch.equal(out.double().cpu(), S.mx_values(*S.mx_quantise(x.cpu(), storage, x.dtype), storage))
