@@ -267,3 +267,40 @@ def test_small_fp16_keys_into_a_cache(down, interleaved, storage, gpu_device):
     at = [torch.tensor(x, dtype=torch.int32, device=gpu_device) for x in ([0], [0, n])]
     c.gather(1, *at, ko, vo)
     assert torch.equal(ko.cpu(), keys.half())
+
+
+@pytest.mark.parametrize("storage", ["rows", None, "mxfp8", "mxfp4"])
+@pytest.mark.parametrize("n,hq,hkv,d", [(2500, 32, 8, 128), (3000, 32, 8, 128), (5200, 8, 2, 128), (5200, 12, 4, 64),
+                                        (8191, 24, 4, 128), (5121, 5, 5, 64), (900, 130, 2, 64), (6000, 2, 1, 128)])
+def test_a_chunk_of_tokens(n, hq, hkv, d, storage, gpu_device):
+    """As many tokens as have their heads in one wave, or shared out over a few: every row the
+    same bits as in calls of 200 tokens, which are shared out more, and those as near as any."""
+    interleaved = hq % 8 == 0
+    q, k, v, positions, inv_freq, w = _inputs(n, hq, hkv, d, d, torch.bfloat16, gpu_device)
+    at = list(range(0, n, 200))
+    few = [prepare_qk_norm_rope(q[a:a + 200], k[a:a + 200], positions[a:a + 200], inv_freq, *w, interleaved=interleaved) for a in at]
+    want_q, want_k = torch.cat([x.q_out for x in few]), torch.cat([x.k_out for x in few])
+    for i in (0, len(few) - 1):
+        a = slice(at[i], at[i] + 200)
+        _near(few[i].q_out, q[a], positions[a], inv_freq, w[0], interleaved=interleaved)
+        _near(few[i].k_out, k[a], positions[a], inv_freq, w[1], interleaved=interleaved)
+    if storage == "rows":
+        plan = prepare_qk_norm_rope(q, k, positions, inv_freq, *w, interleaved=interleaved)
+        assert torch.equal(plan.q_out, want_q) and torch.equal(plan.k_out, want_k)
+        return
+    c, slots = _cached(gpu_device, torch.bfloat16, storage, n, hkv, d)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=gpu_device)
+    plan = prepare_qk_norm_rope(q, k, positions, inv_freq, *w, interleaved=interleaved, k_out=k_out, v=v, cache=c, layer=1)
+    assert torch.equal(plan.q_out, want_q) and torch.equal(k_out, want_k)
+    planes = [t.view(torch.uint8).clone() for t in (c.k, c.v, c.k_scales, c.v_scales) if t is not None]
+    for t in (c.k, c.v, c.k_scales, c.v_scales):
+        if t is not None:
+            t.view(torch.uint8).zero_()
+    every = c.slots.clone()
+    for a in at:  # the cache by calls of few tokens
+        m = min(200, n - a)
+        c.slots[:m] = every[a:a + m]
+        prepare_qk_norm_rope(q[a:a + m], k[a:a + m], positions[a:a + m], inv_freq, *w, interleaved=interleaved, v=v[a:a + m], cache=c,
+                             layer=1)
+    for t, x in zip((c.k, c.v, c.k_scales, c.v_scales), planes):
+        assert torch.equal(t.view(torch.uint8), x)
