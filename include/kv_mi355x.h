@@ -108,7 +108,9 @@ int kv_cache_append(kv_cache *c, int32_t layer, const void *k, const void *v, in
  * tokens' type, to nearest even where that does not hold them (no case of what append
  * wrote).  starts: int32 [n + 1], ascending within [0, tokens] (else a status, and
  * some rows may be left out); tokens <= KV_MAX_GATHER_TOKENS.  Other rows of k and v are
- * left as they were.  k and v share no memory with each other or the cache. */
+ * left as they were.  Token strides are at most 2^30; k and v share no memory with each
+ * other (rows of one may lie between the other's), with rows and starts or with the
+ * cache. */
 int kv_cache_gather(kv_cache *c, int32_t layer, const int32_t *rows, const int32_t *starts, int32_t n, void *k, void *v,
                     int64_t k_stride, int64_t v_stride, int32_t tokens, void *stream);
 /* dst[i] becomes a second holder of the pages of src[i] (int32 [n], n <=

@@ -6,6 +6,7 @@
 #include "../../include/kv_mi355x.h"
 #include "gqa_internal.h"
 #include "kv_internal.h"
+#include "spans.h"
 
 namespace moe {
 int capi_fail(int code, const char *fmt, ...);  // moe_capi.hip (thread-local message)
@@ -13,6 +14,7 @@ int capi_fail(int code, const char *fmt, ...);  // moe_capi.hip (thread-local me
 
 struct kv_cache {
   moe::KvState s;
+  moe::Span memory[11];  // what is the cache's
   int device;
 };
 
@@ -26,6 +28,8 @@ const KvState *kv_state(const kv_cache *c, int *device) {
 namespace {
 
 using moe::capi_fail;
+
+constexpr int64_t kMaxStride = 1LL << 30;  // of rows that are written
 
 bool aligned(const void *p, uintptr_t n) { return p && ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -125,6 +129,15 @@ int kv_cache_create_stored(kv_cache **out, const kv_cache_desc *d, int32_t stora
   s.page_bytes = rows * (storage == KV_STORAGE_16BIT ? 2 * d->head_dim : storage == KV_STORAGE_MXFP8 ? d->head_dim : d->head_dim / 2);
   s.scale_page_bytes = storage == KV_STORAGE_16BIT ? 0 : rows * (d->head_dim / 32);
   moe::kv_bind_workspace(&s, d->workspace);
+  const int64_t planes = (int64_t)d->layers * d->pages;
+  const moe::Span memory[] = {
+      moe::span_of(d->k, planes * s.page_bytes), moe::span_of(d->v, planes * s.page_bytes),
+      moe::span_of(k_scales, planes * s.scale_page_bytes), moe::span_of(v_scales, planes * s.scale_page_bytes),
+      moe::span_of(d->tables, 4 * (int64_t)d->sequences * d->max_pages), moe::span_of(d->lengths, 4 * (int64_t)d->sequences),
+      moe::span_of(d->refs, 4 * (int64_t)d->pages), moe::span_of(d->starts, 4 * ((int64_t)d->sequences + 1)),
+      moe::span_of(d->slots, 8 * (int64_t)d->max_tokens), moe::span_of(d->status, 16), moe::span_of(d->workspace, (int64_t)need)};
+  static_assert(sizeof(memory) == sizeof(c->memory), "spans of a cache");
+  memcpy(c->memory, memory, sizeof(memory));
   c->device = dev;
   *out = c;
   return MOE_OK;
@@ -170,8 +183,16 @@ int kv_cache_gather(kv_cache *c, int32_t layer, const int32_t *rows, const int32
   if (!aligned(rows, 4) || !aligned(starts, 4)) return capi_fail(MOE_EINVAL, "rows and starts must be given");
   if (!aligned(k, 16) || !aligned(v, 16)) return capi_fail(MOE_EINVAL, "k/v must be non-null and 16-byte aligned");
   const int64_t row = (int64_t)c->s.kv_heads * c->s.head_dim;
-  if (k_stride < row || v_stride < row || k_stride % 8 || v_stride % 8)
-    return capi_fail(MOE_EINVAL, "token strides must be >= %lld and multiples of 8", (long long)row);
+  if (k_stride < row || v_stride < row || k_stride % 8 || v_stride % 8 || k_stride > kMaxStride || v_stride > kMaxStride)
+    return capi_fail(MOE_EINVAL, "token strides must be >= %lld, multiples of 8, at most 2^30", (long long)row);
+  // What is written is neither read nor written by another workgroup.
+  const moe::Rows k_rows = {k, 2 * k_stride, 2 * row, tokens}, v_rows = {v, 2 * v_stride, 2 * row, tokens};
+  if (moe::may_meet(k_rows, v_rows)) return capi_fail(MOE_EINVAL, "k and v must share no memory");
+  for (const moe::Span out : {moe::span_of(k_rows), moe::span_of(v_rows)}) {
+    bool shared = moe::meet(out, moe::span_of(rows, 4 * (int64_t)n)) || moe::meet(out, moe::span_of(starts, 4 * ((int64_t)n + 1)));
+    for (const moe::Span own : c->memory) shared |= moe::meet(out, own);
+    if (shared) return capi_fail(MOE_EINVAL, "k and v must share no memory with rows, starts or the cache");
+  }
   return on_device(c, "gather", [&] {
     return moe::launch_kv_gather(c->s, layer, rows, starts, n, (uint16_t *)k, (uint16_t *)v, k_stride, v_stride, tokens,
                                  (hipStream_t)stream);

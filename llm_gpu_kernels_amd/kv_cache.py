@@ -172,7 +172,8 @@ class PagedKVCache:
         ``dtype``, the heads of a token side by side), as the keys and values of
         ``prepare_segmented_gqa`` or ``prepare_packed_gqa`` lie.  ``starts``: int32
         [n + 1], ascending within [0, tokens], tokens at most 2^26.  Other rows of k and v
-        keep what they held; k and v share no memory."""
+        keep what they held.  k and v may be views of one tensor, but share no memory with
+        each other, ``rows``, ``starts`` or the cache."""
         if not isinstance(layer, int) or not 0 <= layer < self.layers:
             raise ValueError(f"layer must be an int in [0, {self.layers}) (got {layer!r})")
         n = self._rows(rows, "rows").shape[0]

@@ -374,3 +374,57 @@ def test_small_fp16_tokens_read_back(storage, gpu_device):
     c.gather(0, _i32([0], gpu_device), _i32([0, 150], gpu_device), ko, vo)
     for out, x in ((ko, k), (vo, v)):
         assert torch.equal(out.double().cpu(), S.mx_values(*S.mx_quantise(x.cpu(), storage, x.dtype), storage))
+
+
+@pytest.mark.parametrize("storage", [None] + STORAGES)
+def test_gather_refuses_memory_that_is_read_or_written_twice(storage, gpu_device):
+    """Before anything is launched; rows of one tensor between each other's are taken."""
+    n, dim, heads = 40, 64, 1
+    c = _cache(gpu_device, storage, heads=heads, dim=dim, layers=1)
+    c.tables[0, :3], c.lengths[0] = _i32([3, 8, 5], gpu_device), n
+    _filled(c, 5)
+    rows, starts = _i32([0], gpu_device), _i32([0, n], gpu_device)
+    want = [_rows_of(c, t, s, 0, 0, n) for t, s in ((c.k, c.k_scales), (c.v, c.v_scales))]
+    before = [_bytes(t) for t in _planes(c)] + [t.cpu() for t in (c.tables, c.lengths, c.refs, c.slots, c.starts)]
+
+    def new(*shape):
+        return torch.zeros(*shape, dtype=c.dtype, device=gpu_device)
+
+    def of(t):  # a tensor of the call's type at a tensor's memory, if it holds that many
+        flat = t.reshape(-1).view(torch.uint8).view(c.dtype)
+        return flat[:flat.numel() // dim * dim].view(-1, heads, dim)
+
+    other, one, wide = new(n, heads, dim), new(2 * n, heads, dim), new(n + 1, heads, 2 * dim)
+    taken = [(new(n, heads, dim), other), (wide[:n, :, dim:], wide[1:, :, :dim]), (one[:n], one[n:]), (one[n:], one[:n]), (one[0::2], one[1::2]), (one[1::2], one[0::2]),
+             new(n, 2 * heads, dim).split(heads, 1), new(n, 3 * heads, dim)[:, 1:].split(heads, 1)]
+    for k, v in taken:
+        c.gather(0, rows, starts, k, v)
+        assert torch.equal(k.cpu().view(torch.int16), want[0].view(torch.int16))
+        assert torch.equal(v.cpu().view(torch.int16), want[1].view(torch.int16))
+    crossing = wide.as_strided((n, heads, dim), (2 * dim, dim, 1), dim + 32)  # from one row to the next
+    refused = [(other, other), (one[:n], one[n - 1:2 * n - 1]), (one[:n], one[0::2]), (one[1::2], one[n:]),
+               (wide[:n, :, :dim], wide[:n, :, 8:dim + 8]), (wide[:n, :, dim:], crossing)]
+    for t in _planes(c) + [c.slots, c.workspace]:
+        m = of(t)
+        if m.shape[0]:
+            few = min(len(m), n)
+            refused += [(m[:few], other[:few]), (other[:few], m[-few:])]
+    both = torch.zeros(4096, dtype=torch.int32, device=gpu_device)  # outputs around rows and starts
+    at = of(both)
+    both[100:101], both[104:106] = rows, starts
+    for k, v in refused:
+        kept = k.clone(), v.clone()
+        with pytest.raises(ValueError, match="share no memory"):
+            c.gather(0, rows, starts if len(k) == n else _i32([0, len(k)], gpu_device), k, v)
+        assert torch.equal(k.view(torch.int16), kept[0].view(torch.int16)) and torch.equal(v.view(torch.int16), kept[1].view(torch.int16))
+    for a, b in ((both[100:101], starts), (rows, both[104:106])):
+        for k, v in ((at[:n], other), (other, at[:n])):
+            with pytest.raises(ValueError, match="share no memory"):
+                c.gather(0, a, b, k, v)
+    c.gather(0, both[100:101], both[104:106], at[n:2 * n], other)
+    after = [_bytes(t) for t in _planes(c)] + [t.cpu() for t in (c.tables, c.lengths, c.refs, c.slots, c.starts)]
+    assert all(torch.equal(a, b) for a, b in zip(before, after))
+    for stride in (1 << 31, (1 << 30) + 8):
+        assert N.lib().kv_cache_gather(c._cache, 0, rows.data_ptr(), starts.data_ptr(), 1, one.data_ptr(), other.data_ptr(), stride,
+                                       64, n, None) == N.MOE_EINVAL
+    c.check_inputs()
