@@ -78,7 +78,9 @@ class PreparedQKNormRope:
         d.v_stride = 0 if v is None else _token_stride(v, "v")
         q_out = _output(q_out, q)
         k_out = None if k_out is None and cache is not None else _output(k_out, k)
-        inputs = [q, k, positions, inv_freq] + weights + ([] if v is None else [v, cache.k, cache.v, cache.slots])
+        inputs = [q, k, positions, inv_freq] + weights
+        if cache is not None:
+            inputs += [v, cache.k, cache.v, cache.slots] + [t for t in (cache.k_scales, cache.v_scales) if t is not None]
         for out in (q_out, k_out):
             if out is not None:
                 check_out_storage(out, inputs)

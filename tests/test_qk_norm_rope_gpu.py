@@ -304,3 +304,16 @@ def test_a_chunk_of_tokens(n, hq, hkv, d, storage, gpu_device):
                              layer=1)
     for t, x in zip((c.k, c.v, c.k_scales, c.v_scales), planes):
         assert torch.equal(t.view(torch.uint8), x)
+
+
+@pytest.mark.parametrize("storage", ["mxfp8", "mxfp4"])
+def test_outputs_in_the_cache_are_refused(storage, gpu_device):
+    """Its scales are written as its elements are."""
+    q, k, v, positions, inv_freq, w = _inputs(20, 8, 2, 128, 128, torch.bfloat16, gpu_device, fused=False)
+    c = PagedKVCache(600, 16, 2, 128, sequences=1, max_pages=2, max_tokens=20, storage=storage, device=gpu_device)
+    for held in (c.k, c.v, c.k_scales, c.v_scales):
+        flat = held.view(torch.uint8).flatten().view(torch.bfloat16)
+        for kw in (dict(q_out=flat[:q.numel()].view(q.shape)), dict(k_out=flat[-k.numel():].view(k.shape))):
+            with pytest.raises(ValueError, match="share storage"):
+                prepare_qk_norm_rope(q, k, positions, inv_freq, *w, v=v, cache=c, **kw)
+        assert (held.view(torch.uint8) == 0).all()
