@@ -321,8 +321,10 @@ def prepare_packed_gqa(q, k, v, starts, out=None, *, scale=None):
     return plan
 
 
-# Elements of a microscaled cache -> the library's storage, elements per entry of a row.
-_STORAGES = {torch.float8_e4m3fn: (N.GQA_STORAGE_MXFP8, 1), torch.float4_e2m1fn_x2: (N.GQA_STORAGE_MXFP4, 2)}
+# Elements of a microscaled cache -> the library's storage, elements per entry of a row (of the
+# types that torch has).
+_STORAGES = {getattr(torch, name): held for name, held in (("float8_e4m3fn", (N.GQA_STORAGE_MXFP8, 1)),
+                                                           ("float4_e2m1fn_x2", (N.GQA_STORAGE_MXFP4, 2))) if hasattr(torch, name)}
 
 
 def _check_stored(t, scales, name, q):
@@ -330,7 +332,7 @@ def _check_stored(t, scales, name, q):
     [P, Hkv, D / 32, page], rows and scales of a page and head side by side."""
     if not isinstance(t, torch.Tensor) or t.dtype not in _STORAGES:
         raise TypeError(f"{name} must be a torch.float8_e4m3fn or torch.float4_e2m1fn_x2 tensor beside scales")
-    if not isinstance(scales, torch.Tensor) or scales.dtype != torch.float8_e8m0fnu:
+    if not isinstance(scales, torch.Tensor) or scales.dtype != getattr(torch, "float8_e8m0fnu", None):
         raise TypeError(f"{name}'s scales must be a torch.float8_e8m0fnu tensor")
     dim = q.shape[2]
     row = dim // _STORAGES[t.dtype][1]

@@ -20,9 +20,10 @@ from .attention import _check_int32, _stream_of
 
 __all__ = ["PagedKVCache"]
 
-# storage -> the library's number, the elements' type (None: the tokens'), elements per entry
-_STORAGES = {None: (N.KV_STORAGE_16BIT, None, 1), "mxfp8": (N.KV_STORAGE_MXFP8, torch.float8_e4m3fn, 1),
-             "mxfp4": (N.KV_STORAGE_MXFP4, torch.float4_e2m1fn_x2, 2)}
+# storage -> the library's number, the elements' type by name (None: the tokens'; a torch may
+# lack it), elements per entry
+_STORAGES = {None: (N.KV_STORAGE_16BIT, None, 1), "mxfp8": (N.KV_STORAGE_MXFP8, "float8_e4m3fn", 1),
+             "mxfp4": (N.KV_STORAGE_MXFP4, "float4_e2m1fn_x2", 2)}
 
 
 class PagedKVCache:
@@ -60,6 +61,11 @@ class PagedKVCache:
             raise TypeError("dtype must be torch.bfloat16 or torch.float16")
         if storage not in _STORAGES:
             raise ValueError(f"storage must be None, 'mxfp8' or 'mxfp4' (got {storage!r})")
+        code, element, per_byte = _STORAGES[storage]
+        missing = [f"torch.{n}" for n in (element, "float8_e8m0fnu") if element and not hasattr(torch, n)]
+        if missing:
+            raise RuntimeError(f"storage {storage!r} needs {' and '.join(missing)}, which this torch does not have")
+        element = element and getattr(torch, element)
         device = torch.device(device)
         d = N.KvCacheDesc()
         sizes = dict(pages=pages, page_size=page_size, kv_heads=kv_heads, head_dim=head_dim, layers=layers,
@@ -77,7 +83,6 @@ class PagedKVCache:
         self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
         self.sequences, self.max_pages, self.max_tokens, self.layers = sequences, max_pages, max_tokens, layers
         self.dtype, self.storage, self.device = dtype, storage, device
-        code, element, per_byte = _STORAGES[storage]
         shape = (layers, pages, kv_heads, page_size, head_dim // per_byte)
         def zeros(shape, kind):  # (torch fills no elements of four bits)
             return torch.zeros(shape, dtype=torch.uint8 if element else kind, device=device).view(kind)

@@ -2,6 +2,9 @@
 GPU: refusals of the C ABI and of the Python layer, and the oracle's own invariants."""
 import ctypes
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -10,6 +13,7 @@ from llm_gpu_kernels_amd import (PagedKVCache, _native as N, prepare_paged_gqa, 
                                  prepare_shared_gqa)
 from oracle import serving_oracle as S
 
+ROOT = Path(__file__).resolve().parents[1]
 BASE = 1 << 20  # an address that is only looked at by the validation
 
 
@@ -232,3 +236,41 @@ def test_attention_python_refusals():
         prepare_paged_gqa(q, eight, eight, tables, lengths, k_scales=scales)
     with pytest.raises(ValueError):  # not on a GPU
         prepare_paged_gqa(q, eight, eight, tables, lengths, k_scales=scales, v_scales=scales)
+
+
+WITHOUT = r"""
+import sys
+import torch
+for name in sys.argv[1].split(","):
+    delattr(torch, name)
+from llm_gpu_kernels_amd import PagedKVCache, prepare_paged_gqa, prepare_moe
+sizes = dict(sequences=4, max_pages=8, max_tokens=64)
+for storage, needs in ((None, ""), ("mxfp8", "float8_e4m3fn,float8_e8m0fnu"), ("mxfp4", "float4_e2m1fn_x2,float8_e8m0fnu")):
+    try:
+        PagedKVCache(10, 16, 2, 64, storage=storage, device="cpu", **sizes)
+    except Exception as e:
+        print(type(e).__name__, e, flush=True)
+    gone = [n for n in needs.split(",") if n in sys.argv[1].split(",")]
+    if not gone:
+        continue
+    try:
+        q, t = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 2, 16, 64, dtype=torch.uint8)
+        prepare_paged_gqa(q, t, t, q, q, k_scales=t, v_scales=t)
+    except TypeError as e:
+        print("attention", e, flush=True)
+"""
+
+
+@pytest.mark.parametrize("gone", ["float4_e2m1fn_x2", "float8_e8m0fnu", "float4_e2m1fn_x2,float8_e8m0fnu,float8_e4m3fn"])
+def test_a_torch_without_the_types_of_a_storage(gone):
+    """The package is imported, and everything else of it works; a storage whose types are
+    missing is refused by name."""
+    done = subprocess.run([sys.executable, "-c", WITHOUT, gone], capture_output=True, text=True, cwd=ROOT)
+    assert done.returncode == 0, done.stderr
+    lines = done.stdout.splitlines()
+    caches = [x for x in lines if not x.startswith("attention")]
+    assert len(caches) == 3 and caches[0] == "ValueError device must be a GPU device"
+    for line, needs in zip(caches[1:], ({"float8_e4m3fn", "float8_e8m0fnu"}, {"float4_e2m1fn_x2", "float8_e8m0fnu"})):
+        missing = needs & set(gone.split(","))
+        assert line.startswith("RuntimeError" if missing else "ValueError device") and all(f"torch.{n}" in line for n in missing)
+    assert any(x.startswith("attention") for x in lines)
