@@ -134,7 +134,8 @@ typedef struct gqa_paged_desc {
   size_t workspace_bytes;
 } gqa_paged_desc;
 typedef struct gqa_paged_plan gqa_paged_plan;
-/* Status words and the partial states of a run. */
+/* Status words and the partial states of a run, of this descriptor: where it needs no states
+ * (each workgroup has all of a sequence), one with fewer sequences may. */
 int gqa_paged_workspace_bytes(const gqa_paged_desc *d, size_t *bytes);
 int gqa_paged_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d);
 /*
@@ -173,7 +174,7 @@ void gqa_paged_plan_destroy(gqa_paged_plan *p);
  * ascend within [0, B] are reported (GQA_STATUS_BAD_BOUNDS) and nothing is shared then; so
  * are negative prefixes, taken as 0.  starts and prefixes lie on the GPU and are read by
  * every run.  G <= 1024; desc as for the paged form, with a workspace of
- * gqa_shared_workspace_bytes().
+ * gqa_shared_workspace_bytes() for the same descriptor.
  */
 typedef struct gqa_shared_plan gqa_shared_plan;
 int gqa_shared_workspace_bytes(const gqa_paged_desc *d, int32_t G, size_t *bytes);

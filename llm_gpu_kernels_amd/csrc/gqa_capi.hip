@@ -215,6 +215,10 @@ size_t paged_workspace(const gqa_paged_desc *d, int storage, int cus) {
                                       : moe::gqa_mx_workspace(d->B, d->Hq, d->Hkv, d->D, storage, keys, cus);
 }
 
+size_t shared_workspace(const gqa_paged_desc *d, int G, int cus) {
+  return moe::gqa_shared_workspace(d->B, d->Hq, d->Hkv, d->D, (int64_t)d->M * d->page, G, cus);
+}
+
 int need_workspace(const void *workspace, size_t have, size_t need) {
   if (!workspace || !aligned16(workspace) || have < need)
     return moe::capi_fail(MOE_ESPACE, "workspace has %zu bytes, needs %zu, 16-byte aligned", have, need);
@@ -349,7 +353,7 @@ int gqa_shared_workspace_bytes(const gqa_paged_desc *d, int32_t G, size_t *bytes
   if (!rc) rc = validate_groups(G);
   if (!rc && !bytes) rc = moe::capi_fail(MOE_EINVAL, "null bytes");
   if (!rc) rc = device_cus(&dev, &cus);
-  if (!rc) *bytes = moe::gqa_shared_workspace(d->B, d->Hq, d->Hkv, d->D, G, cus);
+  if (!rc) *bytes = shared_workspace(d, G, cus);
   return rc;
 }
 
@@ -363,7 +367,7 @@ int gqa_shared_plan_create(gqa_shared_plan **out, const gqa_paged_desc *d, int32
     rc = moe::capi_fail(MOE_EINVAL, "starts and prefixes must be given");
   if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, 256);
   if (!rc) rc = device_cus(&dev, &cus);
-  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, moe::gqa_shared_workspace(d->B, d->Hq, d->Hkv, d->D, G, cus));
+  if (!rc) rc = need_workspace(d->workspace, d->workspace_bytes, shared_workspace(d, G, cus));
   if (rc) return rc;
   gqa_shared_plan *p = new (std::nothrow) gqa_shared_plan();
   if (!p) return moe::capi_fail(MOE_EINVAL, "out of host memory");

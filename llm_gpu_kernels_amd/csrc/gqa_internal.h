@@ -117,15 +117,16 @@ size_t gqa_mx_workspace(int B, int Hq, int Hkv, int D, int storage, int64_t keys
 hipError_t launch_gqa_mx(const GqaPagedArgs &a, int cus, hipStream_t s);
 
 // The same where groups of sequences start with the same keys (gqa_shared.hip), of 16-bit
-// pages: with a.shared.
-size_t gqa_shared_workspace(int B, int Hq, int Hkv, int D, int G, int cus);
+// pages: with a.shared.  keys: of a full table; a call that goes row by row needs the status
+// words alone.
+size_t gqa_shared_workspace(int B, int Hq, int Hkv, int D, int64_t keys, int G, int cus);
 void gqa_shared_bind(GqaPagedArgs *a, int G, const int32_t *starts, const int32_t *prefixes, void *workspace, int cus);
 hipError_t launch_gqa_shared(const GqaPagedArgs &a, int cus, hipStream_t s);
 // Of gqa_paged.hip: workgroups of four waves, and the launch over the planned work.
 int gqa_shared_workgroups(int D, int cus);
 hipError_t launch_gqa_shared_work(const GqaPagedArgs &a, int cus, hipStream_t s);
 // Whether every row is worked on by itself, and that.
-bool gqa_shared_by_rows(const GqaPagedArgs &a, int cus);
+bool gqa_shared_by_rows(int B, int Hq, int Hkv, int D, int64_t keys, int cus);
 hipError_t launch_gqa_shared_rows(const GqaPagedArgs &a, hipStream_t s);
 
 // Synchronises `s`, reads a status word and clears the bits that it had.

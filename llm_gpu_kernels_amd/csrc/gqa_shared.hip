@@ -266,23 +266,29 @@ Layout layout_of(int B, int Hq, int Hkv, int D, int G, int cus) {
 
 }  // namespace
 
-size_t gqa_shared_workspace(int B, int Hq, int Hkv, int D, int G, int cus) { return layout_of(B, Hq, Hkv, D, G, cus).bytes; }
+size_t gqa_shared_workspace(int B, int Hq, int Hkv, int D, int64_t keys, int G, int cus) {
+  return gqa_shared_by_rows(B, Hq, Hkv, D, keys, cus) ? 256 : layout_of(B, Hq, Hkv, D, G, cus).bytes;
+}
 
 void gqa_shared_bind(GqaPagedArgs *a, int G, const int32_t *starts, const int32_t *prefixes, void *workspace, int cus) {
   uint8_t *const w = (uint8_t *)workspace;
-  const Layout l = layout_of(a->B, a->Hq, a->Hkv, a->D, G, cus);
   const int per_page = a->page / 16;
   a->status = (uint32_t *)w;
+  a->shared = GqaSharedState{G, G <= shared::kLocalGroups && a->B <= shared::kLocalRows, starts, prefixes, nullptr, nullptr,
+                             nullptr, nullptr, nullptr, a->Hq / a->Hkv, per_page & (per_page - 1) ? -1 : __builtin_ctz(per_page)};
+  if (gqa_shared_by_rows(a->B, a->Hq, a->Hkv, a->D, (int64_t)a->M * a->page, cus)) return;
+  const Layout l = layout_of(a->B, a->Hq, a->Hkv, a->D, G, cus);
   a->pieces = (int32_t *)(w + l.pieces);
   a->partial = (float *)(w + l.partial);
-  a->shared = GqaSharedState{G, G <= shared::kLocalGroups && a->B <= shared::kLocalRows, starts, prefixes,
-                             (int32_t *)(w + l.header), (int32_t *)(w + l.groups), (int32_t *)(w + l.rows),
-                             (float *)(w + l.heads), (float *)(w + l.more), a->Hq / a->Hkv,
-                             per_page & (per_page - 1) ? -1 : __builtin_ctz(per_page)};
+  a->shared.header = (int32_t *)(w + l.header);
+  a->shared.groups = (int32_t *)(w + l.groups);
+  a->shared.rows = (int32_t *)(w + l.rows);
+  a->shared.heads = (float *)(w + l.heads);
+  a->shared.more = (float *)(w + l.more);
 }
 
 hipError_t launch_gqa_shared(const GqaPagedArgs &p, int cus, hipStream_t s) {
-  if (gqa_shared_by_rows(p, cus)) return launch_gqa_shared_rows(p, s);
+  if (gqa_shared_by_rows(p.B, p.Hq, p.Hkv, p.D, (int64_t)p.M * p.page, cus)) return launch_gqa_shared_rows(p, s);
   if (!p.shared.local)
     hipLaunchKernelGGL(gqa_shared_plan, dim3(1), dim3(kPlanThreads), 0, s, p, gqa_shared_workgroups(p.D, cus));
   if (const hipError_t e = launch_gqa_shared_work(p, cus, s)) return e;

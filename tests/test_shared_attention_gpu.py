@@ -1,6 +1,8 @@
 """Decode attention where groups of sequences start with the same keys, against attention
 in 64 bits of every sequence by its own table (MI355X only).  Tolerances: oracle/
 serving_oracle.py, tolerance(); the two parts of a row are joined in fp32."""
+import ctypes
+
 import pytest
 import torch
 
@@ -390,3 +392,19 @@ def test_prefixes_longer_than_every_member(gpu_device):
         plan.output.zero_()
         plan.run()
         x.check(plan)
+
+
+def test_workspace(gpu_device):
+    """Where every row goes by itself the status words are all that a plan needs, and less than
+    what is asked for is refused."""
+    x = Groups([(64, [70, 80, 90]), (48, [60, 61])], 8, 2, 128, 16, torch.bfloat16, gpu_device, behind=[33])
+    plan = x.plan()
+    assert (plan.workspace.numel() == 256) == (Groups.least_width == 1)
+    x.check(plan)
+    size, handle = ctypes.c_size_t(0), ctypes.c_void_p()
+    d = plan._desc
+    N.check(N.lib().gqa_shared_workspace_bytes(ctypes.byref(d), 2, ctypes.byref(size)), "size")
+    assert size.value == plan.workspace.numel()
+    d.workspace_bytes = size.value - 1
+    assert N.lib().gqa_shared_plan_create(ctypes.byref(handle), ctypes.byref(d), 2, x.gs.data_ptr(), x.gp.data_ptr()) == N.MOE_ESPACE
+    assert not handle.value
