@@ -145,7 +145,8 @@ int gqa_paged_plan_create(gqa_paged_plan **out, const gqa_paged_desc *d);
  * of a (page, head), [D / 32, page] bytes, lie together; page and head strides in bytes,
  * multiples of 16.  Page strides are below 2^31.  Elements are taken in q's type, to
  * nearest even: one whose value is beyond it is an infinity, one between its smallest
- * numbers (multiples of 2^-24 in fp16) is off by half of the smallest.  What append writes
+ * numbers (multiples of 2^-24 in fp16) is off by half of the smallest.  Probabilities are
+ * rounded to q's type for the product with v, as without a storage.  What append writes
  * for tokens of q's type are numbers of that type; what the norm and rotation write for
  * fp16 (qk_mi355x.h) may lie between them.  Run, status and destroy as above.
  */

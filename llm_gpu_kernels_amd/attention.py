@@ -419,8 +419,11 @@ def prepare_paged_gqa(q, k_pages, v_pages, tables, lengths, out=None, *, scale=N
     (torch.float8_e4m3fn [P, Hkv, page, D] or torch.float4_e2m1fn_x2 [P, Hkv, page, D / 2])
     and ``k_scales`` and ``v_scales`` (``cache.k_scales[layer]``) their scales; a page's
     rows of a head lie side by side.  Elements are taken in q's type: one whose value is
-    beyond it is an infinity.  Prepares and runs once; ``run()`` has no host sync and no
-    allocation."""
+    beyond it is an infinity.
+
+    Scores, maxima and sums are fp32, probabilities are rounded to q's type for the product
+    with the values (with or without a storage), and the output once.  Prepares and runs once;
+    ``run()`` has no host sync and no allocation."""
     plan = PreparedPagedGQA(q, k_pages, v_pages, tables, lengths, out, scale, k_scales, v_scales)
     plan.run()
     return plan
@@ -459,8 +462,8 @@ def prepare_shared_gqa(q, k_pages, v_pages, tables, lengths, starts, prefixes, o
     [starts[0], starts[G]) are in no group), and their first ``prefixes[g]`` keys are the
     same.  Members of length 0 are left out; of the others the shortest bounds what is
     shared, in whole blocks of 16 keys.  The table of one member is read for it, every
-    sequence's own for the rest, so the result is that of ``prepare_paged_gqa`` but for
-    the order of sums.  Pages are 16-bit.  Values of all tensors may change in place
+    sequence's own for the rest, so the result is that of ``prepare_paged_gqa``, its
+    roundings too, but for the order of sums.  Pages are 16-bit.  Values of all tensors may change in place
     between runs.  Prepares and runs once; ``run()`` has no host sync and no
     allocation."""
     plan = PreparedSharedGQA(q, k_pages, v_pages, tables, lengths, starts, prefixes, out, scale)

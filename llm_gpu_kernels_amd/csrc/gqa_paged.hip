@@ -798,7 +798,7 @@ hipError_t launch_gqa_shared_work(const GqaPagedArgs &a, int cus, hipStream_t s)
 // Where even a full table is a few steps for each of eight waves per (sequence, head block),
 // and those all run at once, the pages that rows share come from the L2 and one launch
 // beats the two: 8 and 32 rows with a prefix of 1500 keys, tables of 1616, 8 heads of 128,
-// 12.0 and 12.7 us, by groups 19.2 and 25.3.  Beyond, 128 rows of 1000 to 1200 keys 29.4, by groups
+// 11.7 and 13.1 us, by groups 19.2 and 25.3.  Beyond, 128 rows of 1000 to 1200 keys 29.4, by groups
 // 26.5; 8 of 4000 20.2, 21.9; 40 groups of 4 rows of 2000 201, 91.
 bool gqa_shared_by_rows(int B, int Hq, int Hkv, int D, int64_t keys, int cus) {
   const int64_t pairs = (int64_t)B * Hkv * ((Hq / Hkv + kRows - 1) / kRows);

@@ -174,8 +174,11 @@ class PagedKVCache:
         """Read back the first ``starts[i + 1] - starts[i]`` tokens of row ``rows[i]``
         (int32 [n]; fewer if the row is shorter, none if it is negative) of a layer to
         the rows ``starts[i]`` and up of ``k`` and ``v`` ([tokens, kv_heads, head_dim] of
-        ``dtype``, the heads of a token side by side), as the keys and values of
-        ``prepare_segmented_gqa`` or ``prepare_packed_gqa`` lie.  ``starts``: int32
+        ``dtype``, the heads of a token side by side).  They lie as those of a history do in
+        ``prepare_segmented_gqa`` (bf16, heads of 128, one conversation a call).
+        ``prepare_packed_gqa`` takes as many keys as queries, so it has a use for rows read
+        back only where their queries are there too; no call here attends a chunk behind a
+        history in fp16 or with heads of 64.  ``starts``: int32
         [n + 1], ascending within [0, tokens], tokens at most 2^26.  Other rows of k and v
         keep what they held.  k and v may be views of one tensor, but share no memory with
         each other, ``rows``, ``starts`` or the cache."""
