@@ -38,7 +38,7 @@ int validate(const qk_norm_rope_desc *d, const moe::KvState *s) {
   if (d->R < 2 || d->R > d->D || d->R % 2) return capi_fail(MOE_EINVAL, "R must be even, in [2, D] (got %d)", d->R);
   if (d->Hq < 1 || d->Hq > 65536 || d->Hkv < 1 || d->Hkv > 65536)
     return capi_fail(MOE_EINVAL, "Hq and Hkv must be in [1, 65536] (got %d, %d)", d->Hq, d->Hkv);
-  if (d->N < 0 || d->N > (1 << 24))  // (a grid has fewer than 2^32 threads; two parts of 64 a token)
+  if (d->N < 0 || d->N > (1 << 24))  // (a grid has fewer than 2^32 threads; two waves a token there)
     return capi_fail(MOE_EINVAL, "N must be in [0, 2^24] (got %d)", d->N);
   if (!(d->eps >= 0.f && d->eps < INFINITY)) return capi_fail(MOE_EINVAL, "eps must be finite and not negative");
   if (s) {

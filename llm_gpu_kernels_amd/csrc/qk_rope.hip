@@ -216,15 +216,17 @@ hipError_t launch(const QkArgs &a, int cus, hipStream_t s) {
   const int rows = a.Hq + a.Hkv + (a.cached ? a.Hkv : 0), passes = (rows + kRows - 1) / kRows;
   // A token's passes are shared out over waves, each of which computes its angles: over as many
   // as 20 waves a CU allow (24 to 32 run at once, by the variant's registers; 1000 tokens of 32 + 8
-  // heads of 128: 6.4 us, 7.5 with twice as many, 6.8 with 12 a CU), and where those are fewer, so that
-  // a wave has six passes at most (from 2700 tokens on the best of one to five waves a token, or
-  // mostly within 5 % of that).  In one wave, in two and in three, 3000 tokens: 10 passes (32 + 8 of 128) 12.4, 11.4, 12.2 us,
-  // 12 (the same into eight bits) 15.6, 14.5, 15.6, 3 (12 + 4 of 64 into eight bits) 6.5, 7.0, 7.5; 6000:
-  // 27.2, 25.8, 25.3 and 31.0, 29.5, 30.0 and 9.6, 10.6, 11.7.  7000 of 64 + 8, 18 passes, in one to five: 63.1,
-  // 53.6, 49.8, 49.3, 47.7; of 24 + 8, 8 passes, 27.1, 24.0, 24.3; of 16 + 4, 5 passes, 13.6, 13.9, 15.3.
-  constexpr int kMost = 6;
+  // heads of 128: 6.4 us, 7.5 with twice as many, 6.8 with 12 a CU), and where those are fewer, five
+  // passes to a wave by itself, thirteen to two, 21 to three (from 2700 tokens on the best of one to
+  // five waves a token, or mostly within 5 % of that).  In one wave, in two and in three, 3000 tokens:
+  // 10 passes (32 + 8 of 128) 12.4, 11.4, 12.2 us, 12 (the same into eight bits) 15.6, 14.5, 15.6, 3 (12 + 4
+  // of 64 into eight bits) 6.5, 7.0, 7.5; 6000: 27.2, 25.8, 25.3 and 31.0, 29.5, 30.0 and 9.6, 10.6, 11.7.
+  // 7000 of 64 + 8, 18 passes, in one to five: 63.1, 53.6, 49.8, 49.3, 47.7; of 24 + 8, 8 passes, 27.1,
+  // 24.0, 24.3; of 16 + 8, 6 passes, 19.1, 17.9; of 16 + 4, 5 passes, 13.6, 13.9, 15.3.
   const int64_t places = 20 * (int64_t)cus;
-  const int least = (passes + kMost - 1) / kMost, most = max(least, (int)(places / a.N)), each = (passes + most - 1) / most;
+  // (Fewer than 2^26 waves in all: a grid has fewer than 2^32 threads, and N goes up to 2^24.)
+  const int least = min(1 + (passes + 2) / 8, (1 << 25) / a.N), most = max(least, (int)(places / a.N));
+  const int each = (passes + most - 1) / most;
   const int parts = (passes + each - 1) / each;
   const uint32_t grid = (uint32_t)(((int64_t)a.N * parts + kWaves - 1) / kWaves);
   auto go = [&](auto *kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0, s, a, parts, each); };

@@ -317,3 +317,13 @@ def test_outputs_in_the_cache_are_refused(storage, gpu_device):
             with pytest.raises(ValueError, match="share storage"):
                 prepare_qk_norm_rope(q, k, positions, inv_freq, *w, v=v, cache=c, **kw)
         assert (held.view(torch.uint8) == 0).all()
+
+
+def test_as_many_tokens_as_allowed(gpu_device):
+    """2^24 tokens, the same 1024 over and over: every time the same bits."""
+    q, k, _, positions, inv_freq, w = _inputs(1024, 2, 1, 64, 64, torch.bfloat16, gpu_device)
+    few = prepare_qk_norm_rope(q, k, positions, inv_freq, *w)
+    times = 2 ** 14
+    plan = prepare_qk_norm_rope(q.repeat(times, 1, 1), k.repeat(times, 1, 1), positions.repeat(times), inv_freq, *w)
+    for out, one in ((plan.q_out, few.q_out), (plan.k_out, few.k_out)):
+        assert (out.view(times, *one.shape).view(torch.int16) == one.view(torch.int16)).all()
